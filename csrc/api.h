@@ -412,6 +412,39 @@ int zse_attn_prefill_ext(const void* q, int ldq, const void* kv_layer, int64_t b
                          void* out_f16, int ldo, int num_seqs, int max_q_len, int nh, int nkv, int hd, int block_size,
                          float scale, float softcap, int window, void* stream);
 
+// ---- kv_q8.cu: the 8-bit KV cache ---------------------------------------------------------------------------------
+// One layer: data uint8 [num_blocks][2 (K, V)][nkv][block_size][hd], scale fp32 [num_blocks][2][nkv][block_size]; an element
+// is (data - 128) * scale.  hd 64, 96, 128 or 256, block_size a multiple of 16; both 16-byte aligned.  Block ids and slots outside
+// the cache are reported through the status word and taken for holes.
+typedef struct ZseKvQ8 {
+  void* data;
+  void* scale;
+  int32_t num_blocks, nkv, block_size, hd;
+} ZseKvQ8;
+// Rows [M, (nh + 2 nkv) * hd] (fp16, row stride ld; or n_planes fp32 planes [n_planes][M][cols] plus bias_f16): q and k rotated
+// (rotate-half over the first rotary_dim dimensions, a multiple of 16), q to q_out (row stride ld_q; may be qkv), k and v
+// quantised into the cache at `slots` (-1: not stored), each with the scale max|x| / 127 of its head.
+int zse_rope_kv_write_q8(const ZseKvQ8* kv, const void* qkv, int ld, void* q_out, int ld_q, const void* planes, int n_planes,
+                         const void* bias, const void* positions_i32, const void* slots_i64, const void* inv_freq_f32, int M,
+                         int nh, int rotary_dim, void* status, void* stream);
+// Pages of whole sequences as fp16: block j of sequence s -> out[cu_blocks[s] + j] (zeros behind seq_lens[s]), its place to
+// out_tables[s][j] (-1: hole, or behind the sequence).  out: out_blocks pages [2][nkv][block_size][hd].
+int zse_kv_read_q8(const ZseKvQ8* kv, const void* tables_i32, int max_blocks, const void* seq_lens_i32,
+                   const void* cu_blocks_i32, int num_seqs, void* out_f16, int out_blocks, void* out_tables_i32, int out_max_blocks,
+                   void* status, void* stream);
+// ---- attention_q8.cu ----------------------------------------------------------------------------------------------
+// One row per sequence (cu_q null: row s sees seq_lens[s] tokens) or rows cu_q[s] .. cu_q[s + 1] - 1 of sequence s (at most
+// max_q), the first at position q_pos0[s], each seeing the tokens up to its own; window > 0: the last so many of them.
+// num_splits: pieces of a (sequence, kv head); 0: the launcher decides.  More than zse_attn_decode_q8_most_whole() pieces need
+// scratch of zse_attn_decode_q8_scratch_floats.
+int zse_attn_decode_q8_splits(int num_seqs, int max_q, int nh, int nkv, int hd, int block_size, int max_blocks, int window,
+                              int num_splits);
+int64_t zse_attn_decode_q8_scratch_floats(int num_seqs, int max_q, int nh, int hd, int splits);
+int zse_attn_decode_q8(const ZseKvQ8* kv, const void* q_f16, int ldq, const void* tables_i32, int max_blocks,
+                       const void* seq_lens_i32, const void* cu_q_i32, const void* q_pos0_i32, int num_seqs, int max_q,
+                       void* out_f16, int ldo, int nh, void* scratch_f32, int64_t scratch_floats, int num_splits, float scale,
+                       int window, void* status, void* stream);
+
 // ---- sampling.cu --------------------------------------------------------------------------------------------
 int zse_argmax(const void* logits_f16, int ld, void* out_i32, int M, int V, void* stream);
 int zse_sample(const void* logits_f16, int ld, void* out_i32, int M, int V, const void* temperature_f32,

@@ -1,0 +1,430 @@
+"""Kernels of the 8-bit KV cache (csrc/kv_q8.cu, csrc/attention_q8.cu) against 64 bits: sizes, masks and contents where they can go
+wrong, and the three of them together as a layer uses them."""
+import pytest
+import torch
+
+from tests.helpers.kv_q8_oracle import attention, check_write, make_cache, make_tables, scale_of
+from zse_b200.cache.quant_kv import QuantKV
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from zse_b200.ops.backend import make_ops
+    return make_ops(DEV)
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def ints(v, dtype=torch.int32):
+    return torch.tensor(v, dtype=dtype, device=DEV)
+
+
+def freqs_of(rot, theta=1e6):
+    return (theta ** (-torch.arange(0, rot, 2, dtype=torch.float64) / max(rot, 1))).float().to(DEV)
+
+
+# ---- write ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("hd,rot", [(64, 64), (64, 16), (96, 96), (96, 48), (128, 128), (128, 96), (256, 256), (128, 0)])
+@pytest.mark.parametrize("nh,nkv,M", [(4, 2, 1), (7, 1, 5), (40, 8, 33), (16, 16, 200)])
+@pytest.mark.parametrize("planes,bias", [(0, False), (1, False), (3, True), (9, True)])
+def test_write(ops, hd, rot, nh, nkv, M, planes, bias):
+    g = gen(hd * 1000 + rot * 10 + M + planes)
+    bs, blocks, cols = 16, M // 16 + 3, (nh + 2 * nkv) * hd
+    pos = torch.randint(0, 40000, (M,), generator=g, dtype=torch.int32)
+    pos[0] = 2 ** 31 - 1
+    pos[-1] = 131071 if M > 1 else 2 ** 31 - 1
+    slots = torch.randperm(blocks * bs, generator=g)[:M]
+    slots[M // 2] = -1 if M > 1 else slots[0]
+    kv = QuantKV(torch.full((blocks, 2, nkv, bs, hd), 77, dtype=torch.uint8, device=DEV),
+                 torch.full((blocks, 2, nkv, bs), 7.0, device=DEV))
+    qkv = torch.randn(M, cols + 24, generator=g).half().to(DEV)           # rows further apart than they are wide
+    before = qkv.clone()
+    p = b = None
+    x = qkv[:, :cols].double()
+    if planes:
+        p = torch.randn(planes, M, cols, generator=g).to(DEV)
+        b = torch.randn(cols, generator=g).half().to(DEV) if bias else None
+        # the kernel's own sum: the bias, then plane by plane, in fp32
+        acc = b.float().expand(M, cols) if bias else torch.zeros(M, cols, device=DEV)
+        for i in range(planes):
+            acc = acc + p[i]
+        x = acc.double()
+    ops.rope_kv_write_q8(qkv, kv, pos.to(DEV), slots.to(DEV), freqs_of(rot), M, nh, nkv, hd, planes=p, n_planes=planes, bias=b)
+    torch.cuda.synchronize()
+    ops.check()
+    assert torch.equal(qkv[:, nh * hd:], before[:, nh * hd:])
+    kept = slots >= 0
+    blk, off = (slots.clamp_min(0) // bs).to(DEV), (slots.clamp_min(0) % bs).to(DEV)
+    u, sc = kv.data[blk, :, :, off], kv.scale[blk, :, :, off]
+    k = kept.to(DEV)
+    check_write(x[k], pos.to(DEV)[k], freqs_of(rot), nh, nkv, hd, qkv[k, : nh * hd], u[k], sc[k])
+    if not kept.all():                                                     # q of rows that are not stored is rotated too
+        i = int((~kept).nonzero()[0])
+        from tests.helpers.kv_q8_oracle import rotated
+        h, pair = rotated(x[i: i + 1], pos[i: i + 1].to(DEV), freqs_of(rot), nh, nkv, hd)
+        want, wide = h[0, :nh].reshape(-1), pair[0, :nh].reshape(-1)
+        assert ((qkv[i, : nh * hd].double() - want).abs() <= want.abs() * 2.0 ** -11 + wide * 2.0 ** -21 + 2.0 ** -25).all()
+    free = torch.ones(blocks * bs, dtype=torch.bool)
+    free[slots[kept]] = False
+    flat = lambda t: t.transpose(1, 3).reshape(blocks * bs, -1)
+    assert (flat(kv.data)[free.to(DEV)] == 77).all() and (kv.scale.permute(0, 3, 1, 2).reshape(blocks * bs, -1)[free.to(DEV)] == 7).all()
+
+
+def test_write_to_a_place_of_its_own(ops):
+    nh, nkv, hd, M = 6, 2, 64, 19
+    g = gen(3)
+    qkv = torch.randn(M, (nh + 2 * nkv) * hd, generator=g).half().to(DEV)
+    before, q = qkv.clone(), torch.full((M + 1, nh * hd + 8), 5.0, dtype=torch.float16, device=DEV)
+    kv, kv2 = (QuantKV.zeros((2, 2, nkv, 16, hd), DEV) for _ in range(2))
+    args = (ints(list(range(M))), ints(list(range(M)), torch.int64), freqs_of(hd), M, nh, nkv, hd)
+    ops.rope_kv_write_q8(qkv, kv, *args, q_out=q)
+    assert torch.equal(qkv, before) and (q[M] == 5).all() and (q[:, nh * hd:] == 5).all()
+    ops.rope_kv_write_q8(qkv, kv2, *args)
+    assert torch.equal(qkv[:, : nh * hd], q[:M, : nh * hd]) and torch.equal(kv.data, kv2.data) and torch.equal(kv.scale, kv2.scale)
+
+
+def test_rows_of_zeros_infinities_and_nan(ops):
+    nh, nkv, hd, M = 2, 2, 64, 4
+    x = torch.randn(M, (nh + 2 * nkv) * hd, generator=gen(5)).half()
+    k, v = slice(nh * hd, (nh + 1) * hd), slice((nh + nkv) * hd, (nh + nkv + 1) * hd)
+    x[0, k] = 0
+    x[1, v] = 0
+    x[1, v.start + 5] = float("inf")
+    x[2, v.start + 7] = float("-inf")
+    x[3, v.start + 9] = float("nan")
+    kv = QuantKV.zeros((1, 2, nkv, 16, hd), DEV)
+    ops.rope_kv_write_q8(x.to(DEV), kv, ints([0] * M), ints([0, 1, 2, 3], torch.int64), freqs_of(hd), M, nh, nkv, hd)
+    data, scale = kv.data.cpu(), kv.scale.cpu()
+    assert (data[0, 0, 0, 0] == 128).all() and scale[0, 0, 0, 0] == 0
+    one = torch.full((hd,), 128, dtype=torch.uint8)
+    one[5] = 255
+    assert torch.equal(data[0, 1, 0, 1], one) and abs(float(scale[0, 1, 0, 1]) * 127 / 65504 - 1) < 2.0 ** -22
+    assert data[0, 1, 0, 2, 7] == 1 and abs(float(scale[0, 1, 0, 2]) * 127 / 65504 - 1) < 2.0 ** -22
+    assert scale[0, 1, 0, 3].isnan() and not scale[0, 1, 1].isnan().any() and not scale[0, 0].isnan().any()
+
+
+# ---- read back --------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("nkv,bs", [(1, 16), (2, 48), (8, 32)])
+@pytest.mark.parametrize("lens", [[1], [0, 16, 17, 0, 31, 500], [3] * 40, [2049]])
+def test_read(ops, hd, nkv, bs, lens):
+    g = gen(hd + nkv + len(lens))
+    need = [-(-n // bs) for n in lens]
+    blocks = sum(need) + 3
+    data, scale = make_cache(g, blocks, nkv, bs, hd, DEV)
+    kv = QuantKV(data, scale)
+    holes = [(s, j) for s, n in enumerate(need) for j in range(1, n - 1, 3)]
+    tables = make_tables(g, lens, bs, blocks, DEV, width=max(need) + 2, holes=holes)
+    for s, n in enumerate(lens):                                           # what lies behind a sequence is anything
+        if n % bs and tables[s, need[s] - 1] >= 0:
+            scale[tables[s, need[s] - 1].long(), :, :, n % bs:] = float("nan")
+    cu = [1]                                                               # a page that no sequence has, before and behind
+    for n in need:
+        cu.append(cu[-1] + n)
+    out = torch.full((cu[-1] + 1, 2, nkv, bs, hd), 9.0, dtype=torch.float16, device=DEV)
+    places = torch.full((len(lens) + 1, max(need) + 3), 55, dtype=torch.int32, device=DEV)
+    ops.kv_read_q8(kv, tables, ints(lens), ints(cu), len(lens), out, places)
+    torch.cuda.synchronize()
+    ops.check()
+    want = torch.full(out.shape, 9.0, dtype=torch.float64, device=DEV)
+    want_places = torch.full(places.shape, -1, dtype=torch.int32, device=DEV)
+    want_places[len(lens)] = 55
+    for s, n in enumerate(lens):
+        for j in range(need[s]):
+            b = int(tables[s, j])
+            if b < 0:
+                continue
+            want_places[s, j] = cu[s] + j
+            y = (data[b].double() - 128) * scale[b].double()[..., None]
+            y[:, :, max(0, n - j * bs):] = 0
+            want[cu[s] + j] = y
+    assert torch.equal(places, want_places)
+    # one product in fp32, one rounding to fp16
+    assert ((out.double() - want).abs() <= want.abs() * 2.0 ** -11 * 1.001 + 2.0 ** -25).all()
+
+
+# ---- attention --------------------------------------------------------------------------------------------------------------
+def attend(ops, lens, nh, nkv, hd, bs=16, window=0, holes=(), rows=None, splits=0, seed=0, cache=None, width=None, wide=16):
+    """Runs the operator over sequences of ``lens`` tokens (``rows``: new rows of each) and compares with 64 bits."""
+    g = gen(seed + hd + 7 * nkv + len(lens))
+    blocks = sum(-(-n // bs) for n in lens) + 2
+    data, scale = cache(g, blocks) if cache else make_cache(g, blocks, nkv, bs, hd, DEV)
+    tables = make_tables(g, lens, bs, blocks, DEV, width=width, holes=holes)
+    for s, n in enumerate(lens):
+        if n % bs and tables[s, n // bs] >= 0:
+            scale[tables[s, n // bs].long(), :, :, n % bs:] = float("nan")
+    seen = [(s, n) for s, n in enumerate(lens)] if rows is None else [(s, n - r + 1 + i) for s, (n, r) in enumerate(zip(lens, rows))
+                                                                   for i in range(r)]
+    R = len(seen)
+    q = (torch.randn(max(R, 1), nh * hd + wide, generator=g) * 2).half().to(DEV)
+    out = torch.full((R + 2, nh * hd + wide), 3.0, dtype=torch.float16, device=DEV)
+    kw = {}
+    if rows is not None:
+        cu = [0]
+        for r in rows:
+            cu.append(cu[-1] + r)
+        kw = dict(cu_q=ints(cu), q_pos0=ints([n - r for n, r in zip(lens, rows)]), max_q=max(rows))
+        seen = [(s, n - r + i + 1) for s, (n, r) in enumerate(zip(lens, rows)) for i in range(r)]
+    call = lambda: ops.attn_decode_q8(q, QuantKV(data, scale), tables, ints(lens) if rows is None else None, out, len(lens), nh,
+                                      nkv, hd, scale_of(hd), num_splits=splits, window=window, **kw)
+    call()
+    torch.cuda.synchronize()
+    ops.check()
+    want, tol = attention(q, data, scale, tables, seen, nh, scale_of(hd), window)
+    got = out[:R, : nh * hd].double()
+    assert (out[R:] == 3).all() and (out[:, nh * hd:] == 3).all()
+    assert not got.isnan().any()
+    bad = (got - want).abs() - tol
+    assert (bad <= 0).all(), f"{float(bad.max())} over {float(tol.max())} at {tuple(int(i) for i in torch.nonzero(bad == bad.max())[0])}"
+    first = out.clone()
+    call()
+    assert torch.equal(first, out)                                         # the same call gives the same bits
+    return out
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("nh,nkv", [(1, 1), (8, 8), (7, 1), (40, 8), (16, 1), (24, 2)])
+@pytest.mark.parametrize("lens", [[1], [0, 1, 15, 16, 17, 33, 0, 300], [2100]])
+def test_attention_shapes(ops, hd, nh, nkv, lens):
+    attend(ops, lens, nh, nkv, hd)
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("bs", [16, 32, 48, 64])
+@pytest.mark.parametrize("window", [0, 1, 17, 100])
+def test_windows_and_holes(ops, hd, bs, window):
+    lens = [1, 18, 130, 400, 0, 77]
+    holes = [(s, j) for s, n in enumerate(lens) for j in range(0, -(-n // bs), 3)]        # the first block, and the only one
+    attend(ops, lens, 8, 2, hd, bs=bs, window=window, holes=holes, width=40)
+
+
+@pytest.mark.parametrize("splits", [0, 1, 2, 3, 5, 8, 16, 17, 40, 64])
+@pytest.mark.parametrize("lens", [[5], [700, 0, 31, 2000, 1]])
+def test_pieces(ops, splits, lens):
+    attend(ops, lens, 14, 2, 128, splits=splits)
+    attend(ops, lens, 4, 4, 64, splits=splits, window=333)
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("nh,nkv", [(8, 8), (7, 1), (40, 8), (16, 1)])
+@pytest.mark.parametrize("rows", [[5, 1, 3, 5], [2, 2, 2, 2], [1, 17, 4, 9]])
+@pytest.mark.parametrize("window", [0, 50])
+def test_rows_of_a_draft(ops, hd, nh, nkv, rows, window):
+    attend(ops, [400, 1, 77, 18], nh, nkv, hd, rows=[min(r, n) for r, n in zip(rows, [400, 1, 77, 18])], window=window,
+           holes=[(0, 3), (2, 0)])
+
+
+def test_many_sequences(ops):
+    attend(ops, [(37 * i) % 200 for i in range(300)], 8, 2, 64)
+    attend(ops, [1 + (53 * i) % 90 for i in range(130)], 8, 8, 128, rows=[1 + i % 2 if (53 * i) % 90 else 1 for i in range(130)])
+
+
+def test_long_sequence(ops):
+    attend(ops, [40001], 7, 1, 128)
+    attend(ops, [20011, 3], 8, 1, 128, rows=[4, 1])
+
+
+def test_scales_of_every_size(ops):
+    """Values of one token a thousand times those of the next, and values of 1e-6."""
+    def cache(g, blocks):
+        data, scale = make_cache(g, blocks, 2, 16, 128, DEV)
+        factor = torch.exp(torch.randn(blocks, 2, 16, generator=g) * 3.5).to(DEV)
+        scale[:, 1] *= factor
+        return data, scale
+
+    def small(g, blocks):
+        data, scale = make_cache(g, blocks, 2, 16, 128, DEV)
+        scale[:, 1] *= 1e-6
+        scale[:, 0] *= 3.0
+        return data, scale
+    attend(ops, [1000, 20], 8, 2, 128, cache=cache)
+    out = attend(ops, [600, 3], 8, 2, 128, cache=small)
+    assert out[:2, : 8 * 128].float().abs().max() > 0
+
+
+def test_nan_is_seen_and_not_hidden(ops):
+    nh, nkv, hd, bs = 4, 2, 64, 16
+    g = gen(11)
+    data, scale = make_cache(g, 4, nkv, bs, hd, DEV)
+    tables = ints([[0, 1], [2, 3]])
+    q = torch.randn(2, nh * hd, generator=g).half().to(DEV)
+    scale[0, 1, 0, 3] = float("nan")                                       # sequence 0, value of token 3, kv head 0
+    out = torch.zeros(2, nh * hd, dtype=torch.float16, device=DEV)
+    ops.attn_decode_q8(q, QuantKV(data, scale), tables, ints([20, 20]), out, 2, nh, nkv, hd, scale_of(hd))
+    nan = out.isnan().view(2, nkv, -1).all(-1).tolist()
+    assert nan == [[True, False], [False, False]] and not out[1].isnan().any() and not out[0, nh * hd // 2:].isnan().any()
+    scale[0, 1, 0, 3] = 0.01
+    scale[2, 0, 1, 19 % bs] = float("nan")                                 # a key
+    ops.attn_decode_q8(q, QuantKV(data, scale), tables, ints([20, 20]), out, 2, nh, nkv, hd, scale_of(hd))
+    assert out.isnan().view(2, nkv, -1).all(-1).tolist() == [[False, False], [False, True]]
+
+
+def test_cache_of_more_than_four_gigabytes(ops):
+    nkv, bs, hd = 8, 64, 128
+    blocks = 5 * 2 ** 30 // (2 * nkv * bs * hd)
+    data = torch.empty(blocks, 2, nkv, bs, hd, dtype=torch.uint8, device=DEV)
+    scale = torch.empty(blocks, 2, nkv, bs, device=DEV)
+    g = gen(2)
+    ids = [blocks - 1, 0, blocks - 2, blocks // 2]
+    small, small_scale = make_cache(g, 4, nkv, bs, hd, DEV)
+    data[ids], scale[ids] = small, small_scale
+    q = torch.randn(1, 8 * hd, generator=g).half().to(DEV)
+    out = torch.zeros(1, 8 * hd, dtype=torch.float16, device=DEV)
+    tables = ints([ids])
+    ops.attn_decode_q8(q, QuantKV(data, scale), tables, ints([4 * bs - 3]), out, 1, 8, nkv, hd, scale_of(hd))
+    want, tol = attention(q, data, scale, tables, [(0, 4 * bs - 3)], 8, scale_of(hd))
+    assert ((out.double() - want).abs() <= tol).all()
+    qkv = torch.randn(1, (8 + 2 * nkv) * hd, generator=g).half().to(DEV)
+    slot = blocks * bs - 2
+    ops.rope_kv_write_q8(qkv, QuantKV(data, scale), ints([4]), ints([slot], torch.int64), freqs_of(hd), 1, 8, nkv, hd)
+    pages, places = torch.zeros(4, 2, nkv, bs, hd, dtype=torch.float16, device=DEV), torch.zeros(1, 4, dtype=torch.int32, device=DEV)
+    ops.kv_read_q8(QuantKV(data, scale), tables, ints([4 * bs]), ints([0, 4]), 1, pages, places)
+    v = qkv[0, 16 * hd:].view(nkv, hd).double()
+    step = v.abs().amax(-1, keepdim=True) / 127
+    # half a step of the bytes, the fp16 of the page and 1e-3 of a step for fp32
+    assert ((pages[0, 1, :, bs - 2].double() - v).abs() <= step * 0.501 + v.abs() * 2.0 ** -10).all()
+
+
+# ---- what is reported -------------------------------------------------------------------------------------------------------
+def test_ids_outside_the_cache_are_reported_and_not_followed(ops):
+    from zse_b200.ops.native import DeviceStatusError
+    nh, nkv, hd, bs = 4, 2, 64, 16
+    data, scale = make_cache(gen(1), 3, nkv, bs, hd, DEV)
+    kv = QuantKV(data, scale)
+    q = torch.randn(1, nh * hd, generator=gen(2)).half().to(DEV)
+    out = torch.zeros(1, nh * hd, dtype=torch.float16, device=DEV)
+    ops.attn_decode_q8(q, kv, ints([[1, 3]]), ints([20]), out, 1, nh, nkv, hd, scale_of(hd))
+    with pytest.raises(DeviceStatusError):
+        ops.check()
+    want, tol = attention(q, data, scale, ints([[1, -1]]), [(0, 20)], nh, scale_of(hd))
+    assert ((out.double() - want).abs() <= tol).all()
+    ops.attn_decode_q8(q, kv, ints([[1, 2]]), ints([33]), out, 1, nh, nkv, hd, scale_of(hd))     # more tokens than the table holds
+    with pytest.raises(DeviceStatusError):
+        ops.check()
+    pages, places = torch.zeros(2, 2, nkv, bs, hd, dtype=torch.float16, device=DEV), torch.zeros(1, 2, dtype=torch.int32, device=DEV)
+    ops.kv_read_q8(kv, ints([[1, 7]]), ints([20]), ints([0, 2]), 1, pages, places)
+    with pytest.raises(DeviceStatusError):
+        ops.check()
+    assert places.tolist() == [[0, -1]] and (pages[1] == 0).all() and (pages[0] != 0).any()
+    ops.kv_read_q8(kv, ints([[1, 2]]), ints([20]), ints([0, 1]), 1, pages.zero_(), places)          # one page for two blocks
+    with pytest.raises(DeviceStatusError):
+        ops.check()
+    assert (pages == 0).all() and places.tolist() == [[-1, -1]]
+    x = torch.randn(2, (nh + 2 * nkv) * hd, generator=gen(4)).half().to(DEV)
+    before = data.clone()
+    ops.rope_kv_write_q8(x, kv, ints([0, 1]), ints([3 * bs, -5], torch.int64), freqs_of(hd), 2, nh, nkv, hd)
+    with pytest.raises(DeviceStatusError):
+        ops.check()
+    assert torch.equal(before, data)
+    ops.check()
+
+
+def test_refusals_of_the_library(ops):
+    from zse_b200.ops.native import NativeError
+    kv = QuantKV.zeros((2, 2, 2, 16, 80), DEV)                              # a head dimension without kernels
+    q = torch.zeros(1, 4 * 80, dtype=torch.float16, device=DEV)
+    with pytest.raises(NativeError, match="shape"):
+        ops.attn_decode_q8(q, kv, ints([[0]]), ints([1]), q.clone(), 1, 4, 2, 80, 0.1)
+    kv = QuantKV.zeros((2, 2, 2, 8, 64), DEV)                               # blocks of 8
+    q = torch.zeros(1, 4 * 64, dtype=torch.float16, device=DEV)
+    with pytest.raises(NativeError, match="shape"):
+        ops.attn_decode_q8(q, kv, ints([[0]]), ints([1]), q.clone(), 1, 4, 2, 64, 0.1)
+    kv = QuantKV.zeros((2, 2, 2, 16, 64), DEV)
+    x = torch.zeros(1, 8 * 64 + 1, dtype=torch.float16, device=DEV)
+    with pytest.raises(NativeError, match="aligned|stride"):
+        ops.rope_kv_write_q8(x[:, 1:], kv, ints([0]), ints([0], torch.int64), freqs_of(64), 1, 4, 2, 64)
+    with pytest.raises(NativeError, match="contiguous"):
+        ops.attn_decode_q8(q, QuantKV(torch.zeros(4, 2, 2, 16, 64, dtype=torch.uint8, device=DEV)[::2],
+                                      torch.zeros(4, 2, 2, 16, device=DEV)[::2]), ints([[0]]), ints([1]), q.clone(), 1, 4, 2, 64, 0.1)
+
+
+# ---- together ---------------------------------------------------------------------------------------------------------------
+def _step_inputs(g, lens, nh, nkv, hd, bs):
+    blocks = sum(n // bs + 1 for n in lens) + 1
+    data, scale = make_cache(g, blocks, nkv, bs, hd, DEV)
+    tables = make_tables(g, [n + 1 for n in lens], bs, blocks, DEV)
+    slots = ints([int(tables[s, n // bs]) * bs + n % bs for s, n in enumerate(lens)], torch.int64)
+    qkv = torch.randn(len(lens), (nh + 2 * nkv) * hd, generator=g).half().to(DEV)
+    return QuantKV(data, scale), tables, slots, qkv, ints(lens), ints([n + 1 for n in lens])
+
+
+def _step(ops, kv, tables, slots, qkv, pos, lens, nh, nkv, hd, q, out):
+    S = qkv.shape[0]
+    ops.rope_kv_write_q8(qkv, kv, pos, slots, freqs_of_cached(hd), S, nh, nkv, hd, q_out=q)
+    ops.attn_decode_q8(q, kv, tables, lens, out, S, nh, nkv, hd, scale_of(hd))
+
+
+_FREQS = {}
+
+
+def freqs_of_cached(hd):
+    if hd not in _FREQS:
+        _FREQS[hd] = freqs_of(hd)
+    return _FREQS[hd]
+
+
+@pytest.mark.parametrize("hd,nh,nkv", [(64, 8, 2), (128, 14, 2)])
+def test_decode_step_then_prefill_read(ops, hd, nh, nkv):
+    """A step writes and attends; then the same cache, read back, goes through the framework's prefill attention."""
+    lens, bs, S = [31, 0, 200, 16], 16, 4
+    kv, tables, slots, qkv, pos, now = _step_inputs(gen(hd), lens, nh, nkv, hd, bs)
+    q = torch.zeros(S, nh * hd, dtype=torch.float16, device=DEV)
+    out = torch.zeros(S, nh * hd, dtype=torch.float16, device=DEV)
+    _step(ops, kv, tables, slots, qkv, pos, now, nh, nkv, hd, q, out)
+    want, tol = attention(q, kv.data, kv.scale, tables, [(s, n + 1) for s, n in enumerate(lens)], nh, scale_of(hd))
+    assert ((out.double() - want).abs() <= tol).all()
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n // bs + 1)
+    pages = torch.zeros(cu[-1], 2, nkv, bs, hd, dtype=torch.float16, device=DEV)
+    places = torch.zeros(S, tables.shape[1], dtype=torch.int32, device=DEV)
+    ops.kv_read_q8(kv, tables, now, ints(cu), S, pages, places)
+    again = torch.zeros(S, nh * hd, dtype=torch.float16, device=DEV)
+    ops.attn_prefill(q, pages, places, ints(list(range(S + 1))), pos, again, S, S, 1, nh, nkv, hd, bs, scale_of(hd))
+    torch.cuda.synchronize()
+    ops.check()
+    # the pages are rounded to fp16 once more: 2^-11 of every key and value; a key's share in the exponent is |q.k| * scale * 2^-11
+    most = (q.double().view(S, nkv, nh // nkv, hd).abs().sum(-1).amax((1, 2))[:, None]
+            * (kv.scale[:, 0].nan_to_num(0).double().max() * 127) * scale_of(hd) * 2.0 ** -11)
+    size = (kv.scale[:, 1].double().max() * 127)
+    assert ((again.double() - want).abs() <= 2 * tol + (2 * most + 2.0 ** -10) * size).all()
+
+
+def test_graph_of_a_step(ops):
+    """Captured, replayed with other lengths and tables in place, and beside a second graph on another stream."""
+    nh, nkv, hd, bs = 14, 2, 128, 16
+    made = []
+    for seed, lens in ((1, [40, 300, 7]), (2, [900, 1, 64])):
+        kv, tables, slots, qkv, pos, now = _step_inputs(gen(seed), lens, nh, nkv, hd, bs)
+        wide = torch.full((3, 70), -1, dtype=torch.int32, device=DEV)
+        wide[:, : tables.shape[1]] = tables
+        q, out = (torch.zeros(3, nh * hd, dtype=torch.float16, device=DEV) for _ in range(2))
+        args = (ops, kv, wide, slots, qkv, pos, now, nh, nkv, hd, q, out)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _step(*args)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            _step(*args)
+        made.append((graph, side, kv, wide, now, q, out, args))      # a graph's tensors live as long as it does
+    for _ in range(3):
+        for m in made:
+            m[6].zero_()
+        torch.cuda.synchronize()
+        for graph, side, *_ in made:
+            with torch.cuda.stream(side):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, _, kv, wide, now, q, out, _ in made:
+            want, tol = attention(q, kv.data, kv.scale, wide, [(s, int(n)) for s, n in enumerate(now)], nh, scale_of(hd))
+            assert ((out.double() - want).abs() <= tol).all()
+            now.sub_(1)                                                    # shorter sequences for the next replay
+            now.clamp_(min=0)
+    ops.check()

@@ -133,6 +133,99 @@ class TorchOps:
                                                     cu_q[: num_seqs + 1], q_pos0[:num_seqs], nh, nkv, hd, block_size,
                                                     scale, softcap, window)
 
+    # ---- 8-bit KV cache (cache.quant_kv.QuantKV, one layer) ----------------------------------------------
+    @staticmethod
+    def _check_q8(kv, nh: int, nkv: int, hd: int, **tensors) -> None:
+        """``tensors``: name = (tensor or None, dtype, least number of dimensions)."""
+        if kv.data.dim() != 5 or (kv.kv_heads, kv.head_dim) != (nkv, hd):
+            raise ValueError(f"{nkv} kv heads of {hd} do not match one layer of a cache of shape {tuple(kv.shape)}")
+        if nkv < 1 or nh < 1 or nh % nkv:
+            raise ValueError(f"{nh} heads over {nkv} kv heads")
+        dev = kv.data.device
+        for name, (t, dtype, dims) in tensors.items():
+            if t is None:
+                continue
+            if t.dtype != dtype or t.dim() < dims or (t.numel() and t.stride(-1) != 1):
+                raise ValueError(f"{name}: {dtype} with {dims} dimensions and packed rows expected, not {t.dtype} "
+                                 f"{tuple(t.shape)} with strides {t.stride()}")
+            if t.device != dev:
+                raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
+
+    def _check_write_q8(self, qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out, planes, n_planes, bias):
+        cols = (nh + 2 * nkv) * hd
+        self._check_q8(kv, nh, nkv, hd, qkv=(qkv, torch.float16, 2), q_out=(q_out, torch.float16, 2),
+                       planes=(planes, torch.float32, 1), bias=(bias, torch.float16, 1), positions=(positions, torch.int32, 1),
+                       slots=(slots, torch.int64, 1), inv_freq=(inv_freq, torch.float32, 1))
+        if M < 0 or positions.shape[0] < M or slots.shape[0] < M or q_out.shape[0] < M or q_out.shape[1] < nh * hd:
+            raise ValueError(f"{M} rows do not fit positions, slots or q_out {tuple(q_out.shape)}")
+        if planes is None:
+            if qkv is None or qkv.shape[0] < M or qkv.shape[1] < cols:
+                raise ValueError(f"{M} rows of {cols} columns expected in qkv")
+            if bias is not None:
+                raise ValueError("a bias goes with planes")
+        elif n_planes < 1 or planes.numel() < n_planes * M * cols or not planes.is_contiguous():
+            raise ValueError(f"{n_planes} planes of {M} rows of {cols} columns expected")
+        if bias is not None and bias.numel() < cols:
+            raise ValueError(f"a bias of {cols} columns expected")
+        if 2 * inv_freq.numel() > hd or inv_freq.numel() % 8:
+            raise ValueError(f"{2 * inv_freq.numel()} rotated dimensions of {hd}: a multiple of 16 expected")
+
+    def rope_kv_write_q8(self, qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out=None, planes=None, n_planes=0,
+                         bias=None):
+        """Rotates q and k of M rows, writes k and v into the 8-bit cache at ``slots`` (each slot once; -1: not stored) and the
+        rotated q to the first columns of ``q_out`` (None: ``qkv`` itself).  The rows are those of ``qkv`` [M, q | k | v], or the sum
+        of ``planes`` [n_planes, M, q | k | v] and ``bias``.  k and v columns stay as they are."""
+        q_out = qkv if q_out is None else q_out
+        self._check_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out, planes, n_planes, bias)
+        if M == 0:
+            return
+        cols = (nh + 2 * nkv) * hd
+        if planes is None:
+            x = qkv[:M, :cols]
+        else:
+            x = planes.view(-1)[: n_planes * M * cols].view(n_planes, M, cols).sum(0)
+            if bias is not None:
+                x = x + bias[:cols].float()
+        q_out[:M, : nh * hd] = ref.rope_kv_write_q8(x, kv, positions[:M], slots[:M], inv_freq, nh)
+
+    def _check_read_q8(self, kv, block_tables, seq_lens, cu_blocks, S, out, out_tables):
+        self._check_q8(kv, kv.kv_heads, kv.kv_heads, kv.head_dim, block_tables=(block_tables, torch.int32, 2),
+                       seq_lens=(seq_lens, torch.int32, 1), cu_blocks=(cu_blocks, torch.int32, 1), out=(out, torch.float16, 5),
+                       out_tables=(out_tables, torch.int32, 2))
+        if S < 0 or min(block_tables.shape[0], seq_lens.shape[0], cu_blocks.shape[0] - 1, out_tables.shape[0]) < S:
+            raise ValueError(f"tables, lengths and places of {S} sequences expected")
+        if out.shape[1:] != kv.shape[1:] or not out.is_contiguous():
+            raise ValueError(f"pages of {tuple(kv.shape[1:])} expected, not {tuple(out.shape)}")
+
+    def kv_read_q8(self, kv, block_tables, seq_lens, cu_blocks, S, out, out_tables):
+        """Reads the first ``seq_lens[s]`` tokens of S sequences back as fp16 pages: block j of sequence s goes to
+        ``out[cu_blocks[s] + j]``, its place there to ``out_tables[s, j]`` (-1: a hole, or behind the sequence; such a page of
+        ``out`` stays as it was).  ``out`` and ``out_tables`` are what ``attn_prefill`` takes for a cache and its tables."""
+        self._check_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables)
+        ref.kv_read_q8(kv, block_tables[:S], seq_lens[:S], cu_blocks[: S + 1], out, out_tables)
+
+    def _check_attn_q8(self, q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q):
+        self._check_q8(kv, nh, nkv, hd, q=(q, torch.float16, 2), out=(out, torch.float16, 2),
+                       block_tables=(block_tables, torch.int32, 2), seq_lens=(seq_lens, torch.int32, 1),
+                       cu_q=(cu_q, torch.int32, 1), q_pos0=(q_pos0, torch.int32, 1))
+        if nh // nkv > 16:
+            raise ValueError(f"{nh // nkv} query heads per kv head: up to 16 expected")
+        if S < 0 or block_tables.shape[0] < S or q.shape[1] < nh * hd or out.shape[1] < nh * hd or window < 0:
+            raise ValueError(f"{S} sequences of {nh} heads of {hd} do not fit the tables, q {tuple(q.shape)} or out {tuple(out.shape)}")
+        if cu_q is None:
+            if max_q != 1 or seq_lens is None or seq_lens.shape[0] < S or min(q.shape[0], out.shape[0]) < S:
+                raise ValueError(f"lengths and a row each of {S} sequences expected")
+        elif q_pos0 is None or cu_q.shape[0] < S + 1 or q_pos0.shape[0] < S or not 1 <= max_q <= 64:
+            raise ValueError(f"first rows and positions of {S} sequences and up to 64 rows of each expected")
+
+    def attn_decode_q8(self, q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, scale, scratch=None, num_splits=0, window=0,
+                       cu_q=None, q_pos0=None, max_q=1):
+        """Attention of new tokens over an 8-bit cache.  One row per sequence (row s sees the first ``seq_lens[s]`` tokens), or,
+        with ``cu_q``, rows ``cu_q[s] .. cu_q[s + 1] - 1`` of sequence s (at most ``max_q``), the first of them at position
+        ``q_pos0[s]``, each of which sees the tokens up to its own.  ``window`` > 0: only the last so many of them."""
+        self._check_attn_q8(q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q)
+        ref.attn_decode_q8(q, kv, block_tables, seq_lens, out, S, nh, scale, window, cu_q, q_pos0)
+
     # ---- latent attention and routed feed-forward -----------------------------------------------------
     # (activations and cache at the model's own width: bfloat16 or fp32)
     def dense(self, t: torch.Tensor, dtype) -> torch.Tensor:
@@ -1182,6 +1275,22 @@ class CudaOps(TorchOps):
             return
         self.n.attn_prefill_ext(qkv, qkv.stride(0), kv_layer, block_tables, cu_q, q_pos0, out, out.stride(0),
                                 num_seqs, max_q_len, nh, nkv, hd, block_size, scale, softcap, window)
+
+    def rope_kv_write_q8(self, qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out=None, planes=None, n_planes=0,
+                         bias=None):
+        q_out = qkv if q_out is None else q_out
+        self._check_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out, planes, n_planes, bias)
+        self.n.rope_kv_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, q_out, planes, n_planes, bias, self.status.ptr)
+
+    def kv_read_q8(self, kv, block_tables, seq_lens, cu_blocks, S, out, out_tables):
+        self._check_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables)
+        self.n.kv_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables, self.status.ptr)
+
+    def attn_decode_q8(self, q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, scale, scratch=None, num_splits=0, window=0,
+                       cu_q=None, q_pos0=None, max_q=1):
+        self._check_attn_q8(q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q)
+        self.n.attn_decode_q8(q, kv, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch, num_splits, scale, window,
+                              self.status.ptr)
 
     def headnorm_rope_kv_write(self, qkv, kv_layer, positions, slots, freqs, q_norm_w, k_norm_w, norm_v, k_is_v, eps,
                                M, nh, nkv, hd, block_size):

@@ -109,12 +109,24 @@ class Space(Structure):
                 ("state_ld", c_int32)] + [(n, c_void_p) for n in ("conv_w", "conv_b", "dt_bias", "neg_a", "skip")]
 
 
+class KvQ8(Structure):
+    _fields_ = [("data", c_void_p), ("scale", c_void_p)] + [(n, c_int32) for n in ("num_blocks", "nkv", "block_size", "hd")]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 _SIGS = {
     "zse_gemm_w4": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                             c_void_p, c_void_p]),
     "zse_gemm_w4_splits": (c_int, [c_int, c_int, c_int, c_int]),
+    "zse_rope_kv_write_q8": (c_int, [POINTER(KvQ8), c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                                     c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "zse_kv_read_q8": (c_int, [POINTER(KvQ8), c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int,
+                               c_void_p, c_void_p]),
+    "zse_attn_decode_q8_splits": (c_int, [c_int] * 9),
+    "zse_attn_decode_q8_scratch_floats": (c_int64, [c_int] * 5),
+    "zse_attn_decode_q8": (c_int, [POINTER(KvQ8), c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                   c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_float, c_int, c_void_p, c_void_p]),
     "zse_gemm_w8": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                             c_void_p, c_void_p]),
     "zse_gemm_w8_splits": (c_int, [c_int, c_int, c_int, c_int]),
@@ -511,6 +523,53 @@ def rope_kv_write(qkv, kv_layer, positions, slots, inv_freq, M, nh, nkv, hd, rot
                   n_planes=0, bias=None):
     _ck(load().zse_rope_kv_write(_p(qkv), _p(kv_layer), _p(positions), _p(slots), _p(inv_freq), M, nh, nkv, hd,
                                  rotary_dim, block_size, _p(planes), n_planes, _p(bias), _stream()), "rope_kv_write")
+
+
+def kv_q8(kv) -> KvQ8:
+    """One layer of an 8-bit cache (``cache.quant_kv.QuantKV``) as the kernels take it."""
+    if not (kv.data.is_contiguous() and kv.scale.is_contiguous()):
+        raise NativeError("a layer of an 8-bit cache has to be contiguous")
+    if kv.data.device.type != "cuda":
+        raise NativeError(f"the cache is on {kv.data.device}")
+    return KvQ8(_p(kv.data), _p(kv.scale), kv.num_blocks, kv.kv_heads, kv.block_size, kv.head_dim)
+
+
+def _on_current_device(kv) -> None:
+    if kv.data.device.index != torch.cuda.current_device():
+        raise NativeError(f"the cache is on {kv.data.device}, the current device is {torch.cuda.current_device()}")
+
+
+def rope_kv_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, q_out, planes, n_planes, bias, status):
+    _on_current_device(kv)
+    _ck(load().zse_rope_kv_write_q8(byref(kv.native()), _p(qkv), 0 if qkv is None else qkv.stride(0), _p(q_out), q_out.stride(0),
+                                    _p(planes), n_planes, _p(bias), _p(positions), _p(slots), _p(inv_freq), M, nh,
+                                    inv_freq.numel() * 2, status, _stream()), "rope_kv_write_q8")
+
+
+def kv_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables, status):
+    _on_current_device(kv)
+    _ck(load().zse_kv_read_q8(byref(kv.native()), _p(block_tables), block_tables.stride(0), _p(seq_lens), _p(cu_blocks), S,
+                              _p(out), out.shape[0], _p(out_tables), out_tables.stride(0), status, _stream()), "kv_read_q8")
+
+
+def attn_decode_q8_scratch_floats(S, max_q, nh, nkv, hd, block_size, max_blocks, window=0, num_splits=0) -> int:
+    """fp32 values of scratch that ``attn_decode_q8`` needs for such a call (0: none)."""
+    lib = load()
+    return lib.zse_attn_decode_q8_scratch_floats(
+        S, max_q, nh, hd, lib.zse_attn_decode_q8_splits(S, max_q, nh, nkv, hd, block_size, max_blocks, window, num_splits))
+
+
+def attn_decode_q8(q, kv, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch, num_splits, scale, window, status):
+    """``scratch``: fp32, ``attn_decode_q8_scratch_floats`` of it, or None (then the call allocates what it needs)."""
+    _on_current_device(kv)
+    if scratch is None:
+        n = attn_decode_q8_scratch_floats(S, max_q, nh, kv.kv_heads, kv.head_dim, kv.block_size, block_tables.stride(0), window,
+                                          num_splits)
+        scratch = torch.empty(n, dtype=torch.float32, device=kv.device) if n else None
+    _ck(load().zse_attn_decode_q8(byref(kv.native()), _p(q), q.stride(0), _p(block_tables), block_tables.stride(0), _p(seq_lens),
+                                  _p(cu_q), _p(q_pos0), S, max_q, _p(out), out.stride(0), nh, _p(scratch),
+                                  0 if scratch is None else scratch.numel(), num_splits, float(scale), int(window), status,
+                                  _stream()), "attn_decode_q8")
 
 
 def headnorm_rope_kv_write(qkv, kv_layer, positions, slots, freqs, q_norm_w, k_norm_w, norm_v, k_is_v, eps, M, nh, nkv,

@@ -210,6 +210,85 @@ def attn_prefill(q: torch.Tensor, kv_layer: torch.Tensor, block_tables: torch.Te
     return out
 
 
+def rope_kv_write_q8(x: torch.Tensor, kv, positions: torch.Tensor, slots: torch.Tensor, freqs: torch.Tensor, nh: int) -> torch.Tensor:
+    """Rows x [M, (nh + 2 nkv) * hd] in fp32: q and k are rotated (pairs (i, i + rot/2) of the first rot = 2 * len(freqs)
+    dimensions, angles in 64 bits), k and v quantised into ``kv`` (``cache.quant_kv.QuantKV``) at ``slots`` (-1: not stored).
+    Returns the rotated q [M, nh * hd] in fp16.  A row's scale is max|x| / 127 (rows of nothing above 1e-30 are stored as zeros, a
+    NaN makes the scale NaN), infinities count as the largest fp16 number."""
+    M, hd, nkv, bs, half = x.shape[0], kv.head_dim, kv.kv_heads, kv.block_size, freqs.numel()
+    h = x.float().view(M, nh + 2 * nkv, hd)
+    ang = positions.double()[:, None, None] * freqs.to(x.device).double()
+    c, s = torch.cos(ang).float(), torch.sin(ang).float()
+    a, b = h[:, : nh + nkv, :half], h[:, : nh + nkv, half: 2 * half]
+    h = torch.cat([torch.cat([a * c - b * s, b * c + a * s, h[:, : nh + nkv, 2 * half:]], -1), h[:, nh + nkv:]], 1)
+    h = h.clamp(-65504, 65504)
+    ok = slots >= 0
+    if bool(ok.any()):
+        if int(slots.max()) >= kv.num_blocks * bs:
+            raise ValueError(f"slot {int(slots.max())} of a cache of {kv.num_blocks * bs} tokens")
+        y = h[ok, nh:].view(-1, 2, nkv, hd)
+        top = y.abs().amax(-1)
+        none = top <= 1e-30
+        u = torch.round(y * torch.where(none, torch.zeros_like(top), 127.0 / top)[..., None])
+        blk, off = slots[ok] // bs, slots[ok] % bs
+        kv.data[blk, :, :, off] = (u.nan_to_num(0.0) + 128).to(torch.uint8)
+        kv.scale[blk, :, :, off] = torch.where(none, torch.zeros_like(top), top / 127.0)
+    return h[:, :nh].reshape(M, nh * hd).to(torch.float16)
+
+
+def kv_read_q8(kv, block_tables: torch.Tensor, seq_lens: torch.Tensor, cu_blocks: torch.Tensor, out: torch.Tensor,
+               out_tables: torch.Tensor) -> None:
+    """Pages of whole sequences as fp16: block j of sequence s goes to ``out[cu_blocks[s] + j]`` [2, nkv, bs, hd] with zeros behind
+    the sequence's last token, and its place to ``out_tables[s, j]``; holes and what lies behind the last block are -1 there, and
+    ``out`` keeps what it had."""
+    bs = kv.block_size
+    out_tables[: seq_lens.numel()] = -1
+    for s in range(seq_lens.numel()):
+        n = int(seq_lens[s])
+        first, blocks = int(cu_blocks[s]), (n + bs - 1) // bs
+        if n < 0 or blocks > min(block_tables.shape[1], out_tables.shape[1], int(cu_blocks[s + 1]) - first) or first < 0 \
+                or first + blocks > out.shape[0]:
+            raise ValueError(f"sequence {s}: {n} tokens do not fit its tables or its pages {first} .. {int(cu_blocks[s + 1])}")
+        ids = block_tables[s, :blocks].long()
+        if blocks and int(ids.max()) >= kv.num_blocks:
+            raise ValueError(f"block {int(ids.max())} of a cache of {kv.num_blocks}")
+        j = torch.nonzero(ids >= 0)[:, 0]
+        x = (kv.data[ids[j]].float() - 128) * kv.scale[ids[j]][..., None]
+        live = (j[:, None] * bs + torch.arange(bs, device=j.device)) < n
+        out[first + j] = torch.where(live[:, None, None, :, None], x, torch.zeros_like(x)).to(out.dtype)
+        out_tables[s, j] = (first + j).to(out_tables.dtype)
+
+
+def attn_decode_q8(q: torch.Tensor, kv, block_tables: torch.Tensor, seq_lens, out: torch.Tensor, S: int, nh: int, scale: float,
+                   window: int = 0, cu_q=None, q_pos0=None) -> None:
+    """One row per sequence (row s sees the first ``seq_lens[s]`` tokens), or rows ``cu_q[s] .. cu_q[s + 1]`` of sequence s, the
+    first of them at position ``q_pos0[s]``, each of which sees the tokens up to its own; ``window`` > 0: the last so many of
+    them.  A row that sees nothing gives zeros."""
+    nkv, hd, bs = kv.kv_heads, kv.head_dim, kv.block_size
+    for s in range(S):
+        a, e = (s, s + 1) if cu_q is None else (int(cu_q[s]), int(cu_q[s + 1]))
+        n = int(seq_lens[s]) if cu_q is None else int(q_pos0[s]) + e - a
+        if e <= a:
+            continue
+        if n < 0 or -(-n // bs) > block_tables.shape[1]:
+            raise ValueError(f"sequence {s}: {n} tokens, a table of {block_tables.shape[1]} blocks of {bs}")
+        ids = block_tables[s, : -(-n // bs)].long()
+        if n and int(ids.max()) >= kv.num_blocks:
+            raise ValueError(f"block {int(ids.max())} of a cache of {kv.num_blocks}")
+        at = torch.arange(n, device=q.device)
+        blk, off = ids.clamp_min(0)[at // bs], at % bs
+        pos = torch.arange(n - (e - a), n, device=q.device)[:, None]
+        seen = (at <= pos) & (ids >= 0)[at // bs]
+        if window > 0:
+            seen &= at > pos - window
+        # the scales join scores and weights, so a token that a row does not see takes no part in it, whatever its scale
+        z = torch.einsum("rhgd,thd->hgrt", q[a:e, : nh * hd].float().view(e - a, nkv, nh // nkv, hd),
+                         kv.data[blk, 0, :, off].float() - 128) * kv.scale[blk, 0, :, off].T[:, None, None] * scale
+        p = torch.softmax(z.masked_fill(~seen, float("-inf")), -1) * kv.scale[blk, 1, :, off].T[:, None, None]
+        y = torch.einsum("hgrt,thd->rhgd", p.masked_fill(~seen, 0.0), kv.data[blk, 1, :, off].float() - 128)
+        out[a:e, : nh * hd] = y.reshape(e - a, nh * hd).to(out.dtype)
+
+
 def apply_repetition_penalty(logits: torch.Tensor, counts: dict, penalty: float) -> torch.Tensor:
     """``counts``: token -> occurrences.  positive logits are divided, negative multiplied by
     ``penalty^(1+log2(count))`` (zse-engine/zse_engine/orchestrator/sampler.py:64-80)."""
