@@ -428,19 +428,20 @@ int zse_rope_kv_write_q8(const ZseKvQ8* kv, const void* qkv, int ld, void* q_out
                          const void* bias, const void* positions_i32, const void* slots_i64, const void* inv_freq_f32, int M,
                          int nh, int rotary_dim, void* status, void* stream);
 // Pages of whole sequences as fp16: block j of sequence s -> out[cu_blocks[s] + j] (zeros behind seq_lens[s]), its place to
-// out_tables[s][j] (-1: hole, or behind the sequence).  out: out_blocks pages [2][nkv][block_size][hd].
-int zse_kv_read_q8(const ZseKvQ8* kv, const void* tables_i32, int max_blocks, const void* seq_lens_i32,
-                   const void* cu_blocks_i32, int num_seqs, void* out_f16, int out_blocks, void* out_tables_i32, int out_max_blocks,
-                   void* status, void* stream);
+// out_tables[s][j] (-1: hole, or behind the sequence).  out: out_blocks pages [2][nkv][block_size][hd].  Tables: rows of max_blocks,
+// table_ld apart.
+int zse_kv_read_q8(const ZseKvQ8* kv, const void* tables_i32, int table_ld, int max_blocks, const void* seq_lens_i32,
+                   const void* cu_blocks_i32, int num_seqs, void* out_f16, int out_blocks, void* out_tables_i32, int out_table_ld,
+                   int out_max_blocks, void* status, void* stream);
 // ---- attention_q8.cu ----------------------------------------------------------------------------------------------
 // One row per sequence (cu_q null: row s sees seq_lens[s] tokens) or rows cu_q[s] .. cu_q[s + 1] - 1 of sequence s (at most
 // max_q), the first at position q_pos0[s], each seeing the tokens up to its own; window > 0: the last so many of them.
-// num_splits: pieces of a (sequence, kv head); 0: the launcher decides.  More than zse_attn_decode_q8_most_whole() pieces need
-// scratch of zse_attn_decode_q8_scratch_floats.
-int zse_attn_decode_q8_splits(int num_seqs, int max_q, int nh, int nkv, int hd, int block_size, int max_blocks, int window,
-                              int num_splits);
-int64_t zse_attn_decode_q8_scratch_floats(int num_seqs, int max_q, int nh, int hd, int splits);
-int zse_attn_decode_q8(const ZseKvQ8* kv, const void* q_f16, int ldq, const void* tables_i32, int max_blocks,
+// num_splits: pieces of a (sequence, kv head, rows that share the products), rounded up to a power of two or a multiple of 16;
+// 0: the launcher decides.  Above 16 pieces scratch is needed (zse_attn_decode_q8_scratch_floats, 0: none).  q_rows: rows of q and out.
+int zse_attn_decode_q8_pieces(int num_seqs, int max_q, int nh, int nkv, int block_size, int max_blocks, int window, int num_splits);
+int64_t zse_attn_decode_q8_scratch_floats(int num_seqs, int max_q, int nh, int nkv, int hd, int block_size, int max_blocks,
+                                          int window, int num_splits);
+int zse_attn_decode_q8(const ZseKvQ8* kv, const void* q_f16, int ldq, int q_rows, const void* tables_i32, int table_ld, int max_blocks,
                        const void* seq_lens_i32, const void* cu_q_i32, const void* q_pos0_i32, int num_seqs, int max_q,
                        void* out_f16, int ldo, int nh, void* scratch_f32, int64_t scratch_floats, int num_splits, float scale,
                        int window, void* status, void* stream);

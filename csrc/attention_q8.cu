@@ -1,71 +1,543 @@
 // Attention of new tokens (one, or a few, of every sequence) over the 8-bit KV cache.
+//
+//   s[t][c] = scale * kscale[t] * (sum_d q[c][d] (uk[t][d] - 128)),   o[c][d] = sum_t p[t][c] vscale[t] (uv[t][d] - 128) / sum_t p[t][c]
+//
+// An item is one kv head of one sequence with up to 8 * NB columns c: query heads of the group, times rows of a draft.  Its tokens are
+// cut into pieces, one per CTA; four warps of a CTA take every fourth tile of 16 tokens through rings of their own (cp.async) and
+// keep a running maximum, sum and output in registers.  Tokens are the 16 rows of the products, columns their 8 columns.
+//
+// The pieces of an item are a thread-block cluster: its CTAs put what they have into shared memory and every CTA adds up a share
+// of the result from all of them.  No scratch, no second kernel, nothing that two calls could share.  Only where a cluster of 16
+// per item leaves most of the GPU idle (few sequences of few kv heads) are there several clusters per item, which meet in scratch.
+//
+// Bytes become fp16 numbers by byte permutations alone.  Keys: a byte in the low half of an fp16 number is u * 2^-24 (subnormal numbers
+// are exact in the products), so a product sum is 2^-24 (q . (uk - 128)) + 2^-17 sum(q), and the second term is taken off in fp32
+// per tile: half an instruction per element.  Values: 0x64 above the byte makes 1024 + u, and a packed subtraction of 1152 the
+// exact u - 128; with the subnormal form the weights' sum times 128 would cancel against a result that can be a thousand times smaller.
+// Values come as pairs of dimensions of one token out of ldmatrix.trans, so the two rows of a thread are neighbouring dimensions.
+#include <algorithm>
+
 #include "api.h"
 #include "common.cuh"
+#include "typed.cuh"
 
 namespace zse {
 
 namespace {
 
+constexpr int kWarps = 4;
+constexpr int kStages = 3;
+constexpr int kMostCluster = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// The plain form: a CTA has one row of one head, a thread one token of a tile of 128.
+struct Q8Args {
+  const uint8_t* data;
+  const float* scale;
+  const __half* q;
+  const int *tables, *seq_lens, *cu_q, *q_pos0;
+  __half* out;
+  float* scratch;
+  Status* st;
+  int ldq, ldo, q_rows, num_blocks, nkv, block_size, table_ld, max_blocks, nh, max_q, rows_per, row_groups, window, pieces, cluster;
+  float scale_log2;
+};
+
+__device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t turn_8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t minus_1152(uint32_t x) {           // both halves
+  uint32_t y;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x64806480u));
+  return y;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t smem_addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 load_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float load_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Where 16-byte chunk c of a tile's row lies: any eight rows of one chunk are in eight different groups of four banks.
 template <int HD>
-__global__ void __launch_bounds__(128)
-attn_q8_kernel(const uint8_t* __restrict__ data, const float* __restrict__ scale, int num_blocks, int nkv, int block_size,
-               const __half* __restrict__ q, int ldq, const int* __restrict__ tables, int max_blocks,
-               const int* __restrict__ seq_lens, const int* __restrict__ cu_q, const int* __restrict__ q_pos0,
-               __half* __restrict__ out, int ldo, int nh, float scale_log2, int window, Status* st) {
+__device__ __forceinline__ int place(int row, int c) {
+  if constexpr (HD == 64) return row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
+  if constexpr (HD == 96) return row * 96 + ((c ^ ((row >> 2) & 1)) << 4);
+  return row * HD + ((c ^ (row & 7)) << 4);
+}
+
+template <int HD, int NB>
+struct Q8Smem {
+  static constexpr int kTile = 16 * HD;                                // K or V of 16 tokens
+  static constexpr int kSlot = 2 * kTile + 128;                        // K, V, their scales
+  static constexpr int kRing = kStages * kSlot;                        // of a warp; its output at the end
+  static constexpr int kCols = 8 * NB;
+  static constexpr int kPitch = HD + 4;                                // floats of a column of output
+  static constexpr int kTotal = kWarps * kRing + (kWarps + 1) * 2 * kCols * 4;
+  static_assert(kCols * kPitch * 4 <= kRing, "a warp's output fits its ring");
+};
+
+template <int HD, int NB>
+__global__ void __launch_bounds__(kWarps * 32)
+attn_q8_kernel(const Q8Args a) {
+  using S = Q8Smem<HD, NB>;
+  constexpr int kChunks = HD / 16;                                     // 16-byte chunks of a row, and 16-wide steps of the products
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* own_m = reinterpret_cast<float*>(smem + kWarps * S::kRing);   // [warp][column], then the CTA's
+  float* own_l = own_m + (kWarps + 1) * S::kCols;
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float qs[HD], ps[128], red[128];
-  const int head = blockIdx.x, s = blockIdx.z, tid = threadIdx.x, kvh = head / (nh / nkv);
-  const int row = cu_q != nullptr ? cu_q[s] + blockIdx.y : s;
-  if (cu_q != nullptr && row >= cu_q[s + 1]) return;
-  int len = cu_q != nullptr ? q_pos0[s] + int(blockIdx.y) + 1 : seq_lens[s];
-  if (len < 0 || (len + block_size - 1) / block_size > max_blocks) {
-    if (tid == 0) report(st, kBadArgument, 75, unsigned(s));
-    len = max(0, min(len, max_blocks * block_size));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t2 = (lane & 3) * 2;
+  const int piece = blockIdx.x % a.pieces, item = blockIdx.x / a.pieces;
+  const int rg = item % a.row_groups, kvh = (item / a.row_groups) % a.nkv, s = item / a.row_groups / a.nkv;
+  const int G = a.nh / a.nkv, bpt = a.block_size >> 4, cap = a.max_blocks * a.block_size;
+
+  // rows of this item, and how many tokens its first row sees (each further row sees one more)
+  int row0 = s, rows = 1, base_len;
+  if (a.cu_q != nullptr) {
+    const int first = a.cu_q[s], count = a.cu_q[s + 1] - first;
+    row0 = first + rg * a.rows_per;
+    rows = min(a.rows_per, count - rg * a.rows_per);
+    base_len = a.q_pos0[s] + rg * a.rows_per + 1;
+    if (count > 0 && (first < 0 || count > a.max_q || first + count > a.q_rows)) {
+      if (tid == 0 && rg == 0 && kvh == 0 && piece == 0) report(a.st, kBadArgument, 73, unsigned(s));
+      rows = 0;
+    }
+  } else {
+    base_len = a.seq_lens[s];
   }
-  for (int d = tid; d < HD; d += 128) qs[d] = __half2float(q[size_t(row) * ldq + size_t(head) * HD + d]);
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, acc[(HD + 127) / 128] = {};
-  for (int t0 = window > 0 ? max(0, len - window) : 0; t0 < len; t0 += 128) {
-    const int t = t0 + tid;
-    float z = -INFINITY, vs = 0.f;
-    if (t < len) {
-      const int blk = tables[size_t(s) * max_blocks + t / block_size];
-      if (blk >= num_blocks) report(st, kBadArgument, 76, unsigned(blk));
-      if (blk >= 0 && blk < num_blocks) {
-        const size_t r = ((size_t(blk) * 2) * nkv + kvh) * block_size + t % block_size;
-        float dot = 0.f;
-        for (int d = 0; d < HD; ++d) dot += qs[d] * float(int(data[r * HD + d]) - 128);
-        z = dot * scale[r] * scale_log2;
-        vs = scale[r + size_t(nkv) * block_size];
+  if (rows <= 0) return;                                               // the whole cluster
+  if (base_len < (a.cu_q != nullptr ? 1 : 0) || base_len + rows - 1 > cap) {
+    if (tid == 0 && kvh == 0 && piece == 0) report(a.st, kBadArgument, 75, unsigned(s));
+    base_len = max(0, min(base_len, cap));
+  }
+  const int most_len = min(base_len + rows - 1, cap);
+  const int first_tok = a.window > 0 ? max(0, base_len - a.window) : 0;
+  const int last_first = a.window > 0 ? max(0, most_len - a.window) : 0;       // of the last row
+  const int tile0 = first_tok >> 4, tiles = ((most_len + 15) >> 4) - tile0;
+  const int lo = int((long long)tiles * piece / a.pieces), hi = int((long long)tiles * (piece + 1) / a.pieces);
+  const int mine = max(0, (hi - lo - warp + kWarps - 1) / kWarps);     // tiles lo + warp, lo + warp + 4, ...
+
+  // places of the next 32 tiles in the cache, in units of 16 rows, one in every lane (-1: a hole)
+  auto find = [&](int i0) {
+    const int i = i0 + lane;
+    int v = -1;
+    if (i < mine) {
+      const int tile = tile0 + lo + warp + i * kWarps, bi = tile / bpt;
+      const int blk = a.tables[size_t(s) * a.table_ld + bi];
+      if (blk >= a.num_blocks) report(a.st, kBadArgument, 76, unsigned(blk));
+      else if (blk >= 0) v = (blk * 2 * a.nkv + kvh) * bpt + (tile - bi * bpt);
+    }
+    return v;
+  };
+  uint8_t* ring = smem + warp * S::kRing;
+  int now = find(0), next = find(32);
+  uint32_t holes = 0;                                                  // bit: ring slot whose tile is a hole
+  auto issue = [&](int i, int slot) {                                  // always commits a group
+    if (i < mine) {
+      if ((i & 31) == 0 && i > 0) {
+        now = next;
+        next = find(i + 32);
+      }
+      const int at = __shfl_sync(0xffffffffu, now, i & 31);
+      holes &= ~(1u << slot);
+      if (at >= 0) {
+        uint8_t* dst = ring + slot * S::kSlot;
+        const uint8_t* k = a.data + size_t(at) * S::kTile + lane * 16;
+        const size_t half = size_t(a.nkv) * bpt;
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {
+          const int idx = j * 32 + lane, to = place<HD>(idx / kChunks, idx % kChunks);
+          cpa16(dst + to, k + j * 512);
+          cpa16(dst + S::kTile + to, k + half * S::kTile + j * 512);
+        }
+        if (lane < 8)
+          cpa16(dst + 2 * S::kTile + lane * 16, a.scale + (size_t(at) + (lane & 4 ? half : 0)) * 16 + (lane & 3) * 4);
+      } else {
+        holes |= 1u << slot;
       }
     }
-    red[tid] = z;
-    __syncthreads();
-    float top = m;
-    for (int i = 0; i < 128; ++i) top = fmaxf(top, red[i]);
-    __syncthreads();
-    const float base = top == -INFINITY ? 0.f : top, fade = exp2f(m - base), p = exp2f(z - base);
-    m = top;
-    red[tid] = p;
-    ps[tid] = z == -INFINITY ? 0.f : p * vs;
-    __syncthreads();
-    l *= fade;
-    for (int i = 0; i < 128; ++i) l += red[i];
-    for (int k = 0; k * 128 + tid < HD; ++k) acc[k] *= fade;
-    for (int i = 0; i < min(128, len - t0); ++i) {
-      const int t1 = t0 + i, blk = tables[size_t(s) * max_blocks + t1 / block_size];
-      if (blk < 0 || blk >= num_blocks) continue;
-      const size_t r = ((size_t(blk) * 2 + 1) * nkv + kvh) * block_size + t1 % block_size;
-      for (int k = 0; k * 128 + tid < HD; ++k) acc[k] += ps[i] * float(int(data[r * HD + k * 128 + tid]) - 128);
+    cpa_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) issue(i, i);
+
+  // queries: a thread's column nb * 8 + g, dimensions 16 c + 4 (lane & 3) .. + 3; the permutation of the dimensions inside a step is
+  // that of the keys' bytes
+  uint32_t qb[NB][kChunks][2];
+  float sum_q[NB][2];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int c = nb * 8 + g, r = c / G;
+    const __half* src = a.q + size_t(row0 + r) * a.ldq + size_t(kvh * G + c - r * G) * HD + t2 * 2;
+    float sum = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < kChunks; ++kk) {
+      uint2 v = make_uint2(0u, 0u);
+      if (r < rows) v = *reinterpret_cast<const uint2*>(src + kk * 16);
+      qb[nb][kk][0] = v.x;
+      qb[nb][kk][1] = v.y;
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), y = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+      sum += (x.x + x.y) + (y.x + y.y);
     }
-    __syncthreads();
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    sum_q[nb][0] = -128.f * __shfl_sync(0xffffffffu, sum, t2 * 4);     // of columns t2, t2 + 1
+    sum_q[nb][1] = -128.f * __shfl_sync(0xffffffffu, sum, t2 * 4 + 4);
   }
-  for (int k = 0; k * 128 + tid < HD; ++k)
-    out[size_t(row) * ldo + size_t(head) * HD + k * 128 + tid] = __float2half_rn(l == 0.f ? 0.f : acc[k] / l);
+
+  // m: the weights' reference, at most 6 above no score seen yet (a power of two of the largest weight, not its logarithm's maximum);
+  // ref: a power of two that no scale of a value exceeds; o holds sums of weight * vscale / ref
+  float o[NB][kChunks][4], m[NB][2], l[NB][2], ref = 0.f, inv_ref = 0.f;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    m[nb][0] = m[nb][1] = -INFINITY;
+    l[nb][0] = l[nb][1] = 0.f;
+#pragma unroll
+    for (int d = 0; d < kChunks; ++d) o[nb][d][0] = o[nb][d][1] = o[nb][d][2] = o[nb][d][3] = 0.f;
+  }
+  int slot = 0;
+#pragma unroll 1
+  for (int i = 0; i < mine; ++i) {
+    cpa_wait<kStages - 2>();
+    __syncwarp();
+    const bool hole = (holes >> slot) & 1u;
+    issue(i + kStages - 1, slot == 0 ? kStages - 1 : slot - 1);        // the slot of the tile before this one
+    const uint8_t* at = ring + slot * S::kSlot;
+    slot = slot + 1 == kStages ? 0 : slot + 1;
+    if (hole) continue;
+    const uint32_t kbase = smem_u32(at), vbase = kbase + S::kTile;
+    const float* scales = reinterpret_cast<const float*>(at + 2 * S::kTile);
+    const int tok = (tile0 + lo + warp + i * kWarps) << 4;
+    const int mm = lane >> 3, rr = lane & 7;
+    float sc[NB][2][4];                                                // even and odd steps apart: two chains
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[nb][0][e] = sc[nb][1][e] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < kChunks / 2; ++kk) {
+      uint32_t r[4];
+      ldm_x4(kbase + place<HD>((mm & 1) * 8 + rr, kk * 2 + (mm >> 1)), r);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t f[4] = {__byte_perm(r[2 * h], 0u, 0x4140), __byte_perm(r[2 * h + 1], 0u, 0x4140),
+                               __byte_perm(r[2 * h], 0u, 0x4342), __byte_perm(r[2 * h + 1], 0u, 0x4342)};
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) mma_f16(sc[nb][h], f, qb[nb][kk * 2 + h][0], qb[nb][kk * 2 + h][1]);
+      }
+    }
+    const float k0 = scales[g] * a.scale_log2, k1 = scales[g + 8] * a.scale_log2;
+    float w0 = scales[16 + g], w1 = scales[24 + g];
+    const bool ragged = tok + 16 > base_len || tok < last_first;       // some row does not see some token
+    uint32_t dead = 0;                                                 // bit nb * 4 + e
+    if (ragged) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int len = min(base_len + (nb * 8 + t2 + (e & 1)) / G, cap), at_tok = tok + g + (e >> 1) * 8;
+          if (at_tok >= len || (a.window > 0 && at_tok < len - a.window)) dead |= 1u << (nb * 4 + e);
+        }
+      if (tok + g >= most_len) w0 = 0.f;                               // what lies behind the sequence may be anything
+      if (tok + g + 8 >= most_len) w1 = 0.f;
+    }
+    float v[NB][4];
+    bool over = fmaxf(w0, w1) > ref;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[nb][e] = fmaf(sc[nb][0][e] + sc[nb][1][e], 16777216.f, sum_q[nb][e & 1]) * (e < 2 ? k0 : k1);
+        if ((dead >> (nb * 4 + e)) & 1u) v[nb][e] = -INFINITY;
+        over |= v[nb][e] > m[nb][e & 1] + 6.f;
+      }
+    if (__any_sync(0xffffffffu, over)) {
+      // new references: the tile's maxima where they are above, and what has been summed scaled to them
+      float wtop = fmaxf(fmaxf(w0, w1), 0.f);
+#pragma unroll
+      for (int sh = 4; sh < 32; sh <<= 1) wtop = fmaxf(wtop, __shfl_xor_sync(0xffffffffu, wtop, sh));
+      float fade = 1.f;
+      if (wtop > ref) {
+        // the power of two above twice the scale, so that a slowly growing scale does not come here every time
+        const float up = __uint_as_float(((__float_as_uint(fmaxf(wtop, 1e-30f)) >> 23) + 2u) << 23);
+        fade = ref * (1.f / up);
+        ref = up;
+        inv_ref = 1.f / up;
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(v[nb][e], v[nb][e + 2]);
+#pragma unroll
+          for (int sh = 4; sh < 32; sh <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, sh));
+          const float to = fmaxf(m[nb][e], x);
+          const float drop = m[nb][e] == -INFINITY ? 0.f : ex2(m[nb][e] - to);
+          m[nb][e] = to;
+          l[nb][e] *= drop;
+          f[e] = drop * fade;
+        }
+#pragma unroll
+        for (int d = 0; d < kChunks; ++d) {
+          o[nb][d][0] *= f[0];
+          o[nb][d][1] *= f[1];
+          o[nb][d][2] *= f[0];
+          o[nb][d][3] *= f[1];
+        }
+      }
+    }
+    w0 *= inv_ref;
+    w1 *= inv_ref;
+    uint32_t pb[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float p[4], w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float b = m[nb][e & 1] == -INFINITY ? 0.f : m[nb][e & 1];
+        p[e] = ex2(v[nb][e] - b);
+        w[e] = p[e] * (e < 2 ? w0 : w1);
+      }
+      if (ragged) {                                                    // a weight of zero times a scale that is no number
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((dead >> (nb * 4 + e)) & 1u) w[e] = 0.f;
+      }
+      l[nb][0] += p[0] + p[2];
+      l[nb][1] += p[1] + p[3];
+      pb[nb][0] = turn_8x8(pack_half2(w[0], w[1]));                    // [token][column] -> [column][token], the B operand
+      pb[nb][1] = turn_8x8(pack_half2(w[2], w[3]));
+    }
+#pragma unroll
+    for (int dd = 0; dd < kChunks / 2; ++dd) {
+      uint32_t r[4];
+      ldm_x4_t(vbase + place<HD>((mm & 1) * 8 + rr, dd * 2 + (mm >> 1)), r);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t f[4] = {minus_1152(__byte_perm(r[2 * h], 0x64646464u, 0x4240)), minus_1152(__byte_perm(r[2 * h], 0x64646464u, 0x4341)),
+                               minus_1152(__byte_perm(r[2 * h + 1], 0x64646464u, 0x4240)),
+                               minus_1152(__byte_perm(r[2 * h + 1], 0x64646464u, 0x4341))};
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) mma_f16(o[nb][dd * 2 + h], f, pb[nb][0], pb[nb][1]);
+      }
+    }
+  }
+
+  // ---- the warps' results side by side, in their rings
+  cpa_wait<0>();
+  __syncwarp();
+  float* put = reinterpret_cast<float*>(ring);
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int sh = 4; sh < 32; sh <<= 1) l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], sh);
+      const int c = nb * 8 + t2 + e;
+#pragma unroll
+      for (int d = 0; d < kChunks; ++d)
+        *reinterpret_cast<float2*>(put + c * S::kPitch + d * 16 + 2 * g) = make_float2(o[nb][d][e] * ref, o[nb][d][2 + e] * ref);
+      if (g == 0) {
+        own_m[warp * S::kCols + c] = m[nb][e];
+        own_l[warp * S::kCols + c] = l[nb][e];
+      }
+    }
+  __syncthreads();
+  const int cols = rows * G;
+  constexpr int kQuads = HD / 4;
+  auto finish = [&](int c, int d, const float4& acc, float top, float total) {
+    const int r = c / G, clusters = a.pieces / a.cluster;
+    if (clusters == 1) {
+      const float inv = total == 0.f ? 0.f : 1.f / total;              // nothing seen: zeros
+      uint2 h = make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
+      *reinterpret_cast<uint2*>(a.out + size_t(row0 + r) * a.ldo + size_t(kvh * G + c - r * G) * HD + d) = h;
+    } else {
+      float* to = a.scratch + ((size_t(item) * clusters + piece / a.cluster) * S::kCols + c) * (HD + 4);
+      *reinterpret_cast<float4*>(to + d) = acc;
+      if (d == 0) {
+        to[HD] = top;
+        to[HD + 1] = total;
+      }
+    }
+  };
+  for (int idx = tid; idx < cols * kQuads; idx += kWarps * 32) {
+    const int c = idx / kQuads, d = (idx - c * kQuads) * 4;
+    float top = -INFINITY, total = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, own_m[w * S::kCols + c]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float mw = own_m[w * S::kCols + c], f = mw == -INFINITY ? 1.f : ex2(mw - top);   // (nothing, or no number: as it is)
+      const float4 x = *reinterpret_cast<const float4*>(smem + w * S::kRing + (c * S::kPitch + d) * 4);
+      total += own_l[w * S::kCols + c] * f;
+      acc.x += x.x * f;
+      acc.y += x.y * f;
+      acc.z += x.z * f;
+      acc.w += x.w * f;
+    }
+    if (a.cluster == 1) {
+      finish(c, d, acc, top, total);
+    } else {
+      *reinterpret_cast<float4*>(smem + (c * S::kPitch + d) * 4) = acc;            // in place of the first warp's
+      if (d == 0) {
+        own_m[kWarps * S::kCols + c] = top;
+        own_l[kWarps * S::kCols + c] = total;
+      }
+    }
+  }
+  if (a.cluster == 1) return;
+  cluster_sync();
+  const int rank = piece % a.cluster;
+  const uint32_t base = smem_u32(smem), ma = smem_u32(own_m + kWarps * S::kCols), la = smem_u32(own_l + kWarps * S::kCols);
+  for (int idx = rank * kWarps * 32 + tid; idx < cols * kQuads; idx += a.cluster * kWarps * 32) {
+    const int c = idx / kQuads, d = (idx - c * kQuads) * 4;
+    float top = -INFINITY, total = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < a.cluster; ++w) top = fmaxf(top, load_cluster(in_cta(ma + c * 4, w)));
+    for (int w = 0; w < a.cluster; ++w) {
+      const float mw = load_cluster(in_cta(ma + c * 4, w)), f = mw == -INFINITY ? 1.f : ex2(mw - top);
+      const float4 x = load_cluster4(in_cta(base + (c * S::kPitch + d) * 4, w));
+      total += load_cluster(in_cta(la + c * 4, w)) * f;
+      acc.x += x.x * f;
+      acc.y += x.y * f;
+      acc.z += x.z * f;
+      acc.w += x.w * f;
+    }
+    finish(c, d, acc, top, total);
+  }
+  cluster_sync();                                                      // nobody leaves while others read its shared memory
+}
+
+// Joins the clusters of an item.  grid (items), 128 threads.
+template <int HD>
+__global__ void __launch_bounds__(128)
+attn_q8_join_kernel(const Q8Args a, int cols_kept) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int item = blockIdx.x, rg = item % a.row_groups, kvh = (item / a.row_groups) % a.nkv, s = item / a.row_groups / a.nkv;
+  const int G = a.nh / a.nkv, clusters = a.pieces / a.cluster;
+  int row0 = s, rows = 1;
+  if (a.cu_q != nullptr) {
+    const int first = a.cu_q[s], count = a.cu_q[s + 1] - first;
+    row0 = first + rg * a.rows_per;
+    rows = min(a.rows_per, count - rg * a.rows_per);
+    if (first < 0 || count > a.max_q || first + count > a.q_rows) rows = 0;
+  }
+  for (int idx = threadIdx.x; idx < rows * G * (HD / 4); idx += 128) {
+    const int c = idx / (HD / 4), d = (idx - c * (HD / 4)) * 4, r = c / G;
+    const float* from = a.scratch + (size_t(item) * clusters * cols_kept + c) * (HD + 4);
+    const size_t step = size_t(cols_kept) * (HD + 4);
+    float top = -INFINITY, total = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < clusters; ++w) top = fmaxf(top, from[w * step + HD]);
+    for (int w = 0; w < clusters; ++w) {
+      const float mw = from[w * step + HD], f = mw == -INFINITY ? 1.f : ex2(mw - top);
+      const float4 x = *reinterpret_cast<const float4*>(from + w * step + d);
+      total += from[w * step + HD + 1] * f;
+      acc.x += x.x * f;
+      acc.y += x.y * f;
+      acc.z += x.z * f;
+      acc.w += x.w * f;
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    *reinterpret_cast<uint2*>(a.out + size_t(row0 + r) * a.ldo + size_t(kvh * G + c - r * G) * HD + d) =
+        make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
+  }
+}
+
+int sm_count() {
+  static int counts[kMaxDevices];
+  const int slot = current_device_slot();
+  if (counts[slot] == 0 && cudaDeviceGetAttribute(&counts[slot], cudaDevAttrMultiProcessorCount, slot) != cudaSuccess) return 148;
+  return counts[slot];
+}
+
+struct Plan {
+  int nb, rows_per, row_groups, pieces, cluster;
+};
+Plan plan_of(int num_seqs, int max_q, int nh, int nkv, int block_size, int max_blocks, int window, int num_splits) {
+  Plan p;
+  const int G = nh / nkv;
+  p.nb = max_q * G <= 8 ? 1 : 2;
+  p.rows_per = std::max(1, 8 * p.nb / G);
+  p.row_groups = (max_q + p.rows_per - 1) / p.rows_per;
+  const long long items = (long long)num_seqs * nkv * p.row_groups;
+  long long want = num_splits;
+  if (num_splits <= 0) {
+    long long tokens = (long long)max_blocks * block_size;
+    if (window > 0) tokens = std::min(tokens, (long long)window + max_q + 16);
+    const long long most = std::max(1ll, tokens / 64);                 // a tile for every warp of a piece
+    want = std::min(most, (2ll * sm_count() + items - 1) / items);
+  }
+  if (want <= kMostCluster) {
+    p.cluster = 1;
+    while (p.cluster < want) p.cluster *= 2;
+    p.pieces = p.cluster;
+  } else {
+    p.cluster = kMostCluster;
+    p.pieces = int(std::min(64ll, (want + kMostCluster - 1) / kMostCluster) * kMostCluster);
+  }
+  return p;
+}
+
+template <int HD, int NB>
+int launch(const Q8Args& a, int items, cudaStream_t st) {
+  static bool ready[kMaxDevices];
+  const int dev = current_device_slot();
+  auto kernel = attn_q8_kernel<HD, NB>;
+  constexpr int kBytes = Q8Smem<HD, NB>::kTotal;
+  if (!ready[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+      return ZSE_ERR_LAUNCH;
+    ready[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(items * a.pieces);
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = kBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (a.cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = a.cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return ZSE_ERR_LAUNCH;
+  if (a.pieces > a.cluster &&
+      launch_pdl(attn_q8_join_kernel<HD>, dim3(items), dim3(128), 0, st, a, 8 * NB) != cudaSuccess)
+    return ZSE_ERR_LAUNCH;
+  return 0;
 }
 
 }  // namespace
@@ -73,31 +545,50 @@ attn_q8_kernel(const uint8_t* __restrict__ data, const float* __restrict__ scale
 
 using namespace zse;
 
-extern "C" int zse_attn_decode_q8_splits(int, int, int, int, int, int, int, int, int) { return 1; }
-extern "C" int64_t zse_attn_decode_q8_scratch_floats(int, int, int, int, int) { return 0; }
+extern "C" int zse_attn_decode_q8_pieces(int num_seqs, int max_q, int nh, int nkv, int block_size, int max_blocks, int window,
+                                         int num_splits) {
+  if (nkv <= 0 || nh < nkv || max_q <= 0 || num_seqs <= 0) return 1;
+  return plan_of(num_seqs, max_q, nh, nkv, block_size, max_blocks, window, num_splits).pieces;
+}
 
-extern "C" int zse_attn_decode_q8(const ZseKvQ8* kv, const void* q, int ldq, const void* tables, int max_blocks,
+extern "C" int64_t zse_attn_decode_q8_scratch_floats(int num_seqs, int max_q, int nh, int nkv, int hd, int block_size, int max_blocks,
+                                                     int window, int num_splits) {
+  if (nkv <= 0 || nh < nkv || max_q <= 0 || num_seqs <= 0) return 0;
+  const Plan p = plan_of(num_seqs, max_q, nh, nkv, block_size, max_blocks, window, num_splits);
+  if (p.pieces == p.cluster) return 0;
+  return int64_t(num_seqs) * nkv * p.row_groups * (p.pieces / p.cluster) * 8 * p.nb * (hd + 4);
+}
+
+extern "C" int zse_attn_decode_q8(const ZseKvQ8* kv, const void* q, int ldq, int q_rows, const void* tables, int table_ld, int max_blocks,
                                   const void* seq_lens, const void* cu_q, const void* q_pos0, int num_seqs, int max_q, void* out,
                                   int ldo, int nh, void* scratch, int64_t scratch_floats, int num_splits, float scale, int window,
                                   void* status, void* stream) {
   if (num_seqs <= 0 || max_q <= 0) return 0;
+  const int bpt = kv->block_size / 16;
   if (kv->num_blocks <= 0 || kv->nkv <= 0 || kv->block_size <= 0 || kv->block_size % 16 || nh <= 0 || nh % kv->nkv ||
-      nh / kv->nkv > 16 || num_seqs > 65535)
+      nh / kv->nkv > 16 || max_blocks < 0 || (cu_q == nullptr && max_q != 1))
     return ZSE_ERR_SHAPE;
-  auto go = [&](auto kernel) {
-    return launch_pdl(kernel, dim3(nh, max_q, num_seqs), dim3(128), 0, static_cast<cudaStream_t>(stream),
-                      static_cast<const uint8_t*>(kv->data), static_cast<const float*>(kv->scale), kv->num_blocks, kv->nkv,
-                      kv->block_size, static_cast<const __half*>(q), ldq, static_cast<const int*>(tables), max_blocks,
-                      static_cast<const int*>(seq_lens), static_cast<const int*>(cu_q), static_cast<const int*>(q_pos0),
-                      static_cast<__half*>(out), ldo, nh, scale * kLog2e, window, static_cast<Status*>(status)) == cudaSuccess
-               ? 0
-               : ZSE_ERR_LAUNCH;
-  };
+  if ((reinterpret_cast<uintptr_t>(kv->data) | reinterpret_cast<uintptr_t>(kv->scale) | reinterpret_cast<uintptr_t>(scratch)) & 15 ||
+      (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 7 || ldq % 4 || ldo % 4)
+    return ZSE_ERR_ALIGN;
+  const Plan p = plan_of(num_seqs, max_q, nh, kv->nkv, kv->block_size, max_blocks, window, num_splits);
+  const long long items = (long long)num_seqs * kv->nkv * p.row_groups;
+  if (items * p.pieces > 0x7fffffffll || (long long)kv->num_blocks * 2 * kv->nkv * bpt > 0x7fffffffll ||
+      (long long)max_blocks * kv->block_size > 0x7fffff00ll)
+    return ZSE_ERR_LIMIT;
+  if (p.pieces > p.cluster && (scratch == nullptr || scratch_floats < items * (p.pieces / p.cluster) * 8 * p.nb * (kv->hd + 4)))
+    return ZSE_ERR_LIMIT;
+  const Q8Args a{static_cast<const uint8_t*>(kv->data), static_cast<const float*>(kv->scale), static_cast<const __half*>(q),
+                 static_cast<const int*>(tables), static_cast<const int*>(seq_lens), static_cast<const int*>(cu_q),
+                 static_cast<const int*>(q_pos0), static_cast<__half*>(out), static_cast<float*>(scratch),
+                 static_cast<Status*>(status), ldq, ldo, q_rows, kv->num_blocks, kv->nkv, kv->block_size, table_ld, max_blocks, nh, max_q,
+                 p.rows_per, p.row_groups, window, p.pieces, p.cluster, scale * kLog2e};
+  auto go = [&](auto one, auto two) { return p.nb == 1 ? one(a, int(items), static_cast<cudaStream_t>(stream)) : two(a, int(items), static_cast<cudaStream_t>(stream)); };
   switch (kv->hd) {
-    case 64: return go(attn_q8_kernel<64>);
-    case 96: return go(attn_q8_kernel<96>);
-    case 128: return go(attn_q8_kernel<128>);
-    case 256: return go(attn_q8_kernel<256>);
+    case 64: return go(launch<64, 1>, launch<64, 2>);
+    case 96: return go(launch<96, 1>, launch<96, 2>);
+    case 128: return go(launch<128, 1>, launch<128, 2>);
+    case 256: return go(launch<256, 1>, launch<256, 2>);
     default: return ZSE_ERR_SHAPE;
   }
 }

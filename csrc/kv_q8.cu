@@ -132,9 +132,9 @@ rope_kv_write_q8_kernel(const __half* qkv, int ld, __half* q_out, int ld_q, cons
 // reads 16 bytes and writes 32.
 __global__ void __launch_bounds__(256)
 kv_read_q8_kernel(const uint8_t* __restrict__ data, const float* __restrict__ scale, int num_blocks, int nkv, int block_size,
-                  int hd, const int* __restrict__ tables, int max_blocks, const int* __restrict__ seq_lens,
+                  int hd, const int* __restrict__ tables, int table_ld, int max_blocks, const int* __restrict__ seq_lens,
                   const int* __restrict__ cu_blocks, int num_seqs, __half* __restrict__ out, int out_blocks,
-                  int* __restrict__ out_tables, int out_max_blocks, Status* st) {
+                  int* __restrict__ out_tables, int out_table_ld, int out_max_blocks, Status* st) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
@@ -144,9 +144,9 @@ kv_read_q8_kernel(const uint8_t* __restrict__ data, const float* __restrict__ sc
     const int len = seq_lens[s], first = cu_blocks[s], pages = (max(len, 0) + block_size - 1) / block_size;
     const bool fits = first >= 0 && pages <= min(min(max_blocks, out_max_blocks), cu_blocks[s + 1] - first) && first + pages <= out_blocks;
     if (j == 0 && (!fits || len < 0)) report(st, kBadArgument, 71, unsigned(s));
-    const int blk = fits && j < pages ? tables[size_t(s) * max_blocks + j] : -1;
+    const int blk = fits && j < pages ? tables[size_t(s) * table_ld + j] : -1;
     if (blk >= num_blocks) report(st, kBadArgument, 72, unsigned(blk));
-    out_tables[i] = blk >= 0 && blk < num_blocks ? first + j : -1;
+    out_tables[size_t(s) * out_table_ld + j] = blk >= 0 && blk < num_blocks ? first + j : -1;
   }
   const int total = min(cu_blocks[num_seqs], out_blocks);
   const int runs = 2 * nkv * block_size * hd / 16, row16 = hd / 16;
@@ -159,7 +159,7 @@ kv_read_q8_kernel(const uint8_t* __restrict__ data, const float* __restrict__ sc
     if (first < 0 || j < 0 || j >= pages || pages > min(min(max_blocks, out_max_blocks), cu_blocks[s + 1] - first) ||
         first + pages > out_blocks)
       continue;
-    const int blk = tables[size_t(s) * max_blocks + j];
+    const int blk = tables[size_t(s) * table_ld + j];
     if (blk < 0 || blk >= num_blocks) continue;
     const uint4* src = reinterpret_cast<const uint4*>(data) + size_t(blk) * runs;
     const float* sc = scale + size_t(blk) * 2 * nkv * block_size;
@@ -229,9 +229,9 @@ extern "C" int zse_rope_kv_write_q8(const ZseKvQ8* kv, const void* qkv, int ld, 
   }
 }
 
-extern "C" int zse_kv_read_q8(const ZseKvQ8* kv, const void* tables, int max_blocks, const void* seq_lens, const void* cu_blocks,
-                              int num_seqs, void* out, int out_blocks, void* out_tables, int out_max_blocks, void* status,
-                              void* stream) {
+extern "C" int zse_kv_read_q8(const ZseKvQ8* kv, const void* tables, int table_ld, int max_blocks, const void* seq_lens,
+                              const void* cu_blocks, int num_seqs, void* out, int out_blocks, void* out_tables, int out_table_ld,
+                              int out_max_blocks, void* status, void* stream) {
   if (num_seqs <= 0) return 0;
   if (!cache_ok(kv) || max_blocks < 0 || out_blocks < 0 || out_max_blocks < 0) return ZSE_ERR_SHAPE;
   if (!aligned16(kv->data) || !aligned16(kv->scale) || !aligned16(out)) return ZSE_ERR_ALIGN;
@@ -239,9 +239,9 @@ extern "C" int zse_kv_read_q8(const ZseKvQ8* kv, const void* tables, int max_blo
   const int grid = int(std::max(1ll, std::min((long long)sm_count() * 8, std::max((long long)out_blocks, entries))));
   return launch_pdl(kv_read_q8_kernel, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream),
                     static_cast<const uint8_t*>(kv->data), static_cast<const float*>(kv->scale), kv->num_blocks, kv->nkv,
-                    kv->block_size, kv->hd, static_cast<const int*>(tables), max_blocks, static_cast<const int*>(seq_lens),
+                    kv->block_size, kv->hd, static_cast<const int*>(tables), table_ld, max_blocks, static_cast<const int*>(seq_lens),
                     static_cast<const int*>(cu_blocks), num_seqs, static_cast<__half*>(out), out_blocks,
-                    static_cast<int*>(out_tables), out_max_blocks, static_cast<Status*>(status)) == cudaSuccess
+                    static_cast<int*>(out_tables), out_table_ld, out_max_blocks, static_cast<Status*>(status)) == cudaSuccess
              ? 0
              : ZSE_ERR_LAUNCH;
 }

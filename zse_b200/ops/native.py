@@ -121,11 +121,11 @@ _SIGS = {
     "zse_gemm_w4_splits": (c_int, [c_int, c_int, c_int, c_int]),
     "zse_rope_kv_write_q8": (c_int, [POINTER(KvQ8), c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
                                      c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
-    "zse_kv_read_q8": (c_int, [POINTER(KvQ8), c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int,
-                               c_void_p, c_void_p]),
-    "zse_attn_decode_q8_splits": (c_int, [c_int] * 9),
-    "zse_attn_decode_q8_scratch_floats": (c_int64, [c_int] * 5),
-    "zse_attn_decode_q8": (c_int, [POINTER(KvQ8), c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
+    "zse_kv_read_q8": (c_int, [POINTER(KvQ8), c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int,
+                               c_int, c_void_p, c_void_p]),
+    "zse_attn_decode_q8_pieces": (c_int, [c_int] * 8),
+    "zse_attn_decode_q8_scratch_floats": (c_int64, [c_int] * 9),
+    "zse_attn_decode_q8": (c_int, [POINTER(KvQ8), c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                    c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_float, c_int, c_void_p, c_void_p]),
     "zse_gemm_w8": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                             c_void_p, c_void_p]),
@@ -548,28 +548,27 @@ def rope_kv_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, q_out, planes, 
 
 def kv_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables, status):
     _on_current_device(kv)
-    _ck(load().zse_kv_read_q8(byref(kv.native()), _p(block_tables), block_tables.stride(0), _p(seq_lens), _p(cu_blocks), S,
-                              _p(out), out.shape[0], _p(out_tables), out_tables.stride(0), status, _stream()), "kv_read_q8")
+    _ck(load().zse_kv_read_q8(byref(kv.native()), _p(block_tables), block_tables.stride(0), block_tables.shape[1], _p(seq_lens),
+                              _p(cu_blocks), S, _p(out), out.shape[0], _p(out_tables), out_tables.stride(0),
+                              out_tables.shape[1], status, _stream()), "kv_read_q8")
 
 
 def attn_decode_q8_scratch_floats(S, max_q, nh, nkv, hd, block_size, max_blocks, window=0, num_splits=0) -> int:
     """fp32 values of scratch that ``attn_decode_q8`` needs for such a call (0: none)."""
-    lib = load()
-    return lib.zse_attn_decode_q8_scratch_floats(
-        S, max_q, nh, hd, lib.zse_attn_decode_q8_splits(S, max_q, nh, nkv, hd, block_size, max_blocks, window, num_splits))
+    return load().zse_attn_decode_q8_scratch_floats(S, max_q, nh, nkv, hd, block_size, max_blocks, window, num_splits)
 
 
 def attn_decode_q8(q, kv, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch, num_splits, scale, window, status):
     """``scratch``: fp32, ``attn_decode_q8_scratch_floats`` of it, or None (then the call allocates what it needs)."""
     _on_current_device(kv)
-    if scratch is None:
-        n = attn_decode_q8_scratch_floats(S, max_q, nh, kv.kv_heads, kv.head_dim, kv.block_size, block_tables.stride(0), window,
-                                          num_splits)
-        scratch = torch.empty(n, dtype=torch.float32, device=kv.device) if n else None
-    _ck(load().zse_attn_decode_q8(byref(kv.native()), _p(q), q.stride(0), _p(block_tables), block_tables.stride(0), _p(seq_lens),
-                                  _p(cu_q), _p(q_pos0), S, max_q, _p(out), out.stride(0), nh, _p(scratch),
-                                  0 if scratch is None else scratch.numel(), num_splits, float(scale), int(window), status,
-                                  _stream()), "attn_decode_q8")
+    max_blocks = block_tables.shape[1]
+    n = attn_decode_q8_scratch_floats(S, max_q, nh, kv.kv_heads, kv.head_dim, kv.block_size, max_blocks, window, num_splits)
+    if n and scratch is None:
+        scratch = torch.empty(n, dtype=torch.float32, device=kv.device)
+    _ck(load().zse_attn_decode_q8(byref(kv.native()), _p(q), q.stride(0), min(q.shape[0], out.shape[0]), _p(block_tables),
+                                  block_tables.stride(0), max_blocks, _p(seq_lens), _p(cu_q), _p(q_pos0), S, max_q, _p(out), out.stride(0), nh,
+                                  _p(scratch), 0 if scratch is None else scratch.numel(), num_splits, float(scale), int(window),
+                                  status, _stream()), "attn_decode_q8", 2 if n else 1)
 
 
 def headnorm_rope_kv_write(qkv, kv_layer, positions, slots, freqs, q_norm_w, k_norm_w, norm_v, k_is_v, eps, M, nh, nkv,
