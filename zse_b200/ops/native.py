@@ -534,23 +534,27 @@ def kv_q8(kv) -> KvQ8:
     return KvQ8(_p(kv.data), _p(kv.scale), kv.num_blocks, kv.kv_heads, kv.block_size, kv.head_dim)
 
 
-def _on_current_device(kv) -> None:
-    if kv.data.device.index != torch.cuda.current_device():
-        raise NativeError(f"the cache is on {kv.data.device}, the current device is {torch.cuda.current_device()}")
+def _stream_of(kv) -> int:
+    """The current stream of the cache's device, which has to be the current device.  (The two calls below the public ones:
+    ``torch.cuda.current_stream()`` makes a stream object every time and takes longer than everything else in a call here.)"""
+    at = torch._C._cuda_getDevice()
+    if kv.data.device.index != at:
+        raise NativeError(f"the cache is on {kv.data.device}, the current device is {at}")
+    return torch._C._cuda_getCurrentRawStream(at)
 
 
 def rope_kv_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, q_out, planes, n_planes, bias, status):
-    _on_current_device(kv)
+    stream = _stream_of(kv)
     _ck(load().zse_rope_kv_write_q8(byref(kv.native()), _p(qkv), 0 if qkv is None else qkv.stride(0), _p(q_out), q_out.stride(0),
                                     _p(planes), n_planes, _p(bias), _p(positions), _p(slots), _p(inv_freq), M, nh,
-                                    inv_freq.numel() * 2, status, _stream()), "rope_kv_write_q8")
+                                    inv_freq.numel() * 2, status, stream), "rope_kv_write_q8")
 
 
 def kv_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables, status):
-    _on_current_device(kv)
+    stream = _stream_of(kv)
     _ck(load().zse_kv_read_q8(byref(kv.native()), _p(block_tables), block_tables.stride(0), block_tables.shape[1], _p(seq_lens),
                               _p(cu_blocks), S, _p(out), out.shape[0], _p(out_tables), out_tables.stride(0),
-                              out_tables.shape[1], status, _stream()), "kv_read_q8")
+                              out_tables.shape[1], status, stream), "kv_read_q8")
 
 
 def attn_decode_q8_scratch_floats(S, max_q, nh, nkv, hd, block_size, max_blocks, window=0, num_splits=0) -> int:
@@ -560,7 +564,7 @@ def attn_decode_q8_scratch_floats(S, max_q, nh, nkv, hd, block_size, max_blocks,
 
 def attn_decode_q8(q, kv, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch, num_splits, scale, window, status):
     """``scratch``: fp32, ``attn_decode_q8_scratch_floats`` of it, or None (then the call allocates what it needs)."""
-    _on_current_device(kv)
+    stream = _stream_of(kv)
     max_blocks = block_tables.shape[1]
     n = attn_decode_q8_scratch_floats(S, max_q, nh, kv.kv_heads, kv.head_dim, kv.block_size, max_blocks, window, num_splits)
     if n and scratch is None:
@@ -568,7 +572,7 @@ def attn_decode_q8(q, kv, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, n
     _ck(load().zse_attn_decode_q8(byref(kv.native()), _p(q), q.stride(0), min(q.shape[0], out.shape[0]), _p(block_tables),
                                   block_tables.stride(0), max_blocks, _p(seq_lens), _p(cu_q), _p(q_pos0), S, max_q, _p(out), out.stride(0), nh,
                                   _p(scratch), 0 if scratch is None else scratch.numel(), num_splits, float(scale), int(window),
-                                  status, _stream()), "attn_decode_q8", 2 if n else 1)
+                                  status, stream), "attn_decode_q8", 2 if n else 1)
 
 
 def headnorm_rope_kv_write(qkv, kv_layer, positions, slots, freqs, q_norm_w, k_norm_w, norm_v, k_is_v, eps, M, nh, nkv,
