@@ -438,7 +438,8 @@ int zse_kv_read_q8(const ZseKvQ8* kv, const void* tables_i32, int table_ld, int 
 // max_q), the first at position q_pos0[s], each seeing the tokens up to its own; window > 0: the last so many of them.
 // num_splits: pieces of a (sequence, kv head, rows that share the products), rounded up to a power of two or a multiple of 16;
 // 0: the launcher decides.  Above 16 pieces scratch is needed (zse_attn_decode_q8_scratch_floats, 0: none).  q_rows: rows of q and out.
-int zse_attn_decode_q8_pieces(int num_seqs, int max_q, int nh, int nkv, int block_size, int max_blocks, int window, int num_splits);
+int zse_attn_decode_q8_pieces(int num_seqs, int max_q, int nh, int nkv, int hd, int block_size, int max_blocks, int window,
+                              int num_splits);
 int64_t zse_attn_decode_q8_scratch_floats(int num_seqs, int max_q, int nh, int nkv, int hd, int block_size, int max_blocks,
                                           int window, int num_splits);
 int zse_attn_decode_q8(const ZseKvQ8* kv, const void* q_f16, int ldq, int q_rows, const void* tables_i32, int table_ld, int max_blocks,

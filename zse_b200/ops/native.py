@@ -123,7 +123,7 @@ _SIGS = {
                                      c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
     "zse_kv_read_q8": (c_int, [POINTER(KvQ8), c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int,
                                c_int, c_void_p, c_void_p]),
-    "zse_attn_decode_q8_pieces": (c_int, [c_int] * 8),
+    "zse_attn_decode_q8_pieces": (c_int, [c_int] * 9),
     "zse_attn_decode_q8_scratch_floats": (c_int64, [c_int] * 9),
     "zse_attn_decode_q8": (c_int, [POINTER(KvQ8), c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                    c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_float, c_int, c_void_p, c_void_p]),
