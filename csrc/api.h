@@ -10,6 +10,7 @@
 #define ZSE_ERR_DRIVER (-3)
 #define ZSE_ERR_LAUNCH (-4)
 #define ZSE_ERR_LIMIT (-5)
+#define ZSE_ERR_SCRATCH (-6)
 
 #ifdef __cplusplus
 extern "C" {
@@ -417,35 +418,50 @@ int zse_attn_prefill_ext(const void* q, int ldq, const void* kv_layer, int64_t b
 // is (data - 128) * scale.  hd 64, 96, 128 or 256, block_size a multiple of 16; both 16-byte aligned.  Block ids and slots outside
 // the cache are reported through the status word and taken for holes.
 typedef struct ZseKvQ8 {
-  void* data;
-  void* scale;
+  void *data, *scale;
   int32_t num_blocks, nkv, block_size, hd;
 } ZseKvQ8;
-// Rows [M, (nh + 2 nkv) * hd] (fp16, row stride ld; or n_planes fp32 planes [n_planes][M][cols] plus bias_f16): q and k rotated
+// Rows [M, (nh + 2 nkv) * hd] (fp16, row stride ld; or n_planes fp32 planes [n_planes][M][cols] plus bias): q and k rotated
 // (rotate-half over the first rotary_dim dimensions, a multiple of 16), q to q_out (row stride ld_q; may be qkv), k and v
 // quantised into the cache at `slots` (-1: not stored), each with the scale max|x| / 127 of its head.
-int zse_rope_kv_write_q8(const ZseKvQ8* kv, const void* qkv, int ld, void* q_out, int ld_q, const void* planes, int n_planes,
-                         const void* bias, const void* positions_i32, const void* slots_i64, const void* inv_freq_f32, int M,
-                         int nh, int rotary_dim, void* status, void* stream);
+typedef struct ZseWriteQ8 {
+  ZseKvQ8 kv;
+  const void* qkv;
+  void* q_out;
+  const void *planes, *bias;               // fp32 and fp16, or null
+  const void *positions, *slots, *inv_freq;    // int32, int64, fp32 [rotary_dim / 2]
+  void *status, *stream;
+  int32_t ld, ld_q, n_planes, M, nh, rotary_dim;
+} ZseWriteQ8;
+int zse_rope_kv_write_q8(const ZseWriteQ8* a);
 // Pages of whole sequences as fp16: block j of sequence s -> out[cu_blocks[s] + j] (zeros behind seq_lens[s]), its place to
 // out_tables[s][j] (-1: hole, or behind the sequence).  out: out_blocks pages [2][nkv][block_size][hd].  Tables: rows of max_blocks,
 // table_ld apart.
-int zse_kv_read_q8(const ZseKvQ8* kv, const void* tables_i32, int table_ld, int max_blocks, const void* seq_lens_i32,
-                   const void* cu_blocks_i32, int num_seqs, void* out_f16, int out_blocks, void* out_tables_i32, int out_table_ld,
-                   int out_max_blocks, void* status, void* stream);
+typedef struct ZseReadQ8 {
+  ZseKvQ8 kv;
+  const void *tables, *seq_lens, *cu_blocks;   // int32
+  void *out, *out_tables, *status, *stream;
+  int32_t table_ld, max_blocks, num_seqs, out_blocks, out_table_ld, out_max_blocks;
+} ZseReadQ8;
+int zse_kv_read_q8(const ZseReadQ8* a);
 // ---- attention_q8.cu ----------------------------------------------------------------------------------------------
 // One row per sequence (cu_q null: row s sees seq_lens[s] tokens) or rows cu_q[s] .. cu_q[s + 1] - 1 of sequence s (at most
 // max_q), the first at position q_pos0[s], each seeing the tokens up to its own; window > 0: the last so many of them.
-// num_splits: pieces of a (sequence, kv head, rows that share the products), rounded up to a power of two or a multiple of 16;
-// 0: the launcher decides.  Above 16 pieces scratch is needed (zse_attn_decode_q8_scratch_floats, 0: none).  q_rows: rows of q and out.
-int zse_attn_decode_q8_pieces(int num_seqs, int max_q, int nh, int nkv, int hd, int block_size, int max_blocks, int window,
-                              int num_splits);
-int64_t zse_attn_decode_q8_scratch_floats(int num_seqs, int max_q, int nh, int nkv, int hd, int block_size, int max_blocks,
-                                          int window, int num_splits);
-int zse_attn_decode_q8(const ZseKvQ8* kv, const void* q_f16, int ldq, int q_rows, const void* tables_i32, int table_ld, int max_blocks,
-                       const void* seq_lens_i32, const void* cu_q_i32, const void* q_pos0_i32, int num_seqs, int max_q,
-                       void* out_f16, int ldo, int nh, void* scratch_f32, int64_t scratch_floats, int num_splits, float scale,
-                       int window, void* status, void* stream);
+// num_splits: pieces of a (sequence, kv head, rows that share the products), rounded up to a power of two or a multiple of 8;
+// 0: the launcher decides.  Above 8 pieces scratch is needed (ZSE_ERR_SCRATCH without; zse_attn_decode_q8_scratch_floats of it).
+// Returns the number of kernels launched.
+typedef struct ZseAttnQ8 {
+  ZseKvQ8 kv;
+  const void *q, *tables, *seq_lens, *cu_q, *q_pos0;
+  void *out, *scratch, *status, *stream;
+  int64_t scratch_floats;
+  int32_t ldq, ldo, q_rows, table_ld, max_blocks, num_seqs, max_q, nh, num_splits, window;      // q_rows: rows of q and out
+  float scale;
+  int32_t reserved;
+} ZseAttnQ8;
+int64_t zse_attn_decode_q8_scratch_floats(const ZseAttnQ8* a);
+int zse_attn_decode_q8_pieces(const ZseAttnQ8* a);
+int zse_attn_decode_q8(const ZseAttnQ8* a);
 
 // ---- sampling.cu --------------------------------------------------------------------------------------------
 int zse_argmax(const void* logits_f16, int ld, void* out_i32, int M, int V, void* stream);

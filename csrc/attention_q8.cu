@@ -27,7 +27,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kStages = 3;
-constexpr int kMostCluster = 16;
+constexpr int kMostCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -1e30f;                          // below every score, finite so that no difference is not a number
 
@@ -62,23 +62,20 @@ __device__ __forceinline__ uint32_t minus_1152(uint32_t x) {           // both h
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x64806480u));
   return y;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
+// Barrier of the cluster in two halves: the relaxed form only says that a CTA has got there, the other one orders its writes.
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t in_cta(uint32_t smem_addr, int rank) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ float4 load_cluster4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void store_cluster4(uint32_t addr, const float4& v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
-__device__ __forceinline__ float load_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void store_cluster2(uint32_t addr, float x, float y) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1,%2};" ::"r"(addr), "f"(x), "f"(y) : "memory");
 }
 
 // Where 16-byte chunk c of a tile's row lies: any eight rows of one chunk are in eight different groups of four banks.  Written so
@@ -120,10 +117,12 @@ struct Q8Smem {
   static constexpr int kRing = kStages * kSlot > kCols * kPitch * 4 ? kStages * kSlot : kCols * kPitch * 4;   // of a warp
   static constexpr int kQPitch = HD * 2 + 32;                          // bytes: four columns in different groups of eight banks
   static constexpr bool kQShared = NB > 1;                             // queries in shared memory, or in registers
-  static constexpr int kNumbers = kWarps * kRing;                      // own_m, own_l, own_ref, part_m, part_l
-  static constexpr int kQ = kNumbers + ((kWarps + 1) * 2 * kCols + kWarps + 2 * kMostCluster * kCols) * 4;
+  static constexpr int kNumbers = kWarps * kRing;                      // own_m, own_l [warp][column], own_ref [warp]
+  static constexpr int kGot = kNumbers + (2 * kWarps * kCols + kWarps) * 4;            // references and sums, [CTA][column][2]
+  static constexpr int kGotO = kGot + 2 * kMostCluster * kCols * 4;                    // results, [CTA][its share here] of 16 bytes
+  static constexpr int kQ = kGotO + (kCols * HD / 4 + kMostCluster) * 16;
   static constexpr int kTotal = kQ + (kQShared ? kCols * kQPitch : 0);
-  static_assert(kQ % 16 == 0, "16-byte pieces");
+  static_assert(kGot % 16 == 0 && kGotO % 16 == 0 && kQ % 16 == 0, "16-byte pieces");
 };
 
 template <int HD, int NB>
@@ -133,15 +132,22 @@ attn_q8_kernel(const Q8Args a) {
   constexpr int kChunks = HD / 16;                                     // 16-byte chunks of a row, and 16-wide steps of the products
   constexpr int kChains = NB == 1 ? 2 : 1;                             // even and odd steps of a column apart
   extern __shared__ __align__(128) uint8_t smem[];
-  float* own_m = reinterpret_cast<float*>(smem + S::kNumbers);         // [warp][column], then the CTA's
-  float* own_l = own_m + (kWarps + 1) * S::kCols;
-  float* own_ref = own_l + (kWarps + 1) * S::kCols;                    // [warp]
+  float* own_m = reinterpret_cast<float*>(smem + S::kNumbers);         // [warp][column]
+  float* own_l = own_m + kWarps * S::kCols;
+  float* own_ref = own_l + kWarps * S::kCols;                          // [warp]
   pdl_launch_dependents();
   pdl_wait();
   // (what every CTA does once is kept short: with one tile per warp it is most of its instructions)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t2 = (lane & 3) * 2;
   const int piece = blockIdx.x, s = blockIdx.z, kvh = a.row_groups == 1 ? blockIdx.y : blockIdx.y / a.row_groups;
   const int rg = blockIdx.y - kvh * a.row_groups, cap = a.max_blocks * a.bpt * 16;
+
+  // A warp's tile i is 4 (i * pieces + piece) + warp of the item: pieces are equally long, and without a window where the first tiles
+  // lie is known before the length (the entries are loaded beside it, and used if the sequence is that long).
+  const int* table = a.tables + size_t(s) * a.table_ld;
+  const int stride = a.pieces * kWarps, ahead = piece * kWarps + warp + lane * stride;
+  int early = -1;
+  if (a.window == 0 && lane < 4 && ahead < a.max_blocks * a.bpt) early = table[a.bpt_shift >= 0 ? ahead >> a.bpt_shift : ahead / a.bpt];
 
   // rows of this item, and how many tokens its first row sees (each further row sees one more)
   int row0 = s, rows = 1, base_len;
@@ -166,17 +172,16 @@ attn_q8_kernel(const Q8Args a) {
   const int first_tok = a.window > 0 ? max(0, base_len - a.window) : 0;
   const int last_first = a.window > 0 ? max(0, most_len - a.window) : 0;       // of the last row
   const int tile0 = first_tok >> 4, tiles = ((most_len + 15) >> 4) - tile0;
-  const int per = unsigned(tiles + a.pieces - 1) / unsigned(a.pieces), lo = min(tiles, piece * per), hi = min(tiles, lo + per);
-  const int mine = max(0, (hi - lo - warp + kWarps - 1) / kWarps);     // tiles lo + warp, lo + warp + 4, ...
+  const int first_tile = piece * kWarps + warp, mine = first_tile < tiles ? unsigned(tiles - first_tile - 1) / unsigned(stride) + 1 : 0;
+  if (a.cluster > 1) cluster_arrive_relaxed();                         // (waited for before another CTA's memory is written)
 
   // places of the next 32 tiles in the cache, in units of 16 rows, one in every lane (-1: a hole)
-  const int* table = a.tables + size_t(s) * a.table_ld;
   auto find = [&](int i0) {
     const int i = i0 + lane;
     int v = -1;
     if (i < mine) {
-      const int tile = tile0 + lo + warp + i * kWarps, bi = a.bpt_shift >= 0 ? tile >> a.bpt_shift : tile / a.bpt;
-      const int blk = table[bi];
+      const int tile = tile0 + first_tile + i * stride, bi = a.bpt_shift >= 0 ? tile >> a.bpt_shift : tile / a.bpt;
+      const int blk = i < 4 && a.window == 0 ? early : table[bi];
       if (unsigned(blk) < unsigned(a.num_blocks)) v = (blk * 2 * a.nkv + kvh) * a.bpt + (tile - bi * a.bpt);
       else if (blk >= 0) complain(a.st, 76, blk);
     }
@@ -282,7 +287,7 @@ attn_q8_kernel(const Q8Args a) {
     const uint32_t at = ring + slot * S::kSlot, tile = at + step0, scales = at + 2 * S::kTile + g * 4;
     slot = slot + 1 == kStages ? 0 : slot + 1;
     if (hole) continue;
-    const int tok = (tile0 + lo + warp + i * kWarps) << 4;
+    const int tok = (tile0 + first_tile + i * stride) << 4;
     const float k0 = load_shared(scales) * a.scale_log2, k1 = load_shared(scales + 32) * a.scale_log2;      // (with the 2^24 of the bytes)
     float w0 = load_shared(scales + 64), w1 = load_shared(scales + 96);
     float sc[NB][kChains][4];
@@ -443,11 +448,13 @@ attn_q8_kernel(const Q8Args a) {
       float* to = a.scratch + ((size_t(item) * (a.pieces / a.cluster) + piece / a.cluster) * S::kCols + c) * (HD + 4);
       *reinterpret_cast<float4*>(to + d) = acc;
       if (d == 0) {
-        to[HD] = top;
-        to[HD + 1] = total;
+        *reinterpret_cast<float2*>(to + HD) = make_float2(top, total);
       }
     }
   };
+  const int rank = piece & (a.cluster - 1), shift = 31 - __clz(a.cluster), share = (cols * kQuads + a.cluster - 1) >> shift;
+  const uint32_t got = smem_u32(smem) + S::kGot, got_o = smem_u32(smem) + S::kGotO;
+  if (a.cluster > 1) cluster_wait();                                   // all CTAs of the cluster run
   for (int idx = tid; idx < cols * kQuads; idx += kWarps * 32) {
     const int c = idx / kQuads, d = (idx - c * kQuads) * 4;
     float top = kNone, total = 0.f;
@@ -468,67 +475,53 @@ attn_q8_kernel(const Q8Args a) {
     if (a.cluster == 1) {
       finish(c, d, acc, top, total);
     } else {
-      *reinterpret_cast<float4*>(smem + (c * S::kPitch + d) * 4) = acc;            // in place of the first warp's
-      if (d == 0) {
-        own_m[kWarps * S::kCols + c] = top;
-        own_l[kWarps * S::kCols + c] = total;
-      }
+      // to the CTA that adds up this element: every cluster-th is its own
+      const uint32_t to = in_cta(got_o + ((rank * share) + (idx >> shift)) * 16, idx & (a.cluster - 1));
+      store_cluster4(to, acc);
+      if (d == 0)
+        for (int w = 0; w < a.cluster; ++w) store_cluster2(in_cta(got + (rank * S::kCols + c) * 8, w), top, total);
     }
   }
   if (a.cluster == 1) return;
-  // Every CTA has a share of the elements and adds it up over the cluster.  A load from another CTA takes some 200 cycles, so they
-  // go out together: first all references and sums of weights, then the results in batches.
-  cluster_sync();
-  const int rank = piece & (a.cluster - 1);
-  const uint32_t base = smem_u32(smem), ma = smem_u32(own_m + kWarps * S::kCols), la = smem_u32(own_l + kWarps * S::kCols);
-  float* part_m = own_ref + kWarps;                                    // [column][CTA]: factor of its result; sums of weights
-  float* part_l = part_m + S::kCols * kMostCluster;
-  for (int idx = tid; idx < cols * kMostCluster; idx += kWarps * 32) { // the CTAs of a column are neighbouring lanes
-    const int c = idx / kMostCluster, w = idx % kMostCluster;
-    const bool there = w < a.cluster;
-    const float mw = there ? load_cluster(in_cta(ma + c * 4, w)) : kNone, lw = there ? load_cluster(in_cta(la + c * 4, w)) : 0.f;
-    part_m[idx] = mw;
-    part_l[idx] = lw;
-  }
-  __syncthreads();
-  for (int idx = rank * kWarps * 32 + tid; idx < cols * kQuads; idx += a.cluster * kWarps * 32) {
-    const int c = idx / kQuads, d = (idx - c * kQuads) * 4;
+  cluster_arrive();
+  cluster_wait();                                                      // nobody writes here any more, and nobody leaves before
+  const float2* numbers = reinterpret_cast<const float2*>(smem + S::kGot);
+  const float4* parts = reinterpret_cast<const float4*>(smem + S::kGotO);
+  for (int at = tid; at * a.cluster + rank < cols * kQuads; at += kWarps * 32) {
+    const int idx = at * a.cluster + rank, c = idx / kQuads, d = (idx - c * kQuads) * 4;
     float top = kNone, total = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kMostCluster; ++w) top = fmaxf(top, part_m[c * kMostCluster + w]);
+    for (int w = 0; w < kMostCluster; ++w)
+      if (w < a.cluster) top = fmaxf(top, numbers[w * S::kCols + c].x);
 #pragma unroll
-    for (int w0 = 0; w0 < kMostCluster; w0 += 8) {
-      if (w0 < a.cluster) {
-        float4 x[8];
-#pragma unroll
-        for (int w = 0; w < 8; ++w) x[w] = load_cluster4(in_cta(base + (c * S::kPitch + d) * 4, min(w0 + w, a.cluster - 1)));
-#pragma unroll
-        for (int w = 0; w < 8; ++w) {
-          const float mw = part_m[c * kMostCluster + w0 + w], f = ex2(mw - top);
-          if (w0 + w < a.cluster) {
-            total += part_l[c * kMostCluster + w0 + w] * f;
-            acc.x += x[w].x * f;
-            acc.y += x[w].y * f;
-            acc.z += x[w].z * f;
-            acc.w += x[w].w * f;
-          }
-        }
+    for (int w = 0; w < kMostCluster; ++w)
+      if (w < a.cluster) {
+        const float2 n = numbers[w * S::kCols + c];
+        const float4 x = parts[w * share + at];
+        const float f = ex2(n.x - top);
+        total += n.y * f;
+        acc.x += x.x * f;
+        acc.y += x.y * f;
+        acc.z += x.z * f;
+        acc.w += x.w * f;
       }
-    }
     finish(c, d, acc, top, total);
   }
-  cluster_sync();                                                      // nobody leaves while others read its shared memory
 }
 
-// Joins the clusters of an item.  grid (kv heads * row groups, sequences), 128 threads.
+// Joins the clusters of an item.  grid (kv heads * row groups, sequences, columns), 128 threads: kGroups of them share a piece of a
+// column, each takes every kGroups-th cluster.
 template <int HD>
 __global__ void __launch_bounds__(128)
 attn_q8_join_kernel(const Q8Args a, int cols_kept) {
   pdl_launch_dependents();
   pdl_wait();
+  constexpr int kQuads = HD / 4, kGroups = 128 / kQuads;
+  __shared__ float4 part[kGroups][kQuads];
+  __shared__ float2 number[kGroups];
   const int s = blockIdx.y, item = s * gridDim.x + blockIdx.x, kvh = blockIdx.x / a.row_groups, rg = blockIdx.x - kvh * a.row_groups;
-  const int G = a.group, clusters = a.pieces / a.cluster;
+  const int c = blockIdx.z, r = row_of(a, c), clusters = a.pieces / a.cluster;
   int row0 = s, rows = 1;
   if (a.cu_q != nullptr) {
     const int first = a.cu_q[s], count = a.cu_q[s + 1] - first;
@@ -536,26 +529,33 @@ attn_q8_join_kernel(const Q8Args a, int cols_kept) {
     rows = min(a.rows_per, count - rg * a.rows_per);
     if (first < 0 || count > a.max_q || first + count > a.q_rows) rows = 0;
   }
-  for (int idx = threadIdx.x; idx < rows * G * (HD / 4); idx += 128) {
-    const int c = idx / (HD / 4), d = (idx - c * (HD / 4)) * 4, r = row_of(a, c);
-    const float* from = a.scratch + (size_t(item) * clusters * cols_kept + c) * (HD + 4);
-    const size_t step = size_t(cols_kept) * (HD + 4);
-    float top = kNone, total = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int w = 0; w < clusters; ++w) top = fmaxf(top, from[w * step + HD]);
+  if (r >= rows) return;
+  const int grp = threadIdx.x / kQuads, d = (threadIdx.x - grp * kQuads) * 4;
+  const float* from = a.scratch + (size_t(item) * clusters * cols_kept + c) * (HD + 4);
+  const size_t step = size_t(cols_kept) * (HD + 4);
+  float top = kNone, total = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float m, float l, const float4& x) {
+    const float to = fmaxf(top, m), f = ex2(top - to), g = ex2(m - to);
+    top = to;
+    total = total * f + l * g;
+    acc = make_float4(acc.x * f + x.x * g, acc.y * f + x.y * g, acc.z * f + x.z * g, acc.w * f + x.w * g);
+  };
+  if (grp < kGroups) {
 #pragma unroll 4
-    for (int w = 0; w < clusters; ++w) {
-      const float mw = from[w * step + HD], f = ex2(mw - top);
-      const float4 x = *reinterpret_cast<const float4*>(from + w * step + d);
-      total += from[w * step + HD + 1] * f;
-      acc.x += x.x * f;
-      acc.y += x.y * f;
-      acc.z += x.z * f;
-      acc.w += x.w * f;
+    for (int w = grp; w < clusters; w += kGroups) {
+      const float2 n = *reinterpret_cast<const float2*>(from + w * step + HD);
+      add(n.x, n.y, *reinterpret_cast<const float4*>(from + w * step + d));
     }
+    part[grp][d / 4] = acc;
+    if (d == 0) number[grp] = make_float2(top, total);
+  }
+  __syncthreads();
+  if (grp == 0) {
+#pragma unroll
+    for (int w = 1; w < kGroups; ++w) add(number[w].x, number[w].y, part[w][d / 4]);
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    *reinterpret_cast<uint2*>(a.out + size_t(row0 + r) * a.ldo + size_t(kvh * G + c - r * G) * HD + d) =
+    *reinterpret_cast<uint2*>(a.out + size_t(row0 + r) * a.ldo + size_t(kvh * a.group + c - r * a.group) * HD + d) =
         make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
   }
 }
@@ -569,30 +569,33 @@ int sm_count() {
 
 struct Plan {
   int nb, rows_per, row_groups, pieces, cluster;
+  long long scratch_floats;
 };
-Plan plan_of(int num_seqs, int max_q, int nh, int nkv, int hd, int block_size, int max_blocks, int window, int num_splits) {
+Plan plan_of(const ZseAttnQ8& a) {
   Plan p;
-  const int G = nh / nkv;
-  p.nb = max_q * G <= 8 ? 1 : max_q * G <= 16 || hd > 128 ? 2 : 4;
+  const int G = a.nh / a.kv.nkv;
+  p.nb = a.max_q * G <= 8 ? 1 : a.max_q * G <= 16 || a.kv.hd > 128 ? 2 : 4;
   p.rows_per = std::max(1, 8 * p.nb / G);
-  p.row_groups = (max_q + p.rows_per - 1) / p.rows_per;
-  const long long items = (long long)num_seqs * nkv * p.row_groups;
-  long long want = num_splits;
-  if (num_splits <= 0) {
-    long long tokens = (long long)max_blocks * block_size;
-    if (window > 0) tokens = std::min(tokens, (long long)window + max_q + 16);
+  p.row_groups = (a.max_q + p.rows_per - 1) / p.rows_per;
+  const long long items = (long long)a.num_seqs * a.kv.nkv * p.row_groups;
+  long long want = a.num_splits;
+  if (want <= 0) {
+    long long tokens = (long long)a.max_blocks * a.kv.block_size;
+    if (a.window > 0) tokens = std::min(tokens, (long long)a.window + a.max_q + 16);
     const long long most = std::max(1ll, tokens / 64);                 // a tile for every warp of a piece
     want = std::min(most, (2ll * sm_count() + items - 1) / items);
   }
-  if (want <= kMostCluster) {
-    p.cluster = 1;
-    while (p.cluster < want) p.cluster *= 2;
-    p.pieces = p.cluster;
-  } else {
-    p.cluster = kMostCluster;
-    p.pieces = int(std::min(64ll, (want + kMostCluster - 1) / kMostCluster) * kMostCluster);
-  }
+  p.cluster = 1;
+  while (p.cluster < want && p.cluster < kMostCluster) p.cluster *= 2;
+  p.pieces = int(std::min(64ll, (want + p.cluster - 1) / p.cluster) * p.cluster);
+  p.scratch_floats = p.pieces == p.cluster ? 0 : items * (p.pieces / p.cluster) * 8 * p.nb * (a.kv.hd + 4);
   return p;
+}
+bool shape_ok(const ZseAttnQ8& a) {
+  const ZseKvQ8& kv = a.kv;
+  return kv.num_blocks > 0 && kv.nkv > 0 && kv.block_size > 0 && kv.block_size % 16 == 0 && a.nh > 0 && a.nh % kv.nkv == 0 &&
+         a.nh / kv.nkv <= 16 && a.max_blocks >= 0 && a.max_q <= 64 && (a.cu_q != nullptr || a.max_q == 1) &&
+         (kv.hd == 64 || kv.hd == 96 || kv.hd == 128 || kv.hd == 256);
 }
 
 template <int HD, int NB>
@@ -629,9 +632,9 @@ int launch(const Q8Args& a, int num_seqs, cudaStream_t st) {
   cfg.numAttrs = n;
   if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return ZSE_ERR_LAUNCH;
   if (a.pieces > a.cluster &&
-      launch_pdl(attn_q8_join_kernel<HD>, dim3(a.nkv * a.row_groups, num_seqs), dim3(128), 0, st, a, 8 * NB) != cudaSuccess)
+      launch_pdl(attn_q8_join_kernel<HD>, dim3(a.nkv * a.row_groups, num_seqs, a.rows_per * a.group), dim3(128), 0, st, a, 8 * NB) != cudaSuccess)
     return ZSE_ERR_LAUNCH;
-  return 0;
+  return a.pieces > a.cluster ? 2 : 1;
 }
 
 }  // namespace
@@ -639,56 +642,43 @@ int launch(const Q8Args& a, int num_seqs, cudaStream_t st) {
 
 using namespace zse;
 
-extern "C" int zse_attn_decode_q8_pieces(int num_seqs, int max_q, int nh, int nkv, int hd, int block_size, int max_blocks, int window,
-                                         int num_splits) {
-  if (nkv <= 0 || nh < nkv || max_q <= 0 || num_seqs <= 0) return 1;
-  return plan_of(num_seqs, max_q, nh, nkv, hd, block_size, max_blocks, window, num_splits).pieces;
+extern "C" int zse_attn_decode_q8_pieces(const ZseAttnQ8* x) {
+  return x->num_seqs > 0 && x->max_q > 0 && shape_ok(*x) ? plan_of(*x).pieces : 0;
+}
+extern "C" int64_t zse_attn_decode_q8_scratch_floats(const ZseAttnQ8* x) {
+  return x->num_seqs > 0 && x->max_q > 0 && shape_ok(*x) ? plan_of(*x).scratch_floats : 0;
 }
 
-extern "C" int64_t zse_attn_decode_q8_scratch_floats(int num_seqs, int max_q, int nh, int nkv, int hd, int block_size, int max_blocks,
-                                                     int window, int num_splits) {
-  if (nkv <= 0 || nh < nkv || max_q <= 0 || num_seqs <= 0) return 0;
-  const Plan p = plan_of(num_seqs, max_q, nh, nkv, hd, block_size, max_blocks, window, num_splits);
-  if (p.pieces == p.cluster) return 0;
-  return int64_t(num_seqs) * nkv * p.row_groups * (p.pieces / p.cluster) * 8 * p.nb * (hd + 4);
-}
-
-extern "C" int zse_attn_decode_q8(const ZseKvQ8* kv, const void* q, int ldq, int q_rows, const void* tables, int table_ld, int max_blocks,
-                                  const void* seq_lens, const void* cu_q, const void* q_pos0, int num_seqs, int max_q, void* out,
-                                  int ldo, int nh, void* scratch, int64_t scratch_floats, int num_splits, float scale, int window,
-                                  void* status, void* stream) {
-  if (num_seqs <= 0 || max_q <= 0) return 0;
-  const int bpt = kv->block_size / 16;
-  if (kv->num_blocks <= 0 || kv->nkv <= 0 || kv->block_size <= 0 || kv->block_size % 16 || nh <= 0 || nh % kv->nkv ||
-      nh / kv->nkv > 16 || max_blocks < 0 || max_q > 64 || (cu_q == nullptr && max_q != 1) ||
-      (kv->hd != 64 && kv->hd != 96 && kv->hd != 128 && kv->hd != 256))
-    return ZSE_ERR_SHAPE;
-  if ((reinterpret_cast<uintptr_t>(kv->data) | reinterpret_cast<uintptr_t>(kv->scale) | reinterpret_cast<uintptr_t>(scratch) |
-       reinterpret_cast<uintptr_t>(q)) & 15 || reinterpret_cast<uintptr_t>(out) & 7 || ldq % 8 || ldo % 4)
+extern "C" int zse_attn_decode_q8(const ZseAttnQ8* x) {
+  const ZseKvQ8& kv = x->kv;
+  if (x->num_seqs <= 0 || x->max_q <= 0) return 0;
+  if (!shape_ok(*x)) return ZSE_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(kv.data) | reinterpret_cast<uintptr_t>(kv.scale) | reinterpret_cast<uintptr_t>(x->scratch) |
+       reinterpret_cast<uintptr_t>(x->q)) & 15 || reinterpret_cast<uintptr_t>(x->out) & 7 || x->ldq % 8 || x->ldo % 4)
     return ZSE_ERR_ALIGN;
-  const Plan p = plan_of(num_seqs, max_q, nh, kv->nkv, kv->hd, kv->block_size, max_blocks, window, num_splits);
-  if (num_seqs > 65535 || (long long)kv->nkv * p.row_groups > 65535 || (long long)num_seqs * kv->nkv * p.row_groups > 0x7fffffffll ||
-      (long long)kv->num_blocks * 2 * kv->nkv * bpt > 0x7fffffffll || (long long)max_blocks * kv->block_size > 0x7fffff00ll)
+  const Plan p = plan_of(*x);
+  const int bpt = kv.block_size / 16, group = x->nh / kv.nkv;
+  if (x->num_seqs > 65535 || (long long)kv.nkv * p.row_groups > 65535 ||
+      (long long)x->num_seqs * kv.nkv * p.row_groups > 0x7fffffffll || (long long)kv.num_blocks * 2 * kv.nkv * bpt > 0x7fffffffll ||
+      (long long)x->max_blocks * kv.block_size > 0x7fffff00ll || (long long)kv.nkv * kv.block_size * kv.hd > 0x7fffffffll)
     return ZSE_ERR_LIMIT;
-  if (p.pieces > p.cluster &&
-      (scratch == nullptr || scratch_floats < (long long)num_seqs * kv->nkv * p.row_groups * (p.pieces / p.cluster) * 8 * p.nb * (kv->hd + 4)))
-    return ZSE_ERR_LIMIT;
-  const int group = nh / kv->nkv;
+  if (p.scratch_floats > 0 && (x->scratch == nullptr || x->scratch_floats < p.scratch_floats)) return ZSE_ERR_SCRATCH;
   int shift = 0;
   while ((1 << shift) < bpt) ++shift;
-  const Q8Args a{static_cast<const uint8_t*>(kv->data), static_cast<const float*>(kv->scale), static_cast<const __half*>(q),
-                 static_cast<const int*>(tables), static_cast<const int*>(seq_lens), static_cast<const int*>(cu_q),
-                 static_cast<const int*>(q_pos0), static_cast<__half*>(out), static_cast<float*>(scratch),
-                 static_cast<Status*>(status), ldq, ldo, q_rows, kv->num_blocks, kv->nkv, bpt, (1 << shift) == bpt ? shift : -1,
-                 table_ld, max_blocks, group, (65536 + group - 1) / group, max_q, p.rows_per, p.row_groups, window, p.pieces,
-                 p.cluster, scale * kLog2e * 16777216.f};
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define ZSE_Q8_WIDTH(HD) p.nb == 1 ? launch<HD, 1>(a, num_seqs, st) : p.nb == 2 ? launch<HD, 2>(a, num_seqs, st)
-  switch (kv->hd) {
-    case 64: return ZSE_Q8_WIDTH(64) : launch<64, 4>(a, num_seqs, st);
-    case 96: return ZSE_Q8_WIDTH(96) : launch<96, 4>(a, num_seqs, st);
-    case 128: return ZSE_Q8_WIDTH(128) : launch<128, 4>(a, num_seqs, st);
-    default: return p.nb == 1 ? launch<256, 1>(a, num_seqs, st) : launch<256, 2>(a, num_seqs, st);
+  const Q8Args a{static_cast<const uint8_t*>(kv.data), static_cast<const float*>(kv.scale), static_cast<const __half*>(x->q),
+                 static_cast<const int*>(x->tables), static_cast<const int*>(x->seq_lens), static_cast<const int*>(x->cu_q),
+                 static_cast<const int*>(x->q_pos0), static_cast<__half*>(x->out), static_cast<float*>(x->scratch),
+                 static_cast<Status*>(x->status), x->ldq, x->ldo, x->q_rows, kv.num_blocks, kv.nkv, bpt,
+                 (1 << shift) == bpt ? shift : -1, x->table_ld, x->max_blocks, group, (65536 + group - 1) / group, x->max_q,
+                 p.rows_per, p.row_groups, x->window, p.pieces, p.cluster, x->scale * kLog2e * 16777216.f};
+  const int n = x->num_seqs;
+  const cudaStream_t st = static_cast<cudaStream_t>(x->stream);
+#define ZSE_Q8_WIDTH(HD) p.nb == 1 ? launch<HD, 1>(a, n, st) : p.nb == 2 ? launch<HD, 2>(a, n, st)
+  switch (kv.hd) {
+    case 64: return ZSE_Q8_WIDTH(64) : launch<64, 4>(a, n, st);
+    case 96: return ZSE_Q8_WIDTH(96) : launch<96, 4>(a, n, st);
+    case 128: return ZSE_Q8_WIDTH(128) : launch<128, 4>(a, n, st);
+    default: return p.nb == 1 ? launch<256, 1>(a, n, st) : launch<256, 2>(a, n, st);
   }
 #undef ZSE_Q8_WIDTH
 }

@@ -243,9 +243,9 @@ kv_read_q8_kernel(const uint8_t* __restrict__ data, const float* __restrict__ sc
   }
 }
 
-bool cache_ok(const ZseKvQ8* kv) {
-  return kv->num_blocks > 0 && kv->nkv > 0 && kv->block_size > 0 && kv->block_size % 16 == 0 &&
-         (kv->hd == 64 || kv->hd == 96 || kv->hd == 128 || kv->hd == 256);
+bool cache_ok(const ZseKvQ8& kv) {
+  return kv.num_blocks > 0 && kv.nkv > 0 && kv.block_size > 0 && kv.block_size % 16 == 0 &&
+         (kv.hd == 64 || kv.hd == 96 || kv.hd == 128 || kv.hd == 256);
 }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 int sm_count() {
@@ -260,27 +260,28 @@ int sm_count() {
 
 using namespace zse;
 
-extern "C" int zse_rope_kv_write_q8(const ZseKvQ8* kv, const void* qkv, int ld, void* q_out, int ld_q, const void* planes,
-                                    int n_planes, const void* bias, const void* positions, const void* slots,
-                                    const void* inv_freq, int M, int nh, int rotary_dim, void* status, void* stream) {
-  if (M <= 0) return 0;
-  if (!cache_ok(kv) || nh <= 0 || rotary_dim < 0 || rotary_dim % 16 || rotary_dim > kv->hd || (planes == nullptr && qkv == nullptr))
+extern "C" int zse_rope_kv_write_q8(const ZseWriteQ8* w) {
+  const ZseKvQ8& kv = w->kv;
+  if (w->M <= 0) return 0;
+  if (!cache_ok(kv) || w->nh <= 0 || w->rotary_dim < 0 || w->rotary_dim % 16 || w->rotary_dim > kv.hd ||
+      (w->planes == nullptr && w->qkv == nullptr))
     return ZSE_ERR_SHAPE;
-  if (!aligned16(kv->data) || !aligned16(kv->scale) || !aligned16(q_out) || ld_q % 8 ||
-      (planes != nullptr ? !aligned16(planes) || (bias != nullptr && !aligned16(bias)) : !aligned16(qkv) || ld % 8))
+  if (!aligned16(kv.data) || !aligned16(kv.scale) || !aligned16(w->q_out) || w->ld_q % 8 ||
+      (w->planes != nullptr ? !aligned16(w->planes) || (w->bias != nullptr && !aligned16(w->bias)) : !aligned16(w->qkv) || w->ld % 8))
     return ZSE_ERR_ALIGN;
   auto go = [&](auto from_rows, auto from_planes, int lanes) {
-    const int rounds = (nh + 2 * kv->nkv + 256 / lanes - 1) / (256 / lanes);
-    return launch_pdl(planes != nullptr ? from_planes : from_rows, dim3(M, M < 2 * sm_count() ? rounds : 1), dim3(256), 0,
-                      static_cast<cudaStream_t>(stream), static_cast<const __half*>(qkv), ld, static_cast<__half*>(q_out), ld_q,
-                      static_cast<const float*>(planes), n_planes, static_cast<const __half*>(bias),
-                      static_cast<uint8_t*>(kv->data), static_cast<float*>(kv->scale), static_cast<const int*>(positions),
-                      static_cast<const long long*>(slots), static_cast<const float*>(inv_freq), nh, kv->nkv, rotary_dim,
-                      kv->block_size, (long long)kv->num_blocks * kv->block_size, static_cast<Status*>(status)) == cudaSuccess
-               ? 0
+    const int rounds = (w->nh + 2 * kv.nkv + 256 / lanes - 1) / (256 / lanes);
+    return launch_pdl(w->planes != nullptr ? from_planes : from_rows, dim3(w->M, w->M < 2 * sm_count() ? rounds : 1), dim3(256), 0,
+                      static_cast<cudaStream_t>(w->stream), static_cast<const __half*>(w->qkv), w->ld,
+                      static_cast<__half*>(w->q_out), w->ld_q, static_cast<const float*>(w->planes), w->n_planes,
+                      static_cast<const __half*>(w->bias), static_cast<uint8_t*>(kv.data), static_cast<float*>(kv.scale),
+                      static_cast<const int*>(w->positions), static_cast<const long long*>(w->slots),
+                      static_cast<const float*>(w->inv_freq), w->nh, kv.nkv, w->rotary_dim, kv.block_size,
+                      (long long)kv.num_blocks * kv.block_size, static_cast<Status*>(w->status)) == cudaSuccess
+               ? 1
                : ZSE_ERR_LAUNCH;
   };
-  switch (kv->hd) {
+  switch (kv.hd) {
     case 64: return go(rope_kv_write_q8_kernel<64, false>, rope_kv_write_q8_kernel<64, true>, kLanes<64>);
     case 96: return go(rope_kv_write_q8_kernel<96, false>, rope_kv_write_q8_kernel<96, true>, kLanes<96>);
     case 128: return go(rope_kv_write_q8_kernel<128, false>, rope_kv_write_q8_kernel<128, true>, kLanes<128>);
@@ -288,24 +289,24 @@ extern "C" int zse_rope_kv_write_q8(const ZseKvQ8* kv, const void* qkv, int ld, 
   }
 }
 
-extern "C" int zse_kv_read_q8(const ZseKvQ8* kv, const void* tables, int table_ld, int max_blocks, const void* seq_lens,
-                              const void* cu_blocks, int num_seqs, void* out, int out_blocks, void* out_tables, int out_table_ld,
-                              int out_max_blocks, void* status, void* stream) {
-  if (num_seqs <= 0) return 0;
-  if (!cache_ok(kv) || max_blocks < 0 || out_blocks < 0 || out_max_blocks < 0) return ZSE_ERR_SHAPE;
-  if (!aligned16(kv->data) || !aligned16(kv->scale) || !aligned16(out)) return ZSE_ERR_ALIGN;
-  const long long entries = ((long long)num_seqs * out_max_blocks + 255) / 256;
-  const int grid = int(std::max(1ll, std::min((long long)sm_count() * 8, std::max((long long)out_blocks, entries))));
+extern "C" int zse_kv_read_q8(const ZseReadQ8* r) {
+  const ZseKvQ8& kv = r->kv;
+  if (r->num_seqs <= 0) return 0;
+  if (!cache_ok(kv) || r->max_blocks < 0 || r->out_blocks < 0 || r->out_max_blocks < 0) return ZSE_ERR_SHAPE;
+  if (!aligned16(kv.data) || !aligned16(kv.scale) || !aligned16(r->out)) return ZSE_ERR_ALIGN;
+  const long long entries = ((long long)r->num_seqs * r->out_max_blocks + 255) / 256;
+  const int grid = int(std::max(1ll, std::min((long long)sm_count() * 8, std::max((long long)r->out_blocks, entries))));
   auto go = [&](auto kernel) {
-    return launch_pdl(kernel, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(kv->data),
-                      static_cast<const float*>(kv->scale), kv->num_blocks, kv->nkv, kv->block_size,
-                      static_cast<const int*>(tables), table_ld, max_blocks, static_cast<const int*>(seq_lens),
-                      static_cast<const int*>(cu_blocks), num_seqs, static_cast<__half*>(out), out_blocks,
-                      static_cast<int*>(out_tables), out_table_ld, out_max_blocks, static_cast<Status*>(status)) == cudaSuccess
-               ? 0
+    return launch_pdl(kernel, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(r->stream), static_cast<const uint8_t*>(kv.data),
+                      static_cast<const float*>(kv.scale), kv.num_blocks, kv.nkv, kv.block_size,
+                      static_cast<const int*>(r->tables), r->table_ld, r->max_blocks, static_cast<const int*>(r->seq_lens),
+                      static_cast<const int*>(r->cu_blocks), r->num_seqs, static_cast<__half*>(r->out), r->out_blocks,
+                      static_cast<int*>(r->out_tables), r->out_table_ld, r->out_max_blocks,
+                      static_cast<Status*>(r->status)) == cudaSuccess
+               ? 1
                : ZSE_ERR_LAUNCH;
   };
-  switch (kv->hd) {
+  switch (kv.hd) {
     case 64: return go(kv_read_q8_kernel<64>);
     case 96: return go(kv_read_q8_kernel<96>);
     case 128: return go(kv_read_q8_kernel<128>);

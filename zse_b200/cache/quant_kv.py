@@ -18,17 +18,18 @@ HEAD_DIMS = (64, 96, 128, 256)          # what the kernels are built for
 class QuantKV:
     """The whole cache (a leading ``layers`` dimension) or one layer of it; ``kv[i]`` is layer i."""
 
-    __slots__ = ("data", "scale", "_native")
+    __slots__ = ("data", "scale")
 
     def __init__(self, data: torch.Tensor, scale: torch.Tensor):
-        if data.dtype != torch.uint8 or scale.dtype != torch.float32:
+        if data.dtype is not torch.uint8 or scale.dtype is not torch.float32:
             raise TypeError(f"an 8-bit cache is uint8 data and float32 scales, not {data.dtype} and {scale.dtype}")
-        if data.dim() < 5 or data.shape[:-1] != scale.shape or data.shape[-4] != 2:
+        shape = data.shape
+        if len(shape) < 5 or shape[:-1] != scale.shape or shape[-4] != 2:
             raise ValueError(f"data [.., blocks, 2, kv heads, block size, head dim] and scales of its leading dimensions are "
-                             f"needed, not {tuple(data.shape)} and {tuple(scale.shape)}")
-        if data.device != scale.device:
+                             f"needed, not {tuple(shape)} and {tuple(scale.shape)}")
+        if data.get_device() != scale.get_device():
             raise ValueError(f"data on {data.device}, scales on {scale.device}")
-        self.data, self.scale, self._native = data, scale, None
+        self.data, self.scale = data, scale
 
     @classmethod
     def zeros(cls, shape: Tuple[int, ...], device=None) -> "QuantKV":
@@ -66,13 +67,6 @@ class QuantKV:
         """Copies a block of every layer."""
         self.data[:, dst].copy_(self.data[:, src])
         self.scale[:, dst].copy_(self.scale[:, src])
-
-    def native(self):
-        """The C description of this layer (made once; it holds pointers into the two tensors)."""
-        if self._native is None:
-            from ..ops import native
-            self._native = native.kv_q8(self)
-        return self._native
 
 
 def refuses(config, tp_size: int = 1) -> Optional[str]:

@@ -135,40 +135,44 @@ class TorchOps:
 
     # ---- 8-bit KV cache (cache.quant_kv.QuantKV, one layer) ----------------------------------------------
     @staticmethod
-    def _check_q8(kv, nh: int, nkv: int, hd: int, **tensors) -> None:
-        """``tensors``: name = (tensor or None, dtype, least number of dimensions)."""
-        if kv.data.dim() != 5 or (kv.kv_heads, kv.head_dim) != (nkv, hd):
-            raise ValueError(f"{nkv} kv heads of {hd} do not match one layer of a cache of shape {tuple(kv.shape)}")
+    def _check_q8(kv, nh: int, nkv: int, hd: int, *tensors) -> None:
+        """``tensors``: (name, tensor or None, dtype, number of dimensions)."""
+        shape = kv.data.shape
+        if len(shape) != 5 or shape[2] != nkv or shape[4] != hd:
+            raise ValueError(f"{nkv} kv heads of {hd} do not match one layer of a cache of shape {tuple(shape)}")
         if nkv < 1 or nh < 1 or nh % nkv:
             raise ValueError(f"{nh} heads over {nkv} kv heads")
-        dev = kv.data.device
-        for name, (t, dtype, dims) in tensors.items():
+        device = kv.data.get_device()
+        for name, t, dtype, dims in tensors:
             if t is None:
                 continue
-            if t.dtype != dtype or t.dim() < dims or (t.numel() and t.stride(-1) != 1):
+            strides = t.stride()
+            if t.dtype is not dtype or len(strides) != dims or (strides[-1] != 1 and t.shape[-1] > 1):
                 raise ValueError(f"{name}: {dtype} with {dims} dimensions and packed rows expected, not {t.dtype} "
-                                 f"{tuple(t.shape)} with strides {t.stride()}")
-            if t.device != dev:
-                raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
+                                 f"{tuple(t.shape)} with strides {strides}")
+            if t.get_device() != device:
+                raise ValueError(f"{name} is on {t.device}, the cache on {kv.data.device}")
 
     def _check_write_q8(self, qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out, planes, n_planes, bias):
         cols = (nh + 2 * nkv) * hd
-        self._check_q8(kv, nh, nkv, hd, qkv=(qkv, torch.float16, 2), q_out=(q_out, torch.float16, 2),
-                       planes=(planes, torch.float32, 1), bias=(bias, torch.float16, 1), positions=(positions, torch.int32, 1),
-                       slots=(slots, torch.int64, 1), inv_freq=(inv_freq, torch.float32, 1))
-        if M < 0 or positions.shape[0] < M or slots.shape[0] < M or q_out.shape[0] < M or q_out.shape[1] < nh * hd:
-            raise ValueError(f"{M} rows do not fit positions, slots or q_out {tuple(q_out.shape)}")
+        f16, f32 = torch.float16, torch.float32
+        self._check_q8(kv, nh, nkv, hd, ("qkv", qkv, f16, 2), ("q_out", q_out, f16, 2), ("bias", bias, f16, 1),
+                       ("positions", positions, torch.int32, 1), ("slots", slots, torch.int64, 1), ("inv_freq", inv_freq, f32, 1))
+        if q_out is None or M < 0 or positions.shape[0] < M or slots.shape[0] < M or q_out.shape[0] < M or q_out.shape[1] < nh * hd:
+            raise ValueError(f"{M} rows do not fit positions, slots or q_out")
         if planes is None:
             if qkv is None or qkv.shape[0] < M or qkv.shape[1] < cols:
                 raise ValueError(f"{M} rows of {cols} columns expected in qkv")
             if bias is not None:
                 raise ValueError("a bias goes with planes")
-        elif n_planes < 1 or planes.numel() < n_planes * M * cols or not planes.is_contiguous():
-            raise ValueError(f"{n_planes} planes of {M} rows of {cols} columns expected")
-        if bias is not None and bias.numel() < cols:
+        elif (n_planes < 1 or planes.dtype is not f32 or planes.numel() < n_planes * M * cols or not planes.is_contiguous()
+              or planes.get_device() != kv.data.get_device()):
+            raise ValueError(f"{n_planes} planes of {M} rows of {cols} columns expected, packed, beside the cache")
+        if bias is not None and bias.shape[0] < cols:
             raise ValueError(f"a bias of {cols} columns expected")
-        if 2 * inv_freq.numel() > hd or inv_freq.numel() % 8:
-            raise ValueError(f"{2 * inv_freq.numel()} rotated dimensions of {hd}: a multiple of 16 expected")
+        rot = 2 * inv_freq.shape[0]
+        if rot > hd or rot % 16:
+            raise ValueError(f"{rot} rotated dimensions of {hd}: a multiple of 16 expected")
 
     def rope_kv_write_q8(self, qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out=None, planes=None, n_planes=0,
                          bias=None):
@@ -189,13 +193,13 @@ class TorchOps:
         q_out[:M, : nh * hd] = ref.rope_kv_write_q8(x, kv, positions[:M], slots[:M], inv_freq, nh)
 
     def _check_read_q8(self, kv, block_tables, seq_lens, cu_blocks, S, out, out_tables):
-        self._check_q8(kv, kv.kv_heads, kv.kv_heads, kv.head_dim, block_tables=(block_tables, torch.int32, 2),
-                       seq_lens=(seq_lens, torch.int32, 1), cu_blocks=(cu_blocks, torch.int32, 1), out=(out, torch.float16, 5),
-                       out_tables=(out_tables, torch.int32, 2))
+        shape, i32 = kv.data.shape, torch.int32
+        self._check_q8(kv, shape[2], shape[2], shape[-1], ("block_tables", block_tables, i32, 2), ("seq_lens", seq_lens, i32, 1),
+                       ("cu_blocks", cu_blocks, i32, 1), ("out", out, torch.float16, 5), ("out_tables", out_tables, i32, 2))
         if S < 0 or min(block_tables.shape[0], seq_lens.shape[0], cu_blocks.shape[0] - 1, out_tables.shape[0]) < S:
             raise ValueError(f"tables, lengths and places of {S} sequences expected")
-        if out.shape[1:] != kv.shape[1:] or not out.is_contiguous():
-            raise ValueError(f"pages of {tuple(kv.shape[1:])} expected, not {tuple(out.shape)}")
+        if out.shape[1:] != shape[1:] or not out.is_contiguous():
+            raise ValueError(f"pages of {tuple(shape[1:])} expected, not {tuple(out.shape)}")
 
     def kv_read_q8(self, kv, block_tables, seq_lens, cu_blocks, S, out, out_tables):
         """Reads the first ``seq_lens[s]`` tokens of S sequences back as fp16 pages: block j of sequence s goes to
@@ -205,9 +209,10 @@ class TorchOps:
         ref.kv_read_q8(kv, block_tables[:S], seq_lens[:S], cu_blocks[: S + 1], out, out_tables)
 
     def _check_attn_q8(self, q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q):
-        self._check_q8(kv, nh, nkv, hd, q=(q, torch.float16, 2), out=(out, torch.float16, 2),
-                       block_tables=(block_tables, torch.int32, 2), seq_lens=(seq_lens, torch.int32, 1),
-                       cu_q=(cu_q, torch.int32, 1), q_pos0=(q_pos0, torch.int32, 1))
+        i32 = torch.int32
+        self._check_q8(kv, nh, nkv, hd, ("q", q, torch.float16, 2), ("out", out, torch.float16, 2),
+                       ("block_tables", block_tables, i32, 2), ("seq_lens", seq_lens, i32, 1), ("cu_q", cu_q, i32, 1),
+                       ("q_pos0", q_pos0, i32, 1))
         if nh // nkv > 16:
             raise ValueError(f"{nh // nkv} query heads per kv head: up to 16 expected")
         if S < 0 or block_tables.shape[0] < S or q.shape[1] < nh * hd or out.shape[1] < nh * hd or window < 0:

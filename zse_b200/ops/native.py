@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_uint64, c_void_p, POINTER, Structure, byref, c_uint32
 from typing import Optional
 
@@ -16,7 +17,7 @@ import torch
 from . import build as _build
 
 _ERRORS = {-1: "unsupported shape", -2: "misaligned pointer or stride", -3: "CUDA driver call failed",
-           -4: "kernel launch failed", -5: "size beyond a built-in limit"}
+           -4: "kernel launch failed", -5: "size beyond a built-in limit", -6: "scratch is missing or too small"}
 
 
 class NativeError(RuntimeError):
@@ -109,9 +110,11 @@ class Space(Structure):
                 ("state_ld", c_int32)] + [(n, c_void_p) for n in ("conv_w", "conv_b", "dt_bias", "neg_a", "skip")]
 
 
-class KvQ8(Structure):
-    _fields_ = [("data", c_void_p), ("scale", c_void_p)] + [(n, c_int32) for n in ("num_blocks", "nkv", "block_size", "hd")]
-
+# (the calls of the 8-bit cache pack their arguments into bytes of these layouts: a third of what a call of 22 arguments costs)
+_KV_Q8 = "QQiiii"
+_WRITE_Q8 = struct.Struct("<" + _KV_Q8 + "9Q6i")
+_READ_Q8 = struct.Struct("<" + _KV_Q8 + "7Q6i")
+_ATTN_Q8 = struct.Struct("<" + _KV_Q8 + "9Qq10ifi")
 
 _lib: Optional[ctypes.CDLL] = None
 
@@ -119,14 +122,11 @@ _SIGS = {
     "zse_gemm_w4": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                             c_void_p, c_void_p]),
     "zse_gemm_w4_splits": (c_int, [c_int, c_int, c_int, c_int]),
-    "zse_rope_kv_write_q8": (c_int, [POINTER(KvQ8), c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
-                                     c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
-    "zse_kv_read_q8": (c_int, [POINTER(KvQ8), c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int,
-                               c_int, c_void_p, c_void_p]),
-    "zse_attn_decode_q8_pieces": (c_int, [c_int] * 9),
-    "zse_attn_decode_q8_scratch_floats": (c_int64, [c_int] * 9),
-    "zse_attn_decode_q8": (c_int, [POINTER(KvQ8), c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
-                                   c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_float, c_int, c_void_p, c_void_p]),
+    "zse_rope_kv_write_q8": (c_int, [c_char_p]),
+    "zse_kv_read_q8": (c_int, [c_char_p]),
+    "zse_attn_decode_q8_pieces": (c_int, [c_char_p]),
+    "zse_attn_decode_q8_scratch_floats": (c_int64, [c_char_p]),
+    "zse_attn_decode_q8": (c_int, [c_char_p]),
     "zse_gemm_w8": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                             c_void_p, c_void_p]),
     "zse_gemm_w8_splits": (c_int, [c_int, c_int, c_int, c_int]),
@@ -525,54 +525,72 @@ def rope_kv_write(qkv, kv_layer, positions, slots, inv_freq, M, nh, nkv, hd, rot
                                  rotary_dim, block_size, _p(planes), n_planes, _p(bias), _stream()), "rope_kv_write")
 
 
-def kv_q8(kv) -> KvQ8:
-    """One layer of an 8-bit cache (``cache.quant_kv.QuantKV``) as the kernels take it."""
-    if not (kv.data.is_contiguous() and kv.scale.is_contiguous()):
-        raise NativeError("a layer of an 8-bit cache has to be contiguous")
-    if kv.data.device.type != "cuda":
-        raise NativeError(f"the cache is on {kv.data.device}")
-    return KvQ8(_p(kv.data), _p(kv.scale), kv.num_blocks, kv.kv_heads, kv.block_size, kv.head_dim)
-
-
-def _stream_of(kv) -> int:
-    """The current stream of the cache's device, which has to be the current device.  (The two calls below the public ones:
-    ``torch.cuda.current_stream()`` makes a stream object every time and takes longer than everything else in a call here.)"""
+# ---- 8-bit KV cache: ``kv`` is one layer of a ``cache.quant_kv.QuantKV``; every call gives the number of kernels it launched -------
+def _cache_q8(kv) -> tuple:
+    """The layer's address and sizes, and the current stream of its device, which has to be the current device.  (The two calls
+    below the public ones: ``torch.cuda.current_stream()`` makes a stream object and takes longer than the rest of a call here.)"""
+    data, scale = kv.data, kv.scale
     at = torch._C._cuda_getDevice()
-    if kv.data.device.index != at:
-        raise NativeError(f"the cache is on {kv.data.device}, the current device is {at}")
-    return torch._C._cuda_getCurrentRawStream(at)
+    if data.get_device() != at:
+        raise NativeError(f"the cache is on {data.device}, the current device is {at}")
+    if not (data.is_contiguous() and scale.is_contiguous()):
+        raise NativeError("a layer of an 8-bit cache has to be contiguous")
+    blocks, _, nkv, block_size, hd = data.shape
+    return (data.data_ptr(), scale.data_ptr(), blocks, nkv, block_size, hd), torch._C._cuda_getCurrentRawStream(at)
+
+
+def _launched(n: int, what: str) -> None:
+    if n < 0:
+        raise NativeError(f"{what}: {_ERRORS.get(n, n)}")
+    LAUNCHES[0] += n
 
 
 def rope_kv_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, q_out, planes, n_planes, bias, status):
-    stream = _stream_of(kv)
-    _ck(load().zse_rope_kv_write_q8(byref(kv.native()), _p(qkv), 0 if qkv is None else qkv.stride(0), _p(q_out), q_out.stride(0),
-                                    _p(planes), n_planes, _p(bias), _p(positions), _p(slots), _p(inv_freq), M, nh,
-                                    inv_freq.numel() * 2, status, stream), "rope_kv_write_q8")
+    cache, stream = _cache_q8(kv)
+    _launched(load().zse_rope_kv_write_q8(_WRITE_Q8.pack(
+        *cache, 0 if qkv is None else qkv.data_ptr(), q_out.data_ptr(), 0 if planes is None else planes.data_ptr(),
+        0 if bias is None else bias.data_ptr(), positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(), status, stream,
+        0 if qkv is None else qkv.stride(0), q_out.stride(0), n_planes, M, nh, 2 * inv_freq.shape[0])), "rope_kv_write_q8")
 
 
 def kv_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables, status):
-    stream = _stream_of(kv)
-    _ck(load().zse_kv_read_q8(byref(kv.native()), _p(block_tables), block_tables.stride(0), block_tables.shape[1], _p(seq_lens),
-                              _p(cu_blocks), S, _p(out), out.shape[0], _p(out_tables), out_tables.stride(0),
-                              out_tables.shape[1], status, stream), "kv_read_q8")
+    cache, stream = _cache_q8(kv)
+    _launched(load().zse_kv_read_q8(_READ_Q8.pack(
+        *cache, block_tables.data_ptr(), seq_lens.data_ptr(), cu_blocks.data_ptr(), out.data_ptr(), out_tables.data_ptr(), status,
+        stream, block_tables.stride(0), block_tables.shape[1], S, out.shape[0], out_tables.stride(0), out_tables.shape[1])),
+        "kv_read_q8")
 
 
-def attn_decode_q8_scratch_floats(S, max_q, nh, nkv, hd, block_size, max_blocks, window=0, num_splits=0) -> int:
-    """fp32 values of scratch that ``attn_decode_q8`` needs for such a call (0: none)."""
-    return load().zse_attn_decode_q8_scratch_floats(S, max_q, nh, nkv, hd, block_size, max_blocks, window, num_splits)
+def _attn_q8_args(cache, stream, q, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch, num_splits, scale, window,
+                  status) -> bytes:
+    return _ATTN_Q8.pack(
+        *cache, q.data_ptr(), block_tables.data_ptr(), 0 if seq_lens is None else seq_lens.data_ptr(),
+        0 if cu_q is None else cu_q.data_ptr(), 0 if q_pos0 is None else q_pos0.data_ptr(), out.data_ptr(),
+        0 if scratch is None else scratch.data_ptr(), status, stream, 0 if scratch is None else scratch.numel(), q.stride(0),
+        out.stride(0), min(q.shape[0], out.shape[0]), block_tables.stride(0), block_tables.shape[1], S, max_q, nh, num_splits, window,
+        scale, 0)
 
 
 def attn_decode_q8(q, kv, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch, num_splits, scale, window, status):
-    """``scratch``: fp32, ``attn_decode_q8_scratch_floats`` of it, or None (then the call allocates what it needs)."""
-    stream = _stream_of(kv)
-    max_blocks = block_tables.shape[1]
-    n = attn_decode_q8_scratch_floats(S, max_q, nh, kv.kv_heads, kv.head_dim, kv.block_size, max_blocks, window, num_splits)
-    if n and scratch is None:
-        scratch = torch.empty(n, dtype=torch.float32, device=kv.device)
-    _ck(load().zse_attn_decode_q8(byref(kv.native()), _p(q), q.stride(0), min(q.shape[0], out.shape[0]), _p(block_tables),
-                                  block_tables.stride(0), max_blocks, _p(seq_lens), _p(cu_q), _p(q_pos0), S, max_q, _p(out), out.stride(0), nh,
-                                  _p(scratch), 0 if scratch is None else scratch.numel(), num_splits, float(scale), int(window),
-                                  status, stream), "attn_decode_q8", 2 if n else 1)
+    """``scratch``: fp32, ``attn_decode_q8_scratch_floats`` of it, or None (then a call that needs some allocates it)."""
+    lib = load()
+    cache, stream = _cache_q8(kv)
+    n = lib.zse_attn_decode_q8(_attn_q8_args(cache, stream, q, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch,
+                                             num_splits, scale, window, status))
+    if n == -6 and scratch is None:
+        args = (cache, stream, q, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh)
+        need = lib.zse_attn_decode_q8_scratch_floats(_attn_q8_args(*args, None, num_splits, scale, window, status))
+        scratch = torch.empty(need, dtype=torch.float32, device=kv.device)
+        n = lib.zse_attn_decode_q8(_attn_q8_args(*args, scratch, num_splits, scale, window, status))
+    _launched(n, "attn_decode_q8")
+
+
+def attn_decode_q8_plan(S, max_q, nh, nkv, hd, block_size, max_blocks, window=0, num_splits=0) -> tuple:
+    """(pieces of a sequence and kv head, fp32 values of scratch) of such a call."""
+    lib = load()
+    args = _ATTN_Q8.pack(0, 0, 1, nkv, block_size, hd, 0, 0, 0, max_q > 1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, max_blocks, S, max_q, nh,
+                         num_splits, window, 1.0, 0)
+    return lib.zse_attn_decode_q8_pieces(args), lib.zse_attn_decode_q8_scratch_floats(args)
 
 
 def headnorm_rope_kv_write(qkv, kv_layer, positions, slots, freqs, q_norm_w, k_norm_w, norm_v, k_is_v, eps, M, nh, nkv,
