@@ -578,12 +578,22 @@ Plan plan_of(const ZseAttnQ8& a) {
   p.rows_per = std::max(1, 8 * p.nb / G);
   p.row_groups = (a.max_q + p.rows_per - 1) / p.rows_per;
   const long long items = (long long)a.num_seqs * a.kv.nkv * p.row_groups;
+  // Pieces: what fits the GPU at a time (CTAs an SM by registers and shared memory; an eighth less, for clusters need neighbouring
+  // places), at least half a tile a warp.  Measured (HD 128, us by pieces): 1 x 1000 tokens of 8 kv heads 1: 10.5, 4: 5.6, 8: 4.8; 32 x 500
+  // 1: 14.9, 2: 12.6, 4: 16.0; 64 x 6001..8190 1: 157, 2: 148 - a second wave pays where a warp still has 32 tiles of it.  Several
+  // clusters (and the launch that joins them) where eight pieces leave a warp 12 tiles: 1 x 4000 of 4 kv heads 8: 7.9, 32: 7.3; 1 x
+  // 32765 8: 36, 64: 14.9, 112: 14.3.
   long long want = a.num_splits;
   if (want <= 0) {
-    long long tokens = (long long)a.max_blocks * a.kv.block_size;
-    if (a.window > 0) tokens = std::min(tokens, (long long)a.window + a.max_q + 16);
-    const long long most = std::max(1ll, tokens / 64);                 // a tile for every warp of a piece
-    want = std::min(most, (2ll * sm_count() + items - 1) / items);
+    long long tiles = (long long)a.max_blocks * (a.kv.block_size / 16);
+    if (a.window > 0) tiles = std::min(tiles, ((long long)a.window + a.max_q) / 16 + 2);
+    const int per_sm = a.kv.hd > 128 ? (p.nb == 1 ? 2 : 1) : p.nb == 1 ? 4 : p.nb == 2 ? 3 : 2;
+    const long long room = std::max(1ll, (long long)sm_count() * per_sm * 7 / 8 / items);
+    want = 1;
+    while (want < kMostCluster && want * 2 <= room && want * 2 <= (tiles + 1) / 2) want *= 2;
+    if (want < kMostCluster && want * 2 > room && tiles >= want * 2 * kWarps * 32) want *= 2;
+    if (want == kMostCluster && room > kMostCluster && tiles >= kMostCluster * kWarps * 12)
+      want = std::max(want, std::min(room, tiles / (4 * kWarps)) / kMostCluster * kMostCluster);
   }
   p.cluster = 1;
   while (p.cluster < want && p.cluster < kMostCluster) p.cluster *= 2;

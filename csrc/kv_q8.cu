@@ -54,123 +54,185 @@ __device__ __forceinline__ uint4 pack8(const float* x) {
 template <int HD>
 constexpr int kLanes = HD <= 64 ? 4 : HD <= 128 ? 8 : 16;      // threads of a head, a power of two; HD / 16 of them work
 
-// A CTA has one token and blockIdx.y's share of its heads; a thread has 16 elements of a head, two runs of eight that rotate with
-// each other (or neighbouring runs of the part that does not rotate), in 16-byte accesses.  Angles are products in 64 bits brought
-// into one turn, so a rotation is as exact at position 10^9 as at 0; they are computed once per CTA, behind the first loads.
-template <int HD, bool PLANES>
+// What the two write kernels do with a head of a token: a thread has 16 of its elements, two runs of eight that rotate with each
+// other (or neighbouring runs of the part that does not rotate).
+struct Write {
+  __half* q_out;
+  uint8_t* data;
+  float* scale;
+  int ld_q, nh, nkv;
+};
+template <int HD>
+struct Lane {
+  static constexpr int L = kLanes<HD>;
+  int c, ia, ib;                                                       // of a head's threads; first elements of the two runs
+  bool works, turns;
+  __device__ __forceinline__ explicit Lane(int rot) {
+    c = threadIdx.x % L;
+    works = c < HD / 16;
+    turns = works && c < rot / 16;
+    ia = turns ? c * 8 : works ? rot + (c - rot / 16) * 16 : 0;
+    ib = turns ? rot / 2 + c * 8 : ia + 8;
+  }
+};
+// `stored`: the cache row of K head 0 of the token, or -1; the whole warp calls it (live: this thread has something)
+template <int HD>
+__device__ __forceinline__ void put_head(const Write& w, const Lane<HD>& lane, float* a, float* b, const float* sn, const float* cs,
+                                         bool live, int t, int head, long long stored, int block_size) {
+  if (live && lane.turns && head < w.nh + w.nkv) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = a[j], y = b[j], s = sn[lane.c * 8 + j], c = cs[lane.c * 8 + j];
+      a[j] = x * c - y * s;
+      b[j] = y * c + x * s;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a[j] = clamp_nan(a[j]), b[j] = clamp_nan(b[j]);
+  const bool cached = live && head >= w.nh && stored >= 0;
+  if (__any_sync(0xffffffffu, cached)) {
+    float top = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max_nan(top, max_nan(fabsf(a[j]), fabsf(b[j])));
+#pragma unroll
+    for (int o = 1; o < Lane<HD>::L; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (cached) {
+      const bool none = top <= 1e-30f;
+      const float steps = none ? 0.f : __fdiv_rn(127.f, top);
+      const size_t row = size_t(stored) + size_t(head - w.nh) * block_size;            // K heads, then V heads
+      uint8_t* dst = w.data + row * HD;
+      *reinterpret_cast<uint2*>(dst + lane.ia) = quantise8(a, steps);
+      *reinterpret_cast<uint2*>(dst + lane.ib) = quantise8(b, steps);
+      if (lane.c == 0) w.scale[row] = none ? 0.f : __fdiv_rn(top, 127.f);
+    }
+  }
+  if (live && head < w.nh) {
+    __half* dst = w.q_out + size_t(t) * w.ld_q + size_t(head) * HD;
+    *reinterpret_cast<uint4*>(dst + lane.ia) = pack8(a);
+    *reinterpret_cast<uint4*>(dst + lane.ib) = pack8(b);
+  }
+}
+// Sine and cosine of a token's angle for pair i: the product in 64 bits, brought into one turn, so that a rotation is as exact at
+// position 10^9 as at 0.
+__device__ __forceinline__ void turn_of(int position, float freq, float* s, float* c) {
+  const double turn = double(position) * double(freq), n = rint(turn * (1.0 / kTurn));
+  sincosf(float(fma(-n, kTurnLow, fma(-n, kTurn, turn))), s, c);
+}
+// The cache row of K head 0 of a slot, or -1.
+__device__ __forceinline__ long long row_of_slot(long long slot, int t, int nkv, int block_size, long long num_slots, Status* st) {
+  if (slot >= num_slots) {
+    report(st, kBadArgument, 70, unsigned(t));
+    return -1;
+  }
+  if (slot < 0) return -1;
+  const long long blk = slot / block_size;
+  return blk * 2 * nkv * block_size + (slot - blk * block_size);
+}
+
+// Rows of fp16.  A CTA has `tokens` neighbouring tokens: their angles (one per thread), then their heads, each thread's next 32 bytes
+// loaded before those at hand are turned.  With one token a CTA (48 heads of 64 are 3 KB) it is all start: 8080 such tokens took 34 us.
+template <int HD>
 __global__ void __launch_bounds__(256)
-rope_kv_write_q8_kernel(const __half* qkv, int ld, __half* q_out, int ld_q, const float* __restrict__ planes, int n_planes,
-                        const __half* __restrict__ bias, uint8_t* __restrict__ data, float* __restrict__ scale,
-                        const int* __restrict__ positions, const long long* __restrict__ slots,
-                        const float* __restrict__ inv_freq, int nh, int nkv, int rot, int block_size, long long num_slots,
-                        Status* st) {
+rope_kv_write_q8_kernel(const __half* qkv, int ld, Write w, const int* __restrict__ positions, const long long* __restrict__ slots,
+                        const float* __restrict__ inv_freq, int M, int tokens, int rot, int block_size, long long num_slots, Status* st) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int L = kLanes<HD>;
-  constexpr int kHeads = 256 / L;
-  constexpr int kPlanes = 4;                                           // loaded before the first of them is added
-  __shared__ __align__(16) float sin_t[HD / 2], cos_t[HD / 2];
-  const int t = blockIdx.x, M = gridDim.x, half = rot / 2;
-  const int c = threadIdx.x % L;
-  const bool works = c < HD / 16, turns = works && c < rot / 16;
-  const int ia = turns ? c * 8 : works ? rot + (c - rot / 16) * 16 : 0, ib = turns ? half + c * 8 : ia + 8;
-  const int heads = nh + 2 * nkv, cols = heads * HD;
-  float a[8], b[8];
-  auto load = [&](int head) {
-    if constexpr (PLANES) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.f;
-      if (bias != nullptr) {
-        unpack8(*reinterpret_cast<const uint4*>(bias + head * HD + ia), a);
-        unpack8(*reinterpret_cast<const uint4*>(bias + head * HD + ib), b);
-      }
-      const float* src = planes + size_t(t) * cols + size_t(head) * HD;
-      const size_t step = size_t(M) * cols;
-      for (int p = 0; p < n_planes; p += kPlanes) {
-        float4 x[kPlanes][4];
-#pragma unroll
-        for (int k = 0; k < kPlanes; ++k)
-          if (p + k < n_planes) {
-            const float* from = src + (p + k) * step;
-            x[k][0] = __ldcs(reinterpret_cast<const float4*>(from + ia));
-            x[k][1] = __ldcs(reinterpret_cast<const float4*>(from + ia + 4));
-            x[k][2] = __ldcs(reinterpret_cast<const float4*>(from + ib));
-            x[k][3] = __ldcs(reinterpret_cast<const float4*>(from + ib + 4));
-          }
-#pragma unroll
-        for (int k = 0; k < kPlanes; ++k)
-          if (p + k < n_planes) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              a[e] += (&x[k][0].x)[e];
-              a[4 + e] += (&x[k][1].x)[e];
-              b[e] += (&x[k][2].x)[e];
-              b[4 + e] += (&x[k][3].x)[e];
-            }
-          }
-      }
-    } else {
-      const __half* src = qkv + size_t(t) * ld + size_t(head) * HD;
-      unpack8(*reinterpret_cast<const uint4*>(src + ia), a);
-      unpack8(*reinterpret_cast<const uint4*>(src + ib), b);
+  constexpr int kGroups = 256 / kLanes<HD>, kMost = 16;
+  __shared__ float sin_t[256], cos_t[256];                             // [token][rot / 2]
+  __shared__ long long stored[kMost];
+  const Lane<HD> lane(rot);
+  const int half = rot / 2, heads = w.nh + 2 * w.nkv, t0 = blockIdx.x * tokens, n = min(tokens, M - t0);
+  // this thread's heads: every kGroups-th of the tokens' heads in a row (with gridDim.y > 1: of one token, its share)
+  int head = blockIdx.y * kGroups + threadIdx.x / kLanes<HD>, t = 0;
+  const int step = gridDim.y * kGroups;
+  uint4 va = make_uint4(0, 0, 0, 0), vb = va;
+  auto fetch = [&]() {
+    while (head >= heads && t < n) head -= heads, ++t;
+    if (t < n && lane.works) {
+      const __half* src = qkv + size_t(t0 + t) * ld + size_t(head) * HD;
+      va = *reinterpret_cast<const uint4*>(src + lane.ia);
+      vb = *reinterpret_cast<const uint4*>(src + lane.ib);
     }
   };
-  int head = blockIdx.y * kHeads + threadIdx.x / L;
-  bool live = works && head < heads;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.f;
-  if (live) load(head);
-  long long slot = slots[t];
-  if (threadIdx.x < half) {
-    const double turn = double(positions[t]) * double(inv_freq[threadIdx.x]);
-    const double n = rint(turn * (1.0 / kTurn));
-    sincosf(float(fma(-n, kTurnLow, fma(-n, kTurn, turn))), &sin_t[threadIdx.x], &cos_t[threadIdx.x]);
+  if (gridDim.y > 1 && head >= heads) t = n;
+  fetch();
+  for (int i = threadIdx.x; i < n * half; i += 256) {
+    const int k = i / half;
+    turn_of(positions[t0 + k], inv_freq[i - k * half], &sin_t[i], &cos_t[i]);
   }
-  if (slot >= num_slots) {
-    if (threadIdx.x == 0 && blockIdx.y == 0) report(st, kBadArgument, 70, unsigned(t));
-    slot = -1;
-  }
-  const long long blk = slot >= 0 ? slot / block_size : 0;
-  const int off = slot >= 0 ? int(slot - blk * block_size) : 0;
+  if (threadIdx.x < n) stored[threadIdx.x] = row_of_slot(slots[t0 + threadIdx.x], t0 + threadIdx.x, w.nkv, block_size, num_slots, st);
   __syncthreads();
-  float sn[8], cs[8];
+  while (__any_sync(0xffffffffu, t < n)) {
+    const int now = t, at = head;
+    const bool live = t < n && lane.works;
+    float a[8], b[8];
+    unpack8(va, a);
+    unpack8(vb, b);
+    head += step;
+    if (gridDim.y > 1 && head >= heads) t = n;
+    fetch();
+    put_head<HD>(w, lane, a, b, sin_t + now * half, cos_t + now * half, live, t0 + now, at, live ? stored[now] : -1, block_size);
+  }
+}
+
+// Sums of planes (few rows: a decode step).  A CTA has one token and blockIdx.y's share of its heads; four planes are loaded before the
+// first is added.
+template <int HD>
+__global__ void __launch_bounds__(256)
+rope_kv_write_q8_planes_kernel(const float* __restrict__ planes, int n_planes, const __half* __restrict__ bias, Write w,
+                               const int* __restrict__ positions, const long long* __restrict__ slots,
+                               const float* __restrict__ inv_freq, int rot, int block_size, long long num_slots, Status* st) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int kHeads = 256 / kLanes<HD>, kPlanes = 4;
+  __shared__ float sin_t[HD / 2], cos_t[HD / 2];
+  __shared__ long long stored;
+  const Lane<HD> lane(rot);
+  const int t = blockIdx.x, M = gridDim.x, heads = w.nh + 2 * w.nkv, cols = heads * HD;
+  float a[8], b[8];
+  auto load = [&](int head) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) sn[j] = turns ? sin_t[c * 8 + j] : 0.f, cs[j] = turns ? cos_t[c * 8 + j] : 1.f;
+    for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.f;
+    if (!lane.works || head >= heads) return;
+    if (bias != nullptr) {
+      unpack8(*reinterpret_cast<const uint4*>(bias + head * HD + lane.ia), a);
+      unpack8(*reinterpret_cast<const uint4*>(bias + head * HD + lane.ib), b);
+    }
+    const float* src = planes + size_t(t) * cols + size_t(head) * HD;
+    const size_t next = size_t(M) * cols;
+    for (int p = 0; p < n_planes; p += kPlanes) {
+      float4 x[kPlanes][4];
+#pragma unroll
+      for (int k = 0; k < kPlanes; ++k)
+        if (p + k < n_planes) {
+          const float* from = src + (p + k) * next;
+          x[k][0] = __ldcs(reinterpret_cast<const float4*>(from + lane.ia));
+          x[k][1] = __ldcs(reinterpret_cast<const float4*>(from + lane.ia + 4));
+          x[k][2] = __ldcs(reinterpret_cast<const float4*>(from + lane.ib));
+          x[k][3] = __ldcs(reinterpret_cast<const float4*>(from + lane.ib + 4));
+        }
+#pragma unroll
+      for (int k = 0; k < kPlanes; ++k)
+        if (p + k < n_planes) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            a[e] += (&x[k][0].x)[e];
+            a[4 + e] += (&x[k][1].x)[e];
+            b[e] += (&x[k][2].x)[e];
+            b[4 + e] += (&x[k][3].x)[e];
+          }
+        }
+    }
+  };
+  int head = blockIdx.y * kHeads + threadIdx.x / kLanes<HD>;
+  load(head);
+  if (threadIdx.x < rot / 2) turn_of(positions[t], inv_freq[threadIdx.x], &sin_t[threadIdx.x], &cos_t[threadIdx.x]);
+  if (threadIdx.x == 0) stored = row_of_slot(slots[t], t, w.nkv, block_size, num_slots, st);
+  __syncthreads();
   for (int base = blockIdx.y * kHeads; base < heads; base += gridDim.y * kHeads) {     // the same rounds for the whole CTA
-    if (live && head < nh + nkv) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x = a[j], y = b[j];
-        a[j] = x * cs[j] - y * sn[j];
-        b[j] = y * cs[j] + x * sn[j];
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = clamp_nan(a[j]), b[j] = clamp_nan(b[j]);
-    if (base + kHeads > nh) {                                                          // some head here is a key or a value
-      float top = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max_nan(top, max_nan(fabsf(a[j]), fabsf(b[j])));
-#pragma unroll
-      for (int o = 1; o < L; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (live && head >= nh && slot >= 0) {
-        const bool none = top <= 1e-30f;
-        const float steps = none ? 0.f : __fdiv_rn(127.f, top);
-        const size_t row = ((size_t(blk) * 2) * nkv + (head - nh)) * block_size + off;  // K heads, then V heads
-        uint8_t* dst = data + row * HD;
-        *reinterpret_cast<uint2*>(dst + ia) = quantise8(a, steps);
-        *reinterpret_cast<uint2*>(dst + ib) = quantise8(b, steps);
-        if (c == 0) scale[row] = none ? 0.f : __fdiv_rn(top, 127.f);
-      }
-    }
-    if (live && head < nh) {
-      __half* dst = q_out + size_t(t) * ld_q + size_t(head) * HD;
-      *reinterpret_cast<uint4*>(dst + ia) = pack8(a);
-      *reinterpret_cast<uint4*>(dst + ib) = pack8(b);
-    }
+    put_head<HD>(w, lane, a, b, sin_t, cos_t, lane.works && head < heads, t, head, stored, block_size);
     head += gridDim.y * kHeads;
-    live = works && head < heads;
-    if (live) load(head);
+    load(head);
   }
 }
 
@@ -269,23 +331,35 @@ extern "C" int zse_rope_kv_write_q8(const ZseWriteQ8* w) {
   if (!aligned16(kv.data) || !aligned16(kv.scale) || !aligned16(w->q_out) || w->ld_q % 8 ||
       (w->planes != nullptr ? !aligned16(w->planes) || (w->bias != nullptr && !aligned16(w->bias)) : !aligned16(w->qkv) || w->ld % 8))
     return ZSE_ERR_ALIGN;
+  const Write to{static_cast<__half*>(w->q_out), static_cast<uint8_t*>(kv.data), static_cast<float*>(kv.scale), w->ld_q, w->nh, kv.nkv};
+  const long long num_slots = (long long)kv.num_blocks * kv.block_size;
+  const auto* positions = static_cast<const int*>(w->positions);
+  const auto* slots = static_cast<const long long*>(w->slots);
+  const auto* freqs = static_cast<const float*>(w->inv_freq);
+  auto* status = static_cast<Status*>(w->status);
+  const cudaStream_t st = static_cast<cudaStream_t>(w->stream);
   auto go = [&](auto from_rows, auto from_planes, int lanes) {
-    const int rounds = (w->nh + 2 * kv.nkv + 256 / lanes - 1) / (256 / lanes);
-    return launch_pdl(w->planes != nullptr ? from_planes : from_rows, dim3(w->M, w->M < 2 * sm_count() ? rounds : 1), dim3(256), 0,
-                      static_cast<cudaStream_t>(w->stream), static_cast<const __half*>(w->qkv), w->ld,
-                      static_cast<__half*>(w->q_out), w->ld_q, static_cast<const float*>(w->planes), w->n_planes,
-                      static_cast<const __half*>(w->bias), static_cast<uint8_t*>(kv.data), static_cast<float*>(kv.scale),
-                      static_cast<const int*>(w->positions), static_cast<const long long*>(w->slots),
-                      static_cast<const float*>(w->inv_freq), w->nh, kv.nkv, w->rotary_dim, kv.block_size,
-                      (long long)kv.num_blocks * kv.block_size, static_cast<Status*>(w->status)) == cudaSuccess
-               ? 1
-               : ZSE_ERR_LAUNCH;
+    const int rounds = (w->nh + 2 * kv.nkv) * lanes / 256 + ((w->nh + 2 * kv.nkv) * lanes % 256 > 0);
+    cudaError_t e;
+    if (w->planes != nullptr) {
+      e = launch_pdl(from_planes, dim3(w->M, w->M < 2 * sm_count() ? rounds : 1), dim3(256), 0, st,
+                     static_cast<const float*>(w->planes), w->n_planes, static_cast<const __half*>(w->bias), to, positions, slots,
+                     freqs, w->rotary_dim, kv.block_size, num_slots, status);
+    } else {
+      // as many tokens a CTA as its threads have angles, while three CTAs an SM are left; few tokens: a CTA per 256 threads' worth of heads
+      int tokens = 1;
+      while (tokens < 16 && tokens * 2 * std::max(w->rotary_dim / 2, 1) <= 256 && w->M / (tokens * 2) >= 3 * sm_count()) tokens *= 2;
+      e = launch_pdl(from_rows, dim3((w->M + tokens - 1) / tokens, w->M < 2 * sm_count() ? rounds : 1), dim3(256), 0, st,
+                     static_cast<const __half*>(w->qkv), w->ld, to, positions, slots, freqs, w->M, tokens, w->rotary_dim,
+                     kv.block_size, num_slots, status);
+    }
+    return e == cudaSuccess ? 1 : ZSE_ERR_LAUNCH;
   };
   switch (kv.hd) {
-    case 64: return go(rope_kv_write_q8_kernel<64, false>, rope_kv_write_q8_kernel<64, true>, kLanes<64>);
-    case 96: return go(rope_kv_write_q8_kernel<96, false>, rope_kv_write_q8_kernel<96, true>, kLanes<96>);
-    case 128: return go(rope_kv_write_q8_kernel<128, false>, rope_kv_write_q8_kernel<128, true>, kLanes<128>);
-    default: return go(rope_kv_write_q8_kernel<256, false>, rope_kv_write_q8_kernel<256, true>, kLanes<256>);
+    case 64: return go(rope_kv_write_q8_kernel<64>, rope_kv_write_q8_planes_kernel<64>, kLanes<64>);
+    case 96: return go(rope_kv_write_q8_kernel<96>, rope_kv_write_q8_planes_kernel<96>, kLanes<96>);
+    case 128: return go(rope_kv_write_q8_kernel<128>, rope_kv_write_q8_planes_kernel<128>, kLanes<128>);
+    default: return go(rope_kv_write_q8_kernel<256>, rope_kv_write_q8_planes_kernel<256>, kLanes<256>);
   }
 }
 

@@ -575,13 +575,13 @@ def attn_decode_q8(q, kv, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, n
     """``scratch``: fp32, ``attn_decode_q8_scratch_floats`` of it, or None (then a call that needs some allocates it)."""
     lib = load()
     cache, stream = _cache_q8(kv)
-    n = lib.zse_attn_decode_q8(_attn_q8_args(cache, stream, q, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch,
-                                             num_splits, scale, window, status))
-    if n == -6 and scratch is None:
-        args = (cache, stream, q, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh)
-        need = lib.zse_attn_decode_q8_scratch_floats(_attn_q8_args(*args, None, num_splits, scale, window, status))
-        scratch = torch.empty(need, dtype=torch.float32, device=kv.device)
-        n = lib.zse_attn_decode_q8(_attn_q8_args(*args, scratch, num_splits, scale, window, status))
+    args = _attn_q8_args(cache, stream, q, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch, num_splits, scale,
+                         window, status)
+    n = lib.zse_attn_decode_q8(args)
+    if n == -6 and scratch is None:                    # nothing was launched
+        scratch = torch.empty(lib.zse_attn_decode_q8_scratch_floats(args), dtype=torch.float32, device=kv.data.device)
+        n = lib.zse_attn_decode_q8(_attn_q8_args(cache, stream, q, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch,
+                                                 num_splits, scale, window, status))
     _launched(n, "attn_decode_q8")
 
 
