@@ -2,7 +2,9 @@
 //
 //   s[t][c] = scale * kscale[t] * (sum_d q[c][d] (uk[t][d] - 128)),   o[c][d] = sum_t p[t][c] vscale[t] (uv[t][d] - 128) / sum_t p[t][c]
 //
-// An item is one kv head of one sequence with up to 8 * NB columns c: query heads of the group, times rows of a draft.  Its tokens are
+// An item is one kv head of one sequence with up to 8 or 16 columns c: query heads of the group, times rows of a draft (more rows
+// are more items, which read the keys and values again, from L2: with 32 columns a warp needs 240 registers, and 32 drafts of up to five
+// rows of 40 heads over 2001 to 4094 tokens took 78 us instead of 66).  Its tokens are
 // cut into pieces, one per CTA; four warps of a CTA take every fourth tile of 16 tokens through rings of their own (cp.async) and
 // keep a running maximum, sum and output in registers.  Tokens are the 16 rows of the products, columns their 8 columns.
 //
@@ -126,7 +128,7 @@ struct Q8Smem {
 };
 
 template <int HD, int NB>
-__global__ void __launch_bounds__(kWarps * 32, NB == 1 && HD <= 128 ? 4 : NB == 2 && HD <= 128 ? 3 : 1)
+__global__ void __launch_bounds__(kWarps * 32, HD > 128 ? 1 : NB == 1 ? 4 : 3)
 attn_q8_kernel(const Q8Args a) {
   using S = Q8Smem<HD, NB>;
   constexpr int kChunks = HD / 16;                                     // 16-byte chunks of a row, and 16-wide steps of the products
@@ -574,7 +576,7 @@ struct Plan {
 Plan plan_of(const ZseAttnQ8& a) {
   Plan p;
   const int G = a.nh / a.kv.nkv;
-  p.nb = a.max_q * G <= 8 ? 1 : a.max_q * G <= 16 || a.kv.hd > 128 ? 2 : 4;
+  p.nb = a.max_q * G <= 8 ? 1 : 2;
   p.rows_per = std::max(1, 8 * p.nb / G);
   p.row_groups = (a.max_q + p.rows_per - 1) / p.rows_per;
   const long long items = (long long)a.num_seqs * a.kv.nkv * p.row_groups;
@@ -587,7 +589,7 @@ Plan plan_of(const ZseAttnQ8& a) {
   if (want <= 0) {
     long long tiles = (long long)a.max_blocks * (a.kv.block_size / 16);
     if (a.window > 0) tiles = std::min(tiles, ((long long)a.window + a.max_q) / 16 + 2);
-    const int per_sm = a.kv.hd > 128 ? (p.nb == 1 ? 2 : 1) : p.nb == 1 ? 4 : p.nb == 2 ? 3 : 2;
+    const int per_sm = a.kv.hd > 128 ? (p.nb == 1 ? 2 : 1) : p.nb == 1 ? 4 : 3;
     const long long room = std::max(1ll, (long long)sm_count() * per_sm * 7 / 8 / items);
     want = 1;
     while (want < kMostCluster && want * 2 <= room && want * 2 <= (tiles + 1) / 2) want *= 2;
@@ -683,12 +685,10 @@ extern "C" int zse_attn_decode_q8(const ZseAttnQ8* x) {
                  p.rows_per, p.row_groups, x->window, p.pieces, p.cluster, x->scale * kLog2e * 16777216.f};
   const int n = x->num_seqs;
   const cudaStream_t st = static_cast<cudaStream_t>(x->stream);
-#define ZSE_Q8_WIDTH(HD) p.nb == 1 ? launch<HD, 1>(a, n, st) : p.nb == 2 ? launch<HD, 2>(a, n, st)
   switch (kv.hd) {
-    case 64: return ZSE_Q8_WIDTH(64) : launch<64, 4>(a, n, st);
-    case 96: return ZSE_Q8_WIDTH(96) : launch<96, 4>(a, n, st);
-    case 128: return ZSE_Q8_WIDTH(128) : launch<128, 4>(a, n, st);
+    case 64: return p.nb == 1 ? launch<64, 1>(a, n, st) : launch<64, 2>(a, n, st);
+    case 96: return p.nb == 1 ? launch<96, 1>(a, n, st) : launch<96, 2>(a, n, st);
+    case 128: return p.nb == 1 ? launch<128, 1>(a, n, st) : launch<128, 2>(a, n, st);
     default: return p.nb == 1 ? launch<256, 1>(a, n, st) : launch<256, 2>(a, n, st);
   }
-#undef ZSE_Q8_WIDTH
 }

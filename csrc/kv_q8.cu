@@ -246,14 +246,15 @@ __device__ __forceinline__ uint4 values8(const uint2& v, float f) {
   return pack8(x);
 }
 
-// A CTA takes page after page: the sequence a page belongs to is the number of sequences that end at or before it.  A thread reads
-// 8 bytes and writes 16, so that a warp's stores are one run; four such pieces are loaded before the first is converted.
+// A CTA takes part after part of the pages (a page is `parts` of them, for few pages): the sequence a page belongs to is the number of
+// sequences that end at or before it.  Where the next part lies is looked up before this one is copied.  A thread reads 8 bytes and
+// writes 16, so that a warp's stores are one run; four such pieces are loaded before the first is converted.
 template <int HD>
 __global__ void __launch_bounds__(256)
 kv_read_q8_kernel(const uint8_t* __restrict__ data, const float* __restrict__ scale, int num_blocks, int nkv, int block_size,
                   const int* __restrict__ tables, int table_ld, int max_blocks, const int* __restrict__ seq_lens,
                   const int* __restrict__ cu_blocks, int num_seqs, __half* __restrict__ out, int out_blocks,
-                  int* __restrict__ out_tables, int out_table_ld, int out_max_blocks, Status* st) {
+                  int* __restrict__ out_tables, int out_table_ld, int out_max_blocks, int parts, Status* st) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
@@ -268,40 +269,55 @@ kv_read_q8_kernel(const uint8_t* __restrict__ data, const float* __restrict__ sc
     out_tables[size_t(s) * out_table_ld + j] = blk >= 0 && blk < num_blocks ? first + j : -1;
   }
   constexpr int kRow = HD / 8, kAhead = 4;                             // pieces of a row
-  const int total = min(cu_blocks[num_seqs], out_blocks);
-  const int pieces = 2 * nkv * block_size * kRow;
-  for (int page = blockIdx.x; page < total; page += gridDim.x) {
+  const int total = min(cu_blocks[num_seqs], out_blocks) * parts;
+  const int pieces = 2 * nkv * block_size * kRow, per_part = (pieces + parts - 1) / parts;
+  struct Part {
+    int blk, page, inside;                                             // blk -1: nothing to copy; tokens of the sequence in the page
+  };
+  auto look_up = [&](int part) {
+    Part u{-1, part / parts, 0};
+    if (part >= total) return u;
     int s = 0;
     for (int i = lane; i - lane < num_seqs; i += 32)
-      s += __popc(__ballot_sync(0xffffffffu, i < num_seqs && cu_blocks[i + 1] <= page));
-    if (s >= num_seqs) continue;
-    const int first = cu_blocks[s], j = page - first, len = seq_lens[s], pages = max(len, 0) / block_size + (max(len, 0) % block_size > 0);
+      s += __popc(__ballot_sync(0xffffffffu, i < num_seqs && cu_blocks[i + 1] <= u.page));
+    if (s >= num_seqs) return u;
+    const int first = cu_blocks[s], j = u.page - first, len = max(seq_lens[s], 0), pages = len / block_size + (len % block_size > 0);
     if (first < 0 || j < 0 || j >= pages || pages > min(min(max_blocks, out_max_blocks), cu_blocks[s + 1] - first) ||
         first + pages > out_blocks)
-      continue;
+      return u;
     const int blk = tables[size_t(s) * table_ld + j];
-    if (blk < 0 || blk >= num_blocks) continue;
-    const int inside = min(block_size, len - j * block_size);          // tokens of the sequence in this page
-    const uint2* src = reinterpret_cast<const uint2*>(data) + size_t(blk) * pieces;
-    const float* sc = scale + size_t(blk) * 2 * nkv * block_size;
-    uint4* dst = reinterpret_cast<uint4*>(out) + size_t(page) * pieces;
-    for (int i0 = threadIdx.x; i0 < pieces; i0 += 256 * kAhead) {
-      uint2 v[kAhead];
-      float f[kAhead];
+    if (blk >= 0 && blk < num_blocks) u.blk = blk;
+    u.inside = min(block_size, len - j * block_size);
+    return u;
+  };
+  Part now = look_up(blockIdx.x);
+  for (int part = blockIdx.x; part < total; part += gridDim.x) {
+    const Part next = look_up(part + gridDim.x);
+    if (now.blk >= 0) {
+      const uint2* src = reinterpret_cast<const uint2*>(data) + size_t(now.blk) * pieces;
+      const float* sc = scale + size_t(now.blk) * 2 * nkv * block_size;
+      uint4* dst = reinterpret_cast<uint4*>(out) + size_t(now.page) * pieces;
+      const int begin = (part - now.page * parts) * per_part, end = min(pieces, begin + per_part);
+      for (int i0 = begin + threadIdx.x; i0 < end; i0 += 256 * kAhead) {
+        uint2 v[kAhead];
+        float f[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int i = i0 + k * 256;
-        if (i < pieces) {
-          v[k] = __ldcs(src + i);
-          f[k] = sc[i / kRow];
+        for (int k = 0; k < kAhead; ++k) {
+          const int i = i0 + k * 256;
+          if (i < end) {
+            v[k] = __ldcs(src + i);
+            f[k] = sc[i / kRow];
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int i = i0 + k * 256;
+          if (i < end)
+            dst[i] = now.inside == block_size || (i / kRow) % block_size < now.inside ? values8(v[k], f[k]) : make_uint4(0, 0, 0, 0);
         }
       }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int i = i0 + k * 256;
-        if (i < pieces) dst[i] = inside == block_size || (i / kRow) % block_size < inside ? values8(v[k], f[k]) : make_uint4(0, 0, 0, 0);
-      }
     }
+    now = next;
   }
 }
 
@@ -368,14 +384,18 @@ extern "C" int zse_kv_read_q8(const ZseReadQ8* r) {
   if (r->num_seqs <= 0) return 0;
   if (!cache_ok(kv) || r->max_blocks < 0 || r->out_blocks < 0 || r->out_max_blocks < 0) return ZSE_ERR_SHAPE;
   if (!aligned16(kv.data) || !aligned16(kv.scale) || !aligned16(r->out)) return ZSE_ERR_ALIGN;
-  const long long entries = ((long long)r->num_seqs * r->out_max_blocks + 255) / 256;
-  const int grid = int(std::max(1ll, std::min((long long)sm_count() * 8, std::max((long long)r->out_blocks, entries))));
+  // five CTAs an SM fit; pages in parts of 1024 pieces or more where there are fewer pages than that
+  const long long entries = ((long long)r->num_seqs * r->out_max_blocks + 255) / 256, room = (long long)sm_count() * 5;
+  const long long pieces = 2ll * kv.nkv * kv.block_size * kv.hd / 8;
+  if (pieces * 8 > 0x7fffffffll) return ZSE_ERR_LIMIT;
+  const int parts = int(std::max(1ll, std::min((16 * room + r->out_blocks - 1) / std::max(r->out_blocks, 1), pieces / 1024)));
+  const int grid = int(std::max(1ll, std::min(room, std::max((long long)r->out_blocks * parts, entries))));
   auto go = [&](auto kernel) {
     return launch_pdl(kernel, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(r->stream), static_cast<const uint8_t*>(kv.data),
                       static_cast<const float*>(kv.scale), kv.num_blocks, kv.nkv, kv.block_size,
                       static_cast<const int*>(r->tables), r->table_ld, r->max_blocks, static_cast<const int*>(r->seq_lens),
                       static_cast<const int*>(r->cu_blocks), r->num_seqs, static_cast<__half*>(r->out), r->out_blocks,
-                      static_cast<int*>(r->out_tables), r->out_table_ld, r->out_max_blocks,
+                      static_cast<int*>(r->out_tables), r->out_table_ld, r->out_max_blocks, parts,
                       static_cast<Status*>(r->status)) == cudaSuccess
                ? 1
                : ZSE_ERR_LAUNCH;

@@ -168,7 +168,7 @@ def attend(ops, lens, nh, nkv, hd, bs=16, window=0, holes=(), rows=None, splits=
         cu = [0]
         for r in rows:
             cu.append(cu[-1] + r)
-        kw = dict(cu_q=ints(cu), q_pos0=ints([n - r for n, r in zip(lens, rows)]), max_q=max(rows))
+        kw = dict(cu_q=ints(cu), q_pos0=ints([n - r for n, r in zip(lens, rows)]), max_q=max(rows + [1]))
         seen = [(s, n - r + i + 1) for s, (n, r) in enumerate(zip(lens, rows)) for i in range(r)]
     call = lambda: ops.attn_decode_q8(q, QuantKV(data, scale), tables, ints(lens) if rows is None else None, out, len(lens), nh,
                                       nkv, hd, scale_of(hd), num_splits=splits, window=window, **kw)
@@ -204,10 +204,36 @@ def test_windows_and_holes(ops, hd, bs, window):
 
 
 @pytest.mark.parametrize("splits", [0, 1, 2, 3, 5, 8, 16, 17, 40, 64])
-@pytest.mark.parametrize("lens", [[5], [700, 0, 31, 2000, 1]])
+@pytest.mark.parametrize("lens", [[5], [0], [700, 0, 31, 2000, 1], [0, 0, 16, 16, 900, 0]])
 def test_pieces(ops, splits, lens):
     attend(ops, lens, 14, 2, 128, splits=splits)
     attend(ops, lens, 4, 4, 64, splits=splits, window=333)
+    attend(ops, lens, 10, 2, 96, splits=splits, rows=[min(n, 1 + 2 * i) for i, n in enumerate(lens)], holes=[(len(lens) - 2, 1)] if len(lens) > 1 else ())
+
+
+@pytest.mark.parametrize("splits", [0, 2, 32])
+@pytest.mark.parametrize("hd,nh,nkv", [(64, 32, 8), (96, 4, 4), (128, 16, 1), (256, 16, 8)])
+def test_mixed_lengths(ops, splits, hd, nh, nkv):
+    lens = [(97 * i * i) % 400 for i in range(70)]
+    attend(ops, lens, nh, nkv, hd, splits=splits)
+    attend(ops, lens, nh, nkv, hd, splits=splits, rows=[min(n, 1 + i % 5) for i, n in enumerate(lens)], window=90)
+
+
+@pytest.mark.parametrize("hd,rot", [(64, 64), (64, 16), (96, 48), (128, 128), (256, 256), (128, 0)])
+@pytest.mark.parametrize("M", [888, 1801, 7777])
+def test_write_of_many_rows(ops, hd, rot, M):
+    nh, nkv, bs = 6, 2, 16
+    g = gen(hd + M)
+    pos, slots = torch.arange(M, dtype=torch.int32, device=DEV) * 3, torch.randperm(M + 7, generator=g)[:M].to(DEV)
+    slots[M // 3] = -1
+    kv = QuantKV.zeros(((M + 7) // bs + 1, 2, nkv, bs, hd), DEV)
+    qkv = torch.randn(M, (nh + 2 * nkv) * hd, generator=g).half().to(DEV)
+    x, q = qkv.double(), torch.zeros(M, nh * hd, dtype=torch.float16, device=DEV)
+    ops.rope_kv_write_q8(qkv, kv, pos, slots, freqs_of(rot), M, nh, nkv, hd, q_out=q)
+    k = slots >= 0
+    blk, off = slots[k] // bs, slots[k] % bs
+    check_write(x[k], pos[k], freqs_of(rot), nh, nkv, hd, q[k], kv.data[blk, :, :, off], kv.scale[blk, :, :, off])
+    assert int((kv.data != 0).any(-1).sum()) == 2 * nkv * (M - 1)
 
 
 @pytest.mark.parametrize("hd", [64, 96, 128, 256])
