@@ -3,7 +3,8 @@
 The slab is a single fp16 tensor ``[layers, blocks, 2 (K,V), kv_heads, block_size, head_dim]``: per layer every
 block's K (and V) for one kv head is a contiguous ``block_size*head_dim`` run, which is what the attention kernels
 stream.  Models that cache one latent row per token instead of K and V use the same pool with ``planes=1`` and one kv
-head, at the width of their activations.  Bookkeeping (free list, reference counts for shared/forked blocks) is host-side, as in
+head, at the width of their activations.  With ``dtype=torch.uint8`` the slab is an 8-bit cache (``quant_kv.QuantKV``: a tensor of bytes of
+that shape and one of scales).  Bookkeeping (free list, reference counts for shared/forked blocks) is host-side, as in
 zse-engine/zse_engine/cache/block_pool.py:18-282; with ``device=None`` the pool only does bookkeeping, which is
 how the CPU tests and the scheduler simulations use it.
 """
@@ -14,6 +15,8 @@ from dataclasses import dataclass
 from typing import Deque, Dict, Optional
 
 import torch
+
+from .quant_kv import QuantKV
 
 
 @dataclass
@@ -38,6 +41,11 @@ class Block:
         return self.block_id * self.layer_block_bytes
 
 
+def row_bytes(head_dim: int, dtype) -> int:
+    """Memory of one token's keys (or values) of one kv head: 8-bit rows have a scale each."""
+    return head_dim * torch.empty(0, dtype=dtype).element_size() + (4 if dtype == torch.uint8 else 0)
+
+
 class BlockPool:
     def __init__(self, num_blocks: int, block_size_tokens: int, num_layers: int, num_kv_heads: int, head_dim: int,
                  device=None, dtype=torch.float16, planes: int = 2):
@@ -47,19 +55,20 @@ class BlockPool:
         self._block_size = block_size_tokens
         self._shape = (num_layers, num_blocks, planes, num_kv_heads, block_size_tokens, head_dim)
         self._itemsize = torch.empty(0, dtype=dtype).element_size()
-        self._bytes_per_token = num_layers * planes * num_kv_heads * head_dim * self._itemsize
+        self._bytes_per_token = num_layers * planes * num_kv_heads * row_bytes(head_dim, dtype)
         self._free: Deque[int] = deque(range(num_blocks))
         self._blocks: Dict[int, Block] = {}
-        self.slab: Optional[torch.Tensor] = None
-        if device is not None:
+        self.slab: Optional[torch.Tensor] = None          # (or a QuantKV)
+        if device is not None and dtype == torch.uint8:
+            self.slab = QuantKV.zeros(self._shape, device)
+        elif device is not None:
             # zeros: masked-out tail tokens of a block are multiplied by probability 0 and must be finite
             self.slab = torch.zeros(self._shape, dtype=dtype, device=device)
 
     @classmethod
     def from_budget(cls, budget_bytes: int, block_size_tokens: int, num_layers: int, num_kv_heads: int,
                     head_dim: int, device=None, dtype=torch.float16, planes: int = 2) -> "BlockPool":
-        block_bytes = (block_size_tokens * num_layers * planes * num_kv_heads * head_dim
-                       * torch.empty(0, dtype=dtype).element_size())
+        block_bytes = block_size_tokens * num_layers * planes * num_kv_heads * row_bytes(head_dim, dtype)
         return cls(budget_bytes // block_bytes, block_size_tokens, num_layers, num_kv_heads, head_dim, device, dtype,
                    planes)
 
@@ -123,7 +132,7 @@ class BlockPool:
     def _base_ptr(self) -> int:
         if self.slab is None:
             raise RuntimeError("this pool only does bookkeeping (no device slab)")
-        return int(self.slab.data_ptr())
+        return int((self.slab.data if isinstance(self.slab, QuantKV) else self.slab).data_ptr())
 
     def gpu_ptr_for_block_layer(self, block: Block, layer: int) -> int:
         """Address of the block's K run of ``layer`` (``[kv_heads, block_size, head_dim]`` fp16, V follows it)."""
@@ -165,7 +174,9 @@ class BlockPool:
         return block.num_tokens >= self._block_size
 
     def copy_block(self, src: Block, dst: Block) -> None:
-        if self.slab is not None:
+        if isinstance(self.slab, QuantKV):
+            self.slab.copy_block(src.block_id, dst.block_id)
+        elif self.slab is not None:
             self.slab[:, dst.block_id].copy_(self.slab[:, src.block_id])
 
     def stats(self) -> dict:

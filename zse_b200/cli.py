@@ -31,7 +31,8 @@ def _cmd_serve(a) -> int:
                                 max_batch_seqs=a.max_batch_seqs, prefill_chunk_size=a.prefill_chunk_size,
                                 speculative_k=a.speculative_k, speculative_mode=a.speculative_mode,
                                 use_cuda_graphs=not a.no_graphs, comm_backend=a.comm, quiet=a.quiet,
-                                dtype=getattr(a, "dtype", None), device="cpu" if a.cpu else None)
+                                dtype=getattr(a, "dtype", None), kv_dtype=getattr(a, "kv_dtype", None),
+                                device="cpu" if a.cpu else None)
     server = ZSEServer(a.model, a.host, a.port, a.admin_key, a.db_path, a.model_name, a.quiet, a.tp_size,
                        engine_config=cfg, require_auth=a.require_auth)
     loop = asyncio.new_event_loop()
@@ -228,6 +229,9 @@ def build_parser() -> argparse.ArgumentParser:
                         "sequence-parallel prefill (reduce-scatter / all-gather, residual split by rows)")
     s.add_argument("--dtype", default=None, choices=["float16", "bfloat16", "float32"],
                    help="activation type, for the models that offer more than one (default: the model's own)")
+    s.add_argument("--kv-dtype", default=None, choices=["float16", "int8"],
+                   help="int8: the KV cache in bytes with a scale per token and kv head, half the memory and half of what a "
+                        "decode step reads of it (Llama, Mistral, Qwen2, Phi-3)")
     s.add_argument("--require-auth", action="store_true")
     s.add_argument("--cpu", action="store_true", help="run on the CPU reference path")
     s.set_defaults(fn=_cmd_serve)

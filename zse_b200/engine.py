@@ -23,6 +23,7 @@ from typing import Callable, Dict, Iterator, List, Optional
 
 import torch
 
+from .cache.block_pool import row_bytes
 from .cache.cache_manager import KVCacheManager
 from .cache.state_slots import StateSlots
 from .config import EngineConfig
@@ -102,7 +103,7 @@ class ZStreamerEngine:
 
         t1 = time.monotonic()
         self._model = DecoderModel.from_loader(self._loader, self.device, tp_size=cfg.tp_size, rank=tp_rank,
-                                               dtype=cfg.dtype)
+                                               dtype=cfg.dtype, kv_dtype=cfg.kv_dtype)
         self._model.comm = comm
         if on_gpu:
             torch.cuda.synchronize(self.device)
@@ -112,7 +113,7 @@ class ZStreamerEngine:
         t2 = time.monotonic()
         mc = self._config
         self._max_seq_len = min(cfg.max_seq_len or 32768, mc.max_seq_len)
-        act = self._model.act_dtype
+        act = self._model.kv_cache_dtype
         block_size = cfg.block_size or KVCacheManager._auto_block_size(mc)
         nkv_local = self._model.plan.num_kv_heads
         slots = cfg.state_slots or cfg.max_batch_seqs + 1
@@ -122,11 +123,14 @@ class ZStreamerEngine:
             blocks = mc.cache_blocks(cfg.kv_tokens, cfg.max_batch_seqs, block_size)
         elif on_gpu:
             scratch_est = cfg.max_batch_tokens * (mc.hidden_size * 40 + mc.intermediate_size * 2) + (256 << 20)
+            scratch_est += self._model.kv_scratch_bytes(self._max_seq_len, block_size)
             if mc.keeps_state:
                 scratch_est += slots * StateSlots.bytes_per_slot(mc.state_floats)
             plan = VRAMAllocator.for_device(self.device).plan_allocation(
                 mc, 0, scratch_est, block_size, self._max_seq_len, cfg.max_batch_seqs, cfg.tp_size, cfg.kv_fraction)
-            blocks = max(1, plan.kv_blocks * 2 // act.itemsize)       # the plan counts 16-bit elements
+            # the plan counts 16-bit elements
+            blocks = max(1, plan.kv_blocks * 2 * mc.head_dim // row_bytes(mc.head_dim, act) if self._model.kv_int8
+                         else plan.kv_blocks * 2 // act.itemsize)
             self.vram_plan = plan
         else:
             blocks = max(64, (cfg.max_batch_seqs * min(self._max_seq_len, 2048)) // block_size)

@@ -22,6 +22,8 @@ from typing import Dict, List, Optional
 import numpy as np
 import torch
 
+from ..cache import quant_kv
+from ..cache.quant_kv import QuantKV
 from ..format.loader import ZSELoader
 from ..format.config import ModelConfig
 from ..ops import reference as ref
@@ -143,8 +145,21 @@ class StepBuffers:
         return sum(t.numel() * t.element_size() for t in vars(self).values() if isinstance(t, torch.Tensor))
 
 
+@dataclass
+class PageGroup:
+    """Sequences ``first .. last - 1`` of a prefill pass over an 8-bit cache: as many as the scratch pages hold.  Their rows are
+    ``row .. end - 1``; ``at``: where their places in the pages and their first rows stand in ``StepBuffers.page_ints``."""
+    first: int
+    last: int
+    row: int
+    end: int
+    max_q: int
+    blocks: int = 0
+    at: int = 0
+
+
 class DecoderModel:
-    act_dtype = torch.float16       # activations, and the rows of the KV cache
+    act_dtype = torch.float16       # activations, and the rows of the KV cache (unless that is kept in 8 bits)
     kernel_group: Optional[str] = None      # subset of the native library that is enough (ops/build.py); None = all of it
     mixed_passes = False            # prompt chunks and decoding sequences may share one packed pass
 
@@ -166,12 +181,14 @@ class DecoderModel:
         self.weight_bytes = 0
         self.load_stats: Dict[str, float] = {}
         self.embed_scale = math.sqrt(config.hidden_size) if config.embed_scale else 1.0
+        self.kv_int8 = False        # the KV cache holds bytes and scales (cache.quant_kv)
 
     # ---- loading --------------------------------------------------------------------------------------
     @classmethod
     def from_loader(cls, loader: ZSELoader, device="cpu", tp_size: int = 1, rank: int = 0, ops=None,
-                    progress=None, dtype: Optional[str] = None) -> "DecoderModel":
-        """``dtype``: "bfloat16" or "float32" for the models that offer both; None = what the model is served in."""
+                    progress=None, dtype: Optional[str] = None, kv_dtype: Optional[str] = None) -> "DecoderModel":
+        """``dtype``: "bfloat16" or "float32" for the models that offer both; None = what the model is served in.
+        ``kv_dtype``: "int8" for a cache of bytes with a scale per token and kv head; None = as wide as the activations."""
         c = loader.config
         if c.arch not in SUPPORTED_ARCHS:
             raise NotImplementedError(f"architecture '{c.arch}' has a converter but no runtime here yet "
@@ -190,12 +207,32 @@ class DecoderModel:
             cls = TwinModel if c.side_by_side else HybridModel if c.norms_outputs else LoopedModel
         m = cls(c, plan, ops or make_ops(device, cls.kernel_group))
         m.set_dtype(dtype)
+        m.set_kv_dtype(kv_dtype)
         m._load(loader, progress)
         return m
 
     def set_dtype(self, dtype: Optional[str]) -> None:
         if dtype not in (None, "float16"):
             raise ValueError(f"'{self.config.arch}' runs in float16, not {dtype}")
+
+    def set_kv_dtype(self, kv_dtype: Optional[str]) -> None:
+        if kv_dtype in (None, str(self.act_dtype).split(".")[-1]):
+            return
+        if kv_dtype not in quant_kv.KV_DTYPES:
+            raise ValueError(f"a KV cache of {kv_dtype}: one of {', '.join(quant_kv.KV_DTYPES)} expected")
+        why = quant_kv.refuses(self.config) if kv_dtype == "int8" else f"'{self.config.arch}' keeps its cache in {self.act_dtype}"
+        if why is not None:
+            raise ValueError(f"a KV cache of {kv_dtype} is not available here: {why}")
+        self.kv_int8 = True
+
+    @property
+    def kv_cache_dtype(self) -> torch.dtype:
+        return torch.uint8 if self.kv_int8 else self.act_dtype
+
+    def kv_scratch_bytes(self, max_seq_len: int, block_size: int) -> int:
+        """Memory beside the cache: 8-bit caches have the fp16 pages that prefill attention reads."""
+        blocks = (max_seq_len + block_size - 1) // block_size
+        return blocks * block_size * 2 * self.plan.kv_dim * 2 if self.kv_int8 else 0
 
     def _load(self, loader: ZSELoader, progress=None) -> None:
         c, p, ops, dev = self.config, self.plan, self.ops, self.device
@@ -282,7 +319,87 @@ class DecoderModel:
         if sp is not None and sp.shape[0] >= max_tokens and sp.shape[1] == self.config.hidden_size:
             # the normalised activations live in the symmetric buffer other ranks store gathered rows into
             b.xnorm = sp[:max_tokens]
+        if self.kv_int8:
+            self._add_q8_buffers(b)
         return b
+
+    # ---- 8-bit cache ------------------------------------------------------------------------------------
+    DRAFT_ROWS = 8      # passes of at most so many rows a sequence (speculative verification) attend to the bytes themselves
+
+    def _add_q8_buffers(self, b: StepBuffers) -> None:
+        """Pages that prefill passes read sequences back into (one sequence of the longest kind at least), and scratch of decode
+        attention."""
+        p, hd, bs, on_gpu = self.plan, self.config.head_dim, self.cache_block_size, self.device.type == "cuda"
+        self.table_blocks = b.max_blocks
+        z = lambda *shape, dt: torch.zeros(*shape, dtype=dt, device=self.device)
+        b.pages = z(b.max_blocks, 2, p.num_kv_heads, bs, hd, dt=torch.float16)
+        b.page_tables = torch.full((b.max_seqs, b.max_blocks), -1, dtype=torch.int32, device=self.device)
+        ints = 5 * b.max_seqs + 2                      # lengths, then of every group places in the pages and first rows
+        b.page_ints = z(ints, dt=torch.int32)
+        b.h_page_ints = torch.zeros(ints, dtype=torch.int32, pin_memory=on_gpu)
+        b.page_groups = []
+        need = 0
+        if on_gpu:
+            from ..ops import native
+            need = max(native.attn_decode_q8_plan(S, R, p.num_heads, p.num_kv_heads, hd, bs, b.max_blocks, self.window)[1]
+                       for S in range(1, b.max_seqs + 1) for R in range(1, self.DRAFT_ROWS + 1))
+        b.q8_scratch = z(max(1, need), dt=torch.float32)
+
+    def _stage_q8(self, b: StepBuffers, spans) -> None:
+        bs, S, h = self.cache_block_size, len(spans), b.h_page_ints.numpy()
+        groups: List[PageGroup] = []
+        row = 0
+        for s, (start, n) in enumerate(spans):
+            h[s] = start + n
+            blocks = (start + n + bs - 1) // bs
+            if not groups or groups[-1].blocks + blocks > b.pages.shape[0]:
+                groups.append(PageGroup(s, s, row, row, 0))
+            g = groups[-1]
+            row += n
+            g.last, g.end, g.max_q, g.blocks = s + 1, row, max(g.max_q, n), g.blocks + blocks
+        at = S
+        for g in groups:
+            g.at, n = at, g.last - g.first
+            h[at] = h[at + n + 1] = 0
+            for i in range(n):
+                start, rows = spans[g.first + i]
+                h[at + i + 1] = h[at + i] + (start + rows + bs - 1) // bs
+                h[at + n + 2 + i] = h[at + n + 1 + i] + rows
+            at += 2 * (n + 1)
+        b.page_ints[:at].copy_(b.h_page_ints[:at], non_blocking=True)
+        b.page_groups = groups
+
+    def _rope_write(self, layer, b: StepBuffers, M: int, planes=None, n_planes: int = 0, bias=None) -> None:
+        """q and k of the pass's rows rotated, k and v into the cache layer."""
+        c, p = self.config, self.plan
+        if self.kv_int8:
+            self.ops.rope_kv_write_q8(b.qkv, layer, b.positions, b.slots, self.inv_freq, M, p.num_heads, p.num_kv_heads, c.head_dim,
+                                      planes=planes, n_planes=n_planes, bias=bias)
+        else:
+            self.ops.rope_kv_write(b.qkv, layer, b.positions, b.slots, self.inv_freq, M, p.num_heads, p.num_kv_heads, c.head_dim,
+                                   layer.shape[3], planes=planes, n_planes=n_planes, bias=bias)
+
+    def _attend_q8(self, layer, b: StepBuffers, M: int, mode: str, num_seqs: int, max_q_len: int, attn_splits: int) -> None:
+        """Attention over an 8-bit layer: of one row, or a few, per sequence over the bytes; of longer chunks over fp16 pages that
+        the sequences are read back into first."""
+        ops, c, p = self.ops, self.config, self.plan
+        nh, nkv, hd = p.num_heads, p.num_kv_heads, c.head_dim
+        if mode == "decode":
+            ops.attn_decode_q8(b.qkv, layer, b.block_tables, b.seq_lens, b.attn_out, num_seqs, nh, nkv, hd, self.scale, b.q8_scratch,
+                               attn_splits, self.window)
+            return
+        if max_q_len <= self.DRAFT_ROWS:
+            ops.attn_decode_q8(b.qkv, layer, b.block_tables, None, b.attn_out, num_seqs, nh, nkv, hd, self.scale, b.q8_scratch,
+                               0, self.window, b.cu_q, b.q_pos0, max_q_len)
+            return
+        for g in b.page_groups:
+            n = g.last - g.first
+            tables = b.page_tables[: n]
+            ops.kv_read_q8(layer, b.block_tables[g.first: g.last], b.page_ints[g.first: g.last],
+                           b.page_ints[g.at: g.at + n + 1], n, b.pages, tables)
+            ops.attn_prefill(b.qkv[g.row: g.end], b.pages, tables, b.page_ints[g.at + n + 1: g.at + 2 * n + 2],
+                             b.q_pos0[g.first: g.last], b.attn_out[g.row: g.end], n, g.end - g.row, g.max_q, nh, nkv, hd,
+                             self.cache_block_size, self.scale, window=self.window)
 
     @property
     def _sp_weights_ok(self) -> bool:
@@ -301,6 +418,8 @@ class DecoderModel:
 
     def stage_prefill(self, b: StepBuffers, spans) -> None:
         """Called while a packed pass is staged; ``spans[s] = (start, tokens)`` in the pass's order."""
+        if self.kv_int8:
+            self._stage_q8(b, spans)
 
     def attention_splits(self, seqs: int, max_len: int, most: int, sms: int, tokens: Optional[int] = None) -> int:
         """``num_splits`` of the decode kernel for a step over ``seqs`` sequences of up to ``max_len`` tokens, ``tokens`` in all (not
@@ -318,6 +437,14 @@ class DecoderModel:
         whole = max_len * width / 100
         alone = (seqs * max_len if tokens is None else tokens) * self.plan.num_kv_heads * width / 7700
         return most if whole > 3.5 + 0.6 * alone * 148 / sms else 1
+
+    def attention_pieces(self, seqs: int, max_len: int) -> int:
+        """``num_splits`` of the decode kernel over an 8-bit cache: pieces of a sequence and kv head, for contexts of up to 1024 tokens
+        or of any length (again two CUDA graphs of a batch size at most)."""
+        from ..ops import native
+        p, bs = self.plan, self.cache_block_size
+        blocks = self.table_blocks if max_len > 1024 else max(1, min(1024 // bs, self.table_blocks))
+        return native.attn_decode_q8_plan(seqs, 1, p.num_heads, p.num_kv_heads, self.config.head_dim, bs, blocks, self.window)[0]
 
     # ---- forward --------------------------------------------------------------------------------------
     def _add_norm(self, b: StepBuffers, planes: int, weight: torch.Tensor, M: int, add=None) -> None:
@@ -380,10 +507,10 @@ class DecoderModel:
     def forward(self, b: StepBuffers, kv: torch.Tensor, M: int, mode: str, num_seqs: int, max_q_len: int = 1,
                 n_logit_rows: int = 0, attn_splits: int = 1) -> None:
         """Runs the stack over tokens ``b.ids[:M]``; leaves fp16 logits of rows ``b.logit_rows[:n_logit_rows]`` in
-        ``b.logits``.  ``kv``: [layers, blocks, 2, nkv_local, block_size, hd]."""
+        ``b.logits``.  ``kv``: [layers, blocks, 2, nkv_local, block_size, hd] (8-bit caches: a QuantKV of that shape)."""
         c, p, ops = self.config, self.plan, self.ops
         bs = kv.shape[4]
-        if self.comm is None and self.lora is None:
+        if self.comm is None and self.lora is None and not self.kv_int8:
             step = self._native_step_for(b)
             if step is not None:       # one C call launches the whole pass (csrc/step.cu)
                 step.forward(kv, M, mode == "decode", num_seqs, max_q_len, n_logit_rows, attn_splits)
@@ -398,30 +525,30 @@ class DecoderModel:
         for li, L in enumerate(self.layers):
             self._add_norm(b, planes, L.ln1, M, add)
             gather = self.comm._ctx if self._sp_live else None
+            layer = kv[li]
             if gather is not None:
                 ops.linear(L.qkv, b.xnorm, M, b.qkv, gather=gather)
-                ops.rope_kv_write(b.qkv, kv[li], b.positions, b.slots, self.inv_freq, M, p.num_heads,
-                                  p.num_kv_heads, c.head_dim, bs)
-            elif (self.lora is None and self.rope_table is not None
-                    and ops.qkv_rope_fused_ok(L.qkv, M, c.head_dim, kv[li])):
-                ops.qkv_rope_fused(L.qkv, b.xnorm, M, b.qkv, kv[li], b.positions, b.slots, self.rope_table,
+                self._rope_write(layer, b, M)
+            elif (self.lora is None and self.rope_table is not None and not self.kv_int8
+                    and ops.qkv_rope_fused_ok(L.qkv, M, c.head_dim, layer)):
+                ops.qkv_rope_fused(L.qkv, b.xnorm, M, b.qkv, layer, b.positions, b.slots, self.rope_table,
                                    p.num_heads, p.num_kv_heads, bs)
             elif self.lora is None and M <= b.qkv_plane_rows and L.qkv.kind == "w4t":
                 n_q = ops.linear_partial(L.qkv, b.xnorm, M, b.qkv_planes)
-                ops.rope_kv_write(b.qkv, kv[li], b.positions, b.slots, self.inv_freq, M, p.num_heads, p.num_kv_heads,
-                                  c.head_dim, bs, planes=b.qkv_planes, n_planes=n_q, bias=L.qkv.bias)
+                self._rope_write(layer, b, M, b.qkv_planes, n_q, L.qkv.bias)
             else:
                 ops.linear(L.qkv, b.xnorm, M, b.qkv)
                 if self.lora is not None:
                     self.lora.apply_qkv(li, b, M)
-                ops.rope_kv_write(b.qkv, kv[li], b.positions, b.slots, self.inv_freq, M, p.num_heads,
-                                  p.num_kv_heads, c.head_dim, bs)
-            if mode == "decode":
-                ops.attn_decode(b.qkv, kv[li], b.block_tables, b.seq_lens, b.attn_out, num_seqs, p.num_heads,
+                self._rope_write(layer, b, M)
+            if self.kv_int8:
+                self._attend_q8(layer, b, M, mode, num_seqs, max_q_len, attn_splits)
+            elif mode == "decode":
+                ops.attn_decode(b.qkv, layer, b.block_tables, b.seq_lens, b.attn_out, num_seqs, p.num_heads,
                                 p.num_kv_heads, c.head_dim, bs, self.scale, b.attn_scratch, attn_splits,
                                 window=self.window)
             else:
-                ops.attn_prefill(b.qkv, kv[li], b.block_tables, b.cu_q, b.q_pos0, b.attn_out, num_seqs, M, max_q_len,
+                ops.attn_prefill(b.qkv, layer, b.block_tables, b.cu_q, b.q_pos0, b.attn_out, num_seqs, M, max_q_len,
                                  p.num_heads, p.num_kv_heads, c.head_dim, bs, self.scale, window=self.window)
             add = lora.delta(li, "o_proj", b.attn_out, b, M) if lora is not None else None
             planes = self._row_parallel(L.o, b.attn_out, M, b, L.ln2, add)

@@ -289,6 +289,8 @@ class ModelRunner:
     def _pick_splits(self, S: int, max_len: int, tokens: int) -> int:
         if self.device.type != "cuda":
             return 1
+        if self.model.kv_int8:
+            return self.model.attention_pieces(S, max_len)
         return self.model.attention_splits(S, max_len, self.max_attn_splits, self._sm, tokens)
 
     def _apply_penalties(self, penalties, n_rows: int) -> None:
