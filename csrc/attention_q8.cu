@@ -4,7 +4,7 @@
 //
 // An item is one kv head of one sequence with up to 8 or 16 columns c: query heads of the group, times rows of a draft (more rows
 // are more items, which read the keys and values again, from L2: with 32 columns a warp needs 240 registers, and 32 drafts of up to five
-// rows of 40 heads over 2001 to 4094 tokens took 78 us instead of 66).  Its tokens are
+// rows of 40 heads over 2001 to 4094 tokens took 78 us instead of 66 that way).  Its tokens are
 // cut into pieces, one per CTA; four warps of a CTA take every fourth tile of 16 tokens through rings of their own (cp.async) and
 // keep a running maximum, sum and output in registers.  Tokens are the 16 rows of the products, columns their 8 columns.
 //
@@ -17,6 +17,10 @@
 // element.  Values: 0x64 above the byte makes 1024 + u, and a packed subtraction of 1152 the
 // exact u - 128; with the subnormal form the weights' sum times 128 would cancel against a result that can be a thousand times smaller.
 // Values come as pairs of dimensions of one token out of ldmatrix.trans, so the two rows of a thread are neighbouring dimensions.
+// Weights go into the products as two fp16 numbers, rounded and what that leaves: with the first alone results were off by 3.0e-4 of
+// themselves (2-norm), with both by the 2.1e-4 of their own rounding to fp16.  Up to four columns have the second numbers in the
+// four that would be idle; else they are products more (a legacy product of 16 x 8 x 16 keeps a quarter of an SM busy for some 8 cycles:
+// the drafts above took 66 us without them and 77 us with them, 64 sequences of 128 to 2300 tokens of 40 heads 35.7 and 38.2).
 #include <algorithm>
 
 #include "api.h"
@@ -127,7 +131,8 @@ struct Q8Smem {
   static_assert(kGot % 16 == 0 && kGotO % 16 == 0 && kQ % 16 == 0, "16-byte pieces");
 };
 
-template <int HD, int NB>
+// PACKED: up to four columns; they stand a second time in columns 4 .. 7, where the weights are what rounding leaves of the first.
+template <int HD, int NB, bool PACKED>
 __global__ void __launch_bounds__(kWarps * 32, HD > 128 ? 1 : NB == 1 ? 4 : 3)
 attn_q8_kernel(const Q8Args a) {
   using S = Q8Smem<HD, NB>;
@@ -238,8 +243,8 @@ attn_q8_kernel(const Q8Args a) {
     }
     __syncthreads();
   } else {
-    const int r = row_of(a, g);
-    const __half* src = a.q + size_t(row0 + r) * a.ldq + size_t(kvh * a.group + g - r * a.group) * HD + t2 * 2;
+    const int c = PACKED ? g & 3 : g, r = row_of(a, c);
+    const __half* src = a.q + size_t(row0 + r) * a.ldq + size_t(kvh * a.group + c - r * a.group) * HD + t2 * 2;
 #pragma unroll
     for (int kk = 0; kk < kChunks; ++kk) {
       uint2 v = make_uint2(0u, 0u);
@@ -329,7 +334,8 @@ attn_q8_kernel(const Q8Args a) {
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int len = min(base_len + row_of(a, nb * 8 + t2 + (e & 1)), cap), at_tok = tok + g + (e >> 1) * 8;
+          const int c = PACKED ? (t2 & 2) + (e & 1) : nb * 8 + t2 + (e & 1);
+          const int len = min(base_len + row_of(a, c), cap), at_tok = tok + g + (e >> 1) * 8;
           if (at_tok >= len || (a.window > 0 && at_tok < len - a.window)) {
             dead |= 1u << (nb * 4 + e);
             t[nb][e] = -INFINITY;
@@ -384,7 +390,7 @@ attn_q8_kernel(const Q8Args a) {
     }
     w0 *= inv_ref;
     w1 *= inv_ref;
-    uint32_t pb[NB][2];
+    uint32_t pb[NB][2], rest[NB][2];                                   // tokens 0..7 and 8..15, [column][token]: the B operand
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       float w[4];
@@ -399,8 +405,14 @@ attn_q8_kernel(const Q8Args a) {
         for (int e = 0; e < 4; ++e)
           if ((dead >> (nb * 4 + e)) & 1u) w[e] = 0.f;
       }
-      pb[nb][0] = turn_8x8(pack_half2(w[0], w[1]));                    // [token][column] -> [column][token], the B operand
-      pb[nb][1] = turn_8x8(pack_half2(w[2], w[3]));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t x = pack_half2(w[2 * h], w[2 * h + 1]);
+        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&x));
+        const uint32_t y = pack_half2(w[2 * h] - back.x, w[2 * h + 1] - back.y);
+        pb[nb][h] = turn_8x8(PACKED && t2 >= 4 ? y : x);
+        rest[nb][h] = PACKED ? 0u : turn_8x8(y);
+      }
     }
 #pragma unroll
     for (int dd = 0; dd < kChunks / 2; ++dd) {
@@ -413,6 +425,10 @@ attn_q8_kernel(const Q8Args a) {
                                minus_1152(__byte_perm(r[2 * h + 1], 0x64646464u, 0x4341))};
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) mma_f16(o[nb][dd * 2 + h], f, pb[nb][0], pb[nb][1]);
+        if constexpr (!PACKED) {
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) mma_f16(o[nb][dd * 2 + h], f, rest[nb][0], rest[nb][1]);
+        }
       }
     }
   }
@@ -466,7 +482,11 @@ attn_q8_kernel(const Q8Args a) {
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float mw = own_m[w * S::kCols + c], f = ex2(mw - top);
-      const float4 x = *reinterpret_cast<const float4*>(smem + w * S::kRing + (c * S::kPitch + d) * 4);
+      float4 x = *reinterpret_cast<const float4*>(smem + w * S::kRing + (c * S::kPitch + d) * 4);
+      if constexpr (PACKED) {
+        const float4 y = *reinterpret_cast<const float4*>(smem + w * S::kRing + ((c + 4) * S::kPitch + d) * 4);
+        x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+      }
       total += own_l[w * S::kCols + c] * f;
       const float fo = f * own_ref[w];
       acc.x += x.x * fo;
@@ -610,11 +630,11 @@ bool shape_ok(const ZseAttnQ8& a) {
          (kv.hd == 64 || kv.hd == 96 || kv.hd == 128 || kv.hd == 256);
 }
 
-template <int HD, int NB>
+template <int HD, int NB, bool PACKED>
 int launch(const Q8Args& a, int num_seqs, cudaStream_t st) {
   static bool ready[kMaxDevices];
   const int dev = current_device_slot();
-  auto kernel = attn_q8_kernel<HD, NB>;
+  auto kernel = attn_q8_kernel<HD, NB, PACKED>;
   constexpr int kBytes = Q8Smem<HD, NB>::kTotal;
   if (!ready[dev]) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess ||
@@ -685,10 +705,11 @@ extern "C" int zse_attn_decode_q8(const ZseAttnQ8* x) {
                  p.rows_per, p.row_groups, x->window, p.pieces, p.cluster, x->scale * kLog2e * 16777216.f};
   const int n = x->num_seqs;
   const cudaStream_t st = static_cast<cudaStream_t>(x->stream);
+  auto go = [&](auto packed, auto one, auto two) { return (x->max_q * group <= 4 ? packed : p.nb == 1 ? one : two)(a, n, st); };
   switch (kv.hd) {
-    case 64: return p.nb == 1 ? launch<64, 1>(a, n, st) : launch<64, 2>(a, n, st);
-    case 96: return p.nb == 1 ? launch<96, 1>(a, n, st) : launch<96, 2>(a, n, st);
-    case 128: return p.nb == 1 ? launch<128, 1>(a, n, st) : launch<128, 2>(a, n, st);
-    default: return p.nb == 1 ? launch<256, 1>(a, n, st) : launch<256, 2>(a, n, st);
+    case 64: return go(launch<64, 1, true>, launch<64, 1, false>, launch<64, 2, false>);
+    case 96: return go(launch<96, 1, true>, launch<96, 1, false>, launch<96, 2, false>);
+    case 128: return go(launch<128, 1, true>, launch<128, 1, false>, launch<128, 2, false>);
+    default: return go(launch<256, 1, true>, launch<256, 1, false>, launch<256, 2, false>);
   }
 }
