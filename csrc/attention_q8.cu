@@ -46,7 +46,7 @@ struct Q8Args {
   float* scratch;
   Status* st;
   int ldq, ldo, q_rows, num_blocks, nkv, bpt, bpt_shift, table_ld, max_blocks, group, group_inv, max_q, rows_per, row_groups, window,
-      pieces, cluster;
+      pieces, cluster, sort;                                           // sort: sequences, to be taken the longest first (0: as they come)
   float scale_log2;
 };
 // c / group for columns and c < 64: group_inv = ceil(2^16 / group)
@@ -114,6 +114,30 @@ __device__ __forceinline__ float load_shared(uint32_t addr) {
   return v;
 }
 
+// The z-th longest of the (at most 64) sequences.  Items are handed to the SMs in the order of the grid: the longest first, every SM
+// gets one of each size: with two pieces each, 64 sequences of 128 to 2300 tokens took 36.5 us and take 35.0, of 6001 to 8190 151 and 146.
+__device__ __forceinline__ int by_length(const Q8Args& a, int z) {
+  const int lane = threadIdx.x & 31;
+  int key[2], rank[2] = {0, 0};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int i = k * 32 + lane;
+    key[k] = -1;
+    if (i < a.sort) {
+      const int len = a.cu_q != nullptr ? a.q_pos0[i] + (a.cu_q[i + 1] - a.cu_q[i]) : a.seq_lens[i];
+      key[k] = (min(max(a.window > 0 ? min(len, a.window) : len, 0), (1 << 28) - 1) >> 4) * 64 + 63 - i;   // (no two alike)
+    }
+  }
+#pragma unroll 8
+  for (int j = 0; j < 32; ++j) {
+    const int u = __shfl_sync(0xffffffffu, key[0], j), v = __shfl_sync(0xffffffffu, key[1], j);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) rank[k] += (u > key[k]) + (v > key[k]);
+  }
+  const uint32_t low = __ballot_sync(0xffffffffu, key[0] >= 0 && rank[0] == z), high = __ballot_sync(0xffffffffu, key[1] >= 0 && rank[1] == z);
+  return low != 0 ? __ffs(low) - 1 : __ffs(high) + 31;
+}
+
 template <int HD, int NB>
 struct Q8Smem {
   static constexpr int kTile = 16 * HD;                                // K or V of 16 tokens
@@ -146,7 +170,7 @@ attn_q8_kernel(const Q8Args a) {
   pdl_wait();
   // (what every CTA does once is kept short: with one tile per warp it is most of its instructions)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t2 = (lane & 3) * 2;
-  const int piece = blockIdx.x, s = blockIdx.z, kvh = a.row_groups == 1 ? blockIdx.y : blockIdx.y / a.row_groups;
+  const int piece = blockIdx.x, s = a.sort > 0 ? by_length(a, blockIdx.z) : blockIdx.z, kvh = a.row_groups == 1 ? blockIdx.y : blockIdx.y / a.row_groups;
   const int rg = blockIdx.y - kvh * a.row_groups, cap = a.max_blocks * a.bpt * 16;
 
   // A warp's tile i is 4 (i * pieces + piece) + warp of the item: pieces are equally long, and without a window where the first tiles
@@ -590,7 +614,7 @@ int sm_count() {
 }
 
 struct Plan {
-  int nb, rows_per, row_groups, pieces, cluster;
+  int nb, rows_per, row_groups, pieces, cluster, sort;
   long long scratch_floats;
 };
 Plan plan_of(const ZseAttnQ8& a) {
@@ -601,25 +625,31 @@ Plan plan_of(const ZseAttnQ8& a) {
   p.row_groups = (a.max_q + p.rows_per - 1) / p.rows_per;
   const long long items = (long long)a.num_seqs * a.kv.nkv * p.row_groups;
   // Pieces: what fits the GPU at a time (CTAs an SM by registers and shared memory; an eighth less, for clusters need neighbouring
-  // places), at least half a tile a warp.  Measured (HD 128, us by pieces): 1 x 1000 tokens of 8 kv heads 1: 10.5, 4: 5.6, 8: 4.8; 32 x 500
-  // 1: 14.9, 2: 12.6, 4: 16.0; 64 x 6001..8190 1: 157, 2: 148 - a second wave pays where a warp still has 32 tiles of it.  Several
-  // clusters (and the launch that joins them) where eight pieces leave a warp 12 tiles: 1 x 4000 of 4 kv heads 8: 7.9, 32: 7.3; 1 x
-  // 32765 8: 36, 64: 14.9, 112: 14.3.
+  // places), at least half a tile a warp.  Measured (HD 128, us by pieces): 1 x 1000 tokens of 8 kv heads 1: 11.1, 4: 5.9, 8: 5.0; 32 x 500
+  // 1: 15.9, 2: 13.4, 4: 17.6.
+  // Twice as many, a second wave, where there is no more than one and a warp still has 16 tiles: sequences of mixed length are then
+  // shared out better, the longest first.  64 x 128 .. 2300 tokens of 8 kv heads 1: 38.5, 2: 35.0; 128 .. 4600 1: 71, 2: 55; of 32 heads over
+  // 8 of 64 28 and 23; 32 drafts of up to five rows 79 and 71; but 64 x 2300 1: 52.8, 2: 56.2, and windows make sequences alike.
+  // Several clusters (and the launch that joins them) where eight pieces leave a warp 12 tiles: 1 x 4000 of 4 kv heads 8: 8.4, 32: 7.8;
+  // 1 x 32765 8: 38, 64: 15.5, 128: 14.0.
+  const int per_sm = a.kv.hd > 128 ? (p.nb == 1 ? 2 : 1) : p.nb == 1 ? 4 : 3;
   long long want = a.num_splits;
   if (want <= 0) {
     long long tiles = (long long)a.max_blocks * (a.kv.block_size / 16);
     if (a.window > 0) tiles = std::min(tiles, ((long long)a.window + a.max_q) / 16 + 2);
-    const int per_sm = a.kv.hd > 128 ? (p.nb == 1 ? 2 : 1) : p.nb == 1 ? 4 : 3;
     const long long room = std::max(1ll, (long long)sm_count() * per_sm * 7 / 8 / items);
     want = 1;
     while (want < kMostCluster && want * 2 <= room && want * 2 <= (tiles + 1) / 2) want *= 2;
-    if (want < kMostCluster && want * 2 > room && tiles >= want * 2 * kWarps * 32) want *= 2;
+    if (want < kMostCluster && want * 2 > room && a.window == 0 && items * want * 4 <= 5ll * sm_count() * per_sm &&
+        tiles >= want * 2 * kWarps * 16)
+      want *= 2;
     if (want == kMostCluster && room > kMostCluster && tiles >= kMostCluster * kWarps * 12)
       want = std::max(want, std::min(room, tiles / (4 * kWarps)) / kMostCluster * kMostCluster);
   }
   p.cluster = 1;
   while (p.cluster < want && p.cluster < kMostCluster) p.cluster *= 2;
   p.pieces = int(std::min(64ll, (want + p.cluster - 1) / p.cluster) * p.cluster);
+  p.sort = a.num_seqs > 1 && a.num_seqs <= 64 && 2 * items * p.pieces >= 3ll * sm_count() * per_sm ? a.num_seqs : 0;     // several waves
   p.scratch_floats = p.pieces == p.cluster ? 0 : items * (p.pieces / p.cluster) * 8 * p.nb * (a.kv.hd + 4);
   return p;
 }
@@ -702,7 +732,7 @@ extern "C" int zse_attn_decode_q8(const ZseAttnQ8* x) {
                  static_cast<const int*>(x->q_pos0), static_cast<__half*>(x->out), static_cast<float*>(x->scratch),
                  static_cast<Status*>(x->status), x->ldq, x->ldo, x->q_rows, kv.num_blocks, kv.nkv, bpt,
                  (1 << shift) == bpt ? shift : -1, x->table_ld, x->max_blocks, group, (65536 + group - 1) / group, x->max_q,
-                 p.rows_per, p.row_groups, x->window, p.pieces, p.cluster, x->scale * kLog2e * 16777216.f};
+                 p.rows_per, p.row_groups, x->window, p.pieces, p.cluster, p.sort, x->scale * kLog2e * 16777216.f};
   const int n = x->num_seqs;
   const cudaStream_t st = static_cast<cudaStream_t>(x->stream);
   auto go = [&](auto packed, auto one, auto two) { return (x->max_q * group <= 4 ? packed : p.nb == 1 ? one : two)(a, n, st); };
