@@ -2,25 +2,30 @@
 //
 //   s[t][c] = scale * kscale[t] * (sum_d q[c][d] (uk[t][d] - 128)),   o[c][d] = sum_t p[t][c] vscale[t] (uv[t][d] - 128) / sum_t p[t][c]
 //
-// An item is one kv head of one sequence with up to 8 or 16 columns c: query heads of the group, times rows of a draft (more rows
-// are more items, which read the keys and values again, from L2: with 32 columns a warp needs 240 registers, and 32 drafts of up to five
-// rows of 40 heads over 2001 to 4094 tokens took 78 us instead of 66 that way).  Its tokens are
-// cut into pieces, one per CTA; four warps of a CTA take every fourth tile of 16 tokens through rings of their own (cp.async) and
-// keep a running maximum, sum and output in registers.  Tokens are the 16 rows of the products, columns their 8 columns.
+// An item is one kv head of one sequence with up to 16 columns c: query heads of the group, times rows of a draft.  More rows are more
+// items, which read the keys and values again, from L2: with 32 columns a warp needs 240 registers, and 32 drafts of up to five rows of
+// 40 heads over 2001 to 4094 tokens took 78 us instead of 66 (both with weights of one fp16 number, see below).  An item's tokens are
+// cut into pieces, one per CTA; four warps of a CTA take every fourth tile of 16 tokens through rings of their own (cp.async) and keep
+// running references, sums and outputs in registers.  Tokens are the 16 rows of the products, columns their 8 columns.
 //
-// The pieces of an item are a thread-block cluster: its CTAs put what they have into shared memory and every CTA adds up a share
-// of the result from all of them.  No scratch, no second kernel, nothing that two calls could share.  Only where a cluster of 16
-// per item leaves most of the GPU idle (few sequences of few kv heads) are there several clusters per item, which meet in scratch.
+// Up to eight pieces of an item are a thread-block cluster: every CTA stores what it has into the shared memory of the CTAs that add it
+// up, each a share of the elements.  No scratch, no second kernel, nothing that two calls could share.  Only where eight pieces per item
+// leave most of the GPU idle (few long sequences of few kv heads) are there several clusters per item, which meet in scratch.
 //
-// Bytes become fp16 numbers by byte permutations alone.  Keys: a byte in the low half of an fp16 number is u * 2^-24 (subnormal numbers
-// are exact in the products), so a product sum that starts at -2^-17 sum(q) ends at 2^-24 (q . (uk - 128)): half an instruction per
-// element.  Values: 0x64 above the byte makes 1024 + u, and a packed subtraction of 1152 the
-// exact u - 128; with the subnormal form the weights' sum times 128 would cancel against a result that can be a thousand times smaller.
-// Values come as pairs of dimensions of one token out of ldmatrix.trans, so the two rows of a thread are neighbouring dimensions.
+// Bytes become fp16 numbers by byte permutations.  Keys: a byte in the low half of an fp16 number is u * 2^-24 (subnormal numbers are
+// exact in the products), so a sum that starts at -2^-17 sum(q) ends at 2^-24 (q . (uk - 128)): half an instruction per element.
+// Values: 0x64 above the byte makes 1024 + u, and a packed subtraction of 1152 the exact u - 128; in the subnormal form 128 times the
+// weights' sum would cancel against a result that can be a thousand times smaller.  Values come as pairs of dimensions of one token out
+// of ldmatrix.trans, so the two rows of a thread are neighbouring dimensions.
+//
 // Weights go into the products as two fp16 numbers, rounded and what that leaves: with the first alone results were off by 3.0e-4 of
-// themselves (2-norm), with both by the 2.1e-4 of their own rounding to fp16.  Up to four columns have the second numbers in the
-// four that would be idle; else they are products more (a legacy product of 16 x 8 x 16 keeps a quarter of an SM busy for some 8 cycles:
-// the drafts above took 66 us without them and 77 us with them, 64 sequences of 128 to 2300 tokens of 40 heads 35.7 and 38.2).
+// themselves (2-norm), with both by the 2.1e-4 of their own rounding to fp16.  Up to four columns have the second numbers in the four
+// that would be idle; else they are products more (a product of 16 x 8 x 16 keeps a quarter of an SM busy for some 8 cycles: the drafts
+// 66 -> 77 us, 64 sequences of 128 to 2300 tokens of 40 heads 35.7 -> 38.2; longest first, as by_length() has them, 70 and 35).
+//
+// What bounds it: the cache's bytes where there are many of them (64 sequences of 6001 to 8190 tokens, 64 heads over 8: 146 us, 6.6 TB/s,
+// the rate of a plain copy); mixed lengths leave SMs idle at the end (128 to 2300 tokens: 4.8 TB/s); drafts the products (70 us, of
+// which 34 are product time); few short sequences the way length -> table -> tile -> merge (1 x 300 tokens of 28 heads over 4: 4.2 us).
 #include <algorithm>
 
 #include "api.h"

@@ -17,6 +17,7 @@ import torch
 from ..format.layer_specs import GLU
 from . import reference as ref
 
+F16, F32, I32, I64 = torch.float16, torch.float32, torch.int32, torch.int64
 EPI_F16, EPI_SWIGLU, EPI_PARTIAL, EPI_RELU2 = 0, 1, 2, 5
 
 
@@ -44,6 +45,17 @@ def _np_to_dev(a: np.ndarray, device) -> torch.Tensor:
 
 
 np_to_dev = _np_to_dev
+
+
+def _packed(device: int, dtype, dims: int, *tensors) -> bool:
+    """Whether the tensors (None: not given) have that type, so many dimensions and packed rows, on that device.  (A call of the 8-bit
+    cache's operators asks this of all its tensors; the check that names what is wrong takes twice as long.)"""
+    for t in tensors:
+        if t is not None:
+            strides = t.stride()
+            if t.dtype is not dtype or len(strides) != dims or strides[-1] != 1 or t.get_device() != device:
+                return False
+    return True
 
 
 class TorchOps:
@@ -135,29 +147,34 @@ class TorchOps:
 
     # ---- 8-bit KV cache (cache.quant_kv.QuantKV, one layer) ----------------------------------------------
     @staticmethod
-    def _check_q8(kv, nh: int, nkv: int, hd: int, *tensors) -> None:
-        """``tensors``: (name, tensor or None, dtype, number of dimensions)."""
+    def _heads_q8(kv, nh: int, nkv: int, hd: int) -> int:
+        """The device of a layer that has such heads."""
         shape = kv.data.shape
         if len(shape) != 5 or shape[2] != nkv or shape[4] != hd:
             raise ValueError(f"{nkv} kv heads of {hd} do not match one layer of a cache of shape {tuple(shape)}")
         if nkv < 1 or nh < 1 or nh % nkv:
             raise ValueError(f"{nh} heads over {nkv} kv heads")
-        device = kv.data.get_device()
-        for name, t, dtype, dims in tensors:
+        return kv.data.get_device()
+
+    @staticmethod
+    def _tensors_q8(device: int, **tensors) -> None:
+        """``tensors``: name = (tensor or None, dtype, number of dimensions)."""
+        for name, (t, dtype, dims) in tensors.items():
             if t is None:
                 continue
-            strides = t.stride()
-            if t.dtype is not dtype or len(strides) != dims or (strides[-1] != 1 and t.shape[-1] > 1):
+            if t.dtype is not dtype or t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] > 1):
                 raise ValueError(f"{name}: {dtype} with {dims} dimensions and packed rows expected, not {t.dtype} "
-                                 f"{tuple(t.shape)} with strides {strides}")
+                                 f"{tuple(t.shape)} with strides {t.stride()}")
             if t.get_device() != device:
-                raise ValueError(f"{name} is on {t.device}, the cache on {kv.data.device}")
+                raise ValueError(f"{name} is on {t.device}, not beside the cache")
 
     def _check_write_q8(self, qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out, planes, n_planes, bias):
         cols = (nh + 2 * nkv) * hd
-        f16, f32 = torch.float16, torch.float32
-        self._check_q8(kv, nh, nkv, hd, ("qkv", qkv, f16, 2), ("q_out", q_out, f16, 2), ("bias", bias, f16, 1),
-                       ("positions", positions, torch.int32, 1), ("slots", slots, torch.int64, 1), ("inv_freq", inv_freq, f32, 1))
+        device = self._heads_q8(kv, nh, nkv, hd)
+        if not (_packed(device, F16, 2, qkv, q_out) and _packed(device, I32, 1, positions) and _packed(device, I64, 1, slots)
+                and _packed(device, F32, 1, inv_freq) and _packed(device, F16, 1, bias)):
+            self._tensors_q8(device, qkv=(qkv, F16, 2), q_out=(q_out, F16, 2), bias=(bias, F16, 1), positions=(positions, I32, 1),
+                             slots=(slots, I64, 1), inv_freq=(inv_freq, F32, 1))
         if q_out is None or M < 0 or positions.shape[0] < M or slots.shape[0] < M or q_out.shape[0] < M or q_out.shape[1] < nh * hd:
             raise ValueError(f"{M} rows do not fit positions, slots or q_out")
         if planes is None:
@@ -165,8 +182,8 @@ class TorchOps:
                 raise ValueError(f"{M} rows of {cols} columns expected in qkv")
             if bias is not None:
                 raise ValueError("a bias goes with planes")
-        elif (n_planes < 1 or planes.dtype is not f32 or planes.numel() < n_planes * M * cols or not planes.is_contiguous()
-              or planes.get_device() != kv.data.get_device()):
+        elif (n_planes < 1 or planes.dtype is not F32 or planes.numel() < n_planes * M * cols or not planes.is_contiguous()
+              or planes.get_device() != device):
             raise ValueError(f"{n_planes} planes of {M} rows of {cols} columns expected, packed, beside the cache")
         if bias is not None and bias.shape[0] < cols:
             raise ValueError(f"a bias of {cols} columns expected")
@@ -193,9 +210,12 @@ class TorchOps:
         q_out[:M, : nh * hd] = ref.rope_kv_write_q8(x, kv, positions[:M], slots[:M], inv_freq, nh)
 
     def _check_read_q8(self, kv, block_tables, seq_lens, cu_blocks, S, out, out_tables):
-        shape, i32 = kv.data.shape, torch.int32
-        self._check_q8(kv, shape[2], shape[2], shape[-1], ("block_tables", block_tables, i32, 2), ("seq_lens", seq_lens, i32, 1),
-                       ("cu_blocks", cu_blocks, i32, 1), ("out", out, torch.float16, 5), ("out_tables", out_tables, i32, 2))
+        shape = kv.data.shape
+        device = self._heads_q8(kv, shape[2], shape[2], shape[-1])
+        if not (_packed(device, I32, 2, block_tables, out_tables) and _packed(device, I32, 1, seq_lens, cu_blocks)
+                and _packed(device, F16, 5, out)):
+            self._tensors_q8(device, block_tables=(block_tables, I32, 2), seq_lens=(seq_lens, I32, 1), cu_blocks=(cu_blocks, I32, 1),
+                             out=(out, F16, 5), out_tables=(out_tables, I32, 2))
         if S < 0 or min(block_tables.shape[0], seq_lens.shape[0], cu_blocks.shape[0] - 1, out_tables.shape[0]) < S:
             raise ValueError(f"tables, lengths and places of {S} sequences expected")
         if out.shape[1:] != shape[1:] or not out.is_contiguous():
@@ -209,10 +229,11 @@ class TorchOps:
         ref.kv_read_q8(kv, block_tables[:S], seq_lens[:S], cu_blocks[: S + 1], out, out_tables)
 
     def _check_attn_q8(self, q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q):
-        i32 = torch.int32
-        self._check_q8(kv, nh, nkv, hd, ("q", q, torch.float16, 2), ("out", out, torch.float16, 2),
-                       ("block_tables", block_tables, i32, 2), ("seq_lens", seq_lens, i32, 1), ("cu_q", cu_q, i32, 1),
-                       ("q_pos0", q_pos0, i32, 1))
+        device = self._heads_q8(kv, nh, nkv, hd)
+        if not (_packed(device, F16, 2, q, out) and _packed(device, I32, 2, block_tables)
+                and _packed(device, I32, 1, seq_lens, cu_q, q_pos0)):
+            self._tensors_q8(device, q=(q, F16, 2), out=(out, F16, 2), block_tables=(block_tables, I32, 2), seq_lens=(seq_lens, I32, 1),
+                             cu_q=(cu_q, I32, 1), q_pos0=(q_pos0, I32, 1))
         if nh // nkv > 16:
             raise ValueError(f"{nh // nkv} query heads per kv head: up to 16 expected")
         if S < 0 or block_tables.shape[0] < S or q.shape[1] < nh * hd or out.shape[1] < nh * hd or window < 0:
@@ -708,6 +729,7 @@ class CudaOps(TorchOps):
         native.load(build_if_missing=True, group=group, whole=group is None)
         self.device = torch.device(device)
         self.status = native.Status(self.device)
+        self.status_ptr = self.status.ptr
         self.sm_count = torch.cuda.get_device_properties(self.device).multi_processor_count
         # decode-sized passes (<= 64 tokens) of the INT4 layers: bit 0 = gate/up + SwiGLU, bit 1 = fused QKV + bias +
         # RoPE + KV-cache write, bit 2 = every other INT4 linear, through the persistent kernel (csrc/gemm_w4_dec.cu)
@@ -1285,17 +1307,17 @@ class CudaOps(TorchOps):
                          bias=None):
         q_out = qkv if q_out is None else q_out
         self._check_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out, planes, n_planes, bias)
-        self.n.rope_kv_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, q_out, planes, n_planes, bias, self.status.ptr)
+        self.n.rope_kv_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, q_out, planes, n_planes, bias, self.status_ptr)
 
     def kv_read_q8(self, kv, block_tables, seq_lens, cu_blocks, S, out, out_tables):
         self._check_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables)
-        self.n.kv_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables, self.status.ptr)
+        self.n.kv_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables, self.status_ptr)
 
     def attn_decode_q8(self, q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, scale, scratch=None, num_splits=0, window=0,
                        cu_q=None, q_pos0=None, max_q=1):
         self._check_attn_q8(q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q)
         self.n.attn_decode_q8(q, kv, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch, num_splits, scale, window,
-                              self.status.ptr)
+                              self.status_ptr)
 
     def headnorm_rope_kv_write(self, qkv, kv_layer, positions, slots, freqs, q_norm_w, k_norm_w, norm_v, k_is_v, eps,
                                M, nh, nkv, hd, block_size):

@@ -550,14 +550,14 @@ def rope_kv_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, q_out, planes, 
     _launched(load().zse_rope_kv_write_q8(_WRITE_Q8.pack(
         *cache, 0 if qkv is None else qkv.data_ptr(), q_out.data_ptr(), 0 if planes is None else planes.data_ptr(),
         0 if bias is None else bias.data_ptr(), positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(), status, stream,
-        0 if qkv is None else qkv.stride(0), q_out.stride(0), n_planes, M, nh, 2 * inv_freq.shape[0])), "rope_kv_write_q8")
+        0 if qkv is None else qkv.stride()[0], q_out.stride()[0], n_planes, M, nh, 2 * inv_freq.shape[0])), "rope_kv_write_q8")
 
 
 def kv_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables, status):
     cache, stream = _cache_q8(kv)
     _launched(load().zse_kv_read_q8(_READ_Q8.pack(
         *cache, block_tables.data_ptr(), seq_lens.data_ptr(), cu_blocks.data_ptr(), out.data_ptr(), out_tables.data_ptr(), status,
-        stream, block_tables.stride(0), block_tables.shape[1], S, out.shape[0], out_tables.stride(0), out_tables.shape[1])),
+        stream, block_tables.stride()[0], block_tables.shape[1], S, out.shape[0], out_tables.stride()[0], out_tables.shape[1])),
         "kv_read_q8")
 
 
@@ -566,8 +566,8 @@ def _attn_q8_args(cache, stream, q, block_tables, seq_lens, cu_q, q_pos0, S, max
     return _ATTN_Q8.pack(
         *cache, q.data_ptr(), block_tables.data_ptr(), 0 if seq_lens is None else seq_lens.data_ptr(),
         0 if cu_q is None else cu_q.data_ptr(), 0 if q_pos0 is None else q_pos0.data_ptr(), out.data_ptr(),
-        0 if scratch is None else scratch.data_ptr(), status, stream, 0 if scratch is None else scratch.numel(), q.stride(0),
-        out.stride(0), min(q.shape[0], out.shape[0]), block_tables.stride(0), block_tables.shape[1], S, max_q, nh, num_splits, window,
+        0 if scratch is None else scratch.data_ptr(), status, stream, 0 if scratch is None else scratch.numel(), q.stride()[0],
+        out.stride()[0], min(q.shape[0], out.shape[0]), block_tables.stride()[0], block_tables.shape[1], S, max_q, nh, num_splits, window,
         scale, 0)
 
 
