@@ -250,6 +250,68 @@ def test_many_sequences(ops):
     attend(ops, [1 + (53 * i) % 90 for i in range(130)], 8, 8, 128, rows=[1 + i % 2 if (53 * i) % 90 else 1 for i in range(130)])
 
 
+@pytest.mark.parametrize("nh,nkv,rows", [(16, 16, 1), (64, 16, 1), (40, 8, 5), (32, 16, 3)])
+def test_more_pieces_than_fit_at_a_time(ops, nh, nkv, rows):
+    """Up to 64 sequences are then taken the longest first: alike ones, empty ones, ones that windows make alike."""
+    lens = [300, 0, 17, 300, 2, 64, 64, 1] * 8
+    draft = None if rows == 1 else [min(n, 1 + i % rows) for i, n in enumerate(lens)]
+    for S in (64, 63, 33):
+        for window in (0, 40):
+            attend(ops, lens[:S], nh, nkv, 64, rows=draft and draft[:S], window=window, splits=4)
+    attend(ops, list(range(1, 64)), nh, nkv, 128, rows=draft and [min(n, 2) for n in range(1, 64)], splits=8)
+
+
+def test_tables_inside_wider_ones(ops):
+    g = gen(21)
+    nh, nkv, hd, bs, lens = 8, 2, 64, 16, [40, 100, 5]
+    data, scale = make_cache(g, 12, nkv, bs, hd, DEV)
+    wide = torch.full((3, 20), 10 ** 6, dtype=torch.int32, device=DEV)           # what stands beside is no block
+    wide[:, 3:10] = make_tables(g, lens, bs, 12, DEV, width=7)
+    tables = wide[:, 3:10]
+    q = torch.randn(3, nh * hd, generator=g).half().to(DEV)
+    out = torch.zeros(3, nh * hd, dtype=torch.float16, device=DEV)
+    ops.attn_decode_q8(q, QuantKV(data, scale), tables, ints(lens), out, 3, nh, nkv, hd, scale_of(hd))
+    want, tol = attention(q, data, scale, tables, list(enumerate(lens)), nh, scale_of(hd))
+    assert ((out.double() - want).abs() <= tol).all()
+    pages, places = torch.zeros(11, 2, nkv, bs, hd, dtype=torch.float16, device=DEV), torch.full((3, 30), 5, dtype=torch.int32, device=DEV)
+    ops.kv_read_q8(QuantKV(data, scale), tables, ints(lens), ints([0, 3, 10, 11]), 3, pages, places[:, 4:12])
+    assert places[:, 4:12].tolist() == [[0, 1, 2] + [-1] * 5, [3, 4, 5, 6, 7, 8, 9, -1], [10] + [-1] * 7]
+    assert (places[:, :4] == 5).all() and (places[:, 12:] == 5).all()
+    torch.cuda.synchronize()
+    ops.check()
+
+
+def test_calls_of_nothing(ops):
+    nh, nkv, hd = 4, 2, 64
+    kv = QuantKV(*make_cache(gen(1), 2, nkv, 16, hd, DEV))
+    before = kv.data.clone(), kv.scale.clone()
+    e16, e32, e64 = (torch.zeros(0, 8 * hd, dtype=torch.float16, device=DEV), torch.zeros(0, dtype=torch.int32, device=DEV),
+                     torch.zeros(0, dtype=torch.int64, device=DEV))
+    ops.rope_kv_write_q8(e16, kv, e32, e64, freqs_of(hd), 0, nh, nkv, hd)
+    ops.attn_decode_q8(e16, kv, torch.zeros(0, 1, dtype=torch.int32, device=DEV), e32, e16, 0, nh, nkv, hd, scale_of(hd))
+    places = torch.zeros(0, 1, dtype=torch.int32, device=DEV)
+    ops.kv_read_q8(kv, places, e32, ints([0]), 0, torch.zeros(1, 2, nkv, 16, hd, dtype=torch.float16, device=DEV), places)
+    out = torch.full((2, nh * hd), 7.0, dtype=torch.float16, device=DEV)                     # tables without columns: nothing is seen
+    ops.attn_decode_q8(out.clone(), kv, torch.zeros(2, 0, dtype=torch.int32, device=DEV), ints([0, 0]), out, 2, nh, nkv, hd, scale_of(hd))
+    torch.cuda.synchronize()
+    ops.check()
+    assert (out == 0).all() and torch.equal(before[0], kv.data) and torch.equal(before[1], kv.scale)
+
+
+def test_results_over_the_queries(ops):
+    """The result may go where the queries were."""
+    nh, nkv, hd, lens = 14, 2, 128, [700, 31, 2000]
+    g = gen(8)
+    data, scale = make_cache(g, 180, nkv, 16, hd, DEV)
+    tables = make_tables(g, lens, 16, 180, DEV)
+    q = torch.randn(3, nh * hd, generator=g).half().to(DEV)
+    for splits in (0, 1, 8, 64):
+        out, inplace = torch.zeros_like(q), q.clone()
+        for to, src in ((out, q), (inplace, inplace)):
+            ops.attn_decode_q8(src, QuantKV(data, scale), tables, ints(lens), to, 3, nh, nkv, hd, scale_of(hd), num_splits=splits)
+        assert torch.equal(out, inplace)
+
+
 def test_long_sequence(ops):
     attend(ops, [40001], 7, 1, 128)
     attend(ops, [20011, 3], 8, 1, 128, rows=[4, 1])
