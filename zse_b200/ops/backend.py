@@ -47,17 +47,6 @@ def _np_to_dev(a: np.ndarray, device) -> torch.Tensor:
 np_to_dev = _np_to_dev
 
 
-def _packed(device: int, dtype, dims: int, *tensors) -> bool:
-    """Whether the tensors (None: not given) have that type, so many dimensions and packed rows, on that device.  (A call of the 8-bit
-    cache's operators asks this of all its tensors; the check that names what is wrong takes twice as long.)"""
-    for t in tensors:
-        if t is not None:
-            strides = t.stride()
-            if t.dtype is not dtype or len(strides) != dims or strides[-1] != 1 or t.get_device() != device:
-                return False
-    return True
-
-
 class TorchOps:
     name = "torch"
 
@@ -171,10 +160,8 @@ class TorchOps:
     def _check_write_q8(self, qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out, planes, n_planes, bias):
         cols = (nh + 2 * nkv) * hd
         device = self._heads_q8(kv, nh, nkv, hd)
-        if not (_packed(device, F16, 2, qkv, q_out) and _packed(device, I32, 1, positions) and _packed(device, I64, 1, slots)
-                and _packed(device, F32, 1, inv_freq) and _packed(device, F16, 1, bias)):
-            self._tensors_q8(device, qkv=(qkv, F16, 2), q_out=(q_out, F16, 2), bias=(bias, F16, 1), positions=(positions, I32, 1),
-                             slots=(slots, I64, 1), inv_freq=(inv_freq, F32, 1))
+        self._tensors_q8(device, qkv=(qkv, F16, 2), q_out=(q_out, F16, 2), bias=(bias, F16, 1), positions=(positions, I32, 1),
+                         slots=(slots, I64, 1), inv_freq=(inv_freq, F32, 1))
         if q_out is None or M < 0 or positions.shape[0] < M or slots.shape[0] < M or q_out.shape[0] < M or q_out.shape[1] < nh * hd:
             raise ValueError(f"{M} rows do not fit positions, slots or q_out")
         if planes is None:
@@ -212,10 +199,8 @@ class TorchOps:
     def _check_read_q8(self, kv, block_tables, seq_lens, cu_blocks, S, out, out_tables):
         shape = kv.data.shape
         device = self._heads_q8(kv, shape[2], shape[2], shape[-1])
-        if not (_packed(device, I32, 2, block_tables, out_tables) and _packed(device, I32, 1, seq_lens, cu_blocks)
-                and _packed(device, F16, 5, out)):
-            self._tensors_q8(device, block_tables=(block_tables, I32, 2), seq_lens=(seq_lens, I32, 1), cu_blocks=(cu_blocks, I32, 1),
-                             out=(out, F16, 5), out_tables=(out_tables, I32, 2))
+        self._tensors_q8(device, block_tables=(block_tables, I32, 2), seq_lens=(seq_lens, I32, 1), cu_blocks=(cu_blocks, I32, 1),
+                         out=(out, F16, 5), out_tables=(out_tables, I32, 2))
         if S < 0 or min(block_tables.shape[0], seq_lens.shape[0], cu_blocks.shape[0] - 1, out_tables.shape[0]) < S:
             raise ValueError(f"tables, lengths and places of {S} sequences expected")
         if out.shape[1:] != shape[1:] or not out.is_contiguous():
@@ -230,10 +215,8 @@ class TorchOps:
 
     def _check_attn_q8(self, q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q):
         device = self._heads_q8(kv, nh, nkv, hd)
-        if not (_packed(device, F16, 2, q, out) and _packed(device, I32, 2, block_tables)
-                and _packed(device, I32, 1, seq_lens, cu_q, q_pos0)):
-            self._tensors_q8(device, q=(q, F16, 2), out=(out, F16, 2), block_tables=(block_tables, I32, 2), seq_lens=(seq_lens, I32, 1),
-                             cu_q=(cu_q, I32, 1), q_pos0=(q_pos0, I32, 1))
+        self._tensors_q8(device, q=(q, F16, 2), out=(out, F16, 2), block_tables=(block_tables, I32, 2), seq_lens=(seq_lens, I32, 1),
+                         cu_q=(cu_q, I32, 1), q_pos0=(q_pos0, I32, 1))
         if nh // nkv > 16:
             raise ValueError(f"{nh // nkv} query heads per kv head: up to 16 expected")
         if S < 0 or block_tables.shape[0] < S or q.shape[1] < nh * hd or out.shape[1] < nh * hd or window < 0:
@@ -1303,21 +1286,92 @@ class CudaOps(TorchOps):
         self.n.attn_prefill_ext(qkv, qkv.stride(0), kv_layer, block_tables, cu_q, q_pos0, out, out.stride(0),
                                 num_seqs, max_q_len, nh, nkv, hd, block_size, scale, softcap, window)
 
+    # (The three calls of the 8-bit cache are written out flat: outside a CUDA graph a small one is mostly Python.  What is plainly in
+    # order is seen at a glance; the checks of the base class take the rest and name what is wrong.)
     def rope_kv_write_q8(self, qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out=None, planes=None, n_planes=0,
                          bias=None):
-        q_out = qkv if q_out is None else q_out
-        self._check_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out, planes, n_planes, bias)
-        self.n.rope_kv_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, q_out, planes, n_planes, bias, self.status_ptr)
+        if q_out is None:
+            q_out = qkv
+        data, scale = kv.data, kv.scale
+        device, shape, cols, ld = data.get_device(), data.shape, (nh + 2 * nkv) * hd, (0, 1)
+        if qkv is not None:
+            ld, rows = qkv.stride(), qkv.shape
+        ldq = ld if q_out is qkv else q_out.stride()
+        if planes is None:
+            fine = (qkv is not None and bias is None and qkv.dtype is F16 and len(ld) == 2 and ld[1] == 1 and rows[0] >= M
+                    and rows[1] >= cols and qkv.get_device() == device)
+        else:
+            fine = ((qkv is None or qkv is q_out) and q_out is not None and n_planes > 0 and planes.dtype is F32
+                    and planes.is_contiguous() and planes.numel() >= n_planes * M * cols and planes.get_device() == device
+                    and (bias is None or bias.dtype is F16 and bias.stride() == (1,) and bias.shape[0] >= cols
+                         and bias.get_device() == device))
+        if not (fine and len(shape) == 5 and shape[2] == nkv and shape[4] == hd and nkv > 0 and nh > 0 and nh % nkv == 0 and M >= 0
+                and q_out.dtype is F16 and positions.dtype is I32 and slots.dtype is I64 and inv_freq.dtype is F32
+                and len(ldq) == 2 and ldq[1] == 1 and q_out.shape[0] >= M and q_out.shape[1] >= nh * hd
+                and positions.stride() == (1,) and slots.stride() == (1,) and inv_freq.stride() == (1,)
+                and positions.shape[0] >= M and slots.shape[0] >= M and inv_freq.shape[0] % 8 == 0
+                and 2 * inv_freq.shape[0] <= hd and q_out.get_device() == device and positions.get_device() == device
+                and slots.get_device() == device and inv_freq.get_device() == device):
+            self._check_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out, planes, n_planes, bias)
+        n = self.n
+        stream = n.stream_q8(data, scale)
+        n.launched(n.load().zse_rope_kv_write_q8(n.WRITE_Q8.pack(
+            data.data_ptr(), scale.data_ptr(), shape[0], shape[2], shape[3], shape[4], 0 if qkv is None else qkv.data_ptr(),
+            q_out.data_ptr(), 0 if planes is None else planes.data_ptr(), 0 if bias is None else bias.data_ptr(),
+            positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(), self.status_ptr, stream,
+            ld[0], ldq[0], n_planes, M, nh, 2 * inv_freq.shape[0])), "rope_kv_write_q8")
 
     def kv_read_q8(self, kv, block_tables, seq_lens, cu_blocks, S, out, out_tables):
-        self._check_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables)
-        self.n.kv_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables, self.status_ptr)
+        data, scale = kv.data, kv.scale
+        device, shape, pages, ld, ldo = data.get_device(), data.shape, out.shape, block_tables.stride(), out_tables.stride()
+        rows, rows_out = block_tables.shape, out_tables.shape
+        if not (len(shape) == 5 and len(ld) == 2 and ld[1] == 1 and len(ldo) == 2 and ldo[1] == 1 and pages[1:] == shape[1:] and S >= 0
+                and out.is_contiguous() and out.dtype is F16 and block_tables.dtype is I32 and out_tables.dtype is I32
+                and seq_lens.dtype is I32 and cu_blocks.dtype is I32 and seq_lens.stride() == (1,) and cu_blocks.stride() == (1,)
+                and rows[0] >= S and rows_out[0] >= S and seq_lens.shape[0] >= S and cu_blocks.shape[0] > S
+                and out.get_device() == device and block_tables.get_device() == device and out_tables.get_device() == device
+                and seq_lens.get_device() == device and cu_blocks.get_device() == device):
+            self._check_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables)
+        n = self.n
+        stream = n.stream_q8(data, scale)
+        n.launched(n.load().zse_kv_read_q8(n.READ_Q8.pack(
+            data.data_ptr(), scale.data_ptr(), shape[0], shape[2], shape[3], shape[4], block_tables.data_ptr(), seq_lens.data_ptr(),
+            cu_blocks.data_ptr(), out.data_ptr(), out_tables.data_ptr(), self.status_ptr, stream, ld[0], rows[1], S, pages[0], ldo[0],
+            rows_out[1])), "kv_read_q8")
 
     def attn_decode_q8(self, q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, scale, scratch=None, num_splits=0, window=0,
                        cu_q=None, q_pos0=None, max_q=1):
-        self._check_attn_q8(q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q)
-        self.n.attn_decode_q8(q, kv, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch, num_splits, scale, window,
-                              self.status_ptr)
+        data, scales = kv.data, kv.scale
+        device, shape, ld, ldq, ldo = data.get_device(), data.shape, block_tables.stride(), q.stride(), out.stride()
+        tables, rows, rows_out = block_tables.shape, q.shape, out.shape
+        if cu_q is None:
+            fine = max_q == 1 and q_pos0 is None and seq_lens is not None and seq_lens.shape[0] >= S and rows[0] >= S and rows_out[0] >= S
+        else:
+            fine = (q_pos0 is not None and 1 <= max_q <= 64 and cu_q.dtype is I32 and q_pos0.dtype is I32 and cu_q.stride() == (1,)
+                    and q_pos0.stride() == (1,) and cu_q.shape[0] > S and q_pos0.shape[0] >= S and cu_q.get_device() == device
+                    and q_pos0.get_device() == device)
+        if not (fine and len(shape) == 5 and shape[2] == nkv and shape[4] == hd and nkv > 0 and nh > 0 and nh % nkv == 0
+                and nh <= 16 * nkv and S >= 0 and window >= 0 and len(ld) == 2 and ld[1] == 1 and len(ldq) == 2 and ldq[1] == 1 and len(ldo) == 2 and ldo[1] == 1
+                and q.dtype is F16 and out.dtype is F16 and block_tables.dtype is I32 and tables[0] >= S and rows[1] >= nh * hd
+                and rows_out[1] >= nh * hd and q.get_device() == device and out.get_device() == device
+                and block_tables.get_device() == device
+                and (seq_lens is None or seq_lens.dtype is I32 and seq_lens.stride() == (1,) and seq_lens.get_device() == device)):
+            self._check_attn_q8(q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q)
+        n = self.n
+        stream, lib = n.stream_q8(data, scales), n.load()
+        at = lambda t: 0 if t is None else t.data_ptr()
+        while True:
+            args = n.ATTN_Q8.pack(
+                data.data_ptr(), scales.data_ptr(), shape[0], shape[2], shape[3], shape[4], q.data_ptr(), block_tables.data_ptr(),
+                at(seq_lens), at(cu_q), at(q_pos0), out.data_ptr(), at(scratch), self.status_ptr, stream,
+                0 if scratch is None else scratch.numel(), ldq[0], ldo[0], min(rows[0], rows_out[0]), ld[0], tables[1], S, max_q, nh,
+                num_splits, window, scale, 0)
+            launches = lib.zse_attn_decode_q8(args)
+            if launches != n.NEEDS_SCRATCH or scratch is not None:
+                break
+            # nothing was launched
+            scratch = torch.empty(lib.zse_attn_decode_q8_scratch_floats(args), dtype=F32, device=data.device)
+        n.launched(launches, "attn_decode_q8")
 
     def headnorm_rope_kv_write(self, qkv, kv_layer, positions, slots, freqs, q_norm_w, k_norm_w, norm_v, k_is_v, eps,
                                M, nh, nkv, hd, block_size):

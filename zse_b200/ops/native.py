@@ -110,11 +110,13 @@ class Space(Structure):
                 ("state_ld", c_int32)] + [(n, c_void_p) for n in ("conv_w", "conv_b", "dt_bias", "neg_a", "skip")]
 
 
-# (the calls of the 8-bit cache pack their arguments into bytes of these layouts: a third of what a call of 22 arguments costs)
+# The calls of the 8-bit cache take their arguments as bytes of these layouts (ZseWriteQ8, ZseReadQ8, ZseAttnQ8 in csrc/api.h): a third
+# of what a call of 22 arguments costs.
 _KV_Q8 = "QQiiii"
-_WRITE_Q8 = struct.Struct("<" + _KV_Q8 + "9Q6i")
-_READ_Q8 = struct.Struct("<" + _KV_Q8 + "7Q6i")
-_ATTN_Q8 = struct.Struct("<" + _KV_Q8 + "9Qq10ifi")
+WRITE_Q8 = struct.Struct("<" + _KV_Q8 + "9Q6i")
+READ_Q8 = struct.Struct("<" + _KV_Q8 + "7Q6i")
+ATTN_Q8 = struct.Struct("<" + _KV_Q8 + "9Qq10ifi")
+NEEDS_SCRATCH = -6
 
 _lib: Optional[ctypes.CDLL] = None
 
@@ -525,71 +527,30 @@ def rope_kv_write(qkv, kv_layer, positions, slots, inv_freq, M, nh, nkv, hd, rot
                                  rotary_dim, block_size, _p(planes), n_planes, _p(bias), _stream()), "rope_kv_write")
 
 
-# ---- 8-bit KV cache: ``kv`` is one layer of a ``cache.quant_kv.QuantKV``; every call gives the number of kernels it launched -------
-def _cache_q8(kv) -> tuple:
-    """The layer's address and sizes, and the current stream of its device, which has to be the current device.  (The two calls
-    below the public ones: ``torch.cuda.current_stream()`` makes a stream object and takes longer than the rest of a call here.)"""
-    data, scale = kv.data, kv.scale
+# ---- 8-bit KV cache: ``ops.backend.CudaOps`` packs the arguments of its calls itself, see there ------------------------------------
+def stream_q8(data, scale) -> int:
+    """The current stream of the cache's device, which has to be the current device.  (The two calls below the public ones:
+    ``torch.cuda.current_stream()`` makes a stream object and takes longer than the rest of a call.)"""
     at = torch._C._cuda_getDevice()
     if data.get_device() != at:
         raise NativeError(f"the cache is on {data.device}, the current device is {at}")
     if not (data.is_contiguous() and scale.is_contiguous()):
         raise NativeError("a layer of an 8-bit cache has to be contiguous")
-    blocks, _, nkv, block_size, hd = data.shape
-    return (data.data_ptr(), scale.data_ptr(), blocks, nkv, block_size, hd), torch._C._cuda_getCurrentRawStream(at)
+    return torch._C._cuda_getCurrentRawStream(at)
 
 
-def _launched(n: int, what: str) -> None:
+def launched(n: int, what: str) -> None:
+    """``n``: kernels launched, or an error."""
     if n < 0:
         raise NativeError(f"{what}: {_ERRORS.get(n, n)}")
     LAUNCHES[0] += n
 
 
-def rope_kv_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, q_out, planes, n_planes, bias, status):
-    cache, stream = _cache_q8(kv)
-    _launched(load().zse_rope_kv_write_q8(_WRITE_Q8.pack(
-        *cache, 0 if qkv is None else qkv.data_ptr(), q_out.data_ptr(), 0 if planes is None else planes.data_ptr(),
-        0 if bias is None else bias.data_ptr(), positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(), status, stream,
-        0 if qkv is None else qkv.stride()[0], q_out.stride()[0], n_planes, M, nh, 2 * inv_freq.shape[0])), "rope_kv_write_q8")
-
-
-def kv_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables, status):
-    cache, stream = _cache_q8(kv)
-    _launched(load().zse_kv_read_q8(_READ_Q8.pack(
-        *cache, block_tables.data_ptr(), seq_lens.data_ptr(), cu_blocks.data_ptr(), out.data_ptr(), out_tables.data_ptr(), status,
-        stream, block_tables.stride()[0], block_tables.shape[1], S, out.shape[0], out_tables.stride()[0], out_tables.shape[1])),
-        "kv_read_q8")
-
-
-def _attn_q8_args(cache, stream, q, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch, num_splits, scale, window,
-                  status) -> bytes:
-    return _ATTN_Q8.pack(
-        *cache, q.data_ptr(), block_tables.data_ptr(), 0 if seq_lens is None else seq_lens.data_ptr(),
-        0 if cu_q is None else cu_q.data_ptr(), 0 if q_pos0 is None else q_pos0.data_ptr(), out.data_ptr(),
-        0 if scratch is None else scratch.data_ptr(), status, stream, 0 if scratch is None else scratch.numel(), q.stride()[0],
-        out.stride()[0], min(q.shape[0], out.shape[0]), block_tables.stride()[0], block_tables.shape[1], S, max_q, nh, num_splits, window,
-        scale, 0)
-
-
-def attn_decode_q8(q, kv, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch, num_splits, scale, window, status):
-    """``scratch``: fp32, ``attn_decode_q8_scratch_floats`` of it, or None (then a call that needs some allocates it)."""
-    lib = load()
-    cache, stream = _cache_q8(kv)
-    args = _attn_q8_args(cache, stream, q, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch, num_splits, scale,
-                         window, status)
-    n = lib.zse_attn_decode_q8(args)
-    if n == -6 and scratch is None:                    # nothing was launched
-        scratch = torch.empty(lib.zse_attn_decode_q8_scratch_floats(args), dtype=torch.float32, device=kv.data.device)
-        n = lib.zse_attn_decode_q8(_attn_q8_args(cache, stream, q, block_tables, seq_lens, cu_q, q_pos0, S, max_q, out, nh, scratch,
-                                                 num_splits, scale, window, status))
-    _launched(n, "attn_decode_q8")
-
-
 def attn_decode_q8_plan(S, max_q, nh, nkv, hd, block_size, max_blocks, window=0, num_splits=0) -> tuple:
     """(pieces of a sequence and kv head, fp32 values of scratch) of such a call."""
     lib = load()
-    args = _ATTN_Q8.pack(0, 0, 1, nkv, block_size, hd, 0, 0, 0, max_q > 1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, max_blocks, S, max_q, nh,
-                         num_splits, window, 1.0, 0)
+    args = ATTN_Q8.pack(0, 0, 1, nkv, block_size, hd, 0, 0, 0, max_q > 1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, max_blocks, S, max_q, nh,
+                        num_splits, window, 1.0, 0)
     return lib.zse_attn_decode_q8_pieces(args), lib.zse_attn_decode_q8_scratch_floats(args)
 
 
