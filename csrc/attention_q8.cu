@@ -73,6 +73,11 @@ __device__ __forceinline__ uint32_t minus_1152(uint32_t x) {           // both h
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x64806480u));
   return y;
 }
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // Barrier of the cluster in two halves: the relaxed form only says that a CTA has got there, the other one orders its writes.
 __device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -152,8 +157,8 @@ struct Q8Smem {
   static constexpr int kRing = kStages * kSlot > kCols * kPitch * 4 ? kStages * kSlot : kCols * kPitch * 4;   // of a warp
   static constexpr int kQPitch = HD * 2 + 32;                          // bytes: four columns in different groups of eight banks
   static constexpr bool kQShared = NB > 1;                             // queries in shared memory, or in registers
-  static constexpr int kNumbers = kWarps * kRing;                      // own_m, own_l [warp][column], own_ref [warp]
-  static constexpr int kGot = kNumbers + (2 * kWarps * kCols + kWarps) * 4;            // references and sums, [CTA][column][2]
+  static constexpr int kNumbers = kWarps * kRing;                      // own_m, own_l [warp][column]
+  static constexpr int kGot = kNumbers + 2 * kWarps * kCols * 4;       // references and sums, [CTA][column][2]
   static constexpr int kGotO = kGot + 2 * kMostCluster * kCols * 4;                    // results, [CTA][its share here] of 16 bytes
   static constexpr int kQ = kGotO + (kCols * HD / 4 + kMostCluster) * 16;
   static constexpr int kTotal = kQ + (kQShared ? kCols * kQPitch : 0);
@@ -170,7 +175,6 @@ attn_q8_kernel(const Q8Args a) {
   extern __shared__ __align__(128) uint8_t smem[];
   float* own_m = reinterpret_cast<float*>(smem + S::kNumbers);         // [warp][column]
   float* own_l = own_m + kWarps * S::kCols;
-  float* own_ref = own_l + kWarps * S::kCols;                          // [warp]
   pdl_launch_dependents();
   pdl_wait();
   // (what every CTA does once is kept short: with one tile per warp it is most of its instructions)
@@ -192,8 +196,8 @@ attn_q8_kernel(const Q8Args a) {
     row0 = first + rg * a.rows_per;
     rows = min(a.rows_per, count - rg * a.rows_per);
     base_len = a.q_pos0[s] + rg * a.rows_per + 1;
-    if (count > 0 && (first < 0 || count > a.max_q || first + count > a.q_rows)) {
-      if (tid == 0) complain(a.st, 73, s);
+    if (count <= 0 || first < 0 || count > a.max_q || first + count > a.q_rows) {
+      if (tid == 0 && count > 0) complain(a.st, 73, s);
       rows = 0;
     }
   } else {
@@ -301,10 +305,13 @@ attn_q8_kernel(const Q8Args a) {
     sum_q[nb][1] = sum[1] * -7.62939453125e-6f;
   }
 
-  // Weights are 2^(score - m): m is a score of the column that none so far exceeds by more than 6, so that it and what has been summed
-  // change seldom (kNone: nothing seen).  ref: a power of two that no value's scale so far exceeds; o holds sums of weight * vscale /
-  // ref, which fp16 takes.
-  float o[NB][kChunks][4], m[NB][2], l[NB][2], ref = 0.f, inv_ref = 0.f;
+  // Weights are 2^(score - m), and what goes into the products is weight * vscale, in fp16: so m, one for every column, is what makes the
+  // largest of those 64 when it is set, and it and what has been summed change only where one comes out above 2^14 (kNone: nothing seen).
+  // With the largest score and the largest vscale apart, a token of large values and little weight takes the others' bits (values 10^6
+  // times the others': results off by a fifth).  Weights are at most 2^40 then, however small the values: below that fp16 has zero for
+  // the result.
+  constexpr float kMost = 16384.f, kMostSum = 1e27f;
+  float o[NB][kChunks][4], m[NB][2], l[NB][2];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     m[nb][0] = m[nb][1] = kNone;
@@ -325,7 +332,7 @@ attn_q8_kernel(const Q8Args a) {
     if (hole) continue;
     const int tok = (tile0 + first_tile + i * stride) << 4;
     const float k0 = load_shared(scales) * a.scale_log2, k1 = load_shared(scales + 32) * a.scale_log2;      // (with the 2^24 of the bytes)
-    float w0 = load_shared(scales + 64), w1 = load_shared(scales + 96);
+    const float w0 = load_shared(scales + 64), w1 = load_shared(scales + 96);
     float sc[NB][kChains][4];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -370,27 +377,22 @@ attn_q8_kernel(const Q8Args a) {
             t[nb][e] = -INFINITY;
           }
         }
-      if (tok + g >= most_len) w0 = 0.f;                               // what lies behind the sequence may be anything
-      if (tok + g + 8 >= most_len) w1 = 0.f;
     }
-    bool over = fmaxf(w0, w1) > ref;
+    float w[NB][4], sum[NB][2];
+    bool over = false;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) over |= t[nb][e] > 6.f;
-    if (__any_sync(0xffffffffu, over)) {
-      // new references: the tile's maxima where they are above, and what has been summed scaled to them
-      float wtop = fmaxf(fmaxf(w0, w1), 0.f);
-#pragma unroll
-      for (int sh = 4; sh < 32; sh <<= 1) wtop = fmaxf(wtop, __shfl_xor_sync(0xffffffffu, wtop, sh));
-      float fade = 1.f;
-      if (wtop > ref) {
-        // the power of two above twice the scale, so that a slowly growing scale does not come here every time
-        const float up = __uint_as_float(((__float_as_uint(fmaxf(wtop, 1e-30f)) >> 23) + 2u) << 23);
-        inv_ref = 1.f / up;
-        fade = ref * inv_ref;
-        ref = up;
+      for (int e = 0; e < 2; ++e) {
+        const float p0 = ex2(t[nb][e]), p1 = ex2(t[nb][e + 2]);
+        w[nb][e] = p0 * w0;
+        w[nb][e + 2] = p1 * w1;
+        sum[nb][e] = l[nb][e] + (p0 + p1);
+        over |= fmaxf(w[nb][e], w[nb][e + 2]) > kMost || sum[nb][e] > kMostSum;
       }
+    if (__any_sync(0xffffffffu, over)) {
+      // new references, where the tile's are above, and what has been summed scaled to them
+      const float log0 = lg2(w0), log1 = lg2(w1);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         float f[2];
@@ -398,15 +400,16 @@ attn_q8_kernel(const Q8Args a) {
         for (int e = 0; e < 2; ++e) {
           const float v0 = (dead >> (nb * 4 + e)) & 1u ? -INFINITY : sc[nb][0][e] * k0;
           const float v1 = (dead >> (nb * 4 + e + 2)) & 1u ? -INFINITY : sc[nb][0][e + 2] * k1;
-          float x = fmaxf(v0, v1);
+          float to = fmaxf(fmaxf(v0, v1) - 40.f, fmaxf(v0 + log0, v1 + log1) - 6.f);   // (fmaxf passes over what is no number)
 #pragma unroll
-          for (int sh = 4; sh < 32; sh <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, sh));
-          const float to = fmaxf(m[nb][e], x), drop = ex2(m[nb][e] - to);
+          for (int sh = 4; sh < 32; sh <<= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, sh));
+          to = fmaxf(m[nb][e], to);
+          f[e] = ex2(m[nb][e] - to);
           m[nb][e] = to;
-          l[nb][e] *= drop;
-          f[e] = drop * fade;
-          t[nb][e] = v0 - to;
-          t[nb][e + 2] = v1 - to;
+          const float p0 = ex2(v0 - to), p1 = ex2(v1 - to);
+          w[nb][e] = p0 * w0;
+          w[nb][e + 2] = p1 * w1;
+          sum[nb][e] = l[nb][e] * f[e] + (p0 + p1);
         }
 #pragma unroll
         for (int d = 0; d < kChunks; ++d) {
@@ -417,28 +420,21 @@ attn_q8_kernel(const Q8Args a) {
         }
       }
     }
-    w0 *= inv_ref;
-    w1 *= inv_ref;
     uint32_t pb[NB][2], rest[NB][2];                                   // tokens 0..7 and 8..15, [column][token]: the B operand
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      float w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p = ex2(t[nb][e]);
-        l[nb][e & 1] += p;
-        w[e] = p * (e < 2 ? w0 : w1);
-      }
+      l[nb][0] = sum[nb][0];
+      l[nb][1] = sum[nb][1];
       if (dead) {                                                      // (a weight of zero times a scale that is no number)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if ((dead >> (nb * 4 + e)) & 1u) w[e] = 0.f;
+          if ((dead >> (nb * 4 + e)) & 1u) w[nb][e] = 0.f;
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t x = pack_half2(w[2 * h], w[2 * h + 1]);
+        const uint32_t x = pack_half2(w[nb][2 * h], w[nb][2 * h + 1]);
         const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&x));
-        const uint32_t y = pack_half2(w[2 * h] - back.x, w[2 * h + 1] - back.y);
+        const uint32_t y = pack_half2(w[nb][2 * h] - back.x, w[nb][2 * h + 1] - back.y);
         pb[nb][h] = turn_8x8(PACKED && t2 >= 4 ? y : x);
         rest[nb][h] = PACKED ? 0u : turn_8x8(y);
       }
@@ -481,7 +477,6 @@ attn_q8_kernel(const Q8Args a) {
         own_l[warp * S::kCols + c] = l[nb][e];
       }
     }
-  if (lane == 0) own_ref[warp] = ref;
   __syncthreads();
   const int cols = rows * a.group, item = (s * a.nkv + kvh) * a.row_groups + rg;
   constexpr int kQuads = HD / 4;
@@ -510,18 +505,17 @@ attn_q8_kernel(const Q8Args a) {
     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, own_m[w * S::kCols + c]);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float mw = own_m[w * S::kCols + c], f = ex2(mw - top);
+      const float f = ex2(own_m[w * S::kCols + c] - top);
       float4 x = *reinterpret_cast<const float4*>(smem + w * S::kRing + (c * S::kPitch + d) * 4);
       if constexpr (PACKED) {
         const float4 y = *reinterpret_cast<const float4*>(smem + w * S::kRing + ((c + 4) * S::kPitch + d) * 4);
         x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
       }
       total += own_l[w * S::kCols + c] * f;
-      const float fo = f * own_ref[w];
-      acc.x += x.x * fo;
-      acc.y += x.y * fo;
-      acc.z += x.z * fo;
-      acc.w += x.w * fo;
+      acc.x += x.x * f;
+      acc.y += x.y * f;
+      acc.z += x.z * f;
+      acc.w += x.w * f;
     }
     if (a.cluster == 1) {
       finish(c, d, acc, top, total);
@@ -578,7 +572,7 @@ attn_q8_join_kernel(const Q8Args a, int cols_kept) {
     const int first = a.cu_q[s], count = a.cu_q[s + 1] - first;
     row0 = first + rg * a.rows_per;
     rows = min(a.rows_per, count - rg * a.rows_per);
-    if (first < 0 || count > a.max_q || first + count > a.q_rows) rows = 0;
+    if (count <= 0 || first < 0 || count > a.max_q || first + count > a.q_rows) rows = 0;
   }
   if (r >= rows) return;
   const int grp = threadIdx.x / kQuads, d = (threadIdx.x - grp * kQuads) * 4;

@@ -67,11 +67,11 @@ def check_write(x, positions, freqs, nh, nkv, hd, q, u, scale):
 
 
 def attention(q, data, scale, tables, rows, nh, softmax_scale, window=0):
-    """``rows``: (sequence, tokens seen) of every row of q.  Returns the result in 64 bits and how far fp16 weights and results may
-    be off: half a step of the result (2^-11); of every weight (2^-11) with the products' error in its exponent (the bytes'
+    """``rows``: (sequence, tokens seen) of every row of q.  Returns the result in 64 bits and how far it may be off: half a step of
+    the result (2^-11); of every weight the 2^-22 that two fp16 numbers leave, the products' error in its exponent (the bytes'
     products are summed in fp32 with an offset of 128, 24 rounded sums of at most sum|q| * 255 * scale), and 2^-18 for the
-    exponential, the running sums and scales in fp32; T * 2^-26 for T / 16 truncated sums of a row; and a weight below the normal
-    range of fp16 (rounded to 2^-25, the largest value's scale counted as one, up to eight times too large): T * 2^-22 * max|v|."""
+    exponential, the running sums and scales in fp32; T * 2^-26 for T / 16 truncated sums of a row; and what lies below the range of
+    fp16 (2^-25 each, where the largest weight times value scale is counted as 32 or more): T * 2^-30 of the largest weight times value."""
     nkv, bs, hd = data.shape[2], data.shape[3], data.shape[4]
     out = torch.zeros(len(rows), nh * hd, dtype=F64, device=q.device)
     tol = torch.zeros_like(out)
@@ -92,8 +92,8 @@ def attention(q, data, scale, tables, rows, nh, softmax_scale, window=0):
         spread = qi.abs().sum(-1) * 255 * scale[ids, 0, :, at % bs].to(F64).amax(0)[:, None] * softmax_scale * 24 * 2.0 ** -24
         T = len(at)
         out[i] = o.reshape(-1)
-        tol[i] = (o.abs() * 2.0 ** -11 + size * (2.0 ** -11 + 2 * spread[..., None] + 2.0 ** -18 + T * 2.0 ** -26)
-                  + T * 2.0 ** -22 * v.abs().amax((0, 2))[:, None, None] + 2.0 ** -25).reshape(-1)
+        tol[i] = (o.abs() * 2.0 ** -11 + size * (2.0 ** -22 + 2 * spread[..., None] + 2.0 ** -18 + T * 2.0 ** -26)
+                  + T * 2.0 ** -30 * torch.einsum("hgt,th->hgt", p, v.abs().amax(2)).amax(2)[..., None] + 2.0 ** -25).reshape(-1)
     return out, tol
 
 

@@ -335,6 +335,35 @@ def test_scales_of_every_size(ops):
     assert out[:2, : 8 * 128].float().abs().max() > 0
 
 
+@pytest.mark.parametrize("nh,nkv,rows", [(2, 2, None), (14, 2, None), (32, 2, None), (8, 2, [5, 1, 2])])
+@pytest.mark.parametrize("behind", [2200.0, 16.0])
+@pytest.mark.parametrize("window", [0, 250])
+def test_large_values_of_little_weight(ops, nh, nkv, rows, behind, window):
+    """One token's values are a million times the others', its weight zero or about a millionth of theirs; some before the window."""
+    bs, hd, lens, g = 16, 128, [300, 17, 700], gen(nh + int(behind))
+    data, scale = make_cache(g, 70, nkv, bs, hd, DEV)
+    tables = make_tables(g, lens, bs, 70, DEV)
+    for s, n in enumerate(lens):
+        for t in {0, n // 2, n - 3, max(0, n - 252)}:
+            b = tables[s, t // bs].long()
+            scale[b, 1, :, t % bs] *= 1e6                                  # its values
+            data[b, 0, :, t % bs] = 1                                      # its key: -127 times the scale, against q of about 1.5
+            scale[b, 0, :, t % bs] = behind / (127 * 1.5 * hd * scale_of(hd))
+    seen = [(s, n) for s, n in enumerate(lens)] if rows is None else [(s, n - r + i + 1) for s, (n, r) in enumerate(zip(lens, rows))
+                                                                   for i in range(r)]
+    q = (torch.rand(len(seen), nh * hd, generator=g) + 1).half().to(DEV)
+    out = torch.zeros_like(q)
+    kw = {}
+    if rows is not None:
+        kw = dict(cu_q=ints([0, 5, 6, 8]), q_pos0=ints([n - r for n, r in zip(lens, rows)]), max_q=5)
+    want, tol = attention(q, data, scale, tables, seen, nh, scale_of(hd), window)
+    for splits in (0, 1, 4, 32):
+        ops.attn_decode_q8(q, QuantKV(data, scale), tables, None if rows else ints(lens), out, 3, nh, nkv, hd, scale_of(hd),
+                           num_splits=splits, window=window, **kw)
+        bad = (out.double() - want).abs() - tol
+        assert (bad <= 0).all(), f"{splits} pieces: {float(bad.max())} over {float(tol.max())}, results up to {float(want.abs().max())}"
+
+
 def test_nan_is_seen_and_not_hidden(ops):
     nh, nkv, hd, bs = 4, 2, 64, 16
     g = gen(11)
