@@ -177,8 +177,8 @@ rope_kv_write_q8_kernel(const __half* qkv, int ld, Write w, const int* __restric
   }
 }
 
-// Sums of planes (few rows: a decode step; 64 rows of 56 heads from four planes 4.7 us, 1.2 at the rate of a copy).  A CTA has one token and blockIdx.y's share of its heads; four planes are loaded before the
-// first is added.
+// Sums of planes (few rows: a decode step; 64 rows of 56 heads from four planes 4.7 us, 1.2 at the rate of a copy).  A CTA has one token
+// and blockIdx.y's share of its heads; four planes are loaded before the first is added.
 template <int HD>
 __global__ void __launch_bounds__(256)
 rope_kv_write_q8_planes_kernel(const float* __restrict__ planes, int n_planes, const __half* __restrict__ bias, Write w,
@@ -262,10 +262,14 @@ kv_read_q8_kernel(const uint8_t* __restrict__ data, const float* __restrict__ sc
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const long long entries = (long long)num_seqs * out_max_blocks;
+  auto pages_of = [&](int len) { return max(len, 0) / block_size + (max(len, 0) % block_size > 0); };
+  auto fit = [&](int first, int pages, int last) {                     // (no sum of these overflows)
+    return first >= 0 && pages <= min(max_blocks, out_max_blocks) && first <= out_blocks - pages && first + pages <= last;
+  };
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < entries; i += (long long)gridDim.x * 256) {
     const int s = int(i / out_max_blocks), j = int(i - (long long)s * out_max_blocks);
-    const int len = seq_lens[s], first = cu_blocks[s], pages = max(len, 0) / block_size + (max(len, 0) % block_size > 0);
-    const bool fits = first >= 0 && pages <= min(min(max_blocks, out_max_blocks), cu_blocks[s + 1] - first) && first + pages <= out_blocks;
+    const int len = seq_lens[s], first = cu_blocks[s], pages = pages_of(len);
+    const bool fits = fit(first, pages, cu_blocks[s + 1]);
     if (j == 0 && (!fits || len < 0)) report(st, kBadArgument, 71, unsigned(s));
     const int blk = fits && j < pages ? tables[size_t(s) * table_ld + j] : -1;
     if (blk >= num_blocks) report(st, kBadArgument, 72, unsigned(blk));
@@ -284,10 +288,9 @@ kv_read_q8_kernel(const uint8_t* __restrict__ data, const float* __restrict__ sc
     for (int i = lane; i - lane < num_seqs; i += 32)
       s += __popc(__ballot_sync(0xffffffffu, i < num_seqs && cu_blocks[i + 1] <= u.page));
     if (s >= num_seqs) return u;
-    const int first = cu_blocks[s], j = u.page - first, len = max(seq_lens[s], 0), pages = len / block_size + (len % block_size > 0);
-    if (first < 0 || j < 0 || j >= pages || pages > min(min(max_blocks, out_max_blocks), cu_blocks[s + 1] - first) ||
-        first + pages > out_blocks)
-      return u;
+    const int first = cu_blocks[s], len = seq_lens[s], pages = pages_of(len);
+    if (!fit(first, pages, cu_blocks[s + 1]) || u.page < first || u.page - first >= pages) return u;
+    const int j = u.page - first;
     const int blk = tables[size_t(s) * table_ld + j];
     if (blk >= 0 && blk < num_blocks) u.blk = blk;
     u.inside = min(block_size, len - j * block_size);

@@ -441,6 +441,25 @@ def test_ids_outside_the_cache_are_reported_and_not_followed(ops):
     ops.check()
 
 
+def test_scratch_of_another_kind_and_another_device_are_refused(ops, monkeypatch):
+    from zse_b200.ops.native import NativeError, attn_decode_q8_plan
+    q = torch.zeros(1, 4 * 64, dtype=torch.float16, device=DEV)
+    kv = QuantKV.zeros((64, 2, 2, 16, 64), DEV)
+    tables, need = ints([list(range(64))]), attn_decode_q8_plan(1, 1, 4, 2, 64, 16, 64, num_splits=16)[1]
+    call = lambda scratch: ops.attn_decode_q8(q, kv, tables, ints([1000]), q.clone(), 1, 4, 2, 64, 0.125, scratch, num_splits=16)
+    assert need > 0
+    call(torch.zeros(need, device=DEV))
+    for scratch in (torch.zeros(need, device=DEV, dtype=torch.float16), torch.zeros(need), torch.zeros(2 * need, device=DEV)[::2],
+                    torch.zeros(1, need, device=DEV)):
+        with pytest.raises(ValueError, match="scratch"):
+            call(scratch)
+    with pytest.raises(NativeError, match="scratch"):
+        call(torch.zeros(need - 1, device=DEV))
+    monkeypatch.setattr(ops, "home", 1)
+    with pytest.raises(NativeError, match="device"):
+        call(None)
+
+
 def test_refusals_of_the_library(ops):
     from zse_b200.ops.native import NativeError
     kv = QuantKV.zeros((2, 2, 2, 16, 80), DEV)                              # a head dimension without kernels

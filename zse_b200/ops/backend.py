@@ -213,10 +213,10 @@ class TorchOps:
         self._check_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables)
         ref.kv_read_q8(kv, block_tables[:S], seq_lens[:S], cu_blocks[: S + 1], out, out_tables)
 
-    def _check_attn_q8(self, q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q):
+    def _check_attn_q8(self, q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q, scratch):
         device = self._heads_q8(kv, nh, nkv, hd)
         self._tensors_q8(device, q=(q, F16, 2), out=(out, F16, 2), block_tables=(block_tables, I32, 2), seq_lens=(seq_lens, I32, 1),
-                         cu_q=(cu_q, I32, 1), q_pos0=(q_pos0, I32, 1))
+                         cu_q=(cu_q, I32, 1), q_pos0=(q_pos0, I32, 1), scratch=(scratch, F32, 1))
         if nh // nkv > 16:
             raise ValueError(f"{nh // nkv} query heads per kv head: up to 16 expected")
         if S < 0 or block_tables.shape[0] < S or q.shape[1] < nh * hd or out.shape[1] < nh * hd or window < 0:
@@ -231,8 +231,9 @@ class TorchOps:
                        cu_q=None, q_pos0=None, max_q=1):
         """Attention of new tokens over an 8-bit cache.  One row per sequence (row s sees the first ``seq_lens[s]`` tokens), or,
         with ``cu_q``, rows ``cu_q[s] .. cu_q[s + 1] - 1`` of sequence s (at most ``max_q``), the first of them at position
-        ``q_pos0[s]``, each of which sees the tokens up to its own.  ``window`` > 0: only the last so many of them."""
-        self._check_attn_q8(q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q)
+        ``q_pos0[s]``, each of which sees the tokens up to its own.  ``window`` > 0: only the last so many of them.  ``scratch``:
+        fp32, as many as ``native.attn_decode_q8_plan`` says, of no other call at a time (None: allocated where it takes some)."""
+        self._check_attn_q8(q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q, scratch)
         ref.attn_decode_q8(q, kv, block_tables, seq_lens, out, S, nh, scale, window, cu_q, q_pos0)
 
     # ---- latent attention and routed feed-forward -----------------------------------------------------
@@ -713,6 +714,7 @@ class CudaOps(TorchOps):
         self.device = torch.device(device)
         self.status = native.Status(self.device)
         self.status_ptr = self.status.ptr
+        self.home = self.status.buf.get_device()
         self.sm_count = torch.cuda.get_device_properties(self.device).multi_processor_count
         # decode-sized passes (<= 64 tokens) of the INT4 layers: bit 0 = gate/up + SwiGLU, bit 1 = fused QKV + bias +
         # RoPE + KV-cache write, bit 2 = every other INT4 linear, through the persistent kernel (csrc/gemm_w4_dec.cu)
@@ -1314,7 +1316,7 @@ class CudaOps(TorchOps):
                 and slots.get_device() == device and inv_freq.get_device() == device):
             self._check_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out, planes, n_planes, bias)
         n = self.n
-        stream = n.stream_q8(data, scale)
+        stream = n.stream_q8(data, scale, self.home)
         n.launched(n.load().zse_rope_kv_write_q8(n.WRITE_Q8.pack(
             data.data_ptr(), scale.data_ptr(), shape[0], shape[2], shape[3], shape[4], 0 if qkv is None else qkv.data_ptr(),
             q_out.data_ptr(), 0 if planes is None else planes.data_ptr(), 0 if bias is None else bias.data_ptr(),
@@ -1333,7 +1335,7 @@ class CudaOps(TorchOps):
                 and seq_lens.get_device() == device and cu_blocks.get_device() == device):
             self._check_read_q8(kv, block_tables, seq_lens, cu_blocks, S, out, out_tables)
         n = self.n
-        stream = n.stream_q8(data, scale)
+        stream = n.stream_q8(data, scale, self.home)
         n.launched(n.load().zse_kv_read_q8(n.READ_Q8.pack(
             data.data_ptr(), scale.data_ptr(), shape[0], shape[2], shape[3], shape[4], block_tables.data_ptr(), seq_lens.data_ptr(),
             cu_blocks.data_ptr(), out.data_ptr(), out_tables.data_ptr(), self.status_ptr, stream, ld[0], rows[1], S, pages[0], ldo[0],
@@ -1355,10 +1357,11 @@ class CudaOps(TorchOps):
                 and q.dtype is F16 and out.dtype is F16 and block_tables.dtype is I32 and tables[0] >= S and rows[1] >= nh * hd
                 and rows_out[1] >= nh * hd and q.get_device() == device and out.get_device() == device
                 and block_tables.get_device() == device
+                and (scratch is None or scratch.dtype is F32 and scratch.stride() == (1,) and scratch.get_device() == device)
                 and (seq_lens is None or seq_lens.dtype is I32 and seq_lens.stride() == (1,) and seq_lens.get_device() == device)):
-            self._check_attn_q8(q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q)
+            self._check_attn_q8(q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q, scratch)
         n = self.n
-        stream, lib = n.stream_q8(data, scales), n.load()
+        stream, lib = n.stream_q8(data, scales, self.home), n.load()
         at = lambda t: 0 if t is None else t.data_ptr()
         while True:
             args = n.ATTN_Q8.pack(

@@ -528,12 +528,13 @@ def rope_kv_write(qkv, kv_layer, positions, slots, inv_freq, M, nh, nkv, hd, rot
 
 
 # ---- 8-bit KV cache: ``ops.backend.CudaOps`` packs the arguments of its calls itself, see there ------------------------------------
-def stream_q8(data, scale) -> int:
-    """The current stream of the cache's device, which has to be the current device.  (The two calls below the public ones:
-    ``torch.cuda.current_stream()`` makes a stream object and takes longer than the rest of a call.)"""
+def stream_q8(data, scale, home: int) -> int:
+    """The current stream of the cache's device, which has to be the current device and that of the operators (``home``, where their
+    status word is).  (The two calls below the public ones: ``torch.cuda.current_stream()`` makes a stream object and takes longer
+    than the rest of a call.)"""
     at = torch._C._cuda_getDevice()
-    if data.get_device() != at:
-        raise NativeError(f"the cache is on {data.device}, the current device is {at}")
+    if data.get_device() != at or at != home:
+        raise NativeError(f"the cache is on {data.device}, the operators are on device {home}, the current device is {at}")
     if not (data.is_contiguous() and scale.is_contiguous()):
         raise NativeError("a layer of an 8-bit cache has to be contiguous")
     return torch._C._cuda_getCurrentRawStream(at)
