@@ -143,6 +143,41 @@ def test_window_and_partial_rotation(tmp_path):
         eng.destroy(); plain.destroy()
 
 
+def test_adapters_beside_it(model_path, tmp_path):
+    """Requests of one batch keep their own adapter, its keys and values their own blocks."""
+    from zse_b200.lora.weights import random_adapter_file
+    eng = engine(model_path, max_batch_seqs=4)
+    for name, seed in (("a", 1), ("b", 2)):
+        random_adapter_file(str(tmp_path / name), eng.model_config, rank=4, alpha=8.0, seed=seed, std=0.2)
+        eng.lora_manager.load_adapter(name, str(tmp_path / name))
+    prompt = prompts(1, 40, 40, seed=9)[0]
+
+    def gen(*adapters):
+        ids = [eng.add_request_tokens(prompt, max_tokens=8, temperature=0.0, stop_tokens=[], lora_id=x) for x in adapters]
+        eng.run_until_done()
+        return [eng.get_result(i).output_tokens for i in ids]
+    alone = [gen(x)[0] for x in ("a", None, "b")]
+    assert gen("a", None, "b") == alone and len({tuple(x) for x in alone}) > 1
+    eng.destroy()
+
+
+@pytest.mark.timeout(600)
+def test_heads_over_two_ranks(tmp_path):
+    from zse_b200.parallel.tp_engine import TPEngine
+    path = str(tmp_path / "m.zse")
+    synth.write_random_model(path, synth.shape_config("tiny-aligned"), seed=0)
+    cfg = EngineConfig(device="cpu", kv_blocks=64, max_batch_seqs=4, max_batch_tokens=64, max_seq_len=256, kv_dtype="int8")
+    ps = prompts(3, 12, 80, seed=5)
+    want = run(ZStreamerEngine(path, config=cfg), ps, 6)
+    e = TPEngine(path, tp_size=2, config=cfg, start_timeout_s=180)
+    try:
+        ids = [e.add_request_tokens(x, max_tokens=6, temperature=0.0, stop_tokens=[]) for x in ps]
+        e.run_until_done(120)
+        assert e.healthy and [e.get_result(i).output_tokens for i in ids] == want
+    finally:
+        e.stop()
+
+
 def test_memory_is_counted(model_path):
     a, b = engine(model_path, kv_blocks=40), ZStreamerEngine(model_path, config=EngineConfig(device="cpu", kv_blocks=40, max_seq_len=256))
     hd = a.model_config.head_dim
