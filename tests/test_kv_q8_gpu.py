@@ -336,19 +336,20 @@ def test_scales_of_every_size(ops):
 
 
 @pytest.mark.parametrize("nh,nkv,rows", [(2, 2, None), (14, 2, None), (32, 2, None), (8, 2, [5, 1, 2])])
-@pytest.mark.parametrize("behind", [2200.0, 16.0])
+@pytest.mark.parametrize("behind,factor", [(2200.0, 1e6), (16.0, 1e6), (-8.0, 1e-6), (-8.0, 0.0), (-40.0, 1e-6)])
 @pytest.mark.parametrize("window", [0, 250])
-def test_large_values_of_little_weight(ops, nh, nkv, rows, behind, window):
-    """One token's values are a million times the others', its weight zero or about a millionth of theirs; some before the window."""
-    bs, hd, lens, g = 16, 128, [300, 17, 700], gen(nh + int(behind))
+def test_tokens_of_another_size(ops, nh, nkv, rows, behind, factor, window):
+    """A few tokens' values are a million times the others' and their weight zero or about a millionth of theirs, or the other way
+    round; some of them lie before the window."""
+    bs, hd, lens, g = 16, 128, [300, 17, 700], gen(nh + abs(int(behind)))
     data, scale = make_cache(g, 70, nkv, bs, hd, DEV)
     tables = make_tables(g, lens, bs, 70, DEV)
     for s, n in enumerate(lens):
         for t in {0, n // 2, n - 3, max(0, n - 252)}:
             b = tables[s, t // bs].long()
-            scale[b, 1, :, t % bs] *= 1e6                                  # its values
-            data[b, 0, :, t % bs] = 1                                      # its key: -127 times the scale, against q of about 1.5
-            scale[b, 0, :, t % bs] = behind / (127 * 1.5 * hd * scale_of(hd))
+            scale[b, 1, :, t % bs] *= factor                               # its values
+            data[b, 0, :, t % bs] = 1 if behind > 0 else 255               # its key: +-127 times the scale, against q of about 1.5
+            scale[b, 0, :, t % bs] = abs(behind) / (127 * 1.5 * hd * scale_of(hd))
     seen = [(s, n) for s, n in enumerate(lens)] if rows is None else [(s, n - r + i + 1) for s, (n, r) in enumerate(zip(lens, rows))
                                                                    for i in range(r)]
     q = (torch.rand(len(seen), nh * hd, generator=g) + 1).half().to(DEV)

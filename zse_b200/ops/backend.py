@@ -1362,13 +1362,13 @@ class CudaOps(TorchOps):
             self._check_attn_q8(q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q, scratch)
         n = self.n
         stream, lib = n.stream_q8(data, scales, self.home), n.load()
-        at = lambda t: 0 if t is None else t.data_ptr()
         while True:
             args = n.ATTN_Q8.pack(
-                data.data_ptr(), scales.data_ptr(), shape[0], shape[2], shape[3], shape[4], q.data_ptr(), block_tables.data_ptr(),
-                at(seq_lens), at(cu_q), at(q_pos0), out.data_ptr(), at(scratch), self.status_ptr, stream,
-                0 if scratch is None else scratch.numel(), ldq[0], ldo[0], min(rows[0], rows_out[0]), ld[0], tables[1], S, max_q, nh,
-                num_splits, window, scale, 0)
+                data.data_ptr(), scales.data_ptr(), shape[0], nkv, shape[3], hd, q.data_ptr(), block_tables.data_ptr(),
+                0 if seq_lens is None else seq_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
+                0 if cu_q is None else q_pos0.data_ptr(), out.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
+                self.status_ptr, stream, 0 if scratch is None else scratch.numel(), ldq[0], ldo[0], min(rows[0], rows_out[0]), ld[0],
+                tables[1], S, max_q, nh, num_splits, window, scale, 0)
             launches = lib.zse_attn_decode_q8(args)
             if launches != n.NEEDS_SCRATCH or scratch is not None:
                 break
