@@ -167,7 +167,7 @@ struct Q8Smem {
 
 // PACKED: up to four columns; they stand a second time in columns 4 .. 7, where the weights are what rounding leaves of the first.
 template <int HD, int NB, bool PACKED>
-__global__ void __launch_bounds__(kWarps * 32, HD > 128 ? 1 : NB == 1 ? 4 : 3)
+__global__ void __launch_bounds__(kWarps * 32, HD > 128 ? 1 : NB == 1 || HD == 64 ? 4 : 3)
 attn_q8_kernel(const Q8Args a) {
   using S = Q8Smem<HD, NB>;
   constexpr int kChunks = HD / 16;                                     // 16-byte chunks of a row, and 16-wide steps of the products
@@ -631,7 +631,7 @@ Plan plan_of(const ZseAttnQ8& a) {
   // 8 of 64 28 and 23; 32 drafts of up to five rows 79 and 71; but 64 x 2300 1: 52.8, 2: 56.2, and windows make sequences alike.
   // Several clusters (and the launch that joins them) where eight pieces leave a warp 12 tiles: 1 x 4000 of 4 kv heads 8: 8.4, 32: 7.8;
   // 1 x 32765 8: 38, 64: 15.5, 128: 14.0.
-  const int per_sm = a.kv.hd > 128 ? (p.nb == 1 ? 2 : 1) : p.nb == 1 ? 4 : 3;
+  const int per_sm = a.kv.hd > 128 ? (p.nb == 1 ? 2 : 1) : p.nb == 1 || a.kv.hd == 64 ? 4 : 3;
   long long want = a.num_splits;
   if (want <= 0) {
     long long tiles = (long long)a.max_blocks * (a.kv.block_size / 16);
@@ -648,7 +648,11 @@ Plan plan_of(const ZseAttnQ8& a) {
   p.cluster = 1;
   while (p.cluster < want && p.cluster < kMostCluster) p.cluster *= 2;
   p.pieces = int(std::min(64ll, (want + p.cluster - 1) / p.cluster) * p.cluster);
-  p.sort = a.num_seqs > 1 && a.num_seqs <= 64 && 2 * items * p.pieces >= 3ll * sm_count() * per_sm ? a.num_seqs : 0;     // several waves
+  // The longest first where the CTAs do not all run at once.  More than 8 columns: 64 drafts of five rows of 28 heads over 4, 500 .. 2000
+  // tokens, 1.7 waves 68.2 as they come, 57.4 the longest first; 48 of three rows of 64 over 8 53.7, 43.7.  Up to 8 columns from one
+  // and a half waves on: 48 x 100 .. 1700 of 32 heads over 8 of 64, 1.3 waves, 15.4 and 18.0 (a step takes that long to find its sequence).
+  const long long slots = (long long)sm_count() * per_sm;
+  p.sort = a.num_seqs > 1 && a.num_seqs <= 64 && 2 * items * p.pieces >= (p.nb == 1 ? 3 : 2) * slots ? a.num_seqs : 0;
   p.scratch_floats = p.pieces == p.cluster ? 0 : items * (p.pieces / p.cluster) * 8 * p.nb * (a.kv.hd + 4);
   return p;
 }
