@@ -23,9 +23,9 @@
 // that would be idle; else they are products more (a product of 16 x 8 x 16 keeps a quarter of an SM busy for some 8 cycles: the drafts
 // 66 -> 77 us, 64 sequences of 128 to 2300 tokens of 40 heads 35.7 -> 38.2; longest first, as by_length() has them, 70 and 35).
 //
-// What bounds it: the cache's bytes where there are many of them (64 sequences of 6001 to 8190 tokens, 64 heads over 8: 146 us, 6.6 TB/s,
-// the rate of a plain copy); mixed lengths leave SMs idle at the end (128 to 2300 tokens: 4.8 TB/s); drafts the products (70 us, of
-// which 34 are product time); few short sequences the way length -> table -> tile -> merge (1 x 300 tokens of 28 heads over 4: 4.2 us).
+// What bounds it: the cache's bytes where there are many of them (64 sequences of 6001 to 8190 tokens, 64 heads over 8: 147 us, 6.6 TB/s,
+// the rate of a plain copy); mixed lengths leave SMs idle at the end (128 to 2300 tokens: 4.9 TB/s); drafts the products (71 us, of
+// which 34 are product time); few short sequences the way length -> table -> tile -> merge (1 x 300 tokens of 28 heads over 4: 4.1 us).
 #include <algorithm>
 
 #include "api.h"
