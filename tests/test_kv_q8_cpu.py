@@ -147,7 +147,7 @@ def test_write_refuses(ops, change):
     dict(max_q=2), dict(max_q=0), dict(cu_q=i32([0, 1, 2])), dict(cu_q=i32([0, 1]), q_pos0=i32([0, 0])),
     dict(cu_q=i32([0, 1, 2]), q_pos0=i32([0])), dict(cu_q=i32([0, 1, 2]), q_pos0=i32([0, 0]), max_q=65),
     dict(cu_q=i64([0, 1, 2]), q_pos0=i32([0, 0])), dict(scratch=torch.zeros(4096, dtype=torch.float16)),
-    dict(scratch=torch.zeros(64, 64)), dict(scratch=torch.zeros(4096)[::2]),
+    dict(cu_q=i32([0, 2, 2]), q_pos0=i32([0, 0])), dict(cu_q=i32([0, 1, 3]), q_pos0=i32([0, 0]), max_q=2), dict(scratch=torch.zeros(64, 64)), dict(scratch=torch.zeros(4096)[::2]),
 ])
 def test_attention_refuses(ops, change):
     args = dict(q=torch.zeros(2, 256, dtype=torch.float16), kv=QuantKV.zeros((2, 2, 2, 16, 64)), block_tables=i32([[0], [1]]),

@@ -442,6 +442,45 @@ def test_ids_outside_the_cache_are_reported_and_not_followed(ops):
     ops.check()
 
 
+@pytest.mark.parametrize("splits", [0, 8, 32])
+def test_two_streams_and_two_graphs(ops, splits):
+    """Calls that run at once share nothing; graphs of them keep their own scratch, whatever runs between their replays."""
+    nh, nkv, hd, lens, g = 14, 2, 128, [[3000, 17], [900, 2222]], gen(31)
+    data, scale = make_cache(g, 420, nkv, 16, hd, DEV)
+    kv, qs, outs, args = QuantKV(data, scale), [], [], []
+    for n in lens:
+        qs.append(torch.randn(2, nh * hd, generator=g).half().to(DEV))
+        outs.append(torch.zeros_like(qs[-1]))
+        args.append((make_tables(g, n, 16, 420, DEV), ints(n)))
+    call = lambda i: ops.attn_decode_q8(qs[i], kv, *args[i], outs[i], 2, nh, nkv, hd, scale_of(hd), num_splits=splits)
+    want = []
+    for i in range(2):
+        call(i)
+        want.append(outs[i].clone())
+    streams, graphs = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                outs[i].zero_()
+                call(i)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], stream=streams[i]):
+            call(i)
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                outs[i].zero_()
+                graphs[i].replay()
+    call(0)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    ops.check()
+
+
 def test_scratch_of_another_kind_and_another_device_are_refused(ops, monkeypatch):
     from zse_b200.ops.native import NativeError, attn_decode_q8_plan
     q = torch.zeros(1, 4 * 64, dtype=torch.float16, device=DEV)

@@ -234,6 +234,9 @@ class TorchOps:
         ``q_pos0[s]``, each of which sees the tokens up to its own.  ``window`` > 0: only the last so many of them.  ``scratch``:
         fp32, as many as ``native.attn_decode_q8_plan`` says, of no other call at a time (None: allocated where it takes some)."""
         self._check_attn_q8(q, kv, block_tables, seq_lens, out, S, nh, nkv, hd, window, cu_q, q_pos0, max_q, scratch)
+        if cu_q is not None and S and (int((cu_q[1: S + 1] - cu_q[:S]).max()) > max_q or int(cu_q[:S].min()) < 0
+                                       or int(cu_q[1: S + 1].max()) > min(q.shape[0], out.shape[0])):
+            raise ValueError(f"up to {max_q} rows of a sequence expected, inside q and out")
         ref.attn_decode_q8(q, kv, block_tables, seq_lens, out, S, nh, scale, window, cu_q, q_pos0)
 
     # ---- latent attention and routed feed-forward -----------------------------------------------------
