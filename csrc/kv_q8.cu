@@ -52,7 +52,10 @@ __device__ __forceinline__ uint4 pack8(const float* x) {
 }
 
 template <int HD>
-constexpr int kLanes = HD <= 64 ? 4 : HD <= 128 ? 8 : 16;      // threads of a head, a power of two; HD / 16 of them work
+constexpr int kLanes = HD / 16;                                // threads of a head: 4, 6, 8 or 16
+template <int HD>
+constexpr int kWarpHeads = 32 / kLanes<HD>;                    // heads of a warp.  Of 96: five, and two threads idle; as eight
+                                                               // threads a head, two of them idle, 8080 rows of 96 heads took 60 us instead of 53
 
 // What the two write kernels do with a head of a token: a thread has 16 of its elements, two runs of eight that rotate with each
 // other (or neighbouring runs of the part that does not rotate).
@@ -65,11 +68,13 @@ struct Write {
 template <int HD>
 struct Lane {
   static constexpr int L = kLanes<HD>;
-  int c, ia, ib;                                                       // of a head's threads; first elements of the two runs
+  int group, c, ia, ib;                                                // head of the CTA's at a time, thread of it; first elements of the two runs
   bool works, turns;
   __device__ __forceinline__ explicit Lane(int rot) {
-    c = threadIdx.x % L;
-    works = c < HD / 16;
+    const int lane = threadIdx.x & 31;
+    group = (threadIdx.x >> 5) * kWarpHeads<HD> + lane / L;
+    c = lane % L;
+    works = lane < kWarpHeads<HD> * L;
     turns = works && c < rot / 16;
     ia = turns ? c * 8 : works ? rot + (c - rot / 16) * 16 : 0;
     ib = turns ? rot / 2 + c * 8 : ia + 8;
@@ -94,8 +99,14 @@ __device__ __forceinline__ void put_head(const Write& w, const Lane<HD>& lane, f
     float top = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = max_nan(top, max_nan(fabsf(a[j]), fabsf(b[j])));
+    if constexpr (Lane<HD>::L == 6) {                                  // the thread three on, then the two that are one and two on
+      const int first = (threadIdx.x & 31) - lane.c;
+      top = max_nan(top, __shfl_sync(0xffffffffu, top, first + (lane.c + 3) % 6));
+      top = max_nan(top, max_nan(__shfl_sync(0xffffffffu, top, first + (lane.c + 1) % 6), __shfl_sync(0xffffffffu, top, first + (lane.c + 2) % 6)));
+    } else {
 #pragma unroll
-    for (int o = 1; o < Lane<HD>::L; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int o = 1; o < Lane<HD>::L; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
     if (cached) {
       const bool none = top <= 1e-30f;
       const float steps = none ? 0.f : __fdiv_rn(127.f, top);
@@ -139,13 +150,13 @@ rope_kv_write_q8_kernel(const __half* qkv, int ld, Write w, const int* __restric
                         const float* __restrict__ inv_freq, int M, int tokens, int rot, int block_size, long long num_slots, Status* st) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int kGroups = 256 / kLanes<HD>, kMost = 16;
+  constexpr int kGroups = 8 * kWarpHeads<HD>, kMost = 16;
   __shared__ float sin_t[256], cos_t[256];                             // [token][rot / 2]
   __shared__ long long stored[kMost];
   const Lane<HD> lane(rot);
   const int half = rot / 2, heads = w.nh + 2 * w.nkv, t0 = blockIdx.x * tokens, n = min(tokens, M - t0);
   // this thread's heads: every kGroups-th of the tokens' heads in a row (with gridDim.y > 1: of one token, its share)
-  int head = blockIdx.y * kGroups + threadIdx.x / kLanes<HD>, t = 0;
+  int head = blockIdx.y * kGroups + lane.group, t = 0;
   const int step = gridDim.y * kGroups;
   uint4 va = make_uint4(0, 0, 0, 0), vb = va;
   auto fetch = [&]() {
@@ -186,7 +197,7 @@ rope_kv_write_q8_planes_kernel(const float* __restrict__ planes, int n_planes, c
                                const float* __restrict__ inv_freq, int rot, int block_size, long long num_slots, Status* st) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int kHeads = 256 / kLanes<HD>, kPlanes = 4;
+  constexpr int kHeads = 8 * kWarpHeads<HD>, kPlanes = 4;
   __shared__ float sin_t[HD / 2], cos_t[HD / 2];
   __shared__ long long stored;
   const Lane<HD> lane(rot);
@@ -226,7 +237,7 @@ rope_kv_write_q8_planes_kernel(const float* __restrict__ planes, int n_planes, c
         }
     }
   };
-  int head = blockIdx.y * kHeads + threadIdx.x / kLanes<HD>;
+  int head = blockIdx.y * kHeads + lane.group;
   load(head);
   if (threadIdx.x < rot / 2) turn_of(positions[t], inv_freq[threadIdx.x], &sin_t[threadIdx.x], &cos_t[threadIdx.x]);
   if (threadIdx.x == 0) stored = row_of_slot(slots[t], t, w.nkv, block_size, num_slots, st);
@@ -360,8 +371,8 @@ extern "C" int zse_rope_kv_write_q8(const ZseWriteQ8* w) {
   const auto* freqs = static_cast<const float*>(w->inv_freq);
   auto* status = static_cast<Status*>(w->status);
   const cudaStream_t st = static_cast<cudaStream_t>(w->stream);
-  auto go = [&](auto from_rows, auto from_planes, int lanes) {
-    const int rounds = (w->nh + 2 * kv.nkv) * lanes / 256 + ((w->nh + 2 * kv.nkv) * lanes % 256 > 0);
+  auto go = [&](auto from_rows, auto from_planes, int warp_heads) {
+    const int rounds = (w->nh + 2 * kv.nkv + 8 * warp_heads - 1) / (8 * warp_heads);
     cudaError_t e;
     if (w->planes != nullptr) {
       e = launch_pdl(from_planes, dim3(w->M, w->M < 2 * sm_count() ? rounds : 1), dim3(256), 0, st,
@@ -378,10 +389,10 @@ extern "C" int zse_rope_kv_write_q8(const ZseWriteQ8* w) {
     return e == cudaSuccess ? 1 : ZSE_ERR_LAUNCH;
   };
   switch (kv.hd) {
-    case 64: return go(rope_kv_write_q8_kernel<64>, rope_kv_write_q8_planes_kernel<64>, kLanes<64>);
-    case 96: return go(rope_kv_write_q8_kernel<96>, rope_kv_write_q8_planes_kernel<96>, kLanes<96>);
-    case 128: return go(rope_kv_write_q8_kernel<128>, rope_kv_write_q8_planes_kernel<128>, kLanes<128>);
-    default: return go(rope_kv_write_q8_kernel<256>, rope_kv_write_q8_planes_kernel<256>, kLanes<256>);
+    case 64: return go(rope_kv_write_q8_kernel<64>, rope_kv_write_q8_planes_kernel<64>, kWarpHeads<64>);
+    case 96: return go(rope_kv_write_q8_kernel<96>, rope_kv_write_q8_planes_kernel<96>, kWarpHeads<96>);
+    case 128: return go(rope_kv_write_q8_kernel<128>, rope_kv_write_q8_planes_kernel<128>, kWarpHeads<128>);
+    default: return go(rope_kv_write_q8_kernel<256>, rope_kv_write_q8_planes_kernel<256>, kWarpHeads<256>);
   }
 }
 
