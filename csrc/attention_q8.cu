@@ -179,7 +179,8 @@ attn_q8_kernel(const Q8Args a) {
   pdl_wait();
   // (what every CTA does once is kept short: with one tile per warp it is most of its instructions)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t2 = (lane & 3) * 2;
-  const int piece = blockIdx.x, s = a.sort > 0 ? by_length(a, blockIdx.z) : blockIdx.z, kvh = a.row_groups == 1 ? blockIdx.y : blockIdx.y / a.row_groups;
+  const int piece = blockIdx.x, s = a.sort > 0 ? by_length(a, blockIdx.z) : blockIdx.z;
+  const int kvh = a.row_groups == 1 ? blockIdx.y : blockIdx.y / a.row_groups;
   const int rg = blockIdx.y - kvh * a.row_groups, cap = a.max_blocks * a.bpt * 16;
 
   // A warp's tile i is 4 (i * pieces + piece) + warp of the item: pieces are equally long, and without a window where the first tiles
@@ -626,21 +627,23 @@ Plan plan_of(const ZseAttnQ8& a) {
   // Pieces: what fits the GPU at a time (CTAs an SM by registers and shared memory; an eighth less, for clusters need neighbouring
   // places), at least half a tile a warp.  Measured (HD 128, us by pieces): 1 x 1000 tokens of 8 kv heads 1: 11.1, 4: 5.9, 8: 5.0; 32 x 500
   // 1: 15.9, 2: 13.4, 4: 17.6.
-  // Twice as many, a second wave, where there is no more than one and a warp still has 16 tiles: sequences of mixed length are then
+  // Twice as many, a second wave, where there is little more than one (one) and a warp still has 16 (12) tiles: sequences of mixed length are then
   // shared out better, the longest first.  64 x 128 .. 2300 tokens of 8 kv heads 1: 38.5, 2: 35.0; 128 .. 4600 1: 71, 2: 55; of 32 heads over
-  // 8 of 64 28 and 23; 32 drafts of up to five rows 79 and 71; but 64 x 2300 1: 52.8, 2: 56.2, and windows make sequences alike.
+  // 8 of 64 28 and 23; 48 x 100 .. 1700 of 40 over 8 28.5 and 23.8; 32 drafts of up to five rows 79 and 71; but 64 x 2300 1: 52.8, 2: 56.2, 64 x
+  // 1300 .. 1600 36.5 and 41.0, and windows make sequences alike.
   // Several clusters (and the launch that joins them) where eight pieces leave a warp 12 tiles: 1 x 4000 of 4 kv heads 8: 8.4, 32: 7.8;
   // 1 x 32765 8: 38, 64: 15.5, 128: 14.0.
   const int per_sm = a.kv.hd > 128 ? (p.nb == 1 ? 2 : 1) : p.nb == 1 || a.kv.hd == 64 ? 4 : 3;
+  const long long slots = (long long)sm_count() * per_sm;
   long long want = a.num_splits;
   if (want <= 0) {
     long long tiles = (long long)a.max_blocks * (a.kv.block_size / 16);
     if (a.window > 0) tiles = std::min(tiles, ((long long)a.window + a.max_q) / 16 + 2);
-    const long long room = std::max(1ll, (long long)sm_count() * per_sm * 7 / 8 / items);
+    const long long room = std::max(1ll, slots * 7 / 8 / items);
     want = 1;
     while (want < kMostCluster && want * 2 <= room && want * 2 <= (tiles + 1) / 2) want *= 2;
-    if (want < kMostCluster && want * 2 > room && a.window == 0 && items * want * 4 <= 5ll * sm_count() * per_sm &&
-        tiles >= want * 2 * kWarps * 16)
+    if (want < kMostCluster && want * 2 > room && a.window == 0 && items * want * 4 <= 5 * slots &&
+        tiles >= want * 2 * kWarps * (items * want <= slots ? 12 : 16))
       want *= 2;
     if (want == kMostCluster && room > kMostCluster && tiles >= kMostCluster * kWarps * 12)
       want = std::max(want, std::min(room, tiles / (4 * kWarps)) / kMostCluster * kMostCluster);
@@ -651,7 +654,6 @@ Plan plan_of(const ZseAttnQ8& a) {
   // The longest first where the CTAs do not all run at once.  More than 8 columns: 64 drafts of five rows of 28 heads over 4, 500 .. 2000
   // tokens, 1.7 waves 68.2 as they come, 57.4 the longest first; 48 of three rows of 64 over 8 53.7, 43.7.  Up to 8 columns from one
   // and a half waves on: 48 x 100 .. 1700 of 32 heads over 8 of 64, 1.3 waves, 15.4 and 18.0 (a step takes that long to find its sequence).
-  const long long slots = (long long)sm_count() * per_sm;
   p.sort = a.num_seqs > 1 && a.num_seqs <= 64 && 2 * items * p.pieces >= (p.nb == 1 ? 3 : 2) * slots ? a.num_seqs : 0;
   p.scratch_floats = p.pieces == p.cluster ? 0 : items * (p.pieces / p.cluster) * 8 * p.nb * (a.kv.hd + 4);
   return p;

@@ -181,8 +181,8 @@ class TorchOps:
     def rope_kv_write_q8(self, qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out=None, planes=None, n_planes=0,
                          bias=None):
         """Rotates q and k of M rows, writes k and v into the 8-bit cache at ``slots`` (each slot once; -1: not stored) and the
-        rotated q to the first columns of ``q_out`` (None: ``qkv`` itself).  The rows are those of ``qkv`` [M, q | k | v], or the sum
-        of ``planes`` [n_planes, M, q | k | v] and ``bias``.  k and v columns stay as they are."""
+        rotated q to the first columns of ``q_out`` (None: ``qkv`` itself; else memory of its own).  The rows are those of ``qkv``
+        [M, q | k | v], or the sum of ``planes`` [n_planes, M, q | k | v] and ``bias``.  k and v columns stay as they are."""
         q_out = qkv if q_out is None else q_out
         self._check_write_q8(qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out, planes, n_planes, bias)
         if M == 0:
@@ -1356,7 +1356,8 @@ class CudaOps(TorchOps):
                     and q_pos0.stride() == (1,) and cu_q.shape[0] > S and q_pos0.shape[0] >= S and cu_q.get_device() == device
                     and q_pos0.get_device() == device)
         if not (fine and len(shape) == 5 and shape[2] == nkv and shape[4] == hd and nkv > 0 and nh > 0 and nh % nkv == 0
-                and nh <= 16 * nkv and S >= 0 and window >= 0 and len(ld) == 2 and ld[1] == 1 and len(ldq) == 2 and ldq[1] == 1 and len(ldo) == 2 and ldo[1] == 1
+                and nh <= 16 * nkv and S >= 0 and window >= 0
+                and len(ld) == 2 and ld[1] == 1 and len(ldq) == 2 and ldq[1] == 1 and len(ldo) == 2 and ldo[1] == 1
                 and q.dtype is F16 and out.dtype is F16 and block_tables.dtype is I32 and tables[0] >= S and rows[1] >= nh * hd
                 and rows_out[1] >= nh * hd and q.get_device() == device and out.get_device() == device
                 and block_tables.get_device() == device
