@@ -158,6 +158,10 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   const uint32_t tmem = bars->tmem_base;
   const uint32_t tm_s = tmem, tm_p = tmem, tm_o = tmem + 128;
   volatile int* abort_flag = &bars->abort_flag;
+  // q, the cache rows of this chunk and the block tables may come from the kernels before (pages of an 8-bit cache are read back into
+  // fp16 ones just before, and their tables written with them).  The loader and the softmax warps read the tables, so every warp waits.
+  // cu_q and q_pos0, read above, are uploaded before a pass.
+  pdl_wait();
 
   if (warp == 4) {
     // ------------------------------------------------------------------ producer (the whole warp)
@@ -165,7 +169,6 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     // eight block-table entries up one after the other another ~3.5 k: more than the rest of the tile's chain.  So the
     // warp shares the work: lane 2 g + half looks up group g of the NEXT tile while the current one is in flight, and
     // issues one K and one V load; 16 loads leave in one warp-wide instruction.
-    pdl_wait();                                        // q and the cache rows of this chunk come from the previous kernels
     if (lane == 0) {
       if (G > 0) {
         // slot s = rows 16 s .. 16 s + 15 = the chunk's (at most 16) rows of query head kvh * G + s

@@ -604,3 +604,68 @@ def test_graph_of_a_step(ops):
             now.sub_(1)                                                    # shorter sequences for the next replay
             now.clamp_(min=0)
     ops.check()
+
+
+@pytest.mark.parametrize("stale", [-1, 0])
+@pytest.mark.parametrize("groups", [
+    # sequences' tokens in all, new rows of each, dropped blocks; a pass over more context than the pages hold is several groups
+    [([300, 40, 129], [33, 40, 9], [(0, 2), (2, 0)])],
+    [([130, 33], [130, 12], [(0, 0)]), ([50], [50], []), ([400, 16], [200, 16], [(0, 3), (0, 7)])],
+])
+def test_prefill_right_behind_the_read_back(ops, stale, groups):
+    """Everything queued behind a long product, so that each kernel's CTAs are there before the one in front of it has written: the
+    pages and tables of the read-back, not what stood there, are what attention sees.  ``stale``: the tables' contents before (dropped
+    blocks everywhere; page 0 everywhere, over the dropped ones too); later groups find those of the groups before."""
+    nh, nkv, hd, bs, g = 8, 2, 128, 16, gen(len(groups))
+    most = max(sum(-(-n // bs) for n in lens) for lens, _, _ in groups)
+    pages = torch.zeros(most, 2, nkv, bs, hd, dtype=torch.float16, device=DEV)
+    places = torch.zeros(3, 26, dtype=torch.int32, device=DEV)
+    made = []
+    for lens, new, holes in groups:
+        blocks = sum(-(-n // bs) for n in lens) + 1
+        kv = QuantKV(*make_cache(g, blocks, nkv, bs, hd, DEV))
+        full = make_tables(g, lens, bs, blocks, "cpu")
+        pos = [p for n, r in zip(lens, new) for p in range(n - r, n)]
+        slots = [int(full[s, p // bs]) * bs + p % bs for s, (n, r) in enumerate(zip(lens, new)) for p in range(n - r, n)]
+        for s, b in holes:
+            full[s, b] = -1
+        cu, first = [0], [0]
+        for n, r in zip(lens, new):
+            cu.append(cu[-1] + -(-n // bs))
+            first.append(first[-1] + r)
+        x = torch.randn(first[-1], (nh + 2 * nkv) * hd, generator=g).half().to(DEV)
+        made.append((kv, full.to(DEV), ints(lens), ints(cu), ints(first), ints([n - r for n, r in zip(lens, new)]), ints(pos),
+                     ints(slots, torch.int64), x, x.clone(), torch.zeros(first[-1], nh * hd, dtype=torch.float16, device=DEV), max(new)))
+    freqs, filler = freqs_of(hd), torch.randn(8192, 8192, device=DEV).half()
+
+    def run(wait):
+        places.fill_(stale)
+        for m in made:
+            m[9].copy_(m[8])
+            m[10].zero_()
+        if not wait:
+            for _ in range(3):
+                torch.mm(filler, filler)
+        for kv, tables, lens, cu, first, pos0, pos, slots, _, q, out, max_q in made:
+            S, M = lens.shape[0], pos.shape[0]
+            ops.rope_kv_write_q8(q, kv, pos, slots, freqs, M, nh, nkv, hd)
+            wait and torch.cuda.synchronize()
+            ops.kv_read_q8(kv, tables, lens, cu, S, pages, places[:S])
+            wait and torch.cuda.synchronize()
+            ops.attn_prefill(q, pages, places[:S], first, pos0, out, S, M, max_q, nh, nkv, hd, bs, scale_of(hd))
+            wait and torch.cuda.synchronize()
+        return [m[10].clone() for m in made]
+
+    want = run(True)
+    for (lens, new, _), m, got in zip(groups, made, want):
+        seen = [(s, n - r + 1 + i) for s, (n, r) in enumerate(zip(lens, new)) for i in range(r)]
+        exact, tol = attention(m[9], m[0].data, m[0].scale, m[1], seen, nh, scale_of(hd))
+        # keys and values rounded to fp16 once more, 2^-11 of each (of a key in the exponent), and weights that are fp16 numbers
+        off = (m[9][:, : nh * hd].double().abs().view(-1, nh, hd).sum(-1).amax(1)[:, None] * m[0].scale[:, 0].double().max() * 127
+               * scale_of(hd) * 2 + 2) * 2.0 ** -11 * m[0].scale[:, 1].double().max() * 127
+        assert ((got.double() - exact).abs() <= 2 * tol + off).all()
+    for _ in range(20):
+        for got, right in zip(run(False), want):
+            assert torch.equal(got, right)
+    torch.cuda.synchronize()
+    ops.check()
