@@ -372,7 +372,8 @@ attn_q8_kernel(const Q8Args a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int c = PACKED ? (t2 & 2) + (e & 1) : nb * 8 + t2 + (e & 1);
-          const int len = min(base_len + row_of(a, c), cap), at_tok = tok + g + (e >> 1) * 8;
+          // (a column of no row sees nothing: a large value behind the sequence would move the references of them all)
+          const int r = row_of(a, c), len = r < rows ? min(base_len + r, cap) : 0, at_tok = tok + g + (e >> 1) * 8;
           if (at_tok >= len || (a.window > 0 && at_tok < len - a.window)) {
             dead |= 1u << (nb * 4 + e);
             t[nb][e] = -INFINITY;

@@ -669,3 +669,40 @@ def test_prefill_right_behind_the_read_back(ops, stale, groups):
             assert torch.equal(got, right)
     torch.cuda.synchronize()
     ops.check()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("group,draft", [(3, False), (5, False), (7, False), (11, False), (5, True), (1, True), (2, True)])
+@pytest.mark.parametrize("window", [0, 90])
+def test_what_lies_behind_a_sequence_changes_no_bit(ops, hd, group, draft, window):
+    """Columns of the products that stand for no head or no row (groups of 5 or 7, drafts of fewer rows than the longest) see nothing
+    either: scales left behind the last token, however large, move no reference of the columns beside them."""
+    nkv, bs, lens, g = 2, 16, [2 + (29 * i) % 330 for i in range(24)], gen(hd + group)
+    nh, blocks = group * nkv, sum(-(-n // bs) for n in lens)
+    data, scale = make_cache(g, blocks, nkv, bs, hd, DEV)
+    tables = make_tables(g, lens, bs, blocks, DEV)
+    rows = [min(n, 1 + i % 5) for i, n in enumerate(lens)] if draft else [1] * len(lens)
+    seen = [(s, n - r + 1 + i) for s, (n, r) in enumerate(zip(lens, rows)) for i in range(r)]
+    q = (torch.randn(len(seen), nh * hd, generator=g) * 2).half().to(DEV)
+    kw = {}
+    if draft:
+        cu = [0]
+        for r in rows:
+            cu.append(cu[-1] + r)
+        kw = dict(cu_q=ints(cu), q_pos0=ints([n - r for n, r in zip(lens, rows)]), max_q=5)
+    out = torch.zeros_like(q)
+    for splits in (0, 1):
+        first = None
+        for keys, values in ((0.0, 0.0), (0.0, 1e30), (0.01, float("inf")), (1e30, 1e30), (float("inf"), 1e20), (float("nan"), 1e30), (0.0, -1e30)):
+            for s, n in enumerate(lens):
+                if n % bs:
+                    scale[tables[s, n // bs].long(), 0, :, n % bs:] = keys
+                    scale[tables[s, n // bs].long(), 1, :, n % bs:] = values
+            ops.attn_decode_q8(q, QuantKV(data, scale), tables, None if draft else ints(lens), out, len(lens), nh, nkv, hd, scale_of(hd),
+                               num_splits=splits, window=window, **kw)
+            if first is None:
+                first = out.clone()
+                want, tol = attention(q, data, scale, tables, seen, nh, scale_of(hd), window)
+                assert ((out.double() - want).abs() <= tol).all()
+            assert torch.equal(out, first), (splits, keys, values)
+    ops.check()
