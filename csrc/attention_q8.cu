@@ -148,6 +148,7 @@ __device__ __forceinline__ int by_length(const Q8Args& a, int z) {
   return low != 0 ? __ffs(low) - 1 : __ffs(high) + 31;
 }
 
+constexpr int kQ8SmemAlign = 256;                                      // of the dynamic shared memory
 template <int HD, int NB>
 struct Q8Smem {
   static constexpr int kTile = 16 * HD;                                // K or V of 16 tokens
@@ -163,6 +164,10 @@ struct Q8Smem {
   static constexpr int kQ = kGotO + (kCols * HD / 4 + kMostCluster) * 16;
   static constexpr int kTotal = kQ + (kQShared ? kCols * kQPitch : 0);
   static_assert(kGot % 16 == 0 && kGotO % 16 == 0 && kQ % 16 == 0, "16-byte pieces");
+  // copy_place() and step_place() turn bits of whole shared addresses over, up to bit 7 for rows of 256 bytes and bit 6 for the others:
+  // tiles begin where those bits are zero
+  static constexpr int kAlign = HD == 256 ? 256 : 128;
+  static_assert(kAlign <= kQ8SmemAlign && kTile % kAlign == 0 && kSlot % kAlign == 0 && kRing % kAlign == 0, "places of a tile");
 };
 
 // PACKED: up to four columns; they stand a second time in columns 4 .. 7, where the weights are what rounding leaves of the first.
@@ -172,7 +177,7 @@ attn_q8_kernel(const Q8Args a) {
   using S = Q8Smem<HD, NB>;
   constexpr int kChunks = HD / 16;                                     // 16-byte chunks of a row, and 16-wide steps of the products
   constexpr int kChains = NB == 1 ? 2 : 1;                             // even and odd steps of a column apart
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(kQ8SmemAlign) uint8_t smem[];
   float* own_m = reinterpret_cast<float*>(smem + S::kNumbers);         // [warp][column]
   float* own_l = own_m + kWarps * S::kCols;
   pdl_launch_dependents();
