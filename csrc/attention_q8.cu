@@ -201,7 +201,7 @@ attn_q8_kernel(const Q8Args a) {
     const int first = a.cu_q[s], count = a.cu_q[s + 1] - first;
     row0 = first + rg * a.rows_per;
     rows = min(a.rows_per, count - rg * a.rows_per);
-    base_len = a.q_pos0[s] + rg * a.rows_per + 1;
+    base_len = min(a.q_pos0[s], 0x7fffff7f) + rg * a.rows_per + 1;     // (no sum of these overflows, and that is above every cap)
     if (count <= 0 || first < 0 || count > a.max_q || first + count > a.q_rows) {
       if (tid == 0 && count > 0) complain(a.st, 73, s);
       rows = 0;
@@ -210,7 +210,7 @@ attn_q8_kernel(const Q8Args a) {
     base_len = a.seq_lens[s];
   }
   if (rows <= 0) return;                                               // the whole cluster
-  if (base_len < (a.cu_q != nullptr ? 1 : 0) || base_len + rows - 1 > cap) {
+  if (base_len < (a.cu_q != nullptr ? 1 : 0) || base_len > cap - (rows - 1)) {
     if (tid == 0) complain(a.st, 75, s);
     base_len = max(0, min(base_len, cap));
   }

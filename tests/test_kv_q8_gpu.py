@@ -706,3 +706,25 @@ def test_what_lies_behind_a_sequence_changes_no_bit(ops, hd, group, draft, windo
                 assert ((out.double() - want).abs() <= tol).all()
             assert torch.equal(out, first), (splits, keys, values)
     ops.check()
+
+
+@pytest.mark.parametrize("pos", [2 ** 31 - 1, 2 ** 31 - 4, 2 ** 31 - 200, 33, 28, -1, -2 ** 31])
+@pytest.mark.parametrize("nh,window", [(4, 0), (32, 0), (4, 9)])
+def test_positions_outside_the_table_are_reported(ops, pos, nh, window):
+    """The last of five rows is behind a table of 32 tokens, or the first before it; the sequence beside it gets its result."""
+    from zse_b200.ops.native import DeviceStatusError
+    nkv, hd, bs = 2, 64, 16
+    data, scale = make_cache(gen(3), 4, nkv, bs, hd, DEV)
+    tables = ints([[0, 1], [2, 3]])
+    q = torch.randn(10, nh * hd, generator=gen(4)).half().to(DEV)
+    out = torch.zeros_like(q)
+    for p in (27, pos):
+        ops.attn_decode_q8(q, QuantKV(data, scale), tables, None, out, 2, nh, nkv, hd, scale_of(hd), window=window, cu_q=ints([0, 5, 10]),
+                           q_pos0=ints([p, 20]), max_q=5)
+        want, tol = attention(q, data, scale, tables, [(s, n + i) for s, n in ((0, 28), (1, 21)) for i in range(5)], nh, scale_of(hd), window)
+        assert ((out.double() - want).abs() <= tol)[0 if p == 27 else 5:].all()
+        if p == 27:
+            ops.check()
+    with pytest.raises(DeviceStatusError):
+        ops.check()
+    ops.check()
