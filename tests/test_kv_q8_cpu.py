@@ -193,3 +193,15 @@ def test_cache_object():
     layer = kv[2]
     assert (layer.num_blocks, layer.kv_heads, layer.block_size, layer.head_dim) == (4, 1, 16, 64)
     assert layer.data.data_ptr() == kv.data[2].data_ptr()
+
+
+@pytest.mark.parametrize("pos", [-1, -4, -2 ** 31, 28, 33, 2 ** 31 - 1])
+@pytest.mark.parametrize("window", [0, 9])
+def test_positions_outside_the_table_are_refused(ops, pos, window):
+    """Five rows, of which the first is before a table of 32 tokens or the last behind it."""
+    q, kv = torch.ones(5, 256, dtype=torch.float16), QuantKV.zeros((2, 2, 2, 16, 64))
+    call = lambda p: ops.attn_decode_q8(q, kv, i32([[0, 1]]), None, q.clone(), 1, 4, 2, 64, 0.125, window=window, cu_q=i32([0, 5]),
+                                        q_pos0=i32([p]), max_q=5)
+    call(27)
+    with pytest.raises(ValueError):
+        call(pos)

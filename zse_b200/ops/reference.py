@@ -270,7 +270,7 @@ def attn_decode_q8(q: torch.Tensor, kv, block_tables: torch.Tensor, seq_lens, ou
         n = int(seq_lens[s]) if cu_q is None else int(q_pos0[s]) + e - a
         if e <= a:
             continue
-        if n < 0 or -(-n // bs) > block_tables.shape[1]:
+        if n < (0 if cu_q is None else e - a) or -(-n // bs) > block_tables.shape[1]:
             raise ValueError(f"sequence {s}: {n} tokens, a table of {block_tables.shape[1]} blocks of {bs}")
         ids = block_tables[s, : -(-n // bs)].long()
         if n and int(ids.max()) >= kv.num_blocks:
