@@ -84,3 +84,97 @@ def test_many_blocks_fit_in_the_memory_of_an_fp16_cache(tmp_path):
     small, wide = engine(path, kv_blocks=0, kv_fraction=0.01), engine(path, kv_blocks=0, kv_fraction=0.01, kv_dtype=None)
     assert 1.9 < small.kv_cache.num_total_blocks / wide.kv_cache.num_total_blocks <= 2 * 128 / 132 + 1e-3
     small.destroy(); wide.destroy()
+
+
+def close(got, want):
+    return (got - want).abs().max() <= want.abs().max() * 2.0 ** -5
+
+
+@pytest.mark.parametrize("shape,over", [("small-128", {}), ("tiny", {}), ("small-128", dict(arch="mistral", sliding_window=70))])
+def test_passes_over_more_context_than_the_pages_hold(tmp_path, shape, over):
+    """Groups of sequences share the pages and their tables within every layer; what passes of fewer or shorter sequences left there is
+    not seen, also where the GPU is behind the host.  Each sequence's logits are those it gets by itself."""
+    path = str(tmp_path / "m.zse")
+    synth.write_random_model(path, synth.shape_config(shape, "int4" if shape == "small-128" else "fp16", **over), seed=5)
+    eng = engine(path, max_seq_len=320, max_batch_tokens=1200)
+    r, filler = eng.runner, torch.randn(8192, 8192, device="cuda").half()
+    ps = prompts(8, 30, 310, seed=8)
+    done = [0, 40, 0, 100, 0, 29, 17, 0]                                   # of them tokens of an earlier pass
+    done = [min(d, len(p) - 12) for d, p in zip(done, ps)]
+    single = [logits_after(eng, p, [d] if d else []) for p, d in zip(ps, done)]
+    for order in (range(8), reversed(range(8)), (3, 1, 7, 0), (5, 2, 4, 6, 0, 1)):
+        order = list(order)
+        for i in order:
+            r.cache.allocate_sequence(i, num_tokens=0)
+            if done[i]:
+                r.cache.extend_sequence(i, done[i])
+                r.prefill([(i, ps[i][: done[i]], 0)])
+            r.cache.extend_sequence(i, len(ps[i]) - done[i])
+        for _ in range(3):
+            torch.mm(filler, filler)
+        r.prefill([(i, ps[i][done[i]:], done[i]) for i in order])
+        if len(order) == 8:
+            assert len(r.buf.page_groups) > 2
+        for k, i in enumerate(order):
+            assert close(r.buf.logits[k].float().cpu(), single[i]), (order, i)
+            r.cache.free_sequence(i)
+    r.model.ops.check()
+    eng.destroy()
+
+
+def test_sequences_in_more_pieces_than_a_cluster_has(tmp_path):
+    """Long tables: steps beyond 1024 tokens and drafts meet in scratch, steps before do not, each in its own graph.  Crossing from one
+    to the other, drafts between them, and batches of short and long sequences give what the torch path gives."""
+    path = str(tmp_path / "m.zse")
+    synth.write_random_model(path, synth.shape_config("small-128", "int4", max_seq_len=8192), seed=5)
+    kw = dict(max_seq_len=8192, kv_blocks=700, max_batch_tokens=8192)
+    gpu, cpu = engine(path, **kw), engine(path, device="cpu", **kw)
+    m = gpu.runner.model
+    assert m.attention_pieces(1, 1024) <= 8 < m.attention_pieces(1, 1025) and gpu.runner.buf.q8_scratch.numel() > 1
+    toks = prompts(1, 5010, 5010, seed=1)[0]
+    before = gpu.runner.timings["graph_captures"]
+    for n, cuts in ((1031, list(range(1019, 1031))), (1030, [1019, 1024, 1025, 1026]), (3005, [3000]), (5010, [2000, 5003, 5004, 5009])):
+        want = logits_after(cpu, toks[:n], [])
+        assert close(logits_after(gpu, toks[:n], cuts), want), n
+    assert gpu.runner.timings["graph_captures"] - before == 2
+    # a step of a batch, short and long ones, against each alone
+    lens = [5000, 20, 1400, 1023, 0, 3000]
+    r = gpu.runner
+    alone = [logits_after(gpu, toks[: n + 1], [n] if n else []) for n in lens]
+    live = [(i, n) for i, n in enumerate(lens) if n]
+    for i, n in live:
+        r.cache.allocate_sequence(i, num_tokens=0)
+        r.cache.extend_sequence(i, n)
+        r.prefill([(i, toks[:n], 0)])
+        r.cache.extend_sequence(i, 1)
+    r.decode([i for i, _ in live], [toks[n] for _, n in live])
+    for k, (i, n) in enumerate(live):
+        assert close(r.buf.logits[k].float().cpu(), alone[i]), n
+        r.cache.free_sequence(i)
+    m.ops.check()
+    gpu.destroy(); cpu.destroy()
+
+
+def test_adapters_beside_it(tmp_path):
+    """Requests of one batch keep their own adapter: logits as on the CPU path."""
+    from zse_b200.lora.weights import random_adapter_file
+    path = str(tmp_path / "m.zse")
+    synth.write_random_model(path, synth.shape_config("small-128", "int4"), seed=7)
+    prompt, tokens = prompts(1, 40, 40, seed=9)[0], {}
+    for device in (None, "cpu"):
+        eng = engine(path, max_batch_seqs=4, device=device)
+        for name, seed in (("a", 1), ("b", 2)):
+            if device is None:
+                random_adapter_file(str(tmp_path / name), eng.model_config, rank=4, alpha=8.0, seed=seed, std=0.2)
+            eng.lora_manager.load_adapter(name, str(tmp_path / name))
+
+        def gen(*adapters):
+            ids = [eng.add_request_tokens(prompt, max_tokens=8, temperature=0.0, stop_tokens=[], lora_id=x) for x in adapters]
+            eng.run_until_done()
+            return [eng.get_result(i).output_tokens for i in ids]
+        tokens[device] = gen("a", None, "b")
+        assert eng.fatal_error is None and len({tuple(x) for x in tokens[device]}) > 1
+        if device is None:
+            assert [gen(x)[0][0] for x in ("a", None, "b")] == [t[0] for t in tokens[device]]
+        eng.destroy()
+    assert [t[0] for t in tokens[None]] == [t[0] for t in tokens["cpu"]]
