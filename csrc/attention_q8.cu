@@ -612,13 +612,6 @@ attn_q8_join_kernel(const Q8Args a, int cols_kept) {
   }
 }
 
-int sm_count() {
-  static int counts[kMaxDevices];
-  const int slot = current_device_slot();
-  if (counts[slot] == 0 && cudaDeviceGetAttribute(&counts[slot], cudaDevAttrMultiProcessorCount, slot) != cudaSuccess) return 148;
-  return counts[slot];
-}
-
 struct Plan {
   int nb, rows_per, row_groups, pieces, cluster, sort;
   long long scratch_floats;
@@ -678,9 +671,7 @@ int launch(const Q8Args& a, int num_seqs, cudaStream_t st) {
   auto kernel = attn_q8_kernel<HD, NB, PACKED>;
   constexpr int kBytes = Q8Smem<HD, NB>::kTotal;
   if (!ready[dev]) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess ||
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-      return ZSE_ERR_LAUNCH;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess) return ZSE_ERR_LAUNCH;
     ready[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};

@@ -306,6 +306,13 @@ inline int current_device_slot() {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) dev = 0;
   return dev;
 }
+// SMs of the current device.
+inline int sm_count() {
+  static int counts[kMaxDevices];
+  const int slot = current_device_slot();
+  if (counts[slot] == 0 && cudaDeviceGetAttribute(&counts[slot], cudaDevAttrMultiProcessorCount, slot) != cudaSuccess) return 148;
+  return counts[slot];
+}
 
 // ---- host side: launch with the programmatic-serialization attribute (see pdl_wait) ---------------------------
 int pdl_enabled();   // runtime.cu; 1 unless switched off by zse_set_pdl(0) or ZSE_PDL=0

@@ -343,12 +343,6 @@ bool cache_ok(const ZseKvQ8& kv) {
          (kv.hd == 64 || kv.hd == 96 || kv.hd == 128 || kv.hd == 256);
 }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-int sm_count() {
-  static int counts[kMaxDevices];
-  const int slot = current_device_slot();
-  if (counts[slot] == 0 && cudaDeviceGetAttribute(&counts[slot], cudaDevAttrMultiProcessorCount, slot) != cudaSuccess) return 148;
-  return counts[slot];
-}
 
 }  // namespace
 }  // namespace zse

@@ -69,7 +69,7 @@ class QuantKV:
         self.scale[:, dst].copy_(self.scale[:, src])
 
 
-def refuses(config, tp_size: int = 1) -> Optional[str]:
+def refuses(config) -> Optional[str]:
     """Why a model cannot keep its cache in 8 bits, or None where it can."""
     if config.is_gemma or config.is_latent or config.is_hybrid:
         return f"'{config.arch}' keeps its cache at 16 bits or more"
