@@ -23,9 +23,10 @@
 // that would be idle; else they are products more (a product of 16 x 8 x 16 keeps a quarter of an SM busy for some 8 cycles: the drafts
 // 66 -> 77 us, 64 sequences of 128 to 2300 tokens of 40 heads 35.7 -> 38.2; longest first, as by_length() has them, 70 and 35).
 //
-// What bounds it: the cache's bytes where there are many of them (64 sequences of 6001 to 8190 tokens, 64 heads over 8: 147 us, 6.6 TB/s,
-// the rate of a plain copy); mixed lengths leave SMs idle at the end (128 to 2300 tokens: 4.9 TB/s); drafts the products (71 us, of
-// which 34 are product time); few short sequences the way length -> table -> tile -> merge (1 x 300 tokens of 28 heads over 4: 4.1 us).
+// What bounds it: the cache's bytes where there are many of them (64 sequences of 6001 to 8190 tokens, 64 heads over 8: in a CUDA graph
+// 148 us, 6.5 TB/s, the rate of a plain copy; in calls one by one 168 us, 5.8 TB/s); mixed lengths leave SMs idle at the end (128 to 2300
+// tokens: 4.8 TB/s); drafts the products (71 us, of which 34 are product time); few short sequences the way length -> table -> tile ->
+// merge (1 x 300 tokens of 28 heads over 4: 4.1 us).
 #include <algorithm>
 
 #include "api.h"
@@ -629,7 +630,8 @@ Plan plan_of(const ZseAttnQ8& a) {
   // Twice as many, a second wave, where there is little more than one (one) and a warp still has 16 (12) tiles: sequences of mixed length are then
   // shared out better, the longest first.  64 x 128 .. 2300 tokens of 8 kv heads 1: 38.5, 2: 35.0; 128 .. 4600 1: 71, 2: 55; of 32 heads over
   // 8 of 64 28 and 23; 48 x 100 .. 1700 of 40 over 8 28.5 and 23.8; 32 drafts of up to five rows 79 and 71; but 64 x 2300 1: 52.8, 2: 56.2, 64 x
-  // 1300 .. 1600 36.5 and 41.0, and windows make sequences alike.
+  // 1300 .. 1600 36.7 and 40.9, 32 x 6000 .. 8000 of 28 over 4 4: 44.0, 8: 47.7 (the plan has the table's width, not the lengths), and windows make
+  // sequences alike.
   // Several clusters (and the launch that joins them) where eight pieces leave a warp 12 tiles: 1 x 4000 of 4 kv heads 8: 8.4, 32: 7.8;
   // 1 x 32765 8: 38, 64: 15.5, 128: 14.0.
   const int per_sm = a.kv.hd > 128 ? (p.nb == 1 ? 2 : 1) : p.nb == 1 || a.kv.hd == 64 ? 4 : 3;
