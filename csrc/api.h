@@ -463,6 +463,41 @@ int64_t zse_attn_decode_q8_scratch_floats(const ZseAttnQ8* a);
 int zse_attn_decode_q8_pieces(const ZseAttnQ8* a);
 int zse_attn_decode_q8(const ZseAttnQ8* a);
 
+// ---- fp8_rows.cu: rows in 8-bit floating point --------------------------------------------------------------------------
+// data e4m3 [M][columns], ld_data bytes apart; scale fp32 [columns / 128, rounded up][ld_scale], a row's number the last index: an
+// element is data * scale.  Columns: a multiple of 16; data 16-byte aligned.  type 0 fp16, 1 bfloat16, 2 fp32.  The three calls below
+// return the number of kernels launched.
+// residual fp32 [M][H] += the sum of n_planes planes fp32 [M][H] and of add [M][H] (type, or null); data, scale = RMSNorm(residual) *
+// weight (type), which also goes to `normed` [M][H] (type) unless that is null.  type 0 or 1, H up to 32768.
+typedef struct ZseNormFp8 {
+  void* residual;
+  const void *planes, *add, *weight;
+  void *normed, *data, *scale, *stream;
+  int64_t ld_data, ld_scale;
+  double eps;
+  int32_t n_planes, M, H, type;
+} ZseNormFp8;
+int zse_add_rmsnorm_fp8(const ZseNormFp8* a);
+// Rows x (type, ldx elements apart) of C columns, or (act 1: silu, 2: gelu's tanh form) act(x[:, :C]) * x[:, C : 2 C].
+typedef struct ZseQuantFp8 {
+  const void* x;
+  void *data, *scale, *stream;
+  int64_t ldx, ld_data, ld_scale;
+  int32_t M, C, act, type;
+} ZseQuantFp8;
+int zse_quant_fp8(const ZseQuantFp8* a);
+// ---- gemm_fp8.cu --------------------------------------------------------------------------------------------------------
+// x, sx: such rows of K columns; w e4m3 [N][K], ldw bytes apart, sw fp32 [N / 128][K / 128], both rounded up.  out [M][N] (type, ldo
+// elements apart) = x w^T + bias (bias_type, or null).  act 1 or 2: w is [2 N][K], gate rows then up rows, sw [2][N / 128][K / 128],
+// and out (ldo bytes apart), out_scale (ld_os) are rows in 8 bits, act(x gate^T) * (x up^T); N is then a multiple of 16.
+typedef struct ZseGemmFp8 {
+  const void *x, *sx, *w, *sw, *bias;
+  void *out, *out_scale, *status, *stream;
+  int64_t ldx, ldw, ldo, ld_sx, ld_os;
+  int32_t M, N, K, type, bias_type, act;
+} ZseGemmFp8;
+int zse_gemm_fp8(const ZseGemmFp8* a);
+
 // ---- sampling.cu --------------------------------------------------------------------------------------------
 int zse_argmax(const void* logits_f16, int ld, void* out_i32, int M, int V, void* stream);
 int zse_sample(const void* logits_f16, int ld, void* out_i32, int M, int V, const void* temperature_f32,

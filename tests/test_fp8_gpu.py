@@ -1,0 +1,345 @@
+"""Kernels of 8-bit floating point (csrc/fp8_rows.cu, csrc/gemm_fp8.cu) against 64 bits: sizes, types and contents where they can go
+wrong, and the run of them as a feed-forward uses them."""
+import pytest
+import torch
+
+from tests.helpers.fp8_oracle import (blocks, check_out, check_rows, gated, make_rows, make_weight, norm, product, values, weight)
+from zse_b200.ops.fp8 import Fp8Rows, Fp8Weight
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F8 = torch.float8_e4m3fn
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from zse_b200.ops.backend import make_ops
+    return make_ops(DEV)
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def marked(M, C, extra=2, apart=0):
+    """Rows to be written, more of them than M and ``apart`` bytes between them, with values that are not to change behind M."""
+    data = torch.full((M + extra, C + apart), 3.0).to(F8).to(DEV)[:, :C]
+    return Fp8Rows(data, torch.full((blocks(C), M + extra), 7.0, device=DEV))
+
+
+def untouched(rows, M):
+    return bool((rows.data[M:].float() == 3).all() and (rows.scale[:, M:] == 7).all())
+
+
+# ---- norm -------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("H", [16, 112, 128, 144, 1040, 3584, 5120, 8192, 16400, 32768])
+@pytest.mark.parametrize("M", [1, 2, 5, 33, 700])
+@pytest.mark.parametrize("planes,add,keep", [(0, False, False), (1, False, True), (0, True, False), (3, True, True), (9, False, False)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_norm(ops, H, M, planes, add, keep, dtype):
+    if M * H * (planes + 1) > 20_000_000:
+        pytest.skip("a size that another case has")
+    g = gen(H + M * 7 + planes)
+    r, w = (torch.randn(M + 1, H, generator=g) * 3).to(DEV), (1 + torch.randn(H, generator=g) * 0.2).to(dtype).to(DEV)
+    r[M // 2] *= 1e-3
+    p = torch.randn(planes, M, H, generator=g).to(DEV) if planes else None
+    a = torch.randn(M, H, generator=g).to(dtype).to(DEV) if add else None
+    total = r[:M].double() + (p.double().sum(0) if planes else 0) + (a.double() if add else 0)
+    last, out = r[M].clone(), marked(M, H, apart=16 * (M % 2))
+    normed = torch.full((M + 1, H), 5.0, dtype=dtype, device=DEV) if keep else None
+    ops.add_rmsnorm_fp8(r, p, planes, a, w, out, M, 1e-6, normed=normed)
+    torch.cuda.synchronize()
+    assert torch.equal(r[:M], total.float()) and torch.equal(r[M], last) and untouched(out, M)
+    y = norm(r[:M], w, 1e-6)
+    check_rows(y, 5 * 2.0 ** -24, out, M)
+    if keep:
+        check_out(y, 5 * 2.0 ** -24 * y.abs(), normed[:M])
+        assert (normed[M:] == 5).all()
+
+
+def test_norm_of_zeros_infinities_and_nans(ops):
+    H, M = 512, 6
+    r = torch.randn(M, H, generator=gen(1)).to(DEV)
+    r[1] = 0
+    r[2, 300] = float("inf")
+    r[3, 7] = float("nan")
+    r[4] *= 1e25                                                            # its square does not fit 32 bits
+    r[5, :128] = 0
+    out = marked(M, H)
+    ops.add_rmsnorm_fp8(r, None, 0, None, torch.ones(H, device=DEV).half(), out, M, 1e-6)
+    got = out[:M].dequant()
+    assert (got[1] == 0).all() and got[3].isnan().all()
+    assert got[2, 256:384].isnan().all()
+    keep = torch.tensor([0, 4, 5], device=DEV)
+    check_rows(norm(r, torch.ones(H, device=DEV), 1e-6)[keep], 5 * 2.0 ** -24,
+               Fp8Rows(out.data[:M].view(torch.uint8)[keep].view(F8), out.scale[:, :M][:, keep]), 3)
+
+
+def test_norm_does_not_depend_on_the_other_rows(ops):
+    """A row gives the same bytes alone and among others, whatever launch they take."""
+    for H in (1040, 5120):
+        g = gen(H)
+        r, w, p = torch.randn(900, H, generator=g).to(DEV), torch.ones(H, device=DEV).half(), torch.randn(900, H, generator=g).to(DEV)
+        many, copy = marked(900, H), r.clone()
+        ops.add_rmsnorm_fp8(copy, p, 1, None, w, many, 900, 1e-6)
+        for first, M in ((0, 1), (17, 2), (100, 64), (300, 300)):
+            few, mine = marked(M, H), r[first: first + M].clone()
+            ops.add_rmsnorm_fp8(mine, p[first: first + M], 1, None, w, few, M, 1e-6)
+            assert torch.equal(few.data[:M].view(torch.uint8), many.data[first: first + M].view(torch.uint8))
+            assert torch.equal(few.scale[:, :M], many.scale[:, first: first + M])
+
+
+# ---- rows and gated rows ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("C", [16, 128, 144, 1008, 5120, 13824])
+@pytest.mark.parametrize("M", [1, 3, 34, 517])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("act", ["none", "silu", "gelu"])
+def test_quant(ops, C, M, dtype, act):
+    g = gen(C + M)
+    parts = 1 if act == "none" else 2
+    x = (torch.randn(M + 1, parts * C + 8, generator=g) * 3).to(dtype).to(DEV)[:, : parts * C]
+    if M > 2:
+        x[1, :128] = 0
+        x[2] *= 1e-4                                                        # (fp16: numbers below its normal ones)
+    out = marked(M, C, apart=32)
+    if parts == 1:
+        ops.quant_fp8(x, M, out)
+        y, off = x[:M].double(), 0.0
+    else:
+        ops.swiglu_fp8(x, M, out, gelu=act == "gelu")
+        y, off = gated(x[:M, :C].double(), x[:M, C:].double(), 0.0, 0.0, act == "gelu")
+    torch.cuda.synchronize()
+    check_rows(y, off, out, M)
+    assert untouched(out, M)
+
+
+def test_quant_of_extremes(ops):
+    x = torch.zeros(8, 256, device=DEV)
+    x[0], x[1, 3], x[2, 130] = 3.4e38, float("inf"), float("nan")
+    x[3], x[4], x[5] = 1e-30, 1.1e-30, 1e-45
+    x[6, :128] = torch.linspace(-448, 448, 128)
+    x[7, ::2] = -0.0
+    out = Fp8Rows.empty(8, 256, DEV)
+    ops.quant_fp8(x, 8, out)
+    y = out.dequant()
+    assert (out.data[0].float() == 448).all() and y[1, :128].isnan().all() and (y[1, 128:] == 0).all() and y[2, 128:].isnan().all()
+    assert (out.scale[:, 3] == 0).all() and (out.data[4].float() == 448).all() and (y[5] == 0).all() and (y[7] == 0).all()
+    check_rows(x[6:].double(), 0.0, out[6:], 2)
+
+
+# ---- products -----------------------------------------------------------------------------------------------------------------
+def check_linear(ops, M, N, K, dtype, bias, seed=0, ld=0, first=0):
+    g = gen(M * 31 + N * 7 + K + seed)
+    x, w = make_rows(g, M + 2, K, DEV), make_weight(g, N, K, DEV, bias)
+    x.scale[:, M:] = float("nan")                                           # rows behind M are not looked at
+    whole = torch.full((M + 2, first + N + ld), 5.0, dtype=dtype, device=DEV)
+    out = whole[:, first: first + N]
+    ops.linear_fp8(w, x, M, out)
+    torch.cuda.synchronize()
+    ops.check()
+    y, off = product(values(x, M), weight(w)[0])
+    if bias is not None:
+        y = y + w.bias.double()
+        off = off + 2.0 ** -24 * y.abs()
+    check_out(y, off, out[:M])
+    assert (whole[M:] == 5).all() and (whole[:, :first] == 5).all() and (whole[:, first + N:] == 5).all()
+
+
+@pytest.mark.parametrize("M", [1, 2, 8, 17, 32, 33, 64, 65, 128, 129, 200, 384])
+@pytest.mark.parametrize("N,K", [(1, 16), (7, 144), (127, 272), (128, 128), (129, 1040), (640, 512), (1000, 4096)])
+def test_linear(ops, M, N, K):
+    check_linear(ops, M, N, K, F16, None)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("bias", [None, F16, BF16, F32])
+@pytest.mark.parametrize("M,N,K,ld,first", [(5, 256, 640, 0, 0), (130, 200, 400, 3, 1), (300, 520, 144, 8, 8)])
+def test_linear_types_and_strides(ops, dtype, bias, M, N, K, ld, first):
+    check_linear(ops, M, N, K, dtype, bias, ld=ld, first=first)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 4608, 3584), (3, 3584, 18944), (48, 5120, 13824), (777, 2560, 2048), (2050, 5120, 1024),
+                                   (4096, 300, 16384), (1500, 10240, 528), (9000, 1024, 256)])
+def test_linear_large(ops, M, N, K):
+    check_linear(ops, M, N, K, BF16, None)
+
+
+def check_swiglu(ops, M, ff, K, gelu=False, apart=0):
+    g = gen(M * 13 + ff + K)
+    x, w = make_rows(g, M + 2, K, DEV, hot=False), make_weight(g, ff, K, DEV, glu=True)
+    x.scale[:, M:] = float("nan")
+    out = marked(M, ff, apart=apart)
+    ops.linear_swiglu_fp8(w, x, M, out, gelu=gelu)
+    torch.cuda.synchronize()
+    ops.check()
+    (gate, g_off), (up, u_off) = (product(values(x, M), p) for p in weight(w))
+    y, off = gated(gate, up, g_off, u_off, gelu)
+    check_rows(y, off, out, M)
+    assert untouched(out, M)
+
+
+@pytest.mark.parametrize("M", [1, 2, 16, 31, 33, 64, 100, 128, 129, 260])
+@pytest.mark.parametrize("ff,K,gelu", [(16, 16, False), (48, 272, True), (64, 128, False), (128, 144, False), (144, 640, True), (1008, 2048, False)])
+def test_linear_swiglu(ops, M, ff, K, gelu):
+    check_swiglu(ops, M, ff, K, gelu, apart=16 * (M % 3))
+
+
+@pytest.mark.parametrize("M,ff,K", [(1, 18944, 3584), (5, 13824, 5120), (160, 13824, 2048), (777, 4096, 1024), (2049, 8192, 1040), (4100, 2048, 512)])
+def test_linear_swiglu_large(ops, M, ff, K):
+    check_swiglu(ops, M, ff, K)
+
+
+def test_a_nan_stays_in_its_row_or_column(ops):
+    """A NaN or a scale of infinity in a row of x, or in a row of the weight, reaches the outputs of that row or column alone."""
+    g, M, N, K = gen(5), 70, 300, 400
+    x, w = make_rows(g, M, K, DEV, hot=False), make_weight(g, N, K, DEV)
+    clean = torch.empty(M, N, device=DEV)
+    ops.linear_fp8(w, x, M, clean)
+    x.data.view(torch.uint8)[3, 399] = 0x7F
+    x.scale[1, 66] = float("inf")
+    w.data.view(torch.uint8)[299, 0] = 0x7F
+    out = torch.empty(M, N, device=DEV)
+    ops.linear_fp8(w, x, M, out)
+    assert out[3].isnan().all() and out[:, 299].isnan().all() and not out[66, :299].isfinite().any()
+    keep = [t for t in range(M) if t not in (3, 66)]
+    assert torch.equal(out[keep, :299], clean[keep, :299])
+
+
+def test_zero_scales(ops):
+    g = gen(6)
+    x, w = make_rows(g, 9, 256, DEV), make_weight(g, 256, 256, DEV)
+    x.scale[0, :4], x.scale[:, 5], w.scale[1] = 0, 0, 0
+    out = torch.empty(9, 256, device=DEV)
+    ops.linear_fp8(w, x, 9, out)
+    y, off = product(values(x, 9), weight(w)[0])
+    check_out(y, off, out)
+    assert (out[5] == 0).all() and (out[:, 128:] == 0).all()
+
+
+def test_fp16_is_held_within_its_largest(ops):
+    x, w = make_rows(gen(7), 4, 128, DEV, hot=False), make_weight(gen(8), 128, 128, DEV)
+    x.scale *= 1e7
+    out = torch.empty(4, 128, dtype=F16, device=DEV)
+    ops.linear_fp8(w, x, 4, out)
+    assert out.isfinite().all() and (out.abs() == 65504).sum() > 100
+
+
+def test_outputs_more_than_2_31_apart(ops):
+    g, K, N, ld = gen(9), 256, 130, (1 << 31) + 16
+    x, w = make_rows(g, 2, K, DEV), make_weight(g, N, K, DEV)
+    out = torch.empty(ld + N, dtype=F16, device=DEV).as_strided((2, N), (ld, 1))
+    ops.linear_fp8(w, x, 2, out)
+    y, off = product(values(x, 2), weight(w)[0])
+    check_out(y, off, out)
+    data = torch.empty(ld + 256, dtype=torch.uint8, device=DEV).view(F8).as_strided((2, 256), (ld, 1))
+    rows = Fp8Rows(data, torch.empty(2, 2, device=DEV))
+    h = torch.randn(2, 256, generator=g).to(DEV)
+    ops.quant_fp8(h, 2, rows)
+    check_rows(h.double(), 0.0, rows, 2)
+    ops.linear_fp8(w, rows, 2, out)
+    y, off = product(values(rows, 2), weight(w)[0])
+    check_out(y, off, out)
+
+
+# ---- how they are called ------------------------------------------------------------------------------------------------------
+def feed_forward(ops, r, w16, up, down, x, h, plane, M):
+    ops.add_rmsnorm_fp8(r, None, 0, None, w16, x, M, 1e-6)
+    ops.linear_swiglu_fp8(up, x, M, h)
+    ops.linear_fp8(down, h, M, plane[0])
+    ops.add_rmsnorm_fp8(r, plane, 1, None, w16, x, M, 1e-6)
+
+
+def layer(seed, M, H, ff):
+    g = gen(seed)
+    return dict(r=torch.randn(M, H, generator=g).to(DEV), w16=(1 + torch.randn(H, generator=g) * 0.1).half().to(DEV),
+                up=make_weight(g, ff, H, DEV, glu=True), down=make_weight(g, H, ff, DEV), x=Fp8Rows.empty(M, H, DEV),
+                h=Fp8Rows.empty(M, ff, DEV), plane=torch.empty(1, M, H, device=DEV), M=M)
+
+
+@pytest.mark.parametrize("M,H,ff", [(1, 512, 1024), (48, 1040, 2000), (300, 1024, 1920)])
+def test_feed_forward(ops, M, H, ff):
+    """Norm, gate and up, down, norm, each step checked on what the one before left."""
+    s = layer(M, M, H, ff)
+    before = s["r"].clone()
+    first = Fp8Rows.empty(M, H, DEV)
+    ops.add_rmsnorm_fp8(before.clone(), None, 0, None, s["w16"], first, M, 1e-6)
+    feed_forward(ops, **s)
+    check_rows(norm(before, s["w16"], 1e-6), 5 * 2.0 ** -24, first, M)
+    (gate, g_off), (up, u_off) = (product(values(first, M), p) for p in weight(s["up"]))
+    y, off = gated(gate, up, g_off, u_off, False)
+    check_rows(y, off, s["h"], M)
+    y, off = product(values(s["h"], M), weight(s["down"])[0])
+    check_out(y, off, s["plane"][0])
+    assert torch.equal(s["r"], before + s["plane"][0])
+    check_rows(norm(s["r"], s["w16"], 1e-6), 5 * 2.0 ** -24, s["x"], M)
+
+
+def bits(s):
+    return [t.clone() for t in (s["r"], s["plane"], s["x"].data.view(torch.uint8), s["x"].scale, s["h"].data.view(torch.uint8), s["h"].scale)]
+
+
+def test_streams_and_graphs(ops):
+    """The same bits again, on two streams at once, and from two graphs that replay at once with new residuals."""
+    runs = [layer(1, 40, 1024, 2048), layer(2, 200, 1024, 1920)]
+    start = [s["r"].clone() for s in runs]
+    want = []
+    for s in runs:
+        feed_forward(ops, **s)
+        want.append(bits(s))
+
+    def reset():
+        for s, r in zip(runs, start):
+            s["r"].copy_(r)
+            s["plane"].zero_()
+            s["x"].scale.zero_()
+            s["h"].scale.zero_()
+        torch.cuda.synchronize()
+
+    def same():
+        torch.cuda.synchronize()
+        return all(torch.equal(a, b) for s, w in zip(runs, want) for a, b in zip(bits(s), w))
+
+    streams = [torch.cuda.Stream() for _ in runs]
+    for _ in range(5):
+        reset()
+        for s, stream in zip(runs, streams):
+            with torch.cuda.stream(stream):
+                feed_forward(ops, **s)
+        assert same()
+    graphs = []
+    for s, stream in zip(runs, streams):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            feed_forward(ops, **s)
+        graphs.append(graph)
+    for _ in range(5):
+        reset()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        assert same()
+    ops.check()
+
+
+def test_refusals_of_the_kernels(ops):
+    from zse_b200.ops.native import NativeError
+    rows = Fp8Rows.empty(4, 128, DEV)
+    w = Fp8Weight.from_dense(torch.ones(32, 128, device=DEV))
+    odd = torch.empty(4 * 136 + 8, dtype=torch.uint8, device=DEV).view(F8)
+    for data in (odd[8: 8 + 512].view(4, 128), odd.as_strided((4, 128), (136, 1))):          # no TMA copy starts there
+        bad = Fp8Rows(data, rows.scale)
+        with pytest.raises(NativeError):
+            ops.linear_fp8(w, bad, 4, torch.empty(4, 32, device=DEV))
+        with pytest.raises(NativeError):
+            ops.quant_fp8(torch.zeros(4, 128, device=DEV), 4, bad)
+    with pytest.raises(NativeError):
+        ops.add_rmsnorm_fp8(torch.zeros(1, 32784, device=DEV), None, 0, None, torch.ones(32784, device=DEV).half(),
+                            Fp8Rows.empty(1, 32784, DEV), 1, 1e-6)
+    with pytest.raises(ValueError):
+        ops.linear_fp8(w, Fp8Rows.empty(4, 128), 4, torch.empty(4, 32, device=DEV))          # rows on the CPU
+    with pytest.raises(NativeError):
+        ops.quant_fp8(torch.zeros(4, 128), 4, Fp8Rows.empty(4, 128))                         # all of it on the CPU
+    out = marked(4, 128)
+    ops.quant_fp8(torch.zeros(4, 128, device=DEV), 0, out)
+    assert untouched(out, 0)

@@ -18,6 +18,7 @@ from ..format.layer_specs import GLU
 from . import reference as ref
 
 F16, F32, I32, I64 = torch.float16, torch.float32, torch.int32, torch.int64
+FP8_TYPES = {F16: 0, torch.bfloat16: 1, F32: 2}
 EPI_F16, EPI_SWIGLU, EPI_PARTIAL, EPI_RELU2 = 0, 1, 2, 5
 
 
@@ -238,6 +239,130 @@ class TorchOps:
                                        or int(cu_q[1: S + 1].max()) > min(q.shape[0], out.shape[0])):
             raise ValueError(f"up to {max_q} rows of a sequence expected, inside q and out")
         ref.attn_decode_q8(q, kv, block_tables, seq_lens, out, S, nh, scale, window, cu_q, q_pos0)
+
+    # ---- 8-bit floating point (ops.fp8: Fp8Rows, Fp8Weight) ---------------------------------------------
+    @staticmethod
+    def _rows_fp8(name: str, rows, M: int, columns: int, device: int) -> None:
+        data, scale = rows.data, rows.scale
+        if M < 0 or data.shape[0] < M or data.shape[1] != columns or columns < 16 or columns % 16:
+            raise ValueError(f"{name}: {M} rows of {columns} columns, a multiple of 16, do not fit {tuple(data.shape)}")
+        if data.stride(1) != 1 or (scale.shape[1] > 1 and scale.stride(1) != 1) or (data.shape[0] > 1 and data.stride(0) < columns) or (
+                scale.shape[0] > 1 and scale.stride(0) < scale.shape[1]):
+            raise ValueError(f"{name}: packed rows expected, not strides {data.stride()} and {scale.stride()}")
+        if data.get_device() != device:
+            raise ValueError(f"{name} is on {data.device}, not beside the other tensors")
+
+    @staticmethod
+    def _packed_fp8(device: int, **tensors) -> None:
+        """``tensors``: name = (tensor or None, dtypes, shape that it begins with, whether rows may be apart)."""
+        for name, (t, dtypes, shape, apart) in tensors.items():
+            if t is None:
+                continue
+            if t.dtype not in dtypes or t.dim() != len(shape) or t.get_device() != device:
+                raise ValueError(f"{name}: {' or '.join(map(str, dtypes))} with {len(shape)} dimensions expected beside the other "
+                                 f"tensors, not {t.dtype} {tuple(t.shape)} on {t.device}")
+            fits = t.shape[0] >= shape[0] and (len(shape) == 1 or (t.shape[1] >= shape[1] if apart else t.shape[1] == shape[1]))
+            packed = t.stride(-1) == 1 and (t.dim() == 1 or t.shape[0] == 1 or t.stride(0) >= t.shape[1]) if apart else t.is_contiguous()
+            if not fits or not packed:
+                raise ValueError(f"{name}: {'' if apart else 'packed '}rows {shape} expected, not {tuple(t.shape)} with strides {t.stride()}")
+
+    def _check_norm_fp8(self, residual, partials, n_partials, add, weight, out, M, normed):
+        device, H = residual.get_device(), residual.shape[-1]
+        if M < 0 or n_partials < 0:
+            raise ValueError(f"{M} rows, {n_partials} planes")
+        self._rows_fp8("out", out, M, H, device)
+        if weight.dtype not in (F16, torch.bfloat16):
+            raise ValueError(f"weight: fp16 or bfloat16 expected, not {weight.dtype}")
+        t = (weight.dtype,)
+        self._packed_fp8(device, residual=(residual, (F32,), (M, H), False), add=(add, t, (M, H), False), weight=(weight, t, (H,), False),
+                         normed=(normed, t, (M, H), False))
+        if weight.shape[0] != H:
+            raise ValueError(f"weight: {H} numbers expected, not {weight.shape[0]}")
+        if n_partials and (partials is None or partials.dtype is not F32 or partials.numel() < n_partials * M * H
+                           or not partials.is_contiguous() or partials.get_device() != device):
+            raise ValueError(f"{n_partials} fp32 planes of {M} rows of {H} columns expected, packed, beside the residual")
+
+    def add_rmsnorm_fp8(self, residual, partials, n_partials, add, weight, out, M, eps, normed=None):
+        """residual [M, H] += the sum of ``partials`` [n_partials, M, H] and of ``add`` (fp32, fp32, 16 bits; as in ``add_rmsnorm``);
+        out (``Fp8Rows``) = RMSNorm(residual) * weight in 8 bits, rounded from fp32, and ``normed`` the same in 16 bits.  ``weight``,
+        ``add`` and ``normed`` are all fp16 or all bfloat16.  H: a multiple of 16 up to 32768."""
+        self._check_norm_fp8(residual, partials, n_partials, add, weight, out, M, normed)
+        if M == 0:
+            return
+        H, r = residual.shape[1], residual[:M]
+        if n_partials or add is not None:
+            total = r.double()
+            if n_partials:
+                total = total + partials.view(-1)[: n_partials * M * H].view(n_partials, M, H).double().sum(0)
+            if add is not None:
+                total = total + add[:M].double()
+            r.copy_(total)
+        y = r * torch.rsqrt(r.double().square().mean(-1, keepdim=True) + eps).float() * weight.float()
+        ref.put_fp8(y, out[:M])
+        if normed is not None:
+            normed[:M] = y.clamp(-65504, 65504) if normed.dtype is F16 else y
+
+    def _check_quant_fp8(self, x, M, out, parts):
+        device = x.get_device()
+        self._rows_fp8("out", out, M, out.data.shape[1], device)
+        self._packed_fp8(device, x=(x, (F16, torch.bfloat16, F32), (M, parts * out.data.shape[1]), True))
+        if x.shape[1] != parts * out.data.shape[1]:
+            raise ValueError(f"x: {parts * out.data.shape[1]} columns expected, not {x.shape[1]}")
+
+    def quant_fp8(self, x, M, out):
+        """out (``Fp8Rows``) = the first M rows of ``x`` (fp16, bfloat16 or fp32) in 8 bits."""
+        self._check_quant_fp8(x, M, out, 1)
+        if M:
+            ref.put_fp8(x[:M].float(), out[:M])
+
+    def swiglu_fp8(self, gate_up, M, out, gelu=False):
+        """out (``Fp8Rows`` of C columns) = silu(gate) * up in 8 bits, rounded from fp32 (``gelu``: the tanh form of gelu instead);
+        ``gate_up`` [M, gate | up] in fp16, bfloat16 or fp32."""
+        self._check_quant_fp8(gate_up, M, out, 2)
+        C = out.data.shape[1]
+        if M:
+            ref.put_fp8(ref.gated(gate_up[:M, :C].float(), gate_up[:M, C:].float(), gelu), out[:M])
+
+    def _check_linear_fp8(self, w, x, M, out):
+        device = w.data.get_device()
+        if w.glu:
+            raise ValueError("a gate and up weight goes with linear_swiglu_fp8")
+        self._rows_fp8("x", x, M, w.data.shape[1], device)
+        self._weight_fp8(w)
+        self._packed_fp8(device, out=(out, (F16, torch.bfloat16, F32), (M, w.data.shape[0]), True))
+
+    @staticmethod
+    def _weight_fp8(w) -> None:
+        if w.data.shape[0] < 1 or w.data.stride(1) != 1 or (w.data.shape[0] > 1 and w.data.stride(0) < w.data.shape[1]):
+            raise ValueError(f"w: packed rows expected, not {tuple(w.data.shape)} with strides {w.data.stride()}")
+
+    def linear_fp8(self, w, x, M, out):
+        """out [M, N] (fp16, bfloat16 or fp32) = x w^T + bias of the first M rows of ``x`` (``Fp8Rows``); ``w``: ``Fp8Weight``.  Sums in
+        fp32, rounded once; fp16 is held within +-65504.  K: a multiple of 16."""
+        self._check_linear_fp8(w, x, M, out)
+        if M == 0:
+            return
+        y = x[:M].dequant() @ w.dequant().t()
+        if w.bias is not None:
+            y = y + w.bias.float()
+        out[:M, : w.N] = y.clamp(-65504, 65504) if out.dtype is F16 else y
+
+    def _check_linear_swiglu_fp8(self, w, x, M, out):
+        device = w.data.get_device()
+        if not w.glu:
+            raise ValueError("a gate and up weight (glu=True) is expected")
+        self._rows_fp8("x", x, M, w.data.shape[1], device)
+        self._weight_fp8(w)
+        self._rows_fp8("out", out, M, w.data.shape[0] // 2, device)
+
+    def linear_swiglu_fp8(self, w, x, M, out, gelu=False):
+        """out (``Fp8Rows`` of N / 2 columns) = silu(x gate^T) * (x up^T) in 8 bits, rounded from fp32 (``gelu``: the tanh form of gelu
+        instead); ``w``: an ``Fp8Weight`` with ``glu``.  N / 2 and K: multiples of 16."""
+        self._check_linear_swiglu_fp8(w, x, M, out)
+        if M == 0:
+            return
+        gate, up = (x[:M].dequant() @ w.dequant().t()).chunk(2, 1)
+        ref.put_fp8(ref.gated(gate, up, gelu), out[:M])
 
     # ---- latent attention and routed feed-forward -----------------------------------------------------
     # (activations and cache at the model's own width: bfloat16 or fp32)
@@ -1293,6 +1418,46 @@ class CudaOps(TorchOps):
 
     # (The three calls of the 8-bit cache are written out flat: outside a CUDA graph a small one is mostly Python.  What is plainly in
     # order is seen at a glance; the checks of the base class take the rest and name what is wrong.)
+    # ---- 8-bit floating point: a call packs its arguments itself, and only one that is not as it should be is looked at by name -----
+    def add_rmsnorm_fp8(self, residual, partials, n_partials, add, weight, out, M, eps, normed=None):
+        self._check_norm_fp8(residual, partials, n_partials, add, weight, out, M, normed)
+        n, data, scale = self.n, out.data, out.scale
+        n.launched(n.load().zse_add_rmsnorm_fp8(n.NORM_FP8.pack(
+            residual.data_ptr(), partials.data_ptr() if n_partials else 0, 0 if add is None else add.data_ptr(), weight.data_ptr(),
+            0 if normed is None else normed.data_ptr(), data.data_ptr(), scale.data_ptr(), n.stream_of(data.get_device(), self.home),
+            data.stride(0), scale.stride(0), eps, n_partials, M, residual.shape[1], FP8_TYPES[weight.dtype])), "add_rmsnorm_fp8")
+
+    def quant_fp8(self, x, M, out):
+        self._quant_fp8(x, M, out, 1, 0)
+
+    def swiglu_fp8(self, gate_up, M, out, gelu=False):
+        self._quant_fp8(gate_up, M, out, 2, 2 if gelu else 1)
+
+    def _quant_fp8(self, x, M, out, parts, act):
+        self._check_quant_fp8(x, M, out, parts)
+        n, data, scale = self.n, out.data, out.scale
+        n.launched(n.load().zse_quant_fp8(n.QUANT_FP8.pack(
+            x.data_ptr(), data.data_ptr(), scale.data_ptr(), n.stream_of(data.get_device(), self.home), x.stride(0), data.stride(0),
+            scale.stride(0), M, data.shape[1], act, FP8_TYPES[x.dtype])), "quant_fp8")
+
+    def linear_fp8(self, w, x, M, out):
+        self._check_linear_fp8(w, x, M, out)
+        n, wd, xd, xs, bias = self.n, w.data, x.data, x.scale, w.bias
+        N, K = wd.shape
+        n.launched(n.load().zse_gemm_fp8(n.GEMM_FP8.pack(
+            xd.data_ptr(), xs.data_ptr(), wd.data_ptr(), w.scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), 0,
+            self.status_ptr, n.stream_of(wd.get_device(), self.home), xd.stride(0), wd.stride(0), out.stride(0), xs.stride(0), 0, M, N, K,
+            FP8_TYPES[out.dtype], 0 if bias is None else FP8_TYPES[bias.dtype], 0)), "linear_fp8")
+
+    def linear_swiglu_fp8(self, w, x, M, out, gelu=False):
+        self._check_linear_swiglu_fp8(w, x, M, out)
+        n, wd, xd, xs, data, scale = self.n, w.data, x.data, x.scale, out.data, out.scale
+        N, K = wd.shape
+        n.launched(n.load().zse_gemm_fp8(n.GEMM_FP8.pack(
+            xd.data_ptr(), xs.data_ptr(), wd.data_ptr(), w.scale.data_ptr(), 0, data.data_ptr(), scale.data_ptr(), self.status_ptr,
+            n.stream_of(wd.get_device(), self.home), xd.stride(0), wd.stride(0), data.stride(0), xs.stride(0), scale.stride(0), M, N // 2,
+            K, 0, 0, 2 if gelu else 1)), "linear_swiglu_fp8")
+
     def rope_kv_write_q8(self, qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out=None, planes=None, n_planes=0,
                          bias=None):
         if q_out is None:

@@ -117,6 +117,10 @@ WRITE_Q8 = struct.Struct("<" + _KV_Q8 + "9Q6i")
 READ_Q8 = struct.Struct("<" + _KV_Q8 + "7Q6i")
 ATTN_Q8 = struct.Struct("<" + _KV_Q8 + "9Qq10ifi")
 NEEDS_SCRATCH = -6
+# The same for the operators on 8-bit floating point (ZseNormFp8, ZseQuantFp8, ZseGemmFp8).
+NORM_FP8 = struct.Struct("<8Q2qd4i")
+QUANT_FP8 = struct.Struct("<4Q3q4i")
+GEMM_FP8 = struct.Struct("<9Q5q6i")
 
 _lib: Optional[ctypes.CDLL] = None
 
@@ -126,6 +130,9 @@ _SIGS = {
     "zse_gemm_w4_splits": (c_int, [c_int, c_int, c_int, c_int]),
     "zse_rope_kv_write_q8": (c_int, [c_char_p]),
     "zse_kv_read_q8": (c_int, [c_char_p]),
+    "zse_add_rmsnorm_fp8": (c_int, [c_char_p]),
+    "zse_quant_fp8": (c_int, [c_char_p]),
+    "zse_gemm_fp8": (c_int, [c_char_p]),
     "zse_attn_decode_q8_pieces": (c_int, [c_char_p]),
     "zse_attn_decode_q8_scratch_floats": (c_int64, [c_char_p]),
     "zse_attn_decode_q8": (c_int, [c_char_p]),
@@ -537,6 +544,14 @@ def stream_q8(data, scale, home: int) -> int:
         raise NativeError(f"the cache is on {data.device}, the operators are on device {home}, the current device is {at}")
     if not (data.is_contiguous() and scale.is_contiguous()):
         raise NativeError("a layer of an 8-bit cache has to be contiguous")
+    return torch._C._cuda_getCurrentRawStream(at)
+
+
+def stream_of(device: int, home: int) -> int:
+    """The current stream of ``device``, where a call's tensors are: the current device, and that of the operators (``home``)."""
+    at = torch._C._cuda_getDevice()
+    if device != at or at != home:
+        raise NativeError(f"the tensors are on device {device}, the operators on device {home}, the current device is {at}")
     return torch._C._cuda_getCurrentRawStream(at)
 
 

@@ -236,6 +236,23 @@ def rope_kv_write_q8(x: torch.Tensor, kv, positions: torch.Tensor, slots: torch.
     return h[:, :nh].reshape(M, nh * hd).to(torch.float16)
 
 
+def put_fp8(y: torch.Tensor, out) -> None:
+    """Rows y (fp32) into ``out`` (``ops.fp8.Fp8Rows`` of as many rows)."""
+    M, C = y.shape
+    n = out.scale.shape[0]
+    y = torch.nn.functional.pad(y, (0, n * 128 - C)).view(M, n, 128)
+    top = y.abs().amax(-1)
+    none = top <= 1e-30
+    steps = torch.where(none, torch.zeros_like(top), 448 / top)
+    out.data.copy_((y * steps[..., None]).view(M, -1)[:, :C].to(out.data.dtype))
+    out.scale.copy_(torch.where(none, torch.zeros_like(top), top / 448).t())
+
+
+def gated(g: torch.Tensor, u: torch.Tensor, gelu: bool) -> torch.Tensor:
+    z = 1.5957691216057308 * (g + 0.044715 * g * g * g) if gelu else g
+    return g / (1 + torch.exp(-z)) * u
+
+
 def kv_read_q8(kv, block_tables: torch.Tensor, seq_lens: torch.Tensor, cu_blocks: torch.Tensor, out: torch.Tensor,
                out_tables: torch.Tensor) -> None:
     """Pages of whole sequences as fp16: block j of sequence s goes to ``out[cu_blocks[s] + j]`` [2, nkv, bs, hd] with zeros behind
