@@ -11,6 +11,7 @@
 #include "api.h"
 #include "fp8.cuh"
 #include "gemm_common.cuh"
+#include "pair.cuh"
 
 namespace zse {
 
@@ -54,7 +55,12 @@ __device__ __forceinline__ float bias_of(const Fp8Args& a, int n) {
 
 __device__ __forceinline__ float gated(int act, float g, float u) { return act == kFp8Silu ? fp8_gated<kFp8Silu>(g, u) : fp8_gated<kFp8Gelu>(g, u); }
 
-// The row's columns n .. n + C - 1 to memory, rounded to the output's type.
+__device__ __forceinline__ void store32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+               "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+// The row's columns n .. n + C - 1 to memory, rounded to the output's type: 32 bytes, a sector, at a time where the row lies so.
 template <int C>
 __device__ __forceinline__ void put_row(const Fp8Args& a, float* y, int t, int n) {
   if (a.bias != nullptr) {
@@ -63,13 +69,12 @@ __device__ __forceinline__ void put_row(const Fp8Args& a, float* y, int t, int n
       if (n + i < a.N) y[i] += bias_of(a, n + i);
   }
   const size_t at = size_t(t) * a.ldo + n;
-  const int item = a.type == kFp8F32 ? 4 : 2;
-  const bool wide = n + C <= a.N && ((reinterpret_cast<uintptr_t>(a.out) + at * item) & 15) == 0;
+  const bool whole = n + C <= a.N;
   if (a.type == kFp8F32) {
     float* o = static_cast<float*>(a.out) + at;
-    if (wide) {
+    if (whole && (reinterpret_cast<uintptr_t>(o) & 31) == 0) {
 #pragma unroll
-      for (int i = 0; i < C; i += 4) *reinterpret_cast<float4*>(o + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+      for (int i = 0; i < C; i += 8) store32(o + i, reinterpret_cast<const uint32_t*>(y + i));
     } else {
 #pragma unroll
       for (int i = 0; i < C; ++i)
@@ -78,18 +83,67 @@ __device__ __forceinline__ void put_row(const Fp8Args& a, float* y, int t, int n
     return;
   }
   uint16_t* o = static_cast<uint16_t*>(a.out) + at;
+  const bool wide = whole && (reinterpret_cast<uintptr_t>(o) & 31) == 0;
 #pragma unroll
-  for (int i = 0; i < C; i += 8) {
-    uint32_t v[4];
+  for (int i = 0; i < C; i += 16) {
+    uint32_t v[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 8; ++j)
       v[j] = a.type == kFp8BF16 ? pack2<bf16>(y[i + 2 * j], y[i + 2 * j + 1]) : pack2<__half>(y[i + 2 * j], y[i + 2 * j + 1]);
     if (wide) {
-      *reinterpret_cast<uint4*>(o + i) = make_uint4(v[0], v[1], v[2], v[3]);
+      store32(o + i, v);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < 16; ++j)
         if (n + i + j < a.N) o[i + j] = uint16_t(v[j >> 1] >> (16 * (j & 1)));
+    }
+  }
+}
+
+// act(gate) * up of 64 neighbouring outputs of a row (acc: gates, then ups), the other 64 of their block in the thread of the other half.
+// `live` is false where the sums are not there; every warp of the barrier calls it.
+__device__ __forceinline__ void put_gated(const Fp8Args& a, float* acc, int t, int n, int half, float (*tops)[128], int row, int barrier,
+                                          int threads, bool live) {
+  constexpr int O = 64;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < O; ++i) {
+    acc[i] = n + i < a.N ? gated(a.act, acc[i], acc[O + i]) : 0.f;
+    top = max(top, abs_bits(acc[i]));
+  }
+  tops[half][row] = __uint_as_float(top);
+  asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
+  top = max(top, __float_as_uint(tops[half ^ 1][row]));
+  if (live && t < a.M) {
+    const float steps = fp8_steps(__uint_as_float(top));
+    uint8_t* o = static_cast<uint8_t*>(a.out) + t * a.ldo + n;
+#pragma unroll
+    for (int i = 0; i < O; i += 16)                            // (N is a multiple of 16)
+      if (n + i < a.N)
+        *reinterpret_cast<uint4*>(o + i) =
+            make_uint4(fp8_pack4(acc + i, steps), fp8_pack4(acc + i + 4, steps), fp8_pack4(acc + i + 8, steps), fp8_pack4(acc + i + 12, steps));
+    if (half == 0) a.out_scale[(n / kFp8Block) * a.ld_os + t] = fp8_scale(__uint_as_float(top));
+  }
+}
+
+// acc += s * (columns c0 .. of the accumulator): sixteen columns are read while the sixteen before are added
+template <int C, int SPLIT>
+__device__ __forceinline__ void add_block(float* acc, uint32_t taddr, float s, float s_up) {
+  uint32_t r[2][16];
+  ZSE_TMEM_LD_X16(r[0], taddr);
+#pragma unroll
+  for (int c = 0; c < C; c += 16) {
+    uint32_t* now = r[(c >> 4) & 1];
+    uint32_t* next = r[((c >> 4) & 1) ^ 1];
+    tc_wait_ld();
+    if (c + 16 < C) ZSE_TMEM_LD_X16(next, taddr + c + 16);
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const float f = c < SPLIT ? s : s_up;
+      asm("{\n\t.reg .b64 p, f, c;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 f, {%4, %4};\n\tmov.b64 c, {%0, %1};\n\t"
+          "fma.rn.f32x2 c, p, f, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
+          : "+f"(acc[c + i]), "+f"(acc[c + i + 1])
+          : "f"(__uint_as_float(now[i])), "f"(__uint_as_float(now[i + 1])), "f"(f));
     }
   }
 }
@@ -191,40 +245,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
         live = __all_sync(0xffffffffu, mbar_wait(&bars->acc_full[buf], (k >> 1) & 1, abort_flag, a.status, 83, k));
         if (!live) break;
         tc_fence_after_sync();
-#pragma unroll
-        for (int c = 0; c < C; c += 16) {
-          uint32_t r[16];
-          ZSE_TMEM_LD_X16(r, taddr + buf * NT + c);
-          tc_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(__uint_as_float(r[i]), GLU && c >= C / 2 ? s_up : s, acc[c + i]);
-        }
+        add_block<C, GLU ? C / 2 : C>(acc, taddr + buf * NT, s, s_up);
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->acc_empty[buf]);
       }
       if constexpr (GLU) {
-        constexpr int O = C / 2;                               // outputs of a thread
-        const int n = n0 + half * O;
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < O; ++i) {
-          acc[i] = n + i < a.N ? gated(a.act, acc[i], acc[O + i]) : 0.f;
-          top = max(top, abs_bits(acc[i]));
-        }
-        bars->top[half][row] = __uint_as_float(top);
-        asm volatile("bar.sync 1, %0;" ::"r"(64 * quarters) : "memory");
-        top = max(top, __float_as_uint(bars->top[half ^ 1][row]));
-        if (live && t < a.M) {
-          const float steps = fp8_steps(__uint_as_float(top));
-          uint8_t* o = static_cast<uint8_t*>(a.out) + t * a.ldo + n;
-#pragma unroll
-          for (int i = 0; i < O; i += 16)                      // (N is a multiple of 16)
-            if (n + i < a.N)
-              *reinterpret_cast<uint4*>(o + i) = make_uint4(fp8_pack4(acc + i, steps), fp8_pack4(acc + i + 4, steps),
-                                                            fp8_pack4(acc + i + 8, steps), fp8_pack4(acc + i + 12, steps));
-          if (half == 0) a.out_scale[(n0 / kFp8Block) * a.ld_os + t] = fp8_scale(__uint_as_float(top));
-        }
+        put_gated(a, acc, t, n0 + half * 64, half, bars->top, row, 1, 64 * quarters, live);
       } else if (live && t < a.M && n0 + half * C < a.N) {
         put_row<C>(a, acc, t, n0 + half * C);
       }
@@ -239,6 +266,199 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, 2 * NT);
+}
+
+// ---- many tokens: pairs of CTAs, persistent ------------------------------------------------------------------------------------------
+// 256 tokens and NT weight rows a pair (cta_group::2): a CTA has 128 of the tokens, loads those and half of the weight rows, and owns the
+// sums of its tokens.
+constexpr int kPairThreads = 384;                // warp 0 loads, warp 1 issues the products, warps 4 .. 11 add them up
+// Registers: 168 a thread at launch (64512), then 56 for the first four warps and 216 for the other eight (62464): 128 sums and two reads of 16
+// columns do not fit 168.
+constexpr int kPairStagesMax = 8;
+template <int NT>
+constexpr int kPairStages = NT == 256 ? 6 : 8;
+template <int NT>
+constexpr int kPairStage = 128 * 128 + NT / 2 * 128;
+
+struct Fp8PairBars {
+  uint64_t full[kPairStagesMax], empty[kPairStagesMax];
+  uint64_t acc_full[2], acc_empty[2];
+  uint32_t tmem_base;
+  int abort_flag;
+  float top[2][2][128];                          // two units: a warp may be a unit ahead of the one that has the other 64 outputs
+};
+
+// Units (256 tokens x a tile of weight rows) in an order that keeps m_group token tiles in L2 while the weights stream past them once.
+struct Fp8Units {
+  int n_tiles, m_tiles, m_group;
+  __device__ __forceinline__ void at(int i, int* n, int* m) const {
+    const int g = i / (n_tiles * m_group), r = i - g * n_tiles * m_group, gm = min(m_group, m_tiles - g * m_group);
+    *n = r / gm;
+    *m = g * m_group + r % gm;
+  }
+};
+
+__device__ __forceinline__ void umma_fp8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+template <int NT, bool GLU>
+__global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
+gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Fp8Args a,
+                     const Fp8Units units) {
+  constexpr int kA = 128 * 128, kStage = kPairStage<NT>, kStages = kPairStages<NT>;
+  constexpr int C = NT / 2;                                    // columns of a thread
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Fp8PairBars* bars = reinterpret_cast<Fp8PairBars*>(ring + kStages * kStage);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t crank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(crank));
+  const int pair = blockIdx.x >> 1, workers = gridDim.x >> 1, n_units = units.n_tiles * units.m_tiles;
+  const int n_kb = (a.K + kFp8Block - 1) / kFp8Block;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&bars->full[i], 1);
+      mbar_init(&bars->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->acc_full[i], 1);
+      mbar_init(&bars->acc_empty[i], 16);
+    }
+    bars->abort_flag = 0;
+    mbar_fence_init();
+    prefetch_tmap(&tmap_x);
+    prefetch_tmap(&tmap_w);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(2 * NT) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  pair_cluster_sync();                                         // both CTAs' barriers exist before anybody signals them
+  tc_fence_after_sync();
+  const uint32_t tmem = bars->tmem_base;
+  volatile int* abort_flag = &bars->abort_flag;
+  pdl_launch_dependents();                                     // (the TMEM is ours: a dependent cannot take it first)
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0 && lane == 0) {
+      pdl_wait();
+      int s = 0, c = 0;
+      uint32_t ph = 1;
+      bool live = true;
+      for (int i = pair; i < n_units && live; i += workers) {
+        int n, m;
+        units.at(i, &n, &m);
+        const int t0 = m * 256 + int(crank) * 128;
+        for (int k = 0; k < n_kb; ++k, ++c) {
+          if (c >= kStages && !mbar_wait(&bars->empty[s], ph, abort_flag, a.status, 90, c)) {
+            live = false;
+            break;
+          }
+          const uint32_t full = map_to_rank(smem_u32(&bars->full[s]), 0);
+          if (crank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * kStage);
+          const uint32_t to = smem_u32(ring) + s * kStage;
+          tma_load_2d_pair(to, &tmap_x, k * kFp8Block, t0, full);
+          if constexpr (GLU) {                                 // columns 0 .. 127 of the product: 64 gate rows and their up rows; the rest: the next
+            const int g = n * 128 + int(crank) * 64;
+            tma_load_2d_pair(to + kA, &tmap_w, k * kFp8Block, g, full);
+            tma_load_2d_pair(to + kA + 8192, &tmap_w, k * kFp8Block, a.N + g, full);
+          } else {
+#pragma unroll
+            for (int h = 0; h < NT / 128; ++h)
+              tma_load_2d_pair(to + kA + h * 8192, &tmap_w, k * kFp8Block, n * NT + int(crank) * (NT / 2) + h * 64, full);
+          }
+          if (++s == kStages) { s = 0; ph ^= 1; }
+        }
+      }
+    } else if (warp == 1 && crank == 0) {
+      constexpr uint32_t idesc = make_idesc_f16(256, NT);      // (format 0 of kind::f8f6f4 is e4m3)
+      const uint64_t desc = make_desc_sw128(smem_u32(ring));
+      int s = 0, c = 0;
+      uint32_t ph = 0;
+      bool live = true;
+      for (int i = pair; i < n_units && live; i += workers) {
+        for (int k = 0; k < n_kb; ++k, ++c) {
+          const int buf = c & 1;
+          bool ok = c < 2 || mbar_wait_cluster(&bars->acc_empty[buf], ((c >> 1) & 1) ^ 1, abort_flag, a.status, 91, c);
+          ok = ok && mbar_wait_cluster(&bars->full[s], ph, abort_flag, a.status, 92, c);
+          live = __all_sync(0xffffffffu, ok);
+          if (!live) break;
+          tc_fence_after_sync();
+          const uint64_t da = desc + uint64_t((s * kStage) >> 4), db = da + (kA >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) umma_fp8_pair(tmem + buf * NT, da + j * 2, db + j * 2, idesc, j != 0);
+            tc_commit_pair(&bars->empty[s]);
+            tc_commit_pair(&bars->acc_full[buf]);
+          }
+          __syncwarp();
+          if (++s == kStages) { s = 0; ph ^= 1; }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int q = warp & 3, half = (warp - 4) >> 2, row = q * 32 + lane;
+    const uint32_t taddr = tmem + (uint32_t(q * 32) << 16) + half * C;
+    const uint32_t empty_bar = map_to_rank(smem_u32(&bars->acc_empty[0]), 0);
+    const int nbs = (a.N + kFp8Block - 1) / kFp8Block;
+    bool live = true;
+    int c = 0, unit = 0;
+    pdl_wait();
+    for (int i = pair; i < n_units; i += workers, ++unit) {
+      int n, m;
+      units.at(i, &n, &m);
+      const int t = m * 256 + int(crank) * 128 + row;
+      const int nb = GLU ? n : (n * NT + half * C) / kFp8Block;
+      const float* sw = a.sw + size_t(min(nb, nbs - 1)) * n_kb;
+      const float* sw_up = GLU ? sw + size_t(nbs) * n_kb : sw;
+      const float* sx = a.sx + min(t, a.M - 1);
+      float acc[C];
+#pragma unroll
+      for (int j = 0; j < C; ++j) acc[j] = 0.f;
+      float x = sx[0], w = sw[0], w_up = sw_up[0];             // scales of a block are loaded while the one before is added
+      for (int k = 0; k < n_kb; ++k, ++c) {
+        const float f = x * w, f_up = GLU ? x * w_up : f;
+        if (k + 1 < n_kb) {
+          x = sx[size_t(k + 1) * a.ld_sx];
+          w = sw[k + 1];
+          if (GLU) w_up = sw_up[k + 1];
+        }
+        const int buf = c & 1;
+        live = live && __all_sync(0xffffffffu, mbar_wait(&bars->acc_full[buf], (c >> 1) & 1, abort_flag, a.status, 93, c));
+        if (!live) break;
+        tc_fence_after_sync();
+        add_block<C, GLU ? C / 2 : C>(acc, taddr + buf * NT, f, f_up);
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(empty_bar + buf * 8);
+      }
+      if constexpr (GLU) {
+        put_gated(a, acc, t, n * 128 + half * 64, half, bars->top[unit & 1], row, 1 + q, 64, live);
+      } else if (live && t < a.M && n * NT + half * C < a.N) {
+        put_row<C>(a, acc, t, n * NT + half * C);
+      }
+    }
+  }
+  __syncthreads();
+  if (*abort_flag) {                                           // copies in flight must land before the CTA may leave
+    const uint64_t began = globaltimer_ns();
+    while (globaltimer_ns() - began < 1000000ull) {
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  pair_cluster_sync();                                         // nobody leaves while the other CTA may still signal it
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * NT) : "memory");
 }
 
 // e4m3 rows [rows, K], ld bytes apart: box = 128 columns x box_rows rows, 128-byte swizzle, zeros out of bounds
@@ -270,6 +490,25 @@ int launch(const ZseGemmFp8& g, const Fp8Args& a, cudaStream_t st) {
   return launch_pdl(kern, dim3((g.N + cols - 1) / cols, (g.M + 127) / 128), dim3(kThreads), smem, st, tx, tw, a) == cudaSuccess ? 1 : ZSE_ERR_LAUNCH;
 }
 
+template <int NT, bool GLU>
+int launch_pair(const ZseGemmFp8& g, const Fp8Args& a, cudaStream_t st) {
+  CUtensorMap tx, tw;
+  if (int rc = make_map(g.x, g.M, g.K, g.ldx, 128, &tx)) return rc;
+  if (int rc = make_map(g.w, GLU ? 2ull * g.N : g.N, g.K, g.ldw, 64, &tw)) return rc;
+  constexpr int smem = kPairStages<NT> * kPairStage<NT> + int(sizeof(Fp8PairBars)) + 1024;
+  auto kern = gemm_fp8_pair_kernel<NT, GLU>;
+  static bool attr_done[kMaxDevices] = {};
+  const int dev = current_device_slot();
+  if (!attr_done[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return ZSE_ERR_LAUNCH;
+    attr_done[dev] = true;
+  }
+  const int cols = GLU ? NT / 2 : NT, m_tiles = (g.M + 255) / 256, n_tiles = (g.N + cols - 1) / cols, groups = (m_tiles + 7) / 8;
+  const Fp8Units u{n_tiles, m_tiles, (m_tiles + groups - 1) / groups};        // about 2048 tokens at a time
+  const int pairs = std::min<long long>(sm_count() / 2, (long long)n_tiles * m_tiles);
+  return launch_pdl(kern, dim3(2 * pairs), dim3(kPairThreads), smem, st, tx, tw, a, u) == cudaSuccess ? 1 : ZSE_ERR_LAUNCH;
+}
+
 }  // namespace
 }  // namespace zse
 
@@ -289,5 +528,6 @@ extern "C" int zse_gemm_fp8(const ZseGemmFp8* g) {
   const Fp8Args a{static_cast<const float*>(g->sx), static_cast<const float*>(g->sw), g->bias, g->out, static_cast<float*>(g->out_scale),
                   g->ldo, g->ld_sx, g->ld_os, g->M, g->N, g->K, g->type, g->bias_type, g->act, static_cast<Status*>(g->status)};
   const cudaStream_t st = static_cast<cudaStream_t>(g->stream);
+  if (g->M > 256) return glu ? launch_pair<256, true>(*g, a, st) : launch_pair<256, false>(*g, a, st);
   return glu ? launch<256, true>(*g, a, st) : launch<128, false>(*g, a, st);
 }

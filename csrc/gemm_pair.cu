@@ -29,6 +29,7 @@
 // measured cuBLAS burst peak), down 279 -> 181 us (1599), o 131 -> 78 us, QKV 154 -> 115 us; 7B gate/up 77 tokens 50 -> 38 us, INT8
 // 1500 tokens (expanded to fp16 first before) 411 + 74 -> 295 us.
 #include "gemm_common.cuh"
+#include "pair.cuh"
 
 namespace zse {
 
@@ -82,54 +83,6 @@ __device__ __forceinline__ PairUnit pair_unit(const PairArgs& a, int i) {
   return u;
 }
 
-__device__ __forceinline__ uint32_t map_to_rank(uint32_t smem_addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Bounded wait for arrivals that may come from the other CTA of the pair (same contract as mbar_wait).
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag, Status* st,
-                                                  unsigned where, unsigned detail) {
-  if (mbar_try_wait_cluster(bar, parity)) return true;
-  uint64_t t0 = 0;
-  unsigned spins = 0;
-  while (!mbar_try_wait_cluster(bar, parity)) {
-    if ((++spins & 0xFF) == 0) {
-      if (*abort_flag) return false;
-      const uint64_t now = globaltimer_ns();
-      if (t0 == 0) t0 = now;
-      if (now - t0 > kWaitLimitNs) {
-        report(st, kWaitTimeout, where, detail);
-        *abort_flag = 1;
-        __threadfence_block();
-        return false;
-      }
-    }
-  }
-  return true;
-}
-// Tiled load into this CTA's shared memory whose bytes are counted at a barrier of either CTA of the pair.
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap, int x, int y, uint32_t cluster_bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-      "[%4];" ::"r"(dst),
-      "l"(tmap), "r"(x), "r"(y), "r"(cluster_bar)
-      : "memory");
-}
 __device__ __forceinline__ void umma_ts_pair(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                              uint32_t accumulate) {
   asm volatile(
@@ -138,17 +91,6 @@ __device__ __forceinline__ void umma_ts_pair(uint32_t d_tmem, uint32_t a_tmem, u
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {          // arrives at this offset in both CTAs
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          smem_u32(bar)),
-      "h"(uint16_t(3))
-      : "memory");
-}
-__device__ __forceinline__ void pair_cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 // All-gather in the prologue: rows [t0, t1) were written into this GPU's memory by their owners (other GPUs, plain or
 // multicast stores); a row block is complete when its flag holds the pass epoch.  One thread waits (bounded), then orders those
 // writes before the TMA loads it is about to issue (async proxy).
