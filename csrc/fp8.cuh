@@ -28,11 +28,12 @@ __device__ __forceinline__ uint32_t fp8_pack4(const float* y, float steps) {
   return lo | hi << 16;
 }
 
-// act(g) * u.  gelu's tanh form is g * sigmoid(2 z).
+// act(g) * u.  gelu's tanh form is g * sigmoid(2 z).  The special-function unit's sigmoid is off by a few units in the last place of fp32,
+// 2^-17 of half a step of e4m3; with expf and a division rows of 13824 took a third longer.
 template <int ACT>
 __device__ __forceinline__ float fp8_gated(float g, float u) {
   const float z = ACT == kFp8Silu ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
-  return __fdiv_rn(g, 1.f + expf(-z)) * u;
+  return g * sigmoid_fast(z) * u;
 }
 
 // two numbers in 16 bits each; fp16 is held within its largest, and a NaN stays one

@@ -126,7 +126,14 @@ __device__ __forceinline__ void put_gated(const Fp8Args& a, float* acc, int t, i
   }
 }
 
-// acc += s * (columns c0 .. of the accumulator): sixteen columns are read while the sixteen before are added
+// Waits for the loads from TMEM; what they brought are operands, so that nothing that uses it moves before the wait.
+__device__ __forceinline__ void tc_wait_ld16(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
+// acc += s (s_up from column SPLIT on) * the accumulator's columns: sixteen are read while the sixteen before are added.  (Packed pairs,
+// fma.rn.f32x2, took longer: they have to be brought together first.)
 template <int C, int SPLIT>
 __device__ __forceinline__ void add_block(float* acc, uint32_t taddr, float s, float s_up) {
   uint32_t r[2][16];
@@ -134,17 +141,10 @@ __device__ __forceinline__ void add_block(float* acc, uint32_t taddr, float s, f
 #pragma unroll
   for (int c = 0; c < C; c += 16) {
     uint32_t* now = r[(c >> 4) & 1];
-    uint32_t* next = r[((c >> 4) & 1) ^ 1];
-    tc_wait_ld();
-    if (c + 16 < C) ZSE_TMEM_LD_X16(next, taddr + c + 16);
+    tc_wait_ld16(now);
+    if (c + 16 < C) ZSE_TMEM_LD_X16(r[((c >> 4) & 1) ^ 1], taddr + c + 16);
 #pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-      const float f = c < SPLIT ? s : s_up;
-      asm("{\n\t.reg .b64 p, f, c;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 f, {%4, %4};\n\tmov.b64 c, {%0, %1};\n\t"
-          "fma.rn.f32x2 c, p, f, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
-          : "+f"(acc[c + i]), "+f"(acc[c + i + 1])
-          : "f"(__uint_as_float(now[i])), "f"(__uint_as_float(now[i + 1])), "f"(f));
-    }
+    for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(__uint_as_float(now[i]), c < SPLIT ? s : s_up, acc[c + i]);
   }
 }
 
@@ -274,15 +274,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
 constexpr int kPairThreads = 384;                // warp 0 loads, warp 1 issues the products, warps 4 .. 11 add them up
 // Registers: 168 a thread at launch (64512), then 56 for the first four warps and 216 for the other eight (62464): 128 sums and two reads of 16
 // columns do not fit 168.
-constexpr int kPairStagesMax = 8;
-template <int NT>
-constexpr int kPairStages = NT == 256 ? 6 : 8;
-template <int NT>
-constexpr int kPairStage = 128 * 128 + NT / 2 * 128;
+constexpr int kPairStages = 6, kPairStage = 2 * 128 * 128;
 
 struct Fp8PairBars {
-  uint64_t full[kPairStagesMax], empty[kPairStagesMax];
-  uint64_t acc_full[2], acc_empty[2];
+  uint64_t full[kPairStages], done[kPairStages];   // done: a stage's products are complete: it may be filled again, its accumulator read
+  uint64_t acc_empty[2];
   uint32_t tmem_base;
   int abort_flag;
   float top[2][2][128];                          // two units: a warp may be a unit ahead of the one that has the other 64 outputs
@@ -306,27 +302,25 @@ __device__ __forceinline__ void umma_fp8_pair(uint32_t d_tmem, uint64_t a_desc, 
       : "memory");
 }
 
-template <int NT, bool GLU>
+template <bool GLU>
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
 gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Fp8Args a,
                      const Fp8Units units) {
-  constexpr int kA = 128 * 128, kStage = kPairStage<NT>, kStages = kPairStages<NT>;
-  constexpr int C = NT / 2;                                    // columns of a thread
+  constexpr int kA = 128 * 128, C = 128;                       // C: columns of a thread
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Fp8PairBars* bars = reinterpret_cast<Fp8PairBars*>(ring + kStages * kStage);
+  Fp8PairBars* bars = reinterpret_cast<Fp8PairBars*>(ring + kPairStages * kPairStage);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t crank;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(crank));
   const int pair = blockIdx.x >> 1, workers = gridDim.x >> 1, n_units = units.n_tiles * units.m_tiles;
   const int n_kb = (a.K + kFp8Block - 1) / kFp8Block;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < kPairStages; ++i) {
       mbar_init(&bars->full[i], 1);
-      mbar_init(&bars->empty[i], 1);
+      mbar_init(&bars->done[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars->acc_full[i], 1);
       mbar_init(&bars->acc_empty[i], 16);
     }
     bars->abort_flag = 0;
@@ -335,7 +329,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
     prefetch_tmap(&tmap_w);
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(2 * NT) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   tc_fence_before_sync();
@@ -358,28 +352,26 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
         units.at(i, &n, &m);
         const int t0 = m * 256 + int(crank) * 128;
         for (int k = 0; k < n_kb; ++k, ++c) {
-          if (c >= kStages && !mbar_wait(&bars->empty[s], ph, abort_flag, a.status, 90, c)) {
+          if (c >= kPairStages && !mbar_wait(&bars->done[s], ph, abort_flag, a.status, 90, c)) {
             live = false;
             break;
           }
           const uint32_t full = map_to_rank(smem_u32(&bars->full[s]), 0);
-          if (crank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * kStage);
-          const uint32_t to = smem_u32(ring) + s * kStage;
+          if (crank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * kPairStage);
+          const uint32_t to = smem_u32(ring) + s * kPairStage;
           tma_load_2d_pair(to, &tmap_x, k * kFp8Block, t0, full);
           if constexpr (GLU) {                                 // columns 0 .. 127 of the product: 64 gate rows and their up rows; the rest: the next
             const int g = n * 128 + int(crank) * 64;
             tma_load_2d_pair(to + kA, &tmap_w, k * kFp8Block, g, full);
             tma_load_2d_pair(to + kA + 8192, &tmap_w, k * kFp8Block, a.N + g, full);
           } else {
-#pragma unroll
-            for (int h = 0; h < NT / 128; ++h)
-              tma_load_2d_pair(to + kA + h * 8192, &tmap_w, k * kFp8Block, n * NT + int(crank) * (NT / 2) + h * 64, full);
+            tma_load_2d_pair(to + kA, &tmap_w, k * kFp8Block, n * 256 + int(crank) * 128, full);
           }
-          if (++s == kStages) { s = 0; ph ^= 1; }
+          if (++s == kPairStages) { s = 0; ph ^= 1; }
         }
       }
     } else if (warp == 1 && crank == 0) {
-      constexpr uint32_t idesc = make_idesc_f16(256, NT);      // (format 0 of kind::f8f6f4 is e4m3)
+      constexpr uint32_t idesc = make_idesc_f16(256, 256);      // (format 0 of kind::f8f6f4 is e4m3)
       const uint64_t desc = make_desc_sw128(smem_u32(ring));
       int s = 0, c = 0;
       uint32_t ph = 0;
@@ -387,20 +379,19 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
       for (int i = pair; i < n_units && live; i += workers) {
         for (int k = 0; k < n_kb; ++k, ++c) {
           const int buf = c & 1;
-          bool ok = c < 2 || mbar_wait_cluster(&bars->acc_empty[buf], ((c >> 1) & 1) ^ 1, abort_flag, a.status, 91, c);
-          ok = ok && mbar_wait_cluster(&bars->full[s], ph, abort_flag, a.status, 92, c);
+          bool ok = mbar_wait_cluster(&bars->full[s], ph, abort_flag, a.status, 92, c);
+          ok = ok && (c < 2 || mbar_wait_cluster(&bars->acc_empty[buf], ((c >> 1) & 1) ^ 1, abort_flag, a.status, 91, c));
           live = __all_sync(0xffffffffu, ok);
           if (!live) break;
           tc_fence_after_sync();
-          const uint64_t da = desc + uint64_t((s * kStage) >> 4), db = da + (kA >> 4);
+          const uint64_t da = desc + uint64_t((s * kPairStage) >> 4), db = da + (kA >> 4);
           if (elect_one()) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) umma_fp8_pair(tmem + buf * NT, da + j * 2, db + j * 2, idesc, j != 0);
-            tc_commit_pair(&bars->empty[s]);
-            tc_commit_pair(&bars->acc_full[buf]);
+            for (int j = 0; j < 4; ++j) umma_fp8_pair(tmem + buf * 256, da + j * 2, db + j * 2, idesc, j != 0);
+            tc_commit_pair(&bars->done[s]);
           }
           __syncwarp();
-          if (++s == kStages) { s = 0; ph ^= 1; }
+          if (++s == kPairStages) { s = 0; ph ^= 1; }
         }
       }
     }
@@ -411,13 +402,14 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
     const uint32_t empty_bar = map_to_rank(smem_u32(&bars->acc_empty[0]), 0);
     const int nbs = (a.N + kFp8Block - 1) / kFp8Block;
     bool live = true;
-    int c = 0, unit = 0;
+    int c = 0, unit = 0, es = 0;
+    uint32_t eph = 0;
     pdl_wait();
     for (int i = pair; i < n_units; i += workers, ++unit) {
       int n, m;
       units.at(i, &n, &m);
       const int t = m * 256 + int(crank) * 128 + row;
-      const int nb = GLU ? n : (n * NT + half * C) / kFp8Block;
+      const int nb = GLU ? n : (n * 256 + half * C) / kFp8Block;
       const float* sw = a.sw + size_t(min(nb, nbs - 1)) * n_kb;
       const float* sw_up = GLU ? sw + size_t(nbs) * n_kb : sw;
       const float* sx = a.sx + min(t, a.M - 1);
@@ -433,18 +425,18 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
           if (GLU) w_up = sw_up[k + 1];
         }
         const int buf = c & 1;
-        live = live && __all_sync(0xffffffffu, mbar_wait(&bars->acc_full[buf], (c >> 1) & 1, abort_flag, a.status, 93, c));
-        if (!live) break;
+        live = live && __all_sync(0xffffffffu, mbar_wait(&bars->done[es], eph, abort_flag, a.status, 93, c));
         tc_fence_after_sync();
-        add_block<C, GLU ? C / 2 : C>(acc, taddr + buf * NT, f, f_up);
+        add_block<C, GLU ? C / 2 : C>(acc, taddr + buf * 256, f, f_up);
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(empty_bar + buf * 8);
+        if (++es == kPairStages) { es = 0; eph ^= 1; }
       }
       if constexpr (GLU) {
         put_gated(a, acc, t, n * 128 + half * 64, half, bars->top[unit & 1], row, 1 + q, 64, live);
-      } else if (live && t < a.M && n * NT + half * C < a.N) {
-        put_row<C>(a, acc, t, n * NT + half * C);
+      } else if (live && t < a.M && n * 256 + half * C < a.N) {
+        put_row<C>(a, acc, t, n * 256 + half * C);
       }
     }
   }
@@ -458,7 +450,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
   __syncthreads();
   pair_cluster_sync();                                         // nobody leaves while the other CTA may still signal it
   if (warp == 1)
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * NT) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // e4m3 rows [rows, K], ld bytes apart: box = 128 columns x box_rows rows, 128-byte swizzle, zeros out of bounds
@@ -490,20 +482,20 @@ int launch(const ZseGemmFp8& g, const Fp8Args& a, cudaStream_t st) {
   return launch_pdl(kern, dim3((g.N + cols - 1) / cols, (g.M + 127) / 128), dim3(kThreads), smem, st, tx, tw, a) == cudaSuccess ? 1 : ZSE_ERR_LAUNCH;
 }
 
-template <int NT, bool GLU>
+template <bool GLU>
 int launch_pair(const ZseGemmFp8& g, const Fp8Args& a, cudaStream_t st) {
   CUtensorMap tx, tw;
   if (int rc = make_map(g.x, g.M, g.K, g.ldx, 128, &tx)) return rc;
-  if (int rc = make_map(g.w, GLU ? 2ull * g.N : g.N, g.K, g.ldw, 64, &tw)) return rc;
-  constexpr int smem = kPairStages<NT> * kPairStage<NT> + int(sizeof(Fp8PairBars)) + 1024;
-  auto kern = gemm_fp8_pair_kernel<NT, GLU>;
+  if (int rc = make_map(g.w, GLU ? 2ull * g.N : g.N, g.K, g.ldw, GLU ? 64 : 128, &tw)) return rc;
+  constexpr int smem = kPairStages * kPairStage + int(sizeof(Fp8PairBars)) + 1024;
+  auto kern = gemm_fp8_pair_kernel<GLU>;
   static bool attr_done[kMaxDevices] = {};
   const int dev = current_device_slot();
   if (!attr_done[dev]) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return ZSE_ERR_LAUNCH;
     attr_done[dev] = true;
   }
-  const int cols = GLU ? NT / 2 : NT, m_tiles = (g.M + 255) / 256, n_tiles = (g.N + cols - 1) / cols, groups = (m_tiles + 7) / 8;
+  const int cols = GLU ? 128 : 256, m_tiles = (g.M + 255) / 256, n_tiles = (g.N + cols - 1) / cols, groups = (m_tiles + 7) / 8;
   const Fp8Units u{n_tiles, m_tiles, (m_tiles + groups - 1) / groups};        // about 2048 tokens at a time
   const int pairs = std::min<long long>(sm_count() / 2, (long long)n_tiles * m_tiles);
   return launch_pdl(kern, dim3(2 * pairs), dim3(kPairThreads), smem, st, tx, tw, a, u) == cudaSuccess ? 1 : ZSE_ERR_LAUNCH;
@@ -528,6 +520,6 @@ extern "C" int zse_gemm_fp8(const ZseGemmFp8* g) {
   const Fp8Args a{static_cast<const float*>(g->sx), static_cast<const float*>(g->sw), g->bias, g->out, static_cast<float*>(g->out_scale),
                   g->ldo, g->ld_sx, g->ld_os, g->M, g->N, g->K, g->type, g->bias_type, g->act, static_cast<Status*>(g->status)};
   const cudaStream_t st = static_cast<cudaStream_t>(g->stream);
-  if (g->M > 256) return glu ? launch_pair<256, true>(*g, a, st) : launch_pair<256, false>(*g, a, st);
+  if (g->M > 256) return glu ? launch_pair<true>(*g, a, st) : launch_pair<false>(*g, a, st);
   return glu ? launch<256, true>(*g, a, st) : launch<128, false>(*g, a, st);
 }
