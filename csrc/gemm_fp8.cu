@@ -17,17 +17,6 @@ namespace zse {
 
 namespace {
 
-constexpr int kThreads = 320;                    // warp 0 loads, warp 1 issues the products, warps 2 .. 9 add them up
-constexpr int kStageMax = 8;
-
-struct Fp8Bars {
-  uint64_t full[kStageMax], empty[kStageMax];
-  uint64_t acc_full[2], acc_empty[2];
-  uint32_t tmem_base;
-  int abort_flag;
-  float top[2][128];                             // largest of a row's 64 outputs, for the warps that have the other 64
-};
-
 struct Fp8Args {
   const float *sx, *sw;
   const void* bias;
@@ -148,39 +137,84 @@ __device__ __forceinline__ void add_block(float* acc, uint32_t taddr, float s, f
   }
 }
 
-// A CTA has 128 tokens and NT weight rows (GLU: NT / 2 gate rows and their up rows, in runs of 64 that alternate).
+// ---- few tokens: weight rows on the lanes --------------------------------------------------------------------------------------------
+// The product the other way around: 128 weight rows on the TMEM lanes, NT tokens as columns, so that a thread adds NT / 2 numbers a block
+// whatever the rows are, and the weights, whose bytes are the time of such a pass, stream past once.  A step is two tiles of 128 x 128 weights:
+// two blocks of K of the same rows, or (GLU) gate and up rows of one block.  Where there are fewer tiles of rows than SMs, the CTAs of a
+// cluster have a part of K each and add their sums through distributed shared memory: CTA r finishes the tokens r, r + ks, ... in rank order.
 template <int NT, bool GLU>
-__global__ void __launch_bounds__(kThreads, 1)
-gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Fp8Args a) {
-  constexpr int kA = 128 * 128, kB = NT * 128, kStages = NT == 256 ? 4 : 6;
-  constexpr int C = NT / 2;                                    // columns of a thread
+struct Few {
+  static constexpr int kX = NT * 128, kW = 128 * 128;
+  static constexpr int kStage = 2 * kW + (GLU ? 1 : 2) * kX;
+  static constexpr int kRed = (NT + 8) * 512 * (GLU ? 2 : 1);  // sums of the other CTAs for this one's tokens
+  static constexpr int kRoom = 232448 - 1024 - 4608 - kRed;
+  static constexpr int kStages = kRoom / kStage < 6 ? kRoom / kStage : 6;
+  static constexpr int kBufs = kStages >= 4 ? 4 : 2;           // accumulators of two tiles
+  static constexpr int kSmem = kStages * kStage + kRed + 4608 + 1024;
+  static_assert(kStages >= kBufs && 2 * NT * kBufs <= 512, "a stage's barrier stands for its accumulator too");
+};
+
+struct FewBars {
+  uint64_t full[6], done[6], sc_full[6], sc_empty[6], acc_empty[4];
+  uint32_t tmem_base;
+  int abort_flag;
+  float sw[6][2];
+  float sx[6][2][64];
+  float top[4][64];
+};
+static_assert(sizeof(FewBars) <= 4608, "barriers and scales fit their place");
+
+__device__ __forceinline__ void tmem_ld8(uint32_t* r, uint32_t taddr) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+// four bytes of global memory to shared memory, and an arrival at `bar` when this thread's copies so far are there
+__device__ __forceinline__ void copy4(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+struct FewUnits {
+  int n_tiles, m_tiles, ks;                      // units: tiles of 128 rows x tiles of NT tokens; CTAs of a unit (= cluster size)
+};
+
+template <int NT, bool GLU>
+__global__ void __launch_bounds__(384, 1)
+gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Fp8Args a, const FewUnits u) {
+  using F = Few<NT, GLU>;
+  constexpr int J = GLU ? 2 : 1, H = NT / 2;                   // sums of a thread: J x H
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Fp8Bars* bars = reinterpret_cast<Fp8Bars*>(ring + kStages * (kA + kB));
+  float* red = reinterpret_cast<float*>(ring + F::kStages * F::kStage);
+  FewBars* bars = reinterpret_cast<FewBars*>(ring + F::kStages * F::kStage + F::kRed);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t0 = blockIdx.y * 128, n_kb = (a.K + kFp8Block - 1) / kFp8Block;
-  const int n0 = blockIdx.x * (GLU ? NT / 2 : NT);             // first output column
-  const int quarters = min(4, (a.M - t0 + 31) / 32);           // warps of TMEM lanes that have a row
+  const int rank = int(blockIdx.x) % u.ks, first = int(blockIdx.x) / u.ks, stride = int(gridDim.x) / u.ks, n_units = u.n_tiles * u.m_tiles;
+  const int n_kb = (a.K + kFp8Block - 1) / kFp8Block, steps = GLU ? n_kb : (n_kb + 1) / 2;
+  const int s0 = int((long long)steps * rank / u.ks), s1 = int((long long)steps * (rank + 1) / u.ks);
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < F::kStages; ++i) {
       mbar_init(&bars->full[i], 1);
-      mbar_init(&bars->empty[i], 1);
+      mbar_init(&bars->done[i], 1);
+      mbar_init(&bars->sc_full[i], 32);
+      mbar_init(&bars->sc_empty[i], 8);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars->acc_full[i], 1);
-      mbar_init(&bars->acc_empty[i], 2 * quarters);
-    }
+    for (int i = 0; i < F::kBufs; ++i) mbar_init(&bars->acc_empty[i], 8);
     bars->abort_flag = 0;
     mbar_fence_init();
     prefetch_tmap(&tmap_x);
     prefetch_tmap(&tmap_w);
   }
   if (warp == 1) {
-    tmem_alloc(&bars->tmem_base, 2 * NT);
+    tmem_alloc(&bars->tmem_base, 2 * NT * F::kBufs);
     tmem_relinquish();
   }
   tc_fence_before_sync();
   __syncthreads();
+  if (u.ks > 1) pair_cluster_sync();                           // every CTA of the cluster runs before anybody writes to it
   tc_fence_after_sync();
   const uint32_t tmem = bars->tmem_base;
   volatile int* abort_flag = &bars->abort_flag;
@@ -188,72 +222,220 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
 
   if (warp == 0) {
     if (lane == 0) {
+      // weights are constant: the first stages are under way before the kernel before this one is done
+      auto load_w = [&](int s, int unit, int st) {
+        mbar_arrive_expect_tx(&bars->full[s], F::kStage);
+        uint8_t* to = ring + s * F::kStage;
+        const int n0 = unit / u.m_tiles * 128;
+        tma_load_2d(to, &tmap_w, (GLU ? st : 2 * st) * kFp8Block, n0, &bars->full[s]);
+        tma_load_2d(to + F::kW, &tmap_w, (GLU ? st : 2 * st + 1) * kFp8Block, GLU ? a.N + n0 : n0, &bars->full[s]);
+      };
+      auto load_x = [&](int s, int unit, int st) {
+        uint8_t* to = ring + s * F::kStage + 2 * F::kW;
+        const int t0 = unit % u.m_tiles * NT;
+        tma_load_2d(to, &tmap_x, (GLU ? st : 2 * st) * kFp8Block, t0, &bars->full[s]);
+        if (!GLU) tma_load_2d(to + F::kX, &tmap_x, (2 * st + 1) * kFp8Block, t0, &bars->full[s]);
+      };
+      const int ahead = min(F::kStages, s1 - s0);
+      for (int i = 0; i < ahead; ++i) load_w(i, first, s0 + i);
       pdl_wait();
-      for (int k = 0; k < n_kb; ++k) {
-        const int s = k % kStages;
-        if (k >= kStages && !mbar_wait(&bars->empty[s], ((k / kStages) & 1) ^ 1, abort_flag, a.status, 80, k)) break;
-        mbar_arrive_expect_tx(&bars->full[s], kA + kB);
-        uint8_t* to = ring + s * (kA + kB);
-        tma_load_2d(to, &tmap_x, k * kFp8Block, t0, &bars->full[s]);
-        if constexpr (GLU) {
-#pragma unroll
-          for (int h = 0; h < NT / 128; ++h) {
-            tma_load_2d(to + kA + h * 16384, &tmap_w, k * kFp8Block, n0 + h * 64, &bars->full[s]);
-            tma_load_2d(to + kA + h * 16384 + 8192, &tmap_w, k * kFp8Block, a.N + n0 + h * 64, &bars->full[s]);
+      int s = 0, c = 0;
+      uint32_t ph = 1;
+      bool live = true;
+      for (int i = first; i < n_units && live; i += stride) {
+        for (int st = s0; st < s1; ++st, ++c) {
+          if (c >= F::kStages && !mbar_wait(&bars->done[s], ph, abort_flag, a.status, 80, c)) {
+            live = false;
+            break;
           }
-        } else {
-#pragma unroll
-          for (int h = 0; h < NT / 64; ++h) tma_load_2d(to + kA + h * 8192, &tmap_w, k * kFp8Block, n0 + h * 64, &bars->full[s]);
+          if (c >= ahead) load_w(s, i, st);
+          load_x(s, i, st);
+          if (++s == F::kStages) { s = 0; ph ^= 1; }
         }
       }
     }
   } else if (warp == 1) {
     constexpr uint32_t idesc = make_idesc_f16(128, NT);        // (format 0 of kind::f8f6f4 is e4m3)
     const uint64_t desc = make_desc_sw128(smem_u32(ring));
-    for (int k = 0; k < n_kb; ++k) {
-      const int s = k % kStages, buf = k & 1;
-      bool ok = k < 2 || mbar_wait_spin(&bars->acc_empty[buf], ((k >> 1) & 1) ^ 1, abort_flag, a.status, 81, k);
-      ok = ok && mbar_wait_spin(&bars->full[s], (k / kStages) & 1, abort_flag, a.status, 82, k);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after_sync();
-      const uint64_t da = desc + uint64_t((s * (kA + kB)) >> 4), db = da + (kA >> 4);
-      if (elect_one()) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) umma_fp8(tmem + buf * NT, da + j * 2, db + j * 2, idesc, j != 0);
-        tc_commit(&bars->empty[s]);
-        tc_commit(&bars->acc_full[buf]);
-      }
-      __syncwarp();
-    }
-  } else {
-    const int q = warp & 3, half = (warp - 2) >> 2, row = q * 32 + lane, t = t0 + row;
-    if (q < quarters) {
-      const uint32_t taddr = tmem + (uint32_t(q * 32) << 16) + half * C;
-      pdl_wait();
-      // the scales of this thread's columns: all of one block of weight rows, or (GLU) of a gate and an up block
-      const int nb = (n0 + (GLU ? 0 : half * C)) / kFp8Block, nbs = (a.N + kFp8Block - 1) / kFp8Block;
-      const float* sw = a.sw + size_t(min(nb, nbs - 1)) * n_kb;
-      const float* sw_up = sw + size_t(nbs) * n_kb;
-      const float* sx = a.sx + min(t, a.M - 1);
-      float acc[C];
-#pragma unroll
-      for (int i = 0; i < C; ++i) acc[i] = 0.f;
-      bool live = true;
-      for (int k = 0; k < n_kb && live; ++k) {
-        const float x = sx[size_t(k) * a.ld_sx], s = x * sw[k], s_up = GLU ? x * sw_up[k] : s;
-        const int buf = k & 1;
-        live = __all_sync(0xffffffffu, mbar_wait(&bars->acc_full[buf], (k >> 1) & 1, abort_flag, a.status, 83, k));
+    int s = 0, c = 0;
+    uint32_t ph = 0;
+    bool live = true;
+    for (int i = first; i < n_units && live; i += stride) {
+      for (int st = s0; st < s1; ++st, ++c) {
+        const int buf = c % F::kBufs;
+        bool ok = mbar_wait_spin(&bars->full[s], ph, abort_flag, a.status, 82, c);
+        ok = ok && (c < F::kBufs || mbar_wait_spin(&bars->acc_empty[buf], ((c / F::kBufs) & 1) ^ 1, abort_flag, a.status, 81, c));
+        live = __all_sync(0xffffffffu, ok);
         if (!live) break;
         tc_fence_after_sync();
-        add_block<C, GLU ? C / 2 : C>(acc, taddr + buf * NT, s, s_up);
+        const uint64_t dw = desc + uint64_t((s * F::kStage) >> 4), dx = dw + (2 * F::kW >> 4);
+        if (elect_one()) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_fp8(tmem + (buf * 2 + j) * NT, dw + ((j * F::kW) >> 4) + k * 2, dx + ((GLU ? 0 : j * F::kX) >> 4) + k * 2, idesc, k != 0);
+          tc_commit(&bars->done[s]);
+        }
+        __syncwarp();
+        if (++s == F::kStages) { s = 0; ph ^= 1; }
+      }
+    }
+  } else if (warp == 2) {
+    const int nbs = (a.N + kFp8Block - 1) / kFp8Block;
+    int s = 0, c = 0;
+    uint32_t ph = 1;
+    bool live = true;
+    pdl_wait();
+    for (int i = first; i < n_units && live; i += stride) {
+      const int nb = i / u.m_tiles, t0 = i % u.m_tiles * NT;
+      for (int st = s0; st < s1; ++st, ++c) {
+        live = c < F::kStages || __all_sync(0xffffffffu, mbar_wait(&bars->sc_empty[s], ph, abort_flag, a.status, 84, c));
+        if (!live) break;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int k = GLU ? st : 2 * st + j;
+          if (k < n_kb) {
+            if (!GLU || j == 0)
+#pragma unroll
+              for (int l = 0; l < NT; l += 32)
+                if (l + lane < NT) copy4(&bars->sx[s][j][l + lane], a.sx + size_t(k) * a.ld_sx + min(t0 + l + lane, a.M - 1));
+            if (lane == 0) copy4(&bars->sw[s][j], a.sw + size_t(nb + (GLU ? j * nbs : 0)) * n_kb + k);
+          }
+        }
+        copies_arrive(&bars->sc_full[s]);
+        if (++s == F::kStages) { s = 0; ph ^= 1; }
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+
+  const int q = warp & 3, half = (warp - 4) >> 2, row = q * 32 + lane;
+  // one output; `c`: the token's place in bars->top
+  auto put_one = [&](float y, float b, int n, int t) {
+    if (a.bias != nullptr) y += b;
+    const size_t at = size_t(t) * a.ldo + n;
+    if (a.type == kFp8F32) static_cast<float*>(a.out)[at] = y;
+    else if (a.type == kFp8BF16) static_cast<bf16*>(a.out)[at] = __float2bfloat16_rn(y);
+    else static_cast<__half*>(a.out)[at] = __float2half_rn(hold_f16(y));
+  };
+  auto put_byte = [&](float y, int c, int n, int t) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = max(top, __float_as_uint(bars->top[w][c]));
+    y = __fmul_rn(y, fp8_steps(__uint_as_float(top)));
+    if (n < a.N) static_cast<uint8_t*>(a.out)[t * a.ldo + n] = __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+    if (row == 0) a.out_scale[(n / kFp8Block) * a.ld_os + t] = fp8_scale(__uint_as_float(top));
+  };
+  bool live = true;
+  if (warp >= 4) {
+    const uint32_t taddr = tmem + (uint32_t(q * 32) << 16) + half * H;
+    int s = 0, c = 0;
+    uint32_t ph = 0;
+    pdl_wait();
+    for (int i = first; i < n_units; i += stride) {
+      float acc[J * H];
+#pragma unroll
+      for (int j = 0; j < J * H; ++j) acc[j] = 0.f;
+      for (int st = s0; st < s1; ++st, ++c) {
+        const int buf = c % F::kBufs;
+        live = live && __all_sync(0xffffffffu, mbar_wait(&bars->sc_full[s], ph, abort_flag, a.status, 85, c) &&
+                                                   mbar_wait(&bars->done[s], ph, abort_flag, a.status, 83, c));
+        tc_fence_after_sync();
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (GLU || j == 0 || 2 * st + 1 < n_kb) {            // (uniform)
+            const float w = bars->sw[s][j];
+            const float* x = &bars->sx[s][GLU ? 0 : j][half * H];
+            float* sum = acc + (GLU ? j * H : 0);
+            constexpr int B = H < 16 ? 8 : 16;
+            uint32_t r[H / B][B];
+#pragma unroll
+            for (int l = 0; l < H; l += B) {
+              if constexpr (B == 8) tmem_ld8(r[l / B], taddr + (buf * 2 + j) * NT + l);
+              else ZSE_TMEM_LD_X16(r[l / B], taddr + (buf * 2 + j) * NT + l);
+            }
+            tc_wait_ld();
+#pragma unroll
+            for (int l = 0; l < H; ++l) {
+              asm volatile("" : "+r"(r[l / B][l % B]));        // behind the wait
+              sum[l] = fmaf(__uint_as_float(r[l / B][l % B]), x[l] * w, sum[l]);
+            }
+          }
+        }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->acc_empty[buf]);
+        if (lane == 0) {
+          mbar_arrive(&bars->acc_empty[buf]);
+          mbar_arrive(&bars->sc_empty[s]);
+        }
+        if (++s == F::kStages) { s = 0; ph ^= 1; }
       }
+      if (u.ks == 1) {
+        const int n = i / u.m_tiles * 128 + row, t0 = i % u.m_tiles * NT + half * H;
+        if constexpr (GLU) {
+#pragma unroll
+          for (int l = 0; l < H; ++l) {
+            acc[l] = n < a.N ? gated(a.act, acc[l], acc[H + l]) : 0.f;
+            const uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(acc[l]));
+            if (lane == 0) bars->top[q][half * H + l] = __uint_as_float(top);
+          }
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+#pragma unroll
+          for (int l = 0; l < H; ++l)
+            if (live && t0 + l < a.M) put_byte(acc[l], half * H + l, n, t0 + l);
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");    // before the next unit's
+        } else if (live && n < a.N) {
+          const float b = a.bias != nullptr ? bias_of(a, n) : 0.f;
+#pragma unroll
+          for (int l = 0; l < H; ++l)
+            if (t0 + l < a.M) put_one(acc[l], b, n, t0 + l);
+        }
+      } else {
+        // tokens owner * share .. of this thread's row go to the CTA `owner`
+        const int share = (NT + u.ks - 1) / u.ks, there = min(NT, a.M - i % u.m_tiles * NT);
+        const uint32_t mine = smem_u32(red + (rank * J * share) * 128 + row);
+        int owner = half * H / share, slot = half * H - owner * share;
+        uint32_t to = map_to_rank(mine, owner) + slot * 512;
+#pragma unroll
+        for (int l = 0; l < H; ++l) {
+          if (half * H + l < there) {
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+              asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + j * share * 512), "f"(acc[j * H + l]) : "memory");
+            to += 512;
+            if (++slot == share) slot = 0, to = map_to_rank(mine, ++owner < u.ks ? owner : 0);
+          }
+        }
+      }
+    }
+  }
+  if (u.ks > 1) {                                              // one unit a cluster
+    __syncwarp();
+    pair_cluster_sync();
+    if (warp >= 4) {
+      const int share = (NT + u.ks - 1) / u.ks, n = first / u.m_tiles * 128 + row, t0 = first % u.m_tiles * NT + rank * share;
+      const int mine = min(min(share, NT - rank * share), a.M - t0);          // tokens; the two halves of the warps take turns
+      auto sum_of = [&](int j, int slot) {
+        const float* from = red + (j * share + slot) * 128 + row;
+        float sum = 0.f;
+#pragma unroll 4
+        for (int r = 0; r < u.ks; ++r) sum += from[r * J * share * 128];
+        return sum;
+      };
       if constexpr (GLU) {
-        put_gated(a, acc, t, n0 + half * 64, half, bars->top, row, 1, 64 * quarters, live);
-      } else if (live && t < a.M && n0 + half * C < a.N) {
-        put_row<C>(a, acc, t, n0 + half * C);
+        for (int i = half; i < mine; i += 2) {
+          const float y = n < a.N ? gated(a.act, sum_of(0, i), sum_of(1, i)) : 0.f;
+          red[i * 128 + row] = y;                              // (where this thread read its own part of the first sum)
+          const uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(y));
+          if (lane == 0) bars->top[q][i] = __uint_as_float(top);
+        }
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+        for (int i = half; live && i < mine; i += 2) put_byte(red[i * 128 + row], i, n, t0 + i);
+      } else if (live && n < a.N) {
+        const float b = a.bias != nullptr ? bias_of(a, n) : 0.f;
+#pragma unroll 4
+        for (int i = half; i < mine; i += 2) put_one(sum_of(0, i), b, n, t0 + i);
       }
     }
   }
@@ -265,7 +447,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   }
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, 2 * NT);
+  if (warp == 1) tmem_dealloc(tmem, 2 * NT * F::kBufs);
 }
 
 // ---- many tokens: pairs of CTAs, persistent ------------------------------------------------------------------------------------------
@@ -465,21 +647,61 @@ int make_map(const void* p, uint64_t rows, uint64_t K, uint64_t ld, uint32_t box
              : ZSE_ERR_DRIVER;
 }
 
+// CTAs of a unit: as many as leave every one an SM of its own and a step of K.  0: a cluster of that size does not fit the GPU so often.
 template <int NT, bool GLU>
-int launch(const ZseGemmFp8& g, const Fp8Args& a, cudaStream_t st) {
+int few_splits(int units, int steps) {
+  static int fit[kMaxDevices][9];                              // clusters of a size that run at a time, + 1
+  const int dev = current_device_slot();
+  for (int ks = std::min(std::min(8, steps), sm_count() / std::max(units, 1)); ks > 1; --ks) {
+    int& n = fit[dev][ks];
+    if (n == 0) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(ks);
+      cfg.blockDim = dim3(384);
+      cfg.dynamicSmemBytes = Few<NT, GLU>::kSmem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = ks, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr, cfg.numAttrs = 1;
+      int got = 0;
+      if (cudaOccupancyMaxActiveClusters(&got, gemm_fp8_few_kernel<NT, GLU>, &cfg) != cudaSuccess) got = 0;
+      n = got + 1;
+    }
+    if (units <= n - 1) return ks;
+  }
+  return 1;
+}
+
+template <int NT, bool GLU>
+int launch_few(const ZseGemmFp8& g, const Fp8Args& a, cudaStream_t st) {
+  using F = Few<NT, GLU>;
   CUtensorMap tx, tw;
-  if (int rc = make_map(g.x, g.M, g.K, g.ldx, 128, &tx)) return rc;
-  if (int rc = make_map(g.w, GLU ? 2ull * g.N : g.N, g.K, g.ldw, 64, &tw)) return rc;
-  constexpr int smem = (NT == 256 ? 4 : 6) * (128 + NT) * 128 + int(sizeof(Fp8Bars)) + 1024;
-  auto kern = gemm_fp8_kernel<NT, GLU>;
+  if (int rc = make_map(g.x, g.M, g.K, g.ldx, NT, &tx)) return rc;
+  if (int rc = make_map(g.w, GLU ? 2ull * g.N : g.N, g.K, g.ldw, 128, &tw)) return rc;
+  auto kern = gemm_fp8_few_kernel<NT, GLU>;
   static bool attr_done[kMaxDevices] = {};
   const int dev = current_device_slot();
   if (!attr_done[dev]) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return ZSE_ERR_LAUNCH;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem) != cudaSuccess) return ZSE_ERR_LAUNCH;
     attr_done[dev] = true;
   }
-  const int cols = GLU ? NT / 2 : NT;
-  return launch_pdl(kern, dim3((g.N + cols - 1) / cols, (g.M + 127) / 128), dim3(kThreads), smem, st, tx, tw, a) == cudaSuccess ? 1 : ZSE_ERR_LAUNCH;
+  const int n_kb = (g.K + kFp8Block - 1) / kFp8Block;
+  FewUnits u{(g.N + 127) / 128, (g.M + NT - 1) / NT, 1};
+  const int units = u.n_tiles * u.m_tiles;
+  u.ks = few_splits<NT, GLU>(units, GLU ? n_kb : (n_kb + 1) / 2);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(u.ks > 1 ? units * u.ks : std::min(units, sm_count()));
+  cfg.blockDim = dim3(384);
+  cfg.dynamicSmemBytes = F::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = u.ks, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, tx, tw, a, u) == cudaSuccess ? 1 : ZSE_ERR_LAUNCH;
 }
 
 template <bool GLU>
@@ -520,6 +742,8 @@ extern "C" int zse_gemm_fp8(const ZseGemmFp8* g) {
   const Fp8Args a{static_cast<const float*>(g->sx), static_cast<const float*>(g->sw), g->bias, g->out, static_cast<float*>(g->out_scale),
                   g->ldo, g->ld_sx, g->ld_os, g->M, g->N, g->K, g->type, g->bias_type, g->act, static_cast<Status*>(g->status)};
   const cudaStream_t st = static_cast<cudaStream_t>(g->stream);
-  if (g->M > 256) return glu ? launch_pair<true>(*g, a, st) : launch_pair<false>(*g, a, st);
-  return glu ? launch<256, true>(*g, a, st) : launch<128, false>(*g, a, st);
+  if (g->M > 128) return glu ? launch_pair<true>(*g, a, st) : launch_pair<false>(*g, a, st);
+  if (g->M > 32) return glu ? launch_few<64, true>(*g, a, st) : launch_few<64, false>(*g, a, st);
+  if (g->M > 16) return glu ? launch_few<32, true>(*g, a, st) : launch_few<32, false>(*g, a, st);
+  return glu ? launch_few<16, true>(*g, a, st) : launch_few<16, false>(*g, a, st);
 }
