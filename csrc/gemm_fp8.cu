@@ -146,12 +146,12 @@ template <int NT, bool GLU>
 struct Few {
   static constexpr int kX = NT * 128, kW = 128 * 128;
   static constexpr int kStage = 2 * kW + (GLU ? 1 : 2) * kX;
-  static constexpr int kRed = (NT + 8) * 512 * (GLU ? 2 : 1);  // sums of the other CTAs for this one's tokens
-  static constexpr int kRoom = 232448 - 1024 - 4608 - kRed;
-  static constexpr int kStages = kRoom / kStage < 6 ? kRoom / kStage : 6;
-  static constexpr int kBufs = kStages >= 4 ? 4 : 2;           // accumulators of two tiles
-  static constexpr int kSmem = kStages * kStage + kRed + 4608 + 1024;
+  static constexpr int kBars = 8704;
+  static constexpr int kRoom = (232448 - 1024 - kBars) / kStage, kStages = kRoom < 6 ? kRoom : 6;
+  static constexpr int kBufs = NT <= 64 && kStages >= 4 ? 4 : 2;           // accumulators of two tiles
+  static constexpr int kSmem = kStages * kStage + kBars + 1024;
   static_assert(kStages >= kBufs && 2 * NT * kBufs <= 512, "a stage's barrier stands for its accumulator too");
+  static_assert((NT + 8) * 512 * (GLU ? 2 : 1) <= kStages * kStage, "the ring has room for the other CTAs' sums");
 };
 
 struct FewBars {
@@ -159,10 +159,10 @@ struct FewBars {
   uint32_t tmem_base;
   int abort_flag;
   float sw[6][2];
-  float sx[6][2][64];
-  float top[4][64];
+  alignas(16) float sx[6][2][128];
+  float top[4][128];
 };
-static_assert(sizeof(FewBars) <= 4608, "barriers and scales fit their place");
+static_assert(sizeof(FewBars) <= 8704, "barriers and scales fit their place");
 
 __device__ __forceinline__ void tmem_ld8(uint32_t* r, uint32_t taddr) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -189,8 +189,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
   constexpr int J = GLU ? 2 : 1, H = NT / 2;                   // sums of a thread: J x H
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* red = reinterpret_cast<float*>(ring + F::kStages * F::kStage);
-  FewBars* bars = reinterpret_cast<FewBars*>(ring + F::kStages * F::kStage + F::kRed);
+  float* red = reinterpret_cast<float*>(ring);                 // once all products of the cluster are done
+  FewBars* bars = reinterpret_cast<FewBars*>(ring + F::kStages * F::kStage);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = int(blockIdx.x) % u.ks, first = int(blockIdx.x) / u.ks, stride = int(gridDim.x) / u.ks, n_units = u.n_tiles * u.m_tiles;
   const int n_kb = (a.K + kFp8Block - 1) / kFp8Block, steps = GLU ? n_kb : (n_kb + 1) / 2;
@@ -342,24 +342,32 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
         live = live && __all_sync(0xffffffffu, mbar_wait(&bars->sc_full[s], ph, abort_flag, a.status, 85, c) &&
                                                    mbar_wait(&bars->done[s], ph, abort_flag, a.status, 83, c));
         tc_fence_after_sync();
+        constexpr int B = H < 16 ? 8 : 16, R = H < 32 ? H : 32;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           if (GLU || j == 0 || 2 * st + 1 < n_kb) {            // (uniform)
             const float w = bars->sw[s][j];
-            const float* x = &bars->sx[s][GLU ? 0 : j][half * H];
             float* sum = acc + (GLU ? j * H : 0);
-            constexpr int B = H < 16 ? 8 : 16;
-            uint32_t r[H / B][B];
 #pragma unroll
-            for (int l = 0; l < H; l += B) {
-              if constexpr (B == 8) tmem_ld8(r[l / B], taddr + (buf * 2 + j) * NT + l);
-              else ZSE_TMEM_LD_X16(r[l / B], taddr + (buf * 2 + j) * NT + l);
-            }
-            tc_wait_ld();
+            for (int l0 = 0; l0 < H; l0 += R) {
+              uint32_t r[R / B][B];
 #pragma unroll
-            for (int l = 0; l < H; ++l) {
-              asm volatile("" : "+r"(r[l / B][l % B]));        // behind the wait
-              sum[l] = fmaf(__uint_as_float(r[l / B][l % B]), x[l] * w, sum[l]);
+              for (int l = 0; l < R; l += B) {
+                if constexpr (B == 8) tmem_ld8(r[l / B], taddr + (buf * 2 + j) * NT + l0 + l);
+                else ZSE_TMEM_LD_X16(r[l / B], taddr + (buf * 2 + j) * NT + l0 + l);
+              }
+              float f[R];
+#pragma unroll
+              for (int l = 0; l < R; l += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(&bars->sx[s][GLU ? 0 : j][half * H + l0 + l]);
+                f[l] = x.x * w, f[l + 1] = x.y * w, f[l + 2] = x.z * w, f[l + 3] = x.w * w;
+              }
+              tc_wait_ld();
+#pragma unroll
+              for (int l = 0; l < R; ++l) {
+                asm volatile("" : "+r"(r[l / B][l % B]));      // behind the wait
+                sum[l0 + l] = fmaf(__uint_as_float(r[l / B][l % B]), f[l], sum[l0 + l]);
+              }
             }
           }
         }
@@ -392,6 +400,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
             if (t0 + l < a.M) put_one(acc[l], b, n, t0 + l);
         }
       } else {
+        pair_cluster_sync();                                   // nothing is read from or loaded into a ring of the cluster any more
         // tokens owner * share .. of this thread's row go to the CTA `owner`
         const int share = (NT + u.ks - 1) / u.ks, there = min(NT, a.M - i % u.m_tiles * NT);
         const uint32_t mine = smem_u32(red + (rank * J * share) * 128 + row);
@@ -412,6 +421,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
   }
   if (u.ks > 1) {                                              // one unit a cluster
     __syncwarp();
+    if (warp < 4) pair_cluster_sync();
     pair_cluster_sync();
     if (warp >= 4) {
       const int share = (NT + u.ks - 1) / u.ks, n = first / u.m_tiles * 128 + row, t0 = first % u.m_tiles * NT + rank * share;
@@ -451,8 +461,9 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
 }
 
 // ---- many tokens: pairs of CTAs, persistent ------------------------------------------------------------------------------------------
-// 256 tokens and NT weight rows a pair (cta_group::2): a CTA has 128 of the tokens, loads those and half of the weight rows, and owns the
-// sums of its tokens.
+// 256 tokens and 256 weight rows a pair (cta_group::2): a CTA has 128 of the tokens, loads those and half of the weight rows, and owns the
+// sums of its tokens.  Units that do not fill a round of all pairs take a launch of their own with KS pairs a unit, clusters of 2 KS: each pair
+// has a part of K, and the sums of 128 / KS rows go to each of the CTAs that have the same tokens.
 constexpr int kPairThreads = 384;                // warp 0 loads, warp 1 issues the products, warps 4 .. 11 add them up
 // Registers: 168 a thread at launch (64512), then 56 for the first four warps and 216 for the other eight (62464): 128 sums and two reads of 16
 // columns do not fit 168.
@@ -468,7 +479,7 @@ struct Fp8PairBars {
 
 // Units (256 tokens x a tile of weight rows) in an order that keeps m_group token tiles in L2 while the weights stream past them once.
 struct Fp8Units {
-  int n_tiles, m_tiles, m_group;
+  int n_tiles, m_tiles, m_group, first, end;     // units first .. end - 1 belong to this launch
   __device__ __forceinline__ void at(int i, int* n, int* m) const {
     const int g = i / (n_tiles * m_group), r = i - g * n_tiles * m_group, gm = min(m_group, m_tiles - g * m_group);
     *n = r / gm;
@@ -484,8 +495,13 @@ __device__ __forceinline__ void umma_fp8_pair(uint32_t d_tmem, uint64_t a_desc, 
       : "memory");
 }
 
-template <bool GLU>
-__global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
+__device__ __forceinline__ void commit_to(uint64_t* bar, uint16_t ctas) {    // arrives at this offset in the CTAs of the cluster
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"(ctas)
+               : "memory");
+}
+
+template <bool GLU, int KS>
+__global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2 * KS, 1, 1)
 gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Fp8Args a,
                      const Fp8Units units) {
   constexpr int kA = 128 * 128, C = 128;                       // C: columns of a thread
@@ -493,10 +509,13 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Fp8PairBars* bars = reinterpret_cast<Fp8PairBars*>(ring + kPairStages * kPairStage);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint32_t crank;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(crank));
-  const int pair = blockIdx.x >> 1, workers = gridDim.x >> 1, n_units = units.n_tiles * units.m_tiles;
-  const int n_kb = (a.K + kFp8Block - 1) / kFp8Block;
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const uint32_t crank = rank & 1, leader = KS > 1 ? rank & ~1u : 0;       // of the pair
+  const int part = KS > 1 ? int(rank >> 1) : 0;
+  const int pair = units.first + int(blockIdx.x) / (2 * KS), workers = int(gridDim.x) / (2 * KS), n_units = units.end;
+  const int all_kb = (a.K + kFp8Block - 1) / kFp8Block;
+  const int kb0 = KS > 1 ? all_kb * part / KS : 0, n_kb = KS > 1 ? all_kb * (part + 1) / KS - kb0 : all_kb;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kPairStages; ++i) {
       mbar_init(&bars->full[i], 1);
@@ -538,16 +557,16 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
             live = false;
             break;
           }
-          const uint32_t full = map_to_rank(smem_u32(&bars->full[s]), 0);
+          const uint32_t full = map_to_rank(smem_u32(&bars->full[s]), leader);
           if (crank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * kPairStage);
           const uint32_t to = smem_u32(ring) + s * kPairStage;
-          tma_load_2d_pair(to, &tmap_x, k * kFp8Block, t0, full);
+          tma_load_2d_pair(to, &tmap_x, (kb0 + k) * kFp8Block, t0, full);
           if constexpr (GLU) {                                 // columns 0 .. 127 of the product: 64 gate rows and their up rows; the rest: the next
             const int g = n * 128 + int(crank) * 64;
-            tma_load_2d_pair(to + kA, &tmap_w, k * kFp8Block, g, full);
-            tma_load_2d_pair(to + kA + 8192, &tmap_w, k * kFp8Block, a.N + g, full);
+            tma_load_2d_pair(to + kA, &tmap_w, (kb0 + k) * kFp8Block, g, full);
+            tma_load_2d_pair(to + kA + 8192, &tmap_w, (kb0 + k) * kFp8Block, a.N + g, full);
           } else {
-            tma_load_2d_pair(to + kA, &tmap_w, k * kFp8Block, n * 256 + int(crank) * 128, full);
+            tma_load_2d_pair(to + kA, &tmap_w, (kb0 + k) * kFp8Block, n * 256 + int(crank) * 128, full);
           }
           if (++s == kPairStages) { s = 0; ph ^= 1; }
         }
@@ -570,18 +589,23 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
           if (elect_one()) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) umma_fp8_pair(tmem + buf * 256, da + j * 2, db + j * 2, idesc, j != 0);
-            tc_commit_pair(&bars->done[s]);
+            commit_to(&bars->done[s], uint16_t(3u << leader));
           }
           __syncwarp();
           if (++s == kPairStages) { s = 0; ph ^= 1; }
         }
       }
     }
+    if constexpr (KS > 1) {                                    // (the sums' two)
+      __syncwarp();
+      pair_cluster_sync();
+      pair_cluster_sync();
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int q = warp & 3, half = (warp - 4) >> 2, row = q * 32 + lane;
     const uint32_t taddr = tmem + (uint32_t(q * 32) << 16) + half * C;
-    const uint32_t empty_bar = map_to_rank(smem_u32(&bars->acc_empty[0]), 0);
+    const uint32_t empty_bar = map_to_rank(smem_u32(&bars->acc_empty[0]), leader);
     const int nbs = (a.N + kFp8Block - 1) / kFp8Block;
     bool live = true;
     int c = 0, unit = 0, es = 0;
@@ -592,20 +616,19 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
       units.at(i, &n, &m);
       const int t = m * 256 + int(crank) * 128 + row;
       const int nb = GLU ? n : (n * 256 + half * C) / kFp8Block;
-      const float* sw = a.sw + size_t(min(nb, nbs - 1)) * n_kb;
-      const float* sw_up = GLU ? sw + size_t(nbs) * n_kb : sw;
-      const float* sx = a.sx + min(t, a.M - 1);
+      const float* sw = a.sw + size_t(min(nb, nbs - 1)) * all_kb + kb0;
+      const float* sw_up = GLU ? sw + size_t(nbs) * all_kb : sw;
+      const float* sx = a.sx + size_t(kb0) * a.ld_sx + min(t, a.M - 1);
       float acc[C];
 #pragma unroll
       for (int j = 0; j < C; ++j) acc[j] = 0.f;
-      float x = sx[0], w = sw[0], w_up = sw_up[0];             // scales of a block are loaded while the one before is added
-      for (int k = 0; k < n_kb; ++k, ++c) {
-        const float f = x * w, f_up = GLU ? x * w_up : f;
-        if (k + 1 < n_kb) {
-          x = sx[size_t(k + 1) * a.ld_sx];
-          w = sw[k + 1];
-          if (GLU) w_up = sw_up[k + 1];
-        }
+      // One block.  Its rows' scale is in x, where that of the next but one is loaded when it has been used: it comes from the L2, which can take
+      // longer than a block.  (Two blocks a turn of the loop, so that no register with a load under way is copied; from shared memory, which the
+      // products keep busy, the scales took longer: 567 us instead of 536 for 8192 x 5120 x 13824, 595 with loads one block ahead.)
+      float w32 = 0.f, u32 = 0.f;                              // weight scales of 32 blocks, one a lane
+      auto block = [&](int k, float& x) {
+        const float f = x * __shfl_sync(0xffffffffu, w32, k & 31), f_up = GLU ? x * __shfl_sync(0xffffffffu, u32, k & 31) : f;
+        x = sx[size_t(min(k + 2, n_kb - 1)) * a.ld_sx];
         const int buf = c & 1;
         live = live && __all_sync(0xffffffffu, mbar_wait(&bars->done[es], eph, abort_flag, a.status, 93, c));
         tc_fence_after_sync();
@@ -614,6 +637,45 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(empty_bar + buf * 8);
         if (++es == kPairStages) { es = 0; eph ^= 1; }
+        ++c;
+      };
+      float x0 = sx[0], x1 = sx[size_t(min(1, n_kb - 1)) * a.ld_sx];
+      for (int k0 = 0; k0 < n_kb; k0 += 32) {                  // (no way out of these loops but their end: with one, the sums were moved about)
+        const int end = min(k0 + 32, n_kb);
+        w32 = sw[min(k0 + lane, n_kb - 1)];
+        if (GLU) u32 = sw_up[min(k0 + lane, n_kb - 1)];
+        int k = k0;
+        for (; k + 1 < end; k += 2) {
+          block(k, x0);
+          block(k + 1, x1);
+        }
+        if (k < end) block(k, x0);
+      }
+      if constexpr (KS > 1) {
+        // 32 rows of a quarter go to the CTA `owner` of those with the same tokens, from the others in the order of their parts
+        constexpr int kQuarters = 4 / KS;                      // of a CTA
+        const int owner = q / kQuarters;
+        auto place = [&](int src) { return smem_u32(ring) + ((src * kQuarters + q % kQuarters) * 2 + half) * 16384 + lane * 16; };
+        pair_cluster_sync();                                   // nothing is read from or loaded into a ring of the cluster any more
+        if (owner != part) {
+          const uint32_t to = map_to_rank(place(part < owner ? part : part - 1), uint32_t(owner) * 2 + crank);
+#pragma unroll
+          for (int j = 0; j < C; j += 4)
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + j * 128), "f"(acc[j]), "f"(acc[j + 1]), "f"(acc[j + 2]),
+                         "f"(acc[j + 3])
+                         : "memory");
+        }
+        pair_cluster_sync();
+        if (owner != part) continue;
+#pragma unroll
+        for (int src = 0; src < KS - 1; ++src) {
+#pragma unroll
+          for (int j = 0; j < C; j += 4) {
+            float4 v;
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(place(src) + j * 128));
+            acc[j] += v.x, acc[j + 1] += v.y, acc[j + 2] += v.z, acc[j + 3] += v.w;
+          }
+        }
       }
       if constexpr (GLU) {
         put_gated(a, acc, t, n * 128 + half * 64, half, bars->top[unit & 1], row, 1 + q, 64, live);
@@ -647,80 +709,151 @@ int make_map(const void* p, uint64_t rows, uint64_t K, uint64_t ld, uint32_t box
              : ZSE_ERR_DRIVER;
 }
 
-// CTAs of a unit: as many as leave every one an SM of its own and a step of K.  0: a cluster of that size does not fit the GPU so often.
+// Clusters of `ctas` CTAs of a kernel that run on the GPU at a time.
+template <typename Kernel>
+int clusters_at_a_time(Kernel kern, int ctas, int smem) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(384);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = 1;
+  int got = 0;
+  return cudaOccupancyMaxActiveClusters(&got, kern, &cfg) == cudaSuccess ? got : 0;
+}
+
+constexpr int kPairSmem = kPairStages * kPairStage + int(sizeof(Fp8PairBars)) + 1024;
+
+template <bool GLU, int KS>
+int pair_fit() {                                               // units of this form that run at a time
+  static int fit[kMaxDevices];                                 // + 1
+  int& n = fit[current_device_slot()];
+  if (n == 0) {
+    auto kern = gemm_fp8_pair_kernel<GLU, KS>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem) != cudaSuccess) return 0;
+    n = 1 + (KS == 1 ? sm_count() / 2 : clusters_at_a_time(kern, 2 * KS, kPairSmem));
+  }
+  return n - 1;
+}
+
+template <bool GLU, int KS>
+int launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Args& a, Fp8Units u, int first, int end, cudaStream_t st) {
+  if (first == end) return 0;
+  const int fit = pair_fit<GLU, KS>();
+  if (fit == 0) return ZSE_ERR_LAUNCH;
+  u.first = first, u.end = end;
+  const int clusters = KS == 1 ? std::min(fit, end - first) : end - first;
+  return launch_pdl(gemm_fp8_pair_kernel<GLU, KS>, dim3(2 * KS * clusters), dim3(kPairThreads), kPairSmem, st, tx, tw, a, u) == cudaSuccess
+             ? 1
+             : ZSE_ERR_LAUNCH;
+}
+
+// ---- which kernel ------------------------------------------------------------------------------------------------------------------------
+// Times in microseconds, from layers of 1 to 4096 tokens (those of gate and up weights in brackets).  A pair of CTAs takes 0.46 (0.62) a block of K
+// whatever part of its 256 tokens there is; a step of the kernel for few tokens 0.6 with 16 token columns, 0.65 with 32, 0.78 (0.87) with 64 and 1.25
+// (1.9) with 128, but not less than its weights take from memory.  A launch costs 3, sums over a cluster 4.
+struct Fp8Plan {
+  int nt;                                                      // token columns of the kernel for few tokens; 0: pairs
+  int ks;                                                      // pairs: parts of K of the units behind the last whole round
+  float us;
+};
+template <bool GLU>
+Fp8Plan plan_pairs(int units, int n_kb) {
+  const float kb = GLU ? 0.62f : 0.46f;
+  const int at_once = std::max(1, pair_fit<GLU, 1>()), rest = units % at_once;
+  Fp8Plan p{0, 1, 3 + kb * n_kb * ((units + at_once - 1) / at_once)};
+  if (rest == 0) return p;
+  auto with = [&](int ks, int fit) {
+    const float us = 3 + kb * n_kb * (units / at_once) + (units > rest ? 3 : 0) + 4 + kb * ((n_kb + ks - 1) / ks);
+    if (rest <= fit && n_kb >= 4 * ks && us < p.us) p.ks = ks, p.us = us;
+  };
+  with(2, pair_fit<GLU, 2>());
+  with(4, pair_fit<GLU, 4>());
+  return p;
+}
+
+template <int NT, bool GLU>
+int few_ready() {                                              // 0, or an error
+  static bool done[kMaxDevices];
+  bool& d = done[current_device_slot()];
+  if (!d && cudaFuncSetAttribute(gemm_fp8_few_kernel<NT, GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<NT, GLU>::kSmem) != cudaSuccess)
+    return ZSE_ERR_LAUNCH;
+  d = true;
+  return 0;
+}
+// CTAs of a unit: as many as leave every one an SM of its own and a step of K.
 template <int NT, bool GLU>
 int few_splits(int units, int steps) {
   static int fit[kMaxDevices][9];                              // clusters of a size that run at a time, + 1
-  const int dev = current_device_slot();
+  if (few_ready<NT, GLU>()) return 1;
   for (int ks = std::min(std::min(8, steps), sm_count() / std::max(units, 1)); ks > 1; --ks) {
-    int& n = fit[dev][ks];
-    if (n == 0) {
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(ks);
-      cfg.blockDim = dim3(384);
-      cfg.dynamicSmemBytes = Few<NT, GLU>::kSmem;
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = ks, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
-      cfg.attrs = attr, cfg.numAttrs = 1;
-      int got = 0;
-      if (cudaOccupancyMaxActiveClusters(&got, gemm_fp8_few_kernel<NT, GLU>, &cfg) != cudaSuccess) got = 0;
-      n = got + 1;
-    }
+    int& n = fit[current_device_slot()][ks];
+    if (n == 0) n = 1 + clusters_at_a_time(gemm_fp8_few_kernel<NT, GLU>, ks, Few<NT, GLU>::kSmem);
     if (units <= n - 1) return ks;
   }
   return 1;
 }
+template <int NT, bool GLU>
+void plan_few(int M, int N, int n_kb, Fp8Plan* best) {
+  if (M > 4 * NT) return;
+  const int units = (N + 127) / 128 * ((M + NT - 1) / NT), steps = GLU ? n_kb : (n_kb + 1) / 2, ks = few_splits<NT, GLU>(units, steps);
+  const float step = NT == 16 ? 0.6f : NT == 32 ? 0.65f : NT == 64 ? (GLU ? 0.87f : 0.78f) : (GLU ? 1.9f : 1.25f);
+  const float us = 3 + (ks > 1 ? 4 : 0) + std::max(step * ((steps + ks - 1) / ks) * ((units + sm_count() - 1) / sm_count()), 2.f * N * n_kb * (GLU ? 1 : 0.5f) * 128 / 6e6f);
+  if (us < best->us) *best = Fp8Plan{NT, ks, us};
+}
 
 template <int NT, bool GLU>
-int launch_few(const ZseGemmFp8& g, const Fp8Args& a, cudaStream_t st) {
+int launch_few(const ZseGemmFp8& g, const Fp8Args& a, int ks, cudaStream_t st) {
   using F = Few<NT, GLU>;
+  if (int rc = few_ready<NT, GLU>()) return rc;
   CUtensorMap tx, tw;
   if (int rc = make_map(g.x, g.M, g.K, g.ldx, NT, &tx)) return rc;
   if (int rc = make_map(g.w, GLU ? 2ull * g.N : g.N, g.K, g.ldw, 128, &tw)) return rc;
-  auto kern = gemm_fp8_few_kernel<NT, GLU>;
-  static bool attr_done[kMaxDevices] = {};
-  const int dev = current_device_slot();
-  if (!attr_done[dev]) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem) != cudaSuccess) return ZSE_ERR_LAUNCH;
-    attr_done[dev] = true;
-  }
-  const int n_kb = (g.K + kFp8Block - 1) / kFp8Block;
-  FewUnits u{(g.N + 127) / 128, (g.M + NT - 1) / NT, 1};
+  const FewUnits u{(g.N + 127) / 128, (g.M + NT - 1) / NT, ks};
   const int units = u.n_tiles * u.m_tiles;
-  u.ks = few_splits<NT, GLU>(units, GLU ? n_kb : (n_kb + 1) / 2);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(u.ks > 1 ? units * u.ks : std::min(units, sm_count()));
+  cfg.gridDim = dim3(ks > 1 ? units * ks : std::min(units, sm_count()));
   cfg.blockDim = dim3(384);
   cfg.dynamicSmemBytes = F::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = u.ks, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[0].val.clusterDim.x = ks, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kern, tx, tw, a, u) == cudaSuccess ? 1 : ZSE_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, gemm_fp8_few_kernel<NT, GLU>, tx, tw, a, u) == cudaSuccess ? 1 : ZSE_ERR_LAUNCH;
 }
 
 template <bool GLU>
-int launch_pair(const ZseGemmFp8& g, const Fp8Args& a, cudaStream_t st) {
+int run(const ZseGemmFp8& g, const Fp8Args& a, cudaStream_t st) {
+  const int cols = GLU ? 128 : 256, m_tiles = (g.M + 255) / 256, n_tiles = (g.N + cols - 1) / cols, groups = (m_tiles + 7) / 8;
+  const int n_kb = (g.K + kFp8Block - 1) / kFp8Block;
+  if ((long long)m_tiles * n_tiles > 0x3fffffff) return ZSE_ERR_LIMIT;
+  const int units = m_tiles * n_tiles;
+  Fp8Plan p = plan_pairs<GLU>(units, n_kb);
+  plan_few<16, GLU>(g.M, g.N, n_kb, &p);
+  plan_few<32, GLU>(g.M, g.N, n_kb, &p);
+  plan_few<64, GLU>(g.M, g.N, n_kb, &p);
+  plan_few<128, GLU>(g.M, g.N, n_kb, &p);
+  switch (p.nt) {
+    case 16: return launch_few<16, GLU>(g, a, p.ks, st);
+    case 32: return launch_few<32, GLU>(g, a, p.ks, st);
+    case 64: return launch_few<64, GLU>(g, a, p.ks, st);
+    case 128: return launch_few<128, GLU>(g, a, p.ks, st);
+  }
   CUtensorMap tx, tw;
   if (int rc = make_map(g.x, g.M, g.K, g.ldx, 128, &tx)) return rc;
   if (int rc = make_map(g.w, GLU ? 2ull * g.N : g.N, g.K, g.ldw, GLU ? 64 : 128, &tw)) return rc;
-  constexpr int smem = kPairStages * kPairStage + int(sizeof(Fp8PairBars)) + 1024;
-  auto kern = gemm_fp8_pair_kernel<GLU>;
-  static bool attr_done[kMaxDevices] = {};
-  const int dev = current_device_slot();
-  if (!attr_done[dev]) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return ZSE_ERR_LAUNCH;
-    attr_done[dev] = true;
-  }
-  const int cols = GLU ? 128 : 256, m_tiles = (g.M + 255) / 256, n_tiles = (g.N + cols - 1) / cols, groups = (m_tiles + 7) / 8;
-  const Fp8Units u{n_tiles, m_tiles, (m_tiles + groups - 1) / groups};        // about 2048 tokens at a time
-  const int pairs = std::min<long long>(sm_count() / 2, (long long)n_tiles * m_tiles);
-  return launch_pdl(kern, dim3(2 * pairs), dim3(kPairThreads), smem, st, tx, tw, a, u) == cudaSuccess ? 1 : ZSE_ERR_LAUNCH;
+  const Fp8Units u{n_tiles, m_tiles, (m_tiles + groups - 1) / groups, 0, 0};     // about 2048 tokens at a time
+  const int whole = p.ks > 1 ? units - units % pair_fit<GLU, 1>() : units;
+  const int first = launch_pair<GLU, 1>(tx, tw, a, u, 0, whole, st);
+  if (first < 0) return first;
+  const int rest = p.ks == 4 ? launch_pair<GLU, 4>(tx, tw, a, u, whole, units, st) : launch_pair<GLU, 2>(tx, tw, a, u, whole, units, st);
+  return rest < 0 ? rest : first + rest;
 }
 
 }  // namespace
@@ -742,8 +875,5 @@ extern "C" int zse_gemm_fp8(const ZseGemmFp8* g) {
   const Fp8Args a{static_cast<const float*>(g->sx), static_cast<const float*>(g->sw), g->bias, g->out, static_cast<float*>(g->out_scale),
                   g->ldo, g->ld_sx, g->ld_os, g->M, g->N, g->K, g->type, g->bias_type, g->act, static_cast<Status*>(g->status)};
   const cudaStream_t st = static_cast<cudaStream_t>(g->stream);
-  if (g->M > 128) return glu ? launch_pair<true>(*g, a, st) : launch_pair<false>(*g, a, st);
-  if (g->M > 32) return glu ? launch_few<64, true>(*g, a, st) : launch_few<64, false>(*g, a, st);
-  if (g->M > 16) return glu ? launch_few<32, true>(*g, a, st) : launch_few<32, false>(*g, a, st);
-  return glu ? launch_few<16, true>(*g, a, st) : launch_few<16, false>(*g, a, st);
+  return glu ? run<true>(*g, a, st) : run<false>(*g, a, st);
 }
