@@ -44,8 +44,8 @@ __device__ __forceinline__ float4 load4<bf16>(const bf16* p) {
   return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
 }
 
-template <typename T, int J>
-__global__ void __launch_bounds__(1024)
+template <typename T, int J, int THREADS>
+__global__ void __launch_bounds__(THREADS)
 add_rmsnorm_fp8_kernel(const NormFp8 a) {
   __shared__ double red[32];
   pdl_launch_dependents();
@@ -124,16 +124,14 @@ add_rmsnorm_fp8_kernel(const NormFp8 a) {
 // 16 threads have a block, eight columns each.
 template <typename T>
 struct Eight {
-  float v[8];
-  __device__ __forceinline__ explicit Eight(const T* p) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = load4(p), b = load4(p + 4);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-      const uint4 q = *reinterpret_cast<const uint4*>(p);
-      const float4 a = load4(reinterpret_cast<const T*>(&q)), b = load4(reinterpret_cast<const T*>(&q) + 4);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    }
+  uint4 raw[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < int(sizeof(T) / 2); ++i) raw[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void values(float* v) const {
+    const float4 a = load4(reinterpret_cast<const T*>(raw)), b = load4(reinterpret_cast<const T*>(raw) + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
   }
 };
 
@@ -141,53 +139,73 @@ template <typename T, int ACT>
 __global__ void __launch_bounds__(256)
 quant_fp8_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ data, long long ld_data, float* __restrict__ scale,
                  long long ld_scale, int M, int C) {
+  constexpr int kRows = 2;                                     // read before the first of them is worked on
   pdl_launch_dependents();
   pdl_wait();
-  const int blocks = (C + kFp8Block - 1) / kFp8Block, t = threadIdx.x & 15;
-  const long long total = (long long)M * blocks;
-  for (long long i = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); i - (threadIdx.x >> 4) % 2 < total; i += (long long)gridDim.x * 16) {
-    const int row = int(i / blocks), b = int(i - (long long)row * blocks), c = b * kFp8Block + t * 8;
-    const bool live = i < total && c < C;
-    float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (live) {
-      const Eight<T> g(x + row * ldx + c);
-      if constexpr (ACT == kFp8None) {
+  const int t = threadIdx.x & 15, b = blockIdx.x * 16 + (threadIdx.x >> 4), c = b * kFp8Block + t * 8;
+  const bool inside = c < C;
+  for (int row0 = blockIdx.y * kRows; row0 < M; row0 += gridDim.y * kRows) {
+    Eight<T> g[kRows], u[kRows];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) y[k] = g.v[k];
-      } else {
-        const Eight<T> u(x + row * ldx + C + c);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) y[k] = fp8_gated<ACT>(g.v[k], u.v[k]);
+    for (int r = 0; r < kRows; ++r) {
+      if (inside && row0 + r < M) {
+        g[r].load(x + (row0 + r) * ldx + c);
+        if (ACT != kFp8None) u[r].load(x + (row0 + r) * ldx + C + c);
       }
     }
-    uint32_t top = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) top = max(top, abs_bits(y[k]));
+    for (int r = 0; r < kRows; ++r) {
+      const long long row = row0 + r;
+      const bool live = inside && row < M;
+      float y[8], v[8];
+      g[r].values(y);
+      if constexpr (ACT != kFp8None) {
+        u[r].values(v);
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float steps = fp8_steps(__uint_as_float(top));
-    if (live) *reinterpret_cast<uint2*>(data + row * ld_data + c) = make_uint2(fp8_pack4(y, steps), fp8_pack4(y + 4, steps));
-    if (live && t == 0) scale[b * ld_scale + row] = fp8_scale(__uint_as_float(top));
+        for (int k = 0; k < 8; ++k) y[k] = fp8_gated<ACT>(y[k], v[k]);
+      }
+      uint32_t top = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = max(top, abs_bits(y[k]));
+      if (!live) top = 0;
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float steps = fp8_steps(__uint_as_float(top));
+      if (live) *reinterpret_cast<uint2*>(data + row * ld_data + c) = make_uint2(fp8_pack4(y, steps), fp8_pack4(y + 4, steps));
+      if (live && t == 0) scale[b * ld_scale + row] = fp8_scale(__uint_as_float(top));
+    }
   }
 }
 
 template <typename T>
 int norm_fp8(const NormFp8& a, cudaStream_t st) {
-  const int blocks = (a.H + kFp8Block - 1) / kFp8Block;
-  const int J = (blocks + 31) / 32, threads = 32 * ((blocks + J - 1) / J);
-  auto go = [&](auto kernel) { return launch_pdl(kernel, dim3(a.M), dim3(threads), 0, st, a) == cudaSuccess ? 1 : ZSE_ERR_LAUNCH; };
-  if (J == 1) return go(add_rmsnorm_fp8_kernel<T, 1>);
-  if (J == 2) return go(add_rmsnorm_fp8_kernel<T, 2>);
-  if (J <= 4) return go(add_rmsnorm_fp8_kernel<T, 4>);
-  return go(add_rmsnorm_fp8_kernel<T, 8>);
+  const int blocks = (a.H + kFp8Block - 1) / kFp8Block, least = (blocks + 31) / 32;
+  auto go = [&](auto kernel, int J) {
+    return launch_pdl(kernel, dim3(a.M), dim3(32 * ((blocks + J - 1) / J)), 0, st, a) == cudaSuccess ? 1 : ZSE_ERR_LAUNCH;
+  };
+  // many rows: eight warps a row, so that several rows are under way on an SM; few: as soon as possible done with each
+  if (a.M >= 4 * sm_count() && blocks <= 64) {
+    const int J = (blocks + 7) / 8;
+    if (J == 1) return go(add_rmsnorm_fp8_kernel<T, 1, 256>, 1);
+    if (J == 2) return go(add_rmsnorm_fp8_kernel<T, 2, 256>, 2);
+    if (J == 3) return go(add_rmsnorm_fp8_kernel<T, 3, 256>, 3);
+    if (J == 4) return go(add_rmsnorm_fp8_kernel<T, 4, 256>, 4);
+    if (J == 5) return go(add_rmsnorm_fp8_kernel<T, 5, 256>, 5);
+    return go(add_rmsnorm_fp8_kernel<T, 8, 256>, 8);
+  }
+  if (least == 1) return go(add_rmsnorm_fp8_kernel<T, 1, 1024>, 1);
+  if (least == 2) return go(add_rmsnorm_fp8_kernel<T, 2, 1024>, 2);
+  if (least <= 4) return go(add_rmsnorm_fp8_kernel<T, 4, 1024>, 4);
+  return go(add_rmsnorm_fp8_kernel<T, 8, 1024>, 8);
 }
 
 template <typename T>
 int quant_fp8(const ZseQuantFp8& q, cudaStream_t st) {
-  const long long groups = ((long long)q.M * ((q.C + kFp8Block - 1) / kFp8Block) + 15) / 16;
-  const int grid = int(std::min(groups, 8ll * sm_count()));
+  const int across = ((q.C + kFp8Block - 1) / kFp8Block + 15) / 16, room = std::max(1, 8 * sm_count() / across);
+  if (across > 0x7fffffff / 2) return ZSE_ERR_LIMIT;
+  const dim3 grid(across, std::min(std::min((q.M + 1) / 2, room), 65535));
   auto go = [&](auto kernel) {
-    return launch_pdl(kernel, dim3(grid), dim3(256), 0, st, static_cast<const T*>(q.x), q.ldx, static_cast<uint8_t*>(q.data), q.ld_data,
+    return launch_pdl(kernel, grid, dim3(256), 0, st, static_cast<const T*>(q.x), q.ldx, static_cast<uint8_t*>(q.data), q.ld_data,
                       static_cast<float*>(q.scale), q.ld_scale, q.M, q.C) == cudaSuccess
                ? 1
                : ZSE_ERR_LAUNCH;

@@ -49,42 +49,53 @@ __device__ __forceinline__ void store32(void* p, const uint32_t* v) {
                "r"(v[6]), "r"(v[7])
                : "memory");
 }
-// The row's columns n .. n + C - 1 to memory, rounded to the output's type: 32 bytes, a sector, at a time where the row lies so.
-template <int C>
-__device__ __forceinline__ void put_row(const Fp8Args& a, float* y, int t, int n) {
-  if (a.bias != nullptr) {
+// y[0 .. 15] += the bias of columns n .. n + 15
+__device__ __forceinline__ void add_bias(const Fp8Args& a, float* y, int n) {
+  if (a.bias == nullptr) return;
 #pragma unroll
-    for (int i = 0; i < C; ++i)
-      if (n + i < a.N) y[i] += bias_of(a, n + i);
-  }
-  const size_t at = size_t(t) * a.ldo + n;
-  const bool whole = n + C <= a.N;
-  if (a.type == kFp8F32) {
-    float* o = static_cast<float*>(a.out) + at;
-    if (whole && (reinterpret_cast<uintptr_t>(o) & 31) == 0) {
+  for (int j = 0; j < 16; ++j)
+    if (n + j < a.N) y[j] += bias_of(a, n + j);
+}
+__device__ __forceinline__ void put_one(const Fp8Args& a, float y, size_t at) {
+  if (a.type == kFp8F32) static_cast<float*>(a.out)[at] = y;
+  else if (a.type == kFp8BF16) static_cast<bf16*>(a.out)[at] = __float2bfloat16_rn(y);
+  else static_cast<__half*>(a.out)[at] = __float2half_rn(hold_f16(y));
+}
+// Columns n .. n + C - 1 of a warp's 32 rows t - lane .. to memory, rounded to the output's type.  WIDE: the output, its rows and N are multiples of
+// 32 bytes, a sector, which are written at a time; else sixteen columns of two rows at a time, by way of `stage`.  The whole warp calls it.
+template <int C, bool WIDE>
+__device__ __forceinline__ void put_rows(const Fp8Args& a, float* y, int t, int n, float (*stage)[17]) {
+  if constexpr (WIDE) {
+    const int item = a.type == kFp8F32 ? 4 : 2;
+    uint8_t* o = static_cast<uint8_t*>(a.out) + (size_t(min(t, a.M - 1)) * a.ldo + n) * item;
 #pragma unroll
-      for (int i = 0; i < C; i += 8) store32(o + i, reinterpret_cast<const uint32_t*>(y + i));
-    } else {
+    for (int i = 0; i < C; i += 16) {
+      if (n + i < a.N && t < a.M) {
+        add_bias(a, y + i, n + i);
+        if (a.type == kFp8F32) {
+          store32(o + i * 4, reinterpret_cast<const uint32_t*>(y + i));
+          if (n + i + 8 < a.N) store32(o + i * 4 + 32, reinterpret_cast<const uint32_t*>(y + i + 8));
+        } else {
+          uint32_t v[8];
 #pragma unroll
-      for (int i = 0; i < C; ++i)
-        if (n + i < a.N) o[i] = y[i];
+          for (int j = 0; j < 8; ++j)
+            v[j] = a.type == kFp8BF16 ? pack2<bf16>(y[i + 2 * j], y[i + 2 * j + 1]) : pack2<__half>(y[i + 2 * j], y[i + 2 * j + 1]);
+          store32(o + i * 2, v);
+        }
+      }
     }
-    return;
-  }
-  uint16_t* o = static_cast<uint16_t*>(a.out) + at;
-  const bool wide = whole && (reinterpret_cast<uintptr_t>(o) & 31) == 0;
+  } else {
+    const int lane = threadIdx.x & 31, t0 = t - lane;
 #pragma unroll
-  for (int i = 0; i < C; i += 16) {
-    uint32_t v[8];
+    for (int i = 0; i < C; i += 16) {
+      add_bias(a, y + i, n + i);
+      __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      v[j] = a.type == kFp8BF16 ? pack2<bf16>(y[i + 2 * j], y[i + 2 * j + 1]) : pack2<__half>(y[i + 2 * j], y[i + 2 * j + 1]);
-    if (wide) {
-      store32(o + i, v);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (n + i + j < a.N) o[i + j] = uint16_t(v[j >> 1] >> (16 * (j & 1)));
+      for (int j = 0; j < 16; ++j) stage[lane][j] = y[i + j];
+      __syncwarp();
+      const int col = n + i + (lane & 15);
+      for (int r = lane >> 4; r < 32 && t0 + r < a.M; r += 2)
+        if (col < a.N) put_one(a, stage[r][lane & 15], size_t(t0 + r) * a.ldo + col);
     }
   }
 }
@@ -311,14 +322,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
   }
 
   const int q = warp & 3, half = (warp - 4) >> 2, row = q * 32 + lane;
-  // one output; `c`: the token's place in bars->top
-  auto put_one = [&](float y, float b, int n, int t) {
-    if (a.bias != nullptr) y += b;
-    const size_t at = size_t(t) * a.ldo + n;
-    if (a.type == kFp8F32) static_cast<float*>(a.out)[at] = y;
-    else if (a.type == kFp8BF16) static_cast<bf16*>(a.out)[at] = __float2bfloat16_rn(y);
-    else static_cast<__half*>(a.out)[at] = __float2half_rn(hold_f16(y));
-  };
+  // one output (a byte; `c`: the token's place in bars->top)
+  auto put = [&](float y, float b, int n, int t) { put_one(a, a.bias != nullptr ? y + b : y, size_t(t) * a.ldo + n); };
   auto put_byte = [&](float y, int c, int n, int t) {
     uint32_t top = 0;
 #pragma unroll
@@ -397,7 +402,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
           const float b = a.bias != nullptr ? bias_of(a, n) : 0.f;
 #pragma unroll
           for (int l = 0; l < H; ++l)
-            if (t0 + l < a.M) put_one(acc[l], b, n, t0 + l);
+            if (t0 + l < a.M) put(acc[l], b, n, t0 + l);
         }
       } else {
         pair_cluster_sync();                                   // nothing is read from or loaded into a ring of the cluster any more
@@ -445,7 +450,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
       } else if (live && n < a.N) {
         const float b = a.bias != nullptr ? bias_of(a, n) : 0.f;
 #pragma unroll 4
-        for (int i = half; i < mine; i += 2) put_one(sum_of(0, i), b, n, t0 + i);
+        for (int i = half; i < mine; i += 2) put(sum_of(0, i), b, n, t0 + i);
       }
     }
   }
@@ -474,6 +479,7 @@ struct Fp8PairBars {
   uint64_t acc_empty[2];
   uint32_t tmem_base;
   int abort_flag;
+  float stage[8][32][17];
   float top[2][2][128];                          // two units: a warp may be a unit ahead of the one that has the other 64 outputs
 };
 
@@ -500,7 +506,8 @@ __device__ __forceinline__ void commit_to(uint64_t* bar, uint16_t ctas) {    // 
                : "memory");
 }
 
-template <bool GLU, int KS>
+// WIDE: see put_rows (true for GLU).
+template <bool GLU, int KS, bool WIDE>
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2 * KS, 1, 1)
 gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Fp8Args a,
                      const Fp8Units units) {
@@ -679,8 +686,8 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
       }
       if constexpr (GLU) {
         put_gated(a, acc, t, n * 128 + half * 64, half, bars->top[unit & 1], row, 1 + q, 64, live);
-      } else if (live && t < a.M && n * 256 + half * C < a.N) {
-        put_row<C>(a, acc, t, n * 256 + half * C);
+      } else if (live && n * 256 + half * C < a.N) {
+        put_rows<C, WIDE>(a, acc, t, n * 256 + half * C, bars->stage[WIDE ? 0 : warp - 4]);
       }
     }
   }
@@ -709,6 +716,10 @@ int make_map(const void* p, uint64_t rows, uint64_t K, uint64_t ld, uint32_t box
              : ZSE_ERR_DRIVER;
 }
 
+struct Gpu {
+  int slot, sms;                                               // of the current device
+};
+
 // Clusters of `ctas` CTAs of a kernel that run on the GPU at a time.
 template <typename Kernel>
 int clusters_at_a_time(Kernel kern, int ctas, int smem) {
@@ -726,26 +737,26 @@ int clusters_at_a_time(Kernel kern, int ctas, int smem) {
 
 constexpr int kPairSmem = kPairStages * kPairStage + int(sizeof(Fp8PairBars)) + 1024;
 
-template <bool GLU, int KS>
-int pair_fit() {                                               // units of this form that run at a time
+template <bool GLU, int KS, bool WIDE>
+int pair_fit(const Gpu& gpu) {                                 // units of this form that run at a time
   static int fit[kMaxDevices];                                 // + 1
-  int& n = fit[current_device_slot()];
+  int& n = fit[gpu.slot];
   if (n == 0) {
-    auto kern = gemm_fp8_pair_kernel<GLU, KS>;
+    auto kern = gemm_fp8_pair_kernel<GLU, KS, WIDE>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem) != cudaSuccess) return 0;
-    n = 1 + (KS == 1 ? sm_count() / 2 : clusters_at_a_time(kern, 2 * KS, kPairSmem));
+    n = 1 + (KS == 1 ? gpu.sms / 2 : clusters_at_a_time(kern, 2 * KS, kPairSmem));
   }
   return n - 1;
 }
 
-template <bool GLU, int KS>
-int launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Args& a, Fp8Units u, int first, int end, cudaStream_t st) {
+template <bool GLU, int KS, bool WIDE>
+int launch_pair(const Gpu& gpu, const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Args& a, Fp8Units u, int first, int end, cudaStream_t st) {
   if (first == end) return 0;
-  const int fit = pair_fit<GLU, KS>();
+  const int fit = pair_fit<GLU, KS, WIDE>(gpu);
   if (fit == 0) return ZSE_ERR_LAUNCH;
   u.first = first, u.end = end;
   const int clusters = KS == 1 ? std::min(fit, end - first) : end - first;
-  return launch_pdl(gemm_fp8_pair_kernel<GLU, KS>, dim3(2 * KS * clusters), dim3(kPairThreads), kPairSmem, st, tx, tw, a, u) == cudaSuccess
+  return launch_pdl(gemm_fp8_pair_kernel<GLU, KS, WIDE>, dim3(2 * KS * clusters), dim3(kPairThreads), kPairSmem, st, tx, tw, a, u) == cudaSuccess
              ? 1
              : ZSE_ERR_LAUNCH;
 }
@@ -760,24 +771,24 @@ struct Fp8Plan {
   float us;
 };
 template <bool GLU>
-Fp8Plan plan_pairs(int units, int n_kb) {
+Fp8Plan plan_pairs(const Gpu& gpu, int units, int n_kb) {
   const float kb = GLU ? 0.62f : 0.46f;
-  const int at_once = std::max(1, pair_fit<GLU, 1>()), rest = units % at_once;
+  const int at_once = std::max(1, pair_fit<GLU, 1, true>(gpu)), rest = units % at_once;
   Fp8Plan p{0, 1, 3 + kb * n_kb * ((units + at_once - 1) / at_once)};
   if (rest == 0) return p;
   auto with = [&](int ks, int fit) {
     const float us = 3 + kb * n_kb * (units / at_once) + (units > rest ? 3 : 0) + 4 + kb * ((n_kb + ks - 1) / ks);
     if (rest <= fit && n_kb >= 4 * ks && us < p.us) p.ks = ks, p.us = us;
   };
-  with(2, pair_fit<GLU, 2>());
-  with(4, pair_fit<GLU, 4>());
+  with(2, pair_fit<GLU, 2, true>(gpu));
+  with(4, pair_fit<GLU, 4, true>(gpu));
   return p;
 }
 
 template <int NT, bool GLU>
-int few_ready() {                                              // 0, or an error
+int few_ready(const Gpu& gpu) {                                // 0, or an error
   static bool done[kMaxDevices];
-  bool& d = done[current_device_slot()];
+  bool& d = done[gpu.slot];
   if (!d && cudaFuncSetAttribute(gemm_fp8_few_kernel<NT, GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<NT, GLU>::kSmem) != cudaSuccess)
     return ZSE_ERR_LAUNCH;
   d = true;
@@ -785,36 +796,36 @@ int few_ready() {                                              // 0, or an error
 }
 // CTAs of a unit: as many as leave every one an SM of its own and a step of K.
 template <int NT, bool GLU>
-int few_splits(int units, int steps) {
+int few_splits(const Gpu& gpu, int units, int steps) {
   static int fit[kMaxDevices][9];                              // clusters of a size that run at a time, + 1
-  if (few_ready<NT, GLU>()) return 1;
-  for (int ks = std::min(std::min(8, steps), sm_count() / std::max(units, 1)); ks > 1; --ks) {
-    int& n = fit[current_device_slot()][ks];
+  if (few_ready<NT, GLU>(gpu)) return 1;
+  for (int ks = std::min(std::min(8, steps), gpu.sms / std::max(units, 1)); ks > 1; --ks) {
+    int& n = fit[gpu.slot][ks];
     if (n == 0) n = 1 + clusters_at_a_time(gemm_fp8_few_kernel<NT, GLU>, ks, Few<NT, GLU>::kSmem);
     if (units <= n - 1) return ks;
   }
   return 1;
 }
 template <int NT, bool GLU>
-void plan_few(int M, int N, int n_kb, Fp8Plan* best) {
+void plan_few(const Gpu& gpu, int M, int N, int n_kb, Fp8Plan* best) {
   if (M > 4 * NT) return;
-  const int units = (N + 127) / 128 * ((M + NT - 1) / NT), steps = GLU ? n_kb : (n_kb + 1) / 2, ks = few_splits<NT, GLU>(units, steps);
+  const int units = (N + 127) / 128 * ((M + NT - 1) / NT), steps = GLU ? n_kb : (n_kb + 1) / 2, ks = few_splits<NT, GLU>(gpu, units, steps);
   const float step = NT == 16 ? 0.6f : NT == 32 ? 0.65f : NT == 64 ? (GLU ? 0.87f : 0.78f) : (GLU ? 1.9f : 1.25f);
-  const float us = 3 + (ks > 1 ? 4 : 0) + std::max(step * ((steps + ks - 1) / ks) * ((units + sm_count() - 1) / sm_count()), 2.f * N * n_kb * (GLU ? 1 : 0.5f) * 128 / 6e6f);
+  const float us = 3 + (ks > 1 ? 4 : 0) + std::max(step * ((steps + ks - 1) / ks) * ((units + gpu.sms - 1) / gpu.sms), 2.f * N * n_kb * (GLU ? 1 : 0.5f) * 128 / 6e6f);
   if (us < best->us) *best = Fp8Plan{NT, ks, us};
 }
 
 template <int NT, bool GLU>
-int launch_few(const ZseGemmFp8& g, const Fp8Args& a, int ks, cudaStream_t st) {
+int launch_few(const Gpu& gpu, const ZseGemmFp8& g, const Fp8Args& a, int ks, cudaStream_t st) {
   using F = Few<NT, GLU>;
-  if (int rc = few_ready<NT, GLU>()) return rc;
+  if (int rc = few_ready<NT, GLU>(gpu)) return rc;
   CUtensorMap tx, tw;
   if (int rc = make_map(g.x, g.M, g.K, g.ldx, NT, &tx)) return rc;
   if (int rc = make_map(g.w, GLU ? 2ull * g.N : g.N, g.K, g.ldw, 128, &tw)) return rc;
   const FewUnits u{(g.N + 127) / 128, (g.M + NT - 1) / NT, ks};
   const int units = u.n_tiles * u.m_tiles;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ks > 1 ? units * ks : std::min(units, sm_count()));
+  cfg.gridDim = dim3(ks > 1 ? units * ks : std::min(units, gpu.sms));
   cfg.blockDim = dim3(384);
   cfg.dynamicSmemBytes = F::kSmem;
   cfg.stream = st;
@@ -828,32 +839,41 @@ int launch_few(const ZseGemmFp8& g, const Fp8Args& a, int ks, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, gemm_fp8_few_kernel<NT, GLU>, tx, tw, a, u) == cudaSuccess ? 1 : ZSE_ERR_LAUNCH;
 }
 
+template <bool GLU, bool WIDE>
+int run_pairs(const Gpu& gpu, const ZseGemmFp8& g, const Fp8Args& a, const Fp8Units& u, int units, int ks, cudaStream_t st) {
+  CUtensorMap tx, tw;
+  if (int rc = make_map(g.x, g.M, g.K, g.ldx, 128, &tx)) return rc;
+  if (int rc = make_map(g.w, GLU ? 2ull * g.N : g.N, g.K, g.ldw, GLU ? 64 : 128, &tw)) return rc;
+  const int whole = ks > 1 ? units - units % pair_fit<GLU, 1, WIDE>(gpu) : units;
+  const int first = launch_pair<GLU, 1, WIDE>(gpu, tx, tw, a, u, 0, whole, st);
+  if (first < 0) return first;
+  const int rest = ks == 4 ? launch_pair<GLU, 4, WIDE>(gpu, tx, tw, a, u, whole, units, st) : launch_pair<GLU, 2, WIDE>(gpu, tx, tw, a, u, whole, units, st);
+  return rest < 0 ? rest : first + rest;
+}
+
 template <bool GLU>
 int run(const ZseGemmFp8& g, const Fp8Args& a, cudaStream_t st) {
   const int cols = GLU ? 128 : 256, m_tiles = (g.M + 255) / 256, n_tiles = (g.N + cols - 1) / cols, groups = (m_tiles + 7) / 8;
   const int n_kb = (g.K + kFp8Block - 1) / kFp8Block;
   if ((long long)m_tiles * n_tiles > 0x3fffffff) return ZSE_ERR_LIMIT;
   const int units = m_tiles * n_tiles;
-  Fp8Plan p = plan_pairs<GLU>(units, n_kb);
-  plan_few<16, GLU>(g.M, g.N, n_kb, &p);
-  plan_few<32, GLU>(g.M, g.N, n_kb, &p);
-  plan_few<64, GLU>(g.M, g.N, n_kb, &p);
-  plan_few<128, GLU>(g.M, g.N, n_kb, &p);
+  const Gpu gpu{current_device_slot(), sm_count()};
+  Fp8Plan p = plan_pairs<GLU>(gpu, units, n_kb);
+  plan_few<16, GLU>(gpu, g.M, g.N, n_kb, &p);
+  plan_few<32, GLU>(gpu, g.M, g.N, n_kb, &p);
+  plan_few<64, GLU>(gpu, g.M, g.N, n_kb, &p);
+  plan_few<128, GLU>(gpu, g.M, g.N, n_kb, &p);
   switch (p.nt) {
-    case 16: return launch_few<16, GLU>(g, a, p.ks, st);
-    case 32: return launch_few<32, GLU>(g, a, p.ks, st);
-    case 64: return launch_few<64, GLU>(g, a, p.ks, st);
-    case 128: return launch_few<128, GLU>(g, a, p.ks, st);
+    case 16: return launch_few<16, GLU>(gpu, g, a, p.ks, st);
+    case 32: return launch_few<32, GLU>(gpu, g, a, p.ks, st);
+    case 64: return launch_few<64, GLU>(gpu, g, a, p.ks, st);
+    case 128: return launch_few<128, GLU>(gpu, g, a, p.ks, st);
   }
-  CUtensorMap tx, tw;
-  if (int rc = make_map(g.x, g.M, g.K, g.ldx, 128, &tx)) return rc;
-  if (int rc = make_map(g.w, GLU ? 2ull * g.N : g.N, g.K, g.ldw, GLU ? 64 : 128, &tw)) return rc;
   const Fp8Units u{n_tiles, m_tiles, (m_tiles + groups - 1) / groups, 0, 0};     // about 2048 tokens at a time
-  const int whole = p.ks > 1 ? units - units % pair_fit<GLU, 1>() : units;
-  const int first = launch_pair<GLU, 1>(tx, tw, a, u, 0, whole, st);
-  if (first < 0) return first;
-  const int rest = p.ks == 4 ? launch_pair<GLU, 4>(tx, tw, a, u, whole, units, st) : launch_pair<GLU, 2>(tx, tw, a, u, whole, units, st);
-  return rest < 0 ? rest : first + rest;
+  const int item = a.type == kFp8F32 ? 4 : 2;
+  if (GLU || ((reinterpret_cast<uintptr_t>(a.out) | size_t(a.ldo) * item | size_t(a.N) * item) & 31) == 0)
+    return run_pairs<GLU, true>(gpu, g, a, u, units, p.ks, st);
+  return run_pairs<GLU, GLU>(gpu, g, a, u, units, p.ks, st);
 }
 
 }  // namespace

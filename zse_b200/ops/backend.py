@@ -19,6 +19,7 @@ from . import reference as ref
 
 F16, F32, I32, I64 = torch.float16, torch.float32, torch.int32, torch.int64
 FP8_TYPES = {F16: 0, torch.bfloat16: 1, F32: 2}
+NORM_TYPES = {F16: 0, torch.bfloat16: 1}
 EPI_F16, EPI_SWIGLU, EPI_PARTIAL, EPI_RELU2 = 0, 1, 2, 5
 
 
@@ -1418,14 +1419,27 @@ class CudaOps(TorchOps):
 
     # (The three calls of the 8-bit cache are written out flat: outside a CUDA graph a small one is mostly Python.  What is plainly in
     # order is seen at a glance; the checks of the base class take the rest and name what is wrong.)
-    # ---- 8-bit floating point: a call packs its arguments itself, and only one that is not as it should be is looked at by name -----
+    # ---- 8-bit floating point -----------------------------------------------------------------------------
+    # (A call packs its arguments itself; only one that is not plainly as it should be is looked at by name.)
     def add_rmsnorm_fp8(self, residual, partials, n_partials, add, weight, out, M, eps, normed=None):
-        self._check_norm_fp8(residual, partials, n_partials, add, weight, out, M, normed)
-        n, data, scale = self.n, out.data, out.scale
+        data, scale, shape, t = out.data, out.scale, residual.shape, weight.dtype
+        device, rows, ld, lds, H = residual.get_device(), data.shape, data.stride(), scale.stride(), shape[-1]
+        kind = NORM_TYPES.get(t)
+        if not (len(shape) == 2 and 0 <= M <= shape[0] and M <= rows[0] and rows[1] == H and H >= 16 and H % 16 == 0 and kind is not None
+                and residual.dtype is F32 and residual.is_contiguous() and ld[1] == 1 and ld[0] >= H and lds[1] == 1 and lds[0] >= rows[0]
+                and data.get_device() == device and weight.shape == (H,) and weight.is_contiguous() and weight.get_device() == device
+                and (n_partials == 0 or n_partials > 0 and partials is not None and partials.dtype is F32 and partials.is_contiguous()
+                     and partials.numel() >= n_partials * M * H and partials.get_device() == device)
+                and (add is None or add.dtype is t and add.is_contiguous() and add.dim() == 2 and add.shape[0] >= M and add.shape[1] == H
+                     and add.get_device() == device)
+                and (normed is None or normed.dtype is t and normed.is_contiguous() and normed.dim() == 2 and normed.shape[0] >= M
+                     and normed.shape[1] == H and normed.get_device() == device)):
+            self._check_norm_fp8(residual, partials, n_partials, add, weight, out, M, normed)
+        n = self.n
         n.launched(n.load().zse_add_rmsnorm_fp8(n.NORM_FP8.pack(
             residual.data_ptr(), partials.data_ptr() if n_partials else 0, 0 if add is None else add.data_ptr(), weight.data_ptr(),
-            0 if normed is None else normed.data_ptr(), data.data_ptr(), scale.data_ptr(), n.stream_of(data.get_device(), self.home),
-            data.stride(0), scale.stride(0), eps, n_partials, M, residual.shape[1], FP8_TYPES[weight.dtype])), "add_rmsnorm_fp8")
+            0 if normed is None else normed.data_ptr(), data.data_ptr(), scale.data_ptr(), n.stream_of(device, self.home),
+            ld[0], lds[0], eps, n_partials, M, H, kind)), "add_rmsnorm_fp8")
 
     def quant_fp8(self, x, M, out):
         self._quant_fp8(x, M, out, 1, 0)
@@ -1434,29 +1448,44 @@ class CudaOps(TorchOps):
         self._quant_fp8(gate_up, M, out, 2, 2 if gelu else 1)
 
     def _quant_fp8(self, x, M, out, parts, act):
-        self._check_quant_fp8(x, M, out, parts)
-        n, data, scale = self.n, out.data, out.scale
+        data, scale, shape, ldx, kind = out.data, out.scale, x.shape, x.stride(), FP8_TYPES.get(x.dtype)
+        device, (rows, C), ld, lds = x.get_device(), data.shape, data.stride(), scale.stride()
+        if not (kind is not None and len(shape) == 2 and 0 <= M <= shape[0] and M <= rows and shape[1] == parts * C and ldx[1] == 1
+                and ldx[0] >= shape[1] and C >= 16 and C % 16 == 0 and ld[1] == 1 and ld[0] >= C and lds[1] == 1 and lds[0] >= rows
+                and data.get_device() == device):
+            self._check_quant_fp8(x, M, out, parts)
+        n = self.n
         n.launched(n.load().zse_quant_fp8(n.QUANT_FP8.pack(
-            x.data_ptr(), data.data_ptr(), scale.data_ptr(), n.stream_of(data.get_device(), self.home), x.stride(0), data.stride(0),
-            scale.stride(0), M, data.shape[1], act, FP8_TYPES[x.dtype])), "quant_fp8")
+            x.data_ptr(), data.data_ptr(), scale.data_ptr(), n.stream_of(device, self.home), ldx[0], ld[0], lds[0], M, C, act, kind)),
+            "quant_fp8")
 
     def linear_fp8(self, w, x, M, out):
-        self._check_linear_fp8(w, x, M, out)
-        n, wd, xd, xs, bias = self.n, w.data, x.data, x.scale, w.bias
-        N, K = wd.shape
+        wd, xd, xs, bias = w.data, x.data, x.scale, w.bias
+        (N, K), (rows, cols), shape, ldw, ldx, lds, ldo = wd.shape, xd.shape, out.shape, wd.stride(), xd.stride(), xs.stride(), out.stride()
+        device, kind = wd.get_device(), FP8_TYPES.get(out.dtype)
+        if not (kind is not None and not w.glu and cols == K and K % 16 == 0 and K and N and 0 <= M <= rows and len(shape) == 2
+                and shape[0] >= M and shape[1] >= N and ldo[1] == 1 and ldo[0] >= shape[1] and ldw[1] == 1 and ldw[0] >= K and ldx[1] == 1
+                and ldx[0] >= K and lds[1] == 1 and lds[0] >= rows and xd.get_device() == device and out.get_device() == device):
+            self._check_linear_fp8(w, x, M, out)
+        n = self.n
         n.launched(n.load().zse_gemm_fp8(n.GEMM_FP8.pack(
             xd.data_ptr(), xs.data_ptr(), wd.data_ptr(), w.scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), 0,
-            self.status_ptr, n.stream_of(wd.get_device(), self.home), xd.stride(0), wd.stride(0), out.stride(0), xs.stride(0), 0, M, N, K,
-            FP8_TYPES[out.dtype], 0 if bias is None else FP8_TYPES[bias.dtype], 0)), "linear_fp8")
+            self.status_ptr, n.stream_of(device, self.home), ldx[0], ldw[0], ldo[0], lds[0], 0, M, N, K, kind,
+            0 if bias is None else FP8_TYPES[bias.dtype], 0)), "linear_fp8")
 
     def linear_swiglu_fp8(self, w, x, M, out, gelu=False):
-        self._check_linear_swiglu_fp8(w, x, M, out)
-        n, wd, xd, xs, data, scale = self.n, w.data, x.data, x.scale, out.data, out.scale
-        N, K = wd.shape
+        wd, xd, xs, od, os = w.data, x.data, x.scale, out.data, out.scale
+        (N, K), (rows, cols), (room, ff), ldw, ldx, lds, ldo, ldos = (wd.shape, xd.shape, od.shape, wd.stride(), xd.stride(), xs.stride(),
+                                                                      od.stride(), os.stride())
+        device = wd.get_device()
+        if not (w.glu and cols == K and K % 16 == 0 and K and ff * 2 == N and ff % 16 == 0 and ff and 0 <= M <= rows and M <= room
+                and ldw[1] == 1 and ldw[0] >= K and ldx[1] == 1 and ldx[0] >= K and lds[1] == 1 and lds[0] >= rows and ldo[1] == 1
+                and ldo[0] >= ff and ldos[1] == 1 and ldos[0] >= room and xd.get_device() == device and od.get_device() == device):
+            self._check_linear_swiglu_fp8(w, x, M, out)
+        n = self.n
         n.launched(n.load().zse_gemm_fp8(n.GEMM_FP8.pack(
-            xd.data_ptr(), xs.data_ptr(), wd.data_ptr(), w.scale.data_ptr(), 0, data.data_ptr(), scale.data_ptr(), self.status_ptr,
-            n.stream_of(wd.get_device(), self.home), xd.stride(0), wd.stride(0), data.stride(0), xs.stride(0), scale.stride(0), M, N // 2,
-            K, 0, 0, 2 if gelu else 1)), "linear_swiglu_fp8")
+            xd.data_ptr(), xs.data_ptr(), wd.data_ptr(), w.scale.data_ptr(), 0, od.data_ptr(), os.data_ptr(), self.status_ptr,
+            n.stream_of(device, self.home), ldx[0], ldw[0], ldo[0], lds[0], ldos[0], M, ff, K, 0, 0, 2 if gelu else 1)), "linear_swiglu_fp8")
 
     def rope_kv_write_q8(self, qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out=None, planes=None, n_planes=0,
                          bias=None):

@@ -16,6 +16,7 @@ import torch
 
 BLOCK, TOP, LEAST = 128, 448.0, 1e-30
 F8, F32 = torch.float8_e4m3fn, torch.float32
+BIAS_TYPES = frozenset((torch.float16, torch.bfloat16, F32))
 
 
 def blocks(n: int) -> int:
@@ -63,10 +64,11 @@ class Fp8Weight:
                 2 * ((shape[0] // 2 + 127) // 128) if glu else (shape[0] + 127) // 128, (shape[1] + 127) // 128):
             raise ValueError(f"data [N, K] and scales of blocks of {BLOCK} x {BLOCK}{' of each half' if glu else ''} are needed, not "
                              f"{tuple(shape)} and {tuple(scale.shape)}")
-        if not scale.is_contiguous() or data.get_device() != scale.get_device():
+        device = data.get_device()
+        if not scale.is_contiguous() or device != scale.get_device():
             raise ValueError("the scales have to be contiguous, and on the device of the data")
-        if bias is not None and (glu or bias.shape != shape[:1] or bias.get_device() != data.get_device()
-                                 or bias.dtype not in (torch.float16, torch.bfloat16, F32) or not bias.is_contiguous()):
+        if bias is not None and (glu or bias.dtype not in BIAS_TYPES or bias.stride() != (1,) or len(bias) != shape[0]
+                                 or bias.get_device() != device):
             raise ValueError(f"a bias of {shape[0]} numbers in fp16, bfloat16 or fp32 is expected beside the data, none for a gate and up weight")
         self.data, self.scale, self.bias, self.glu = data, scale, bias, glu
 
