@@ -497,6 +497,9 @@ typedef struct ZseGemmFp8 {
   int32_t M, N, K, type, bias_type, act;
 } ZseGemmFp8;
 int zse_gemm_fp8(const ZseGemmFp8* a);
+// How the current device takes such a call (M, N, K and act count): token columns of the kernel for few tokens with `parts` CTAs a tile of 128
+// rows, or 0 tokens: pairs of CTAs, with `parts` pairs for each of the tiles that are no whole round of the GPU.
+int zse_gemm_fp8_plan(const ZseGemmFp8* a, int32_t* tokens, int32_t* parts);
 
 // ---- sampling.cu --------------------------------------------------------------------------------------------
 int zse_argmax(const void* logits_f16, int ld, void* out_i32, int M, int V, void* stream);

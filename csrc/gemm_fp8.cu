@@ -233,22 +233,6 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
 
   if (warp == 0) {
     if (lane == 0) {
-      // weights are constant: the first stages are under way before the kernel before this one is done
-      auto load_w = [&](int s, int unit, int st) {
-        mbar_arrive_expect_tx(&bars->full[s], F::kStage);
-        uint8_t* to = ring + s * F::kStage;
-        const int n0 = unit / u.m_tiles * 128;
-        tma_load_2d(to, &tmap_w, (GLU ? st : 2 * st) * kFp8Block, n0, &bars->full[s]);
-        tma_load_2d(to + F::kW, &tmap_w, (GLU ? st : 2 * st + 1) * kFp8Block, GLU ? a.N + n0 : n0, &bars->full[s]);
-      };
-      auto load_x = [&](int s, int unit, int st) {
-        uint8_t* to = ring + s * F::kStage + 2 * F::kW;
-        const int t0 = unit % u.m_tiles * NT;
-        tma_load_2d(to, &tmap_x, (GLU ? st : 2 * st) * kFp8Block, t0, &bars->full[s]);
-        if (!GLU) tma_load_2d(to + F::kX, &tmap_x, (2 * st + 1) * kFp8Block, t0, &bars->full[s]);
-      };
-      const int ahead = min(F::kStages, s1 - s0);
-      for (int i = 0; i < ahead; ++i) load_w(i, first, s0 + i);
       pdl_wait();
       int s = 0, c = 0;
       uint32_t ph = 1;
@@ -259,8 +243,13 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
             live = false;
             break;
           }
-          if (c >= ahead) load_w(s, i, st);
-          load_x(s, i, st);
+          mbar_arrive_expect_tx(&bars->full[s], F::kStage);
+          uint8_t* to = ring + s * F::kStage;
+          const int n0 = i / u.m_tiles * 128, t0 = i % u.m_tiles * NT, k = (GLU ? st : 2 * st) * kFp8Block;
+          tma_load_2d(to, &tmap_w, k, n0, &bars->full[s]);
+          tma_load_2d(to + F::kW, &tmap_w, GLU ? k : k + kFp8Block, GLU ? a.N + n0 : n0, &bars->full[s]);
+          tma_load_2d(to + 2 * F::kW, &tmap_x, k, t0, &bars->full[s]);
+          if (!GLU) tma_load_2d(to + 2 * F::kW + F::kX, &tmap_x, k + kFp8Block, t0, &bars->full[s]);
           if (++s == F::kStages) { s = 0; ph ^= 1; }
         }
       }
@@ -762,9 +751,11 @@ int launch_pair(const Gpu& gpu, const CUtensorMap& tx, const CUtensorMap& tw, co
 }
 
 // ---- which kernel ------------------------------------------------------------------------------------------------------------------------
-// Times in microseconds, from layers of 1 to 4096 tokens (those of gate and up weights in brackets).  A pair of CTAs takes 0.46 (0.62) a block of K
-// whatever part of its 256 tokens there is; a step of the kernel for few tokens 0.6 with 16 token columns, 0.65 with 32, 0.78 (0.87) with 64 and 1.25
-// (1.9) with 128, but not less than its weights take from memory.  A launch costs 3, sums over a cluster 4.
+// Times in microseconds, from layers of 1 to 4096 tokens (those of gate and up weights in brackets).  A pair of CTAs takes 0.44 (0.6) a block of K
+// whatever part of its 256 tokens there is, and 5 besides; the kernel for few tokens 0.6 a step with 16 token columns, 0.65 with 32, 0.78 (0.87)
+// with 64 and 1.25 with 128 (gate and up weights: 1.9, which pairs beat), but not less than its weights take from memory, and 2 besides.  Sums over
+// a cluster cost 3 or 4.  Both sides of the line, measured: 128 tokens of 5120 x 13824 30 us with 128 columns and 47 in pairs, 128 of 10240 x 8192 38
+// and 32; 64 of 2 x 13824 x 5120 38 and 48, 128 69 and 49.
 struct Fp8Plan {
   int nt;                                                      // token columns of the kernel for few tokens; 0: pairs
   int ks;                                                      // pairs: parts of K of the units behind the last whole round
@@ -772,12 +763,12 @@ struct Fp8Plan {
 };
 template <bool GLU>
 Fp8Plan plan_pairs(const Gpu& gpu, int units, int n_kb) {
-  const float kb = GLU ? 0.62f : 0.46f;
+  const float kb = GLU ? 0.6f : 0.44f;
   const int at_once = std::max(1, pair_fit<GLU, 1, true>(gpu)), rest = units % at_once;
-  Fp8Plan p{0, 1, 3 + kb * n_kb * ((units + at_once - 1) / at_once)};
+  Fp8Plan p{0, 1, 5 + kb * n_kb * ((units + at_once - 1) / at_once)};
   if (rest == 0) return p;
   auto with = [&](int ks, int fit) {
-    const float us = 3 + kb * n_kb * (units / at_once) + (units > rest ? 3 : 0) + 4 + kb * ((n_kb + ks - 1) / ks);
+    const float us = 5 + kb * n_kb * (units / at_once) + (units > rest ? 3 : 0) + 4 + kb * ((n_kb + ks - 1) / ks);
     if (rest <= fit && n_kb >= 4 * ks && us < p.us) p.ks = ks, p.us = us;
   };
   with(2, pair_fit<GLU, 2, true>(gpu));
@@ -810,8 +801,8 @@ template <int NT, bool GLU>
 void plan_few(const Gpu& gpu, int M, int N, int n_kb, Fp8Plan* best) {
   if (M > 4 * NT) return;
   const int units = (N + 127) / 128 * ((M + NT - 1) / NT), steps = GLU ? n_kb : (n_kb + 1) / 2, ks = few_splits<NT, GLU>(gpu, units, steps);
-  const float step = NT == 16 ? 0.6f : NT == 32 ? 0.65f : NT == 64 ? (GLU ? 0.87f : 0.78f) : (GLU ? 1.9f : 1.25f);
-  const float us = 3 + (ks > 1 ? 4 : 0) + std::max(step * ((steps + ks - 1) / ks) * ((units + gpu.sms - 1) / gpu.sms), 2.f * N * n_kb * (GLU ? 1 : 0.5f) * 128 / 6e6f);
+  const float step = NT == 16 ? 0.6f : NT == 32 ? 0.65f : NT == 64 ? (GLU ? 0.87f : 0.78f) : 1.25f;
+  const float us = 2 + (ks > 1 ? 3 : 0) + std::max(step * ((steps + ks - 1) / ks) * ((units + gpu.sms - 1) / gpu.sms), 2.f * N * n_kb * (GLU ? 1 : 0.5f) * 128 / 6e6f);
   if (us < best->us) *best = Fp8Plan{NT, ks, us};
 }
 
@@ -852,24 +843,34 @@ int run_pairs(const Gpu& gpu, const ZseGemmFp8& g, const Fp8Args& a, const Fp8Un
 }
 
 template <bool GLU>
-int run(const ZseGemmFp8& g, const Fp8Args& a, cudaStream_t st) {
+int plan(const Gpu& gpu, const ZseGemmFp8& g, Fp8Units* u, int* units, Fp8Plan* p) {
   const int cols = GLU ? 128 : 256, m_tiles = (g.M + 255) / 256, n_tiles = (g.N + cols - 1) / cols, groups = (m_tiles + 7) / 8;
   const int n_kb = (g.K + kFp8Block - 1) / kFp8Block;
   if ((long long)m_tiles * n_tiles > 0x3fffffff) return ZSE_ERR_LIMIT;
-  const int units = m_tiles * n_tiles;
+  *u = Fp8Units{n_tiles, m_tiles, (m_tiles + groups - 1) / groups, 0, 0};      // about 2048 tokens at a time
+  *units = m_tiles * n_tiles;
+  *p = plan_pairs<GLU>(gpu, *units, n_kb);
+  plan_few<16, GLU>(gpu, g.M, g.N, n_kb, p);
+  plan_few<32, GLU>(gpu, g.M, g.N, n_kb, p);
+  plan_few<64, GLU>(gpu, g.M, g.N, n_kb, p);
+  if constexpr (!GLU) plan_few<128, GLU>(gpu, g.M, g.N, n_kb, p);
+  return 0;
+}
+
+template <bool GLU>
+int run(const ZseGemmFp8& g, const Fp8Args& a, cudaStream_t st) {
   const Gpu gpu{current_device_slot(), sm_count()};
-  Fp8Plan p = plan_pairs<GLU>(gpu, units, n_kb);
-  plan_few<16, GLU>(gpu, g.M, g.N, n_kb, &p);
-  plan_few<32, GLU>(gpu, g.M, g.N, n_kb, &p);
-  plan_few<64, GLU>(gpu, g.M, g.N, n_kb, &p);
-  plan_few<128, GLU>(gpu, g.M, g.N, n_kb, &p);
+  Fp8Units u;
+  Fp8Plan p;
+  int units;
+  if (int rc = plan<GLU>(gpu, g, &u, &units, &p)) return rc;
   switch (p.nt) {
     case 16: return launch_few<16, GLU>(gpu, g, a, p.ks, st);
     case 32: return launch_few<32, GLU>(gpu, g, a, p.ks, st);
     case 64: return launch_few<64, GLU>(gpu, g, a, p.ks, st);
-    case 128: return launch_few<128, GLU>(gpu, g, a, p.ks, st);
+    case 128:
+      if constexpr (!GLU) return launch_few<128, GLU>(gpu, g, a, p.ks, st);
   }
-  const Fp8Units u{n_tiles, m_tiles, (m_tiles + groups - 1) / groups, 0, 0};     // about 2048 tokens at a time
   const int item = a.type == kFp8F32 ? 4 : 2;
   if (GLU || ((reinterpret_cast<uintptr_t>(a.out) | size_t(a.ldo) * item | size_t(a.N) * item) & 31) == 0)
     return run_pairs<GLU, true>(gpu, g, a, u, units, p.ks, st);
@@ -881,13 +882,34 @@ int run(const ZseGemmFp8& g, const Fp8Args& a, cudaStream_t st) {
 
 using namespace zse;
 
+namespace {
+int fp8_shape(const ZseGemmFp8* g) {
+  const bool glu = g->act != kFp8None;
+  return g->N <= 0 || g->K <= 0 || g->K % 16 || g->act < kFp8None || g->act > kFp8Gelu || g->type < kFp8F16 || g->type > kFp8F32 ||
+                 g->bias_type < kFp8F16 || g->bias_type > kFp8F32 || (glu && (g->N % 16 || g->bias != nullptr))
+             ? ZSE_ERR_SHAPE
+             : 0;
+}
+}  // namespace
+
+extern "C" int zse_gemm_fp8_plan(const ZseGemmFp8* g, int32_t* tokens, int32_t* parts) {
+  if (g->M <= 0) return ZSE_ERR_SHAPE;
+  if (int rc = fp8_shape(g)) return rc;
+  const Gpu gpu{current_device_slot(), sm_count()};
+  Fp8Units u;
+  Fp8Plan p;
+  int units;
+  if (int rc = g->act != kFp8None ? plan<true>(gpu, *g, &u, &units, &p) : plan<false>(gpu, *g, &u, &units, &p)) return rc;
+  *tokens = p.nt;
+  *parts = p.ks;
+  return 0;
+}
+
 extern "C" int zse_gemm_fp8(const ZseGemmFp8* g) {
   if (g->M <= 0) return 0;
+  if (int rc = fp8_shape(g)) return rc;
   const bool glu = g->act != kFp8None;
-  if (g->N <= 0 || g->K <= 0 || g->K % 16 || g->act < kFp8None || g->act > kFp8Gelu || g->type < kFp8F16 || g->type > kFp8F32 ||
-      g->bias_type < kFp8F16 || g->bias_type > kFp8F32 || (glu && (g->N % 16 || g->bias != nullptr || g->out_scale == nullptr)))
-    return ZSE_ERR_SHAPE;
-  if (g->M > 65535 * 128) return ZSE_ERR_LIMIT;
+  if (glu && g->out_scale == nullptr) return ZSE_ERR_SHAPE;
   auto aligned = [](const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; };
   if (!aligned(g->x, 16) || !aligned(g->w, 16) || g->ldx % 16 || g->ldw % 16 || !aligned(g->sx, 4) || !aligned(g->sw, 4) ||
       (glu ? !aligned(g->out, 16) || g->ldo % 16 : !aligned(g->out, g->type == kFp8F32 ? 4 : 2)))

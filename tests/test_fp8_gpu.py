@@ -165,6 +165,32 @@ def test_linear_large(ops, M, N, K):
     check_linear(ops, M, N, K, BF16, None)
 
 
+EVERY_FORM = [
+    (3, 100, 2064), (9, 5120, 2048), (1, 19200, 272), (20, 1000, 4096), (31, 20000, 144), (50, 5110, 4096), (64, 19210, 400), (120, 5120, 8192),
+    (270, 120, 4112), (250, 10240, 2048), (255, 5120, 8192), (257, 2200, 8208), (700, 1001, 4096), (300, 4099, 2560), (300, 4001, 8192),
+    (1200, 8000, 4096), (2100, 5121, 4096)]
+EVERY_FORM_GLU = [
+    (2, 112, 2064), (7, 5120, 2048), (1, 19200, 144), (18, 4096, 2048), (32, 13808, 400), (60, 5120, 4096), (33, 9600, 272), (200, 9600, 528),
+    (256, 2048, 4096), (300, 400, 8192), (1300, 1936, 2048)]
+
+
+def test_the_forms_are_all_there(ops):
+    """The two lists reach every kernel, with K whole and in parts (on a GPU of 148 SMs)."""
+    from zse_b200.ops.native import gemm_fp8_plan
+    if torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("another GPU, other plans")
+    form = lambda p: p if p[0] == 0 else (p[0], p[1] > 1)                   # noqa: E731
+    few = {(n, split) for n in (16, 32, 64) for split in (False, True)}
+    assert {form(gemm_fp8_plan(*c)) for c in EVERY_FORM} == few | {(128, True), (0, 1), (0, 2), (0, 4)}
+    assert {form(gemm_fp8_plan(*c, glu=True)) for c in EVERY_FORM_GLU} == few | {(0, 1), (0, 2), (0, 4)}
+
+
+@pytest.mark.parametrize("M,N,K", EVERY_FORM)
+@pytest.mark.parametrize("dtype,bias", [(F16, F16), (F32, None)])
+def test_linear_in_every_form(ops, M, N, K, dtype, bias):
+    check_linear(ops, M, N, K, dtype, bias, ld=8 if N % 8 == 0 else 0)
+
+
 def check_swiglu(ops, M, ff, K, gelu=False, apart=0):
     g = gen(M * 13 + ff + K)
     x, w = make_rows(g, M + 2, K, DEV, hot=False), make_weight(g, ff, K, DEV, glu=True)
@@ -188,6 +214,11 @@ def test_linear_swiglu(ops, M, ff, K, gelu):
 @pytest.mark.parametrize("M,ff,K", [(1, 18944, 3584), (5, 13824, 5120), (160, 13824, 2048), (777, 4096, 1024), (2049, 8192, 1040), (4100, 2048, 512)])
 def test_linear_swiglu_large(ops, M, ff, K):
     check_swiglu(ops, M, ff, K)
+
+
+@pytest.mark.parametrize("M,ff,K", EVERY_FORM_GLU)
+def test_linear_swiglu_in_every_form(ops, M, ff, K):
+    check_swiglu(ops, M, ff, K, gelu=M % 2 == 0)
 
 
 def test_a_nan_stays_in_its_row_or_column(ops):
@@ -320,6 +351,58 @@ def test_streams_and_graphs(ops):
                 graph.replay()
         assert same()
     ops.check()
+
+
+def test_a_weight_written_just_before(ops):
+    """A call sees what the call before it on the stream has written, weights and their scales among it."""
+    for M, N, K in ((1, 4096, 4096), (300, 2048, 2048)):
+        g = gen(M)
+        x, ws = make_rows(g, M, K, DEV), [make_weight(g, N, K, DEV) for _ in range(2)]
+        want = []
+        for w in ws:
+            out = torch.empty(M, N, device=DEV)
+            ops.linear_fp8(w, x, M, out)
+            want.append(out)
+        w, out = Fp8Weight(ws[0].data.clone(), ws[0].scale.clone()), torch.empty(M, N, device=DEV)
+        for i in range(20):
+            w.data.view(torch.uint8).copy_(ws[i % 2].data.view(torch.uint8))
+            w.scale.copy_(ws[i % 2].scale)
+            ops.linear_fp8(w, x, M, out)
+            assert torch.equal(out, want[i % 2])
+
+
+def test_first_calls_inside_a_graph():
+    """What a call sets up for itself the first time does not disturb a capture."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from tests.helpers.fp8_oracle import make_rows, make_weight
+from zse_b200.ops.backend import make_ops
+from zse_b200.ops.fp8 import Fp8Rows
+ops, g = make_ops("cuda"), torch.Generator().manual_seed(1)
+x = {M: make_rows(g, M, 1024, "cuda", hot=False) for M in (1, 40, 600)}
+w, up = make_weight(g, 512, 1024, "cuda"), make_weight(g, 512, 1024, "cuda", glu=True)
+out = {M: torch.zeros(M, 512, device="cuda") for M in x}
+rows = {M: Fp8Rows(torch.zeros(M, 512, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn), torch.zeros(4, M, device="cuda")) for M in x}
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    for M in x:
+        ops.linear_fp8(w, x[M], M, out[M])
+        ops.linear_swiglu_fp8(up, x[M], M, rows[M])
+        ops.quant_fp8(out[M], M, rows[M])
+graph.replay()
+torch.cuda.synchronize()
+ops.check()
+for M in x:
+    again, r = torch.empty(M, 512, device="cuda"), Fp8Rows.empty(M, 512, "cuda")
+    ops.linear_fp8(w, x[M], M, again)
+    ops.quant_fp8(again, M, r)
+    assert torch.equal(again, out[M]) and torch.equal(r.data.view(torch.uint8), rows[M].data.view(torch.uint8)) and torch.equal(r.scale, rows[M].scale)
+print("FINE")
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
+    assert "FINE" in done.stdout, done.stderr[-2000:]
 
 
 def test_refusals_of_the_kernels(ops):

@@ -133,6 +133,7 @@ _SIGS = {
     "zse_add_rmsnorm_fp8": (c_int, [c_char_p]),
     "zse_quant_fp8": (c_int, [c_char_p]),
     "zse_gemm_fp8": (c_int, [c_char_p]),
+    "zse_gemm_fp8_plan": (c_int, [c_char_p, POINTER(c_int32), POINTER(c_int32)]),
     "zse_attn_decode_q8_pieces": (c_int, [c_char_p]),
     "zse_attn_decode_q8_scratch_floats": (c_int64, [c_char_p]),
     "zse_attn_decode_q8": (c_int, [c_char_p]),
@@ -568,6 +569,13 @@ def attn_decode_q8_plan(S, max_q, nh, nkv, hd, block_size, max_blocks, window=0,
     args = ATTN_Q8.pack(0, 0, 1, nkv, block_size, hd, 0, 0, 0, max_q > 1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, max_blocks, S, max_q, nh,
                         num_splits, window, 1.0, 0)
     return lib.zse_attn_decode_q8_pieces(args), lib.zse_attn_decode_q8_scratch_floats(args)
+
+
+def gemm_fp8_plan(M, N, K, glu: bool = False) -> tuple:
+    """(token columns of the kernel for few tokens or 0: pairs of CTAs, parts of K) of such a product."""
+    tokens, parts = c_int32(), c_int32()
+    _ck(load().zse_gemm_fp8_plan(GEMM_FP8.pack(*[0] * 14, M, N, K, 0, 0, int(glu)), byref(tokens), byref(parts)), "gemm_fp8_plan", 0)
+    return tokens.value, parts.value
 
 
 def headnorm_rope_kv_write(qkv, kv_layer, positions, slots, freqs, q_norm_w, k_norm_w, norm_v, k_is_v, eps, M, nh, nkv,
