@@ -44,8 +44,9 @@ __device__ __forceinline__ float4 load4<bf16>(const bf16* p) {
   return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
 }
 
-template <typename T, int J, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+// SEVERAL: more than one addend.  (One, and 256 threads: as many rows on an SM as registers allow.)
+template <typename T, int J, int THREADS, bool SEVERAL>
+__global__ void __launch_bounds__(THREADS, THREADS > 256 || SEVERAL ? 1 : J <= 5 ? 6 : 4)
 add_rmsnorm_fp8_kernel(const NormFp8 a) {
   __shared__ double red[32];
   pdl_launch_dependents();
@@ -53,7 +54,6 @@ add_rmsnorm_fp8_kernel(const NormFp8 a) {
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row = blockIdx.x, H = a.H, blocks = (H + kFp8Block - 1) / kFp8Block;
   const size_t base = size_t(row) * H, plane = size_t(a.M) * H;
-  const bool several = a.n_planes + (a.add != nullptr) > 1;
   float4 x[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) {
@@ -65,7 +65,7 @@ add_rmsnorm_fp8_kernel(const NormFp8 a) {
     for (int j = 0; j < J; ++j) {
       const int c = (warp + j * warps) * kFp8Block + lane * 4;
       if (c < H) {
-        if (several) {
+        if constexpr (SEVERAL) {
           double s[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
 #pragma unroll 4
           for (int p = 0; p < a.n_planes; ++p) {
@@ -177,7 +177,7 @@ quant_fp8_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ d
   }
 }
 
-template <typename T>
+template <typename T, bool SEVERAL>
 int norm_fp8(const NormFp8& a, cudaStream_t st) {
   const int blocks = (a.H + kFp8Block - 1) / kFp8Block, least = (blocks + 31) / 32;
   auto go = [&](auto kernel, int J) {
@@ -186,24 +186,23 @@ int norm_fp8(const NormFp8& a, cudaStream_t st) {
   // many rows: eight warps a row, so that several rows are under way on an SM; few: as soon as possible done with each
   if (a.M >= 4 * sm_count() && blocks <= 64) {
     const int J = (blocks + 7) / 8;
-    if (J == 1) return go(add_rmsnorm_fp8_kernel<T, 1, 256>, 1);
-    if (J == 2) return go(add_rmsnorm_fp8_kernel<T, 2, 256>, 2);
-    if (J == 3) return go(add_rmsnorm_fp8_kernel<T, 3, 256>, 3);
-    if (J == 4) return go(add_rmsnorm_fp8_kernel<T, 4, 256>, 4);
-    if (J == 5) return go(add_rmsnorm_fp8_kernel<T, 5, 256>, 5);
-    return go(add_rmsnorm_fp8_kernel<T, 8, 256>, 8);
+    if (J == 1) return go(add_rmsnorm_fp8_kernel<T, 1, 256, SEVERAL>, 1);
+    if (J == 2) return go(add_rmsnorm_fp8_kernel<T, 2, 256, SEVERAL>, 2);
+    if (J == 3) return go(add_rmsnorm_fp8_kernel<T, 3, 256, SEVERAL>, 3);
+    if (J == 4) return go(add_rmsnorm_fp8_kernel<T, 4, 256, SEVERAL>, 4);
+    if (J == 5) return go(add_rmsnorm_fp8_kernel<T, 5, 256, SEVERAL>, 5);
+    return go(add_rmsnorm_fp8_kernel<T, 8, 256, SEVERAL>, 8);
   }
-  if (least == 1) return go(add_rmsnorm_fp8_kernel<T, 1, 1024>, 1);
-  if (least == 2) return go(add_rmsnorm_fp8_kernel<T, 2, 1024>, 2);
-  if (least <= 4) return go(add_rmsnorm_fp8_kernel<T, 4, 1024>, 4);
-  return go(add_rmsnorm_fp8_kernel<T, 8, 1024>, 8);
+  if (least == 1) return go(add_rmsnorm_fp8_kernel<T, 1, 1024, SEVERAL>, 1);
+  if (least == 2) return go(add_rmsnorm_fp8_kernel<T, 2, 1024, SEVERAL>, 2);
+  if (least <= 4) return go(add_rmsnorm_fp8_kernel<T, 4, 1024, SEVERAL>, 4);
+  return go(add_rmsnorm_fp8_kernel<T, 8, 1024, SEVERAL>, 8);
 }
 
 template <typename T>
 int quant_fp8(const ZseQuantFp8& q, cudaStream_t st) {
-  const int across = ((q.C + kFp8Block - 1) / kFp8Block + 15) / 16, room = std::max(1, 8 * sm_count() / across);
-  if (across > 0x7fffffff / 2) return ZSE_ERR_LIMIT;
-  const dim3 grid(across, std::min(std::min((q.M + 1) / 2, room), 65535));
+  const int across = ((q.C + kFp8Block - 1) / kFp8Block + 15) / 16;
+  const dim3 grid(across, std::min((q.M + 1) / 2, 65535));
   auto go = [&](auto kernel) {
     return launch_pdl(kernel, grid, dim3(256), 0, st, static_cast<const T*>(q.x), q.ldx, static_cast<uint8_t*>(q.data), q.ld_data,
                       static_cast<float*>(q.scale), q.ld_scale, q.M, q.C) == cudaSuccess
@@ -231,8 +230,10 @@ extern "C" int zse_add_rmsnorm_fp8(const ZseNormFp8* n) {
   const NormFp8 a{static_cast<float*>(n->residual), static_cast<const float*>(n->planes), n->add, n->weight, n->normed,
                   static_cast<uint8_t*>(n->data), static_cast<float*>(n->scale), n->ld_data, n->ld_scale, n->eps, n->n_planes, n->M, n->H};
   const cudaStream_t st = static_cast<cudaStream_t>(n->stream);
-  if (n->type == kFp8F16) return norm_fp8<__half>(a, st);
-  return n->type == kFp8BF16 ? norm_fp8<bf16>(a, st) : ZSE_ERR_SHAPE;
+  const bool several = n->n_planes + (n->add != nullptr) > 1;
+  if (n->type == kFp8F16) return several ? norm_fp8<__half, true>(a, st) : norm_fp8<__half, false>(a, st);
+  if (n->type == kFp8BF16) return several ? norm_fp8<bf16, true>(a, st) : norm_fp8<bf16, false>(a, st);
+  return ZSE_ERR_SHAPE;
 }
 
 extern "C" int zse_quant_fp8(const ZseQuantFp8* q) {
