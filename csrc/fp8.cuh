@@ -11,6 +11,7 @@ namespace zse {
 constexpr int kFp8Block = 128;                  // columns of a scale, and rows of a weight's
 constexpr float kFp8Top = 448.f;                // the largest e4m3
 constexpr float kFp8Least = 1e-30f;             // a block whose largest number is not above it is written as zeros
+constexpr int kFp8Most = 1 << 30;               // rows or columns of a call: their numbers, rounded up to a tile, stay ints
 
 enum Fp8Type : int { kFp8F16 = 0, kFp8BF16 = 1, kFp8F32 = 2 };
 enum Fp8Act : int { kFp8None = 0, kFp8Silu = 1, kFp8Gelu = 2 };
@@ -48,5 +49,14 @@ __device__ __forceinline__ float hold_f16(float x) {
 }
 template <>
 __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) { return pack_half2(hold_f16(a), hold_f16(b)); }
+
+// Whether `rows` rows of `bytes` bytes, ld bytes apart, at p share none with those at q: apart as a whole, or columns of the same rows.
+inline bool rows_apart(const void* p, long long bytes, long long ld, const void* q, long long q_bytes, long long q_ld, int rows) {
+  const long long d = reinterpret_cast<const uint8_t*>(q) - reinterpret_cast<const uint8_t*>(p);
+  if (d >= (rows - 1) * ld + bytes || -d >= (rows - 1) * q_ld + q_bytes) return true;
+  if (rows == 1 || ld != q_ld || ld <= 0) return false;
+  const long long column = (d % ld + ld) % ld;
+  return column >= bytes && column + q_bytes <= ld;
+}
 
 }  // namespace zse

@@ -223,12 +223,13 @@ extern "C" int zse_add_rmsnorm_fp8(const ZseNormFp8* n) {
   if (n->M <= 0) return 0;
   if (n->H <= 0 || n->H % 16 || n->n_planes < 0 || n->residual == nullptr || n->weight == nullptr || (n->n_planes > 0 && n->planes == nullptr))
     return ZSE_ERR_SHAPE;
-  if (n->H > 32768) return ZSE_ERR_LIMIT;
+  if (n->H > 32768 || n->M > kFp8Most) return ZSE_ERR_LIMIT;
+  const int64_t ld_data = n->M == 1 ? 0 : n->ld_data;          // (a single row may have any)
   if (!aligned(n->residual, 16) || !aligned(n->planes, 16) || !aligned(n->add, 8) || !aligned(n->weight, 8) || !aligned(n->normed, 8) ||
-      !aligned(n->data, 16) || n->ld_data % 16 || !aligned(n->scale, 4))
+      !aligned(n->data, 16) || ld_data % 16 || !aligned(n->scale, 4))
     return ZSE_ERR_ALIGN;
   const NormFp8 a{static_cast<float*>(n->residual), static_cast<const float*>(n->planes), n->add, n->weight, n->normed,
-                  static_cast<uint8_t*>(n->data), static_cast<float*>(n->scale), n->ld_data, n->ld_scale, n->eps, n->n_planes, n->M, n->H};
+                  static_cast<uint8_t*>(n->data), static_cast<float*>(n->scale), ld_data, n->ld_scale, n->eps, n->n_planes, n->M, n->H};
   const cudaStream_t st = static_cast<cudaStream_t>(n->stream);
   const bool several = n->n_planes + (n->add != nullptr) > 1;
   if (n->type == kFp8F16) return several ? norm_fp8<__half, true>(a, st) : norm_fp8<__half, false>(a, st);
@@ -239,8 +240,12 @@ extern "C" int zse_add_rmsnorm_fp8(const ZseNormFp8* n) {
 extern "C" int zse_quant_fp8(const ZseQuantFp8* q) {
   if (q->M <= 0) return 0;
   if (q->C <= 0 || q->C % 16 || q->act < kFp8None || q->act > kFp8Gelu) return ZSE_ERR_SHAPE;
-  if (!aligned(q->x, 16) || q->ldx % (q->type == kFp8F32 ? 4 : 8) || !aligned(q->data, 16) || q->ld_data % 16 || !aligned(q->scale, 4))
-    return ZSE_ERR_ALIGN;
+  if (q->M > kFp8Most || q->C > kFp8Most) return ZSE_ERR_LIMIT;
+  ZseQuantFp8 one = *q;
+  if (q->M == 1) one.ldx = one.ld_data = 0, q = &one;          // (a single row may have any)
+  const int item = q->type == kFp8F32 ? 4 : 2;
+  if (!aligned(q->x, 16) || q->ldx * item % 16 || !aligned(q->data, 16) || q->ld_data % 16 || !aligned(q->scale, 4)) return ZSE_ERR_ALIGN;
+  if (!rows_apart(q->x, (q->act == kFp8None ? 1ll : 2ll) * q->C * item, q->ldx * item, q->data, q->C, q->ld_data, q->M)) return ZSE_ERR_SHAPE;
   const cudaStream_t st = static_cast<cudaStream_t>(q->stream);
   switch (q->type) {
     case kFp8F16: return quant_fp8<__half>(*q, st);

@@ -6,8 +6,9 @@
 // a block is a product by itself (four tcgen05.mma of 32 columns) in one of two TMEM accumulators, and the warps that own its rows add it,
 // times both scales, to fp32 sums in their registers while the next block's product runs in the other.
 //
-// Tokens lie on the TMEM lanes: a thread has one row, so both scales are one number of its own per block, the gated activation pairs columns
-// of the same thread, and the largest number of a row's 128 outputs needs two threads.
+// Two kernels.  For many tokens pairs of CTAs have the tokens on the TMEM lanes: a thread has one row, so both scales are one number of its own
+// per block, the gated activation pairs columns of the same thread, and the largest number of a row's 128 outputs needs two threads.  For few
+// tokens the weight rows lie on the lanes.
 #include "api.h"
 #include "fp8.cuh"
 #include "gemm_common.cuh"
@@ -835,7 +836,7 @@ int run_pairs(const Gpu& gpu, const ZseGemmFp8& g, const Fp8Args& a, const Fp8Un
   CUtensorMap tx, tw;
   if (int rc = make_map(g.x, g.M, g.K, g.ldx, 128, &tx)) return rc;
   if (int rc = make_map(g.w, GLU ? 2ull * g.N : g.N, g.K, g.ldw, GLU ? 64 : 128, &tw)) return rc;
-  const int whole = ks > 1 ? units - units % pair_fit<GLU, 1, WIDE, TYPE>(gpu) : units;
+  const int whole = ks > 1 ? units - units % std::max(1, pair_fit<GLU, 1, WIDE, TYPE>(gpu)) : units;
   const int first = launch_pair<GLU, 1, WIDE, TYPE>(gpu, tx, tw, a, u, 0, whole, st);
   if (first < 0) return first;
   const int rest = ks == 4 ? launch_pair<GLU, 4, WIDE, TYPE>(gpu, tx, tw, a, u, whole, units, st) : launch_pair<GLU, 2, WIDE, TYPE>(gpu, tx, tw, a, u, whole, units, st);
@@ -890,7 +891,8 @@ int fp8_shape(const ZseGemmFp8* g) {
   return g->N <= 0 || g->K <= 0 || g->K % 16 || g->act < kFp8None || g->act > kFp8Gelu || g->type < kFp8F16 || g->type > kFp8F32 ||
                  g->bias_type < kFp8F16 || g->bias_type > kFp8F32 || (glu && (g->N % 16 || g->bias != nullptr))
              ? ZSE_ERR_SHAPE
-             : 0;
+         : g->M > kFp8Most || g->N > (glu ? kFp8Most / 2 : kFp8Most) || g->K > kFp8Most ? ZSE_ERR_LIMIT
+                                                                                       : 0;
 }
 }  // namespace
 
@@ -912,10 +914,16 @@ extern "C" int zse_gemm_fp8(const ZseGemmFp8* g) {
   if (int rc = fp8_shape(g)) return rc;
   const bool glu = g->act != kFp8None;
   if (glu && g->out_scale == nullptr) return ZSE_ERR_SHAPE;
+  ZseGemmFp8 one = *g;                                         // (a single row may be any distance from the next)
+  if (g->M == 1) one.ldx = g->K, one.ldo = g->N;
+  if (!glu && g->N == 1) one.ldw = g->K;
+  g = &one;
+  const int item = glu ? 1 : g->type == kFp8F32 ? 4 : 2;
   auto aligned = [](const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; };
   if (!aligned(g->x, 16) || !aligned(g->w, 16) || g->ldx % 16 || g->ldw % 16 || !aligned(g->sx, 4) || !aligned(g->sw, 4) ||
-      (glu ? !aligned(g->out, 16) || g->ldo % 16 : !aligned(g->out, g->type == kFp8F32 ? 4 : 2)))
+      (glu ? !aligned(g->out, 16) || g->ldo % 16 : !aligned(g->out, item) || !aligned(g->bias, g->bias_type == kFp8F32 ? 4 : 2)))
     return ZSE_ERR_ALIGN;
+  if (!rows_apart(g->x, g->K, g->ldx, g->out, (long long)g->N * item, g->ldo * item, g->M)) return ZSE_ERR_SHAPE;
   const Fp8Args a{static_cast<const float*>(g->sx), static_cast<const float*>(g->sw), g->bias, g->out, static_cast<float*>(g->out_scale),
                   g->ldo, g->ld_sx, g->ld_os, g->M, g->N, g->K, g->type, g->bias_type, g->act, static_cast<Status*>(g->status)};
   const cudaStream_t st = static_cast<cudaStream_t>(g->stream);

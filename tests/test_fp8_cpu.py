@@ -176,3 +176,32 @@ def test_layer(ops):
     check_out(y, off, plane[0])
     assert torch.equal(r, before + plane[0])
     check_rows(norm(r, w16, 1e-6), 5 * 2.0 ** -24, x, M)
+
+
+def test_refusals_of_the_entries():
+    """What the C entries refuse before they touch a GPU (the addresses are not read)."""
+    from zse_b200.ops import native as n
+    lib = n.load()
+    at = [(i + 1) << 30 for i in range(9)]
+    SHAPE, ALIGN, LIMIT = -1, -2, -5
+
+    def quant(x=at[0], data=at[1], ldx=64, ld=64, M=4, C=64, act=0, kind=2):
+        return lib.zse_quant_fp8(n.QUANT_FP8.pack(x, data, at[2], 0, ldx, ld, M, M, C, act, kind))
+
+    def gemm(x=at[0], w=at[2], bias=0, out=at[5], ldx=64, ldw=64, ldo=64, M=4, N=64, K=64, kind=2, act=0):
+        return lib.zse_gemm_fp8(n.GEMM_FP8.pack(x, at[1], w, at[3], bias, out, at[6], at[7], 0, ldx, ldw, ldo, M, M, M, N, K, kind, 2, act))
+
+    def rms(M=4, H=64, data=at[2], ld=64, weight=at[1]):
+        return lib.zse_add_rmsnorm_fp8(n.NORM_FP8.pack(at[0], 0, 0, weight, 0, data, at[3], 0, ld, M, 1e-6, 0, M, H, 0))
+    assert quant(C=60) == quant(act=3) == quant(kind=3) == SHAPE
+    assert quant(x=at[0] + 8) == quant(ldx=66) == quant(data=at[1] + 8) == quant(ld=72) == ALIGN
+    assert quant(M=(1 << 30) + 1) == quant(C=(1 << 30) + 16) == LIMIT
+    assert quant(data=at[0]) == quant(data=at[0] + 3 * 256 + 240) == quant(x=at[1] + 3 * 64 + 48) == SHAPE       # bytes of both
+    assert gemm(N=0) == gemm(K=72) == gemm(act=3) == gemm(act=1, N=72) == gemm(act=1, bias=at[4]) == SHAPE
+    assert gemm(x=at[0] + 8) == gemm(w=at[2] + 4) == gemm(ldx=72) == gemm(ldw=72) == gemm(out=at[5] + 2) == gemm(bias=at[4] + 2) == ALIGN
+    assert gemm(act=1, out=at[5] + 8) == gemm(act=1, ldo=72) == ALIGN
+    assert gemm(M=(1 << 30) + 1) == gemm(N=(1 << 30) + 1) == gemm(act=1, N=(1 << 29) + 16) == gemm(K=(1 << 30) + 16) == LIMIT
+    assert gemm(out=at[0], ldx=0, ldo=0) == gemm(out=at[0]) == gemm(out=at[0] + 48) == gemm(act=1, out=at[0] + 32, ldx=128, ldo=128) == SHAPE
+    assert rms(H=60) == rms(weight=0) == SHAPE
+    assert rms(data=at[2] + 8) == rms(ld=72) == rms(weight=at[1] + 2) == ALIGN
+    assert rms(H=32784) == rms(M=(1 << 30) + 1) == LIMIT

@@ -273,6 +273,87 @@ def test_outputs_more_than_2_31_apart(ops):
     check_out(y, off, out)
 
 
+def test_pairs_with_outputs_more_than_2_31_apart(ops):
+    g, M, N, K, ld = gen(10), 300, 256, 4096, (1 << 23) + 16
+    x, w = make_rows(g, M, K, DEV), make_weight(g, N, K, DEV)
+    for shift in (0, 1):                                                    # written 32 bytes at a time, and not
+        out = torch.empty(ld * M + 1, dtype=BF16, device=DEV)[shift:].as_strided((M, N), (ld, 1))
+        ops.linear_fp8(w, x, M, out)
+        ops.check()
+        y, off = product(values(x, M), weight(w)[0])
+        check_out(y, off, out)
+        del out
+
+
+def test_a_single_row_may_have_any_stride(ops):
+    """A tensor of one row says nothing by its stride: that of a transposed column is 1."""
+    K, N, ff = 272, 200, 144
+    g = gen(11)
+    x, w, up, one = make_rows(g, 1, K, DEV, hot=False), make_weight(g, N, K, DEV), make_weight(g, ff, K, DEV, glu=True), make_weight(g, 1, K, DEV)
+
+    def odd(t, ld):
+        flat = torch.empty(t.numel() + ld, dtype=t.dtype, device=DEV)
+        flat.view(torch.uint8)[: t.numel() * t.element_size()] = t.contiguous().view(torch.uint8).flatten()
+        return flat.as_strided(t.shape, (ld, 1))
+    for ld in (0, 1, 7, 1001):
+        xs = Fp8Rows(odd(x.data, ld), x.scale)
+        out = odd(torch.zeros(1, N, device=DEV), ld)
+        ops.linear_fp8(w, xs, 1, out)
+        y, off = product(values(x, 1), weight(w)[0])
+        check_out(y, off, out)
+        rows = Fp8Rows(odd(torch.zeros(1, ff, dtype=torch.uint8, device=DEV).view(F8), ld), torch.empty(2, 1, device=DEV))
+        ops.linear_swiglu_fp8(up, xs, 1, rows)
+        (gate, g_off), (u, u_off) = (product(values(x, 1), p) for p in weight(up))
+        check_rows(*gated(gate, u, g_off, u_off, False), rows, 1)
+        h = odd(torch.randn(1, K, generator=g).to(DEV), ld)
+        rows = Fp8Rows(odd(torch.zeros(1, K, dtype=torch.uint8, device=DEV).view(F8), ld), torch.empty(3, 1, device=DEV))
+        ops.quant_fp8(h, 1, rows)
+        check_rows(h.double(), 0.0, rows, 1)
+        ops.add_rmsnorm_fp8(h.contiguous(), None, 0, None, torch.ones(K, device=DEV).half(), rows, 1, 1e-6)
+        check_rows(norm(h, torch.ones(K, device=DEV), 1e-6), 5 * 2.0 ** -24, rows, 1)
+        out = torch.empty(1, 1, device=DEV)
+        ops.linear_fp8(Fp8Weight(odd(one.data, ld), one.scale), xs, 1, out)
+        y, off = product(values(x, 1), weight(one)[0])
+        check_out(y, off, out)
+
+
+@pytest.mark.parametrize("M", [3, 700])
+def test_outputs_beside_what_they_are_made_of(ops, M):
+    """Rows that are read and rows that are written are columns of one buffer; the same bytes for both are refused."""
+    from zse_b200.ops.native import NativeError
+    K, ff = 256, 128
+    g = gen(12)
+    x, up, w = make_rows(g, M, K, DEV, hot=False), make_weight(g, ff, K, DEV, glu=True), make_weight(g, 64, K, DEV)
+    whole = torch.zeros(M, K + ff + 256, dtype=torch.uint8, device=DEV)
+    whole[:, :K] = x.data.view(torch.uint8)
+    xs, out = Fp8Rows(whole[:, :K].view(F8), x.scale), Fp8Rows(whole[:, K: K + ff].view(F8), torch.empty(1, M, device=DEV))
+    plane = whole[:, K + ff:].view(F32)
+    ops.linear_swiglu_fp8(up, xs, M, out)
+    ops.linear_fp8(w, xs, M, plane)
+    (gate, g_off), (u, u_off) = (product(values(x, M), p) for p in weight(up))
+    check_rows(*gated(gate, u, g_off, u_off, False), out, M)
+    y, off = product(values(x, M), weight(w)[0])
+    check_out(y, off, plane)
+    assert torch.equal(whole[:, :K], x.data.view(torch.uint8))
+    for call in (lambda: ops.linear_swiglu_fp8(up, xs, M, Fp8Rows(whole[:, K - 16: K - 16 + ff].view(F8), out.scale)),
+                 lambda: ops.linear_fp8(w, xs, M, whole[:, :256].view(F32)),
+                 lambda: ops.quant_fp8(plane, M, Fp8Rows(whole[:, K + ff + 64: K + ff + 128].view(F8), out.scale))):
+        with pytest.raises(NativeError):
+            call()
+
+
+@pytest.mark.parametrize("M,H", [(2, 144), (700, 5120)])
+def test_normed_in_the_place_of_add(ops, M, H):
+    g = gen(13)
+    r, a, w = torch.randn(M, H, generator=g).to(DEV), torch.randn(M, H, generator=g).half().to(DEV), torch.ones(H, device=DEV).half()
+    total, out = (r.double() + a.double()).float(), Fp8Rows.empty(M, H, DEV)
+    ops.add_rmsnorm_fp8(r, None, 0, a, w, out, M, 1e-6, normed=a)
+    y = norm(total, w, 1e-6)
+    assert torch.equal(r, total)
+    check_rows(y, 5 * 2.0 ** -24, out, M)
+    check_out(y, 5 * 2.0 ** -24 * y.abs(), a)
+
+
 # ---- how they are called ------------------------------------------------------------------------------------------------------
 def feed_forward(ops, r, w16, up, down, x, h, plane, M):
     ops.add_rmsnorm_fp8(r, None, 0, None, w16, x, M, 1e-6)

@@ -1417,10 +1417,8 @@ class CudaOps(TorchOps):
         self.n.attn_prefill_ext(qkv, qkv.stride(0), kv_layer, block_tables, cu_q, q_pos0, out, out.stride(0),
                                 num_seqs, max_q_len, nh, nkv, hd, block_size, scale, softcap, window)
 
-    # (The three calls of the 8-bit cache are written out flat: outside a CUDA graph a small one is mostly Python.  What is plainly in
-    # order is seen at a glance; the checks of the base class take the rest and name what is wrong.)
     # ---- 8-bit floating point -----------------------------------------------------------------------------
-    # (A call packs its arguments itself; only one that is not plainly as it should be is looked at by name.)
+    # (Flat as well: a call packs its arguments itself; only one that is not plainly as it should be is looked at by name.)
     def add_rmsnorm_fp8(self, residual, partials, n_partials, add, weight, out, M, eps, normed=None):
         data, scale, shape, t = out.data, out.scale, residual.shape, weight.dtype
         device, rows, ld, lds, H = residual.get_device(), data.shape, data.stride(), scale.stride(), shape[-1]
@@ -1487,6 +1485,8 @@ class CudaOps(TorchOps):
             xd.data_ptr(), xs.data_ptr(), wd.data_ptr(), w.scale.data_ptr(), 0, od.data_ptr(), os.data_ptr(), self.status_ptr,
             n.stream_of(device, self.home), ldx[0], ldw[0], ldo[0], lds[0], ldos[0], M, ff, K, 0, 0, 2 if gelu else 1)), "linear_swiglu_fp8")
 
+    # (The three calls of the 8-bit cache are written out flat: outside a CUDA graph a small one is mostly Python.  What is plainly in
+    # order is seen at a glance; the checks of the base class take the rest and name what is wrong.)
     def rope_kv_write_q8(self, qkv, kv, positions, slots, inv_freq, M, nh, nkv, hd, q_out=None, planes=None, n_planes=0,
                          bias=None):
         if q_out is None:
