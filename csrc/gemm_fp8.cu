@@ -9,6 +9,8 @@
 // Two kernels.  For many tokens pairs of CTAs have the tokens on the TMEM lanes: a thread has one row, so both scales are one number of its own
 // per block, the gated activation pairs columns of the same thread, and the largest number of a row's 128 outputs needs two threads.  For few
 // tokens the weight rows lie on the lanes.
+#include <type_traits>
+
 #include "api.h"
 #include "fp8.cuh"
 #include "gemm_common.cuh"
@@ -43,7 +45,11 @@ __device__ __forceinline__ float bias_of(const Fp8Args& a, int n) {
                                    : __half2float(static_cast<const __half*>(a.bias)[n]);
 }
 
-__device__ __forceinline__ float gated(int act, float g, float u) { return act == kFp8Silu ? fp8_gated<kFp8Silu>(g, u) : fp8_gated<kFp8Gelu>(g, u); }
+// (fp8_gated with the activation as an argument, without a branch)
+__device__ __forceinline__ float gated(int act, float g, float u) {
+  const float z = act == kFp8Silu ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
+  return g * sigmoid_fast(z) * u;
+}
 
 __device__ __forceinline__ void store32(void* p, const uint32_t* v) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
@@ -102,16 +108,23 @@ __device__ __forceinline__ void put_rows(const Fp8Args& a, float* y, int t, int 
 }
 
 // act(gate) * up of 64 neighbouring outputs of a row (acc: gates, then ups), the other 64 of their block in the thread of the other half.
+// No branch an output: with one, each had to be done before the next began, 9000 cycles a unit instead of 1500 (4096 x 2 x 13824 x 5120 674 us
+// instead of 571).
 // `live` is false where the sums are not there; every warp of the barrier calls it.
 __device__ __forceinline__ void put_gated(const Fp8Args& a, float* acc, int t, int n, int half, float (*tops)[128], int row, int barrier,
                                           int threads, bool live) {
   constexpr int O = 64;
   uint32_t top = 0;
+  auto gate = [&](auto act) {
 #pragma unroll
-  for (int i = 0; i < O; ++i) {
-    acc[i] = n + i < a.N ? gated(a.act, acc[i], acc[O + i]) : 0.f;
-    top = max(top, abs_bits(acc[i]));
-  }
+    for (int i = 0; i < O; ++i) {
+      const float y = fp8_gated<decltype(act)::value>(acc[i], acc[O + i]);
+      acc[i] = n + (i & ~15) < a.N ? y : 0.f;
+      top = max(top, abs_bits(acc[i]));
+    }
+  };
+  if (a.act == kFp8Silu) gate(std::integral_constant<int, kFp8Silu>());
+  else gate(std::integral_constant<int, kFp8Gelu>());
   tops[half][row] = __uint_as_float(top);
   asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
   top = max(top, __float_as_uint(tops[half ^ 1][row]));
@@ -379,7 +392,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
         if constexpr (GLU) {
 #pragma unroll
           for (int l = 0; l < H; ++l) {
-            acc[l] = n < a.N ? gated(a.act, acc[l], acc[H + l]) : 0.f;
+            const float y = gated(a.act, acc[l], acc[H + l]);
+            acc[l] = n < a.N ? y : 0.f;
             const uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(acc[l]));
             if (lane == 0) bars->top[q][half * H + l] = __uint_as_float(top);
           }
