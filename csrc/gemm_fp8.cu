@@ -63,10 +63,18 @@ __device__ __forceinline__ void add_bias(const Fp8Args& a, float* y, int n) {
   for (int j = 0; j < 16; ++j)
     if (n + j < a.N) y[j] += bias_of(a, n + j);
 }
+template <int TYPE>
 __device__ __forceinline__ void put_one(const Fp8Args& a, float y, size_t at) {
-  if (a.type == kFp8F32) static_cast<float*>(a.out)[at] = y;
-  else if (a.type == kFp8BF16) static_cast<bf16*>(a.out)[at] = __float2bfloat16_rn(y);
+  if (TYPE == kFp8F32) static_cast<float*>(a.out)[at] = y;
+  else if (TYPE == kFp8BF16) static_cast<bf16*>(a.out)[at] = __float2bfloat16_rn(y);
   else static_cast<__half*>(a.out)[at] = __float2half_rn(hold_f16(y));
+}
+// f(the type as a constant): one branch a row of outputs, not one an output
+template <typename F>
+__device__ __forceinline__ void of_type(int type, F f) {
+  if (type == kFp8F32) f(std::integral_constant<int, kFp8F32>());
+  else if (type == kFp8BF16) f(std::integral_constant<int, kFp8BF16>());
+  else f(std::integral_constant<int, kFp8F16>());
 }
 // Columns n .. n + C - 1 of a warp's 32 rows t - lane .. to memory, rounded to the output's type.  WIDE: the output, its rows and N are multiples of
 // 32 bytes, a sector, which are written at a time; else sixteen columns of two rows at a time, by way of `stage`.  The whole warp calls it.
@@ -101,8 +109,13 @@ __device__ __forceinline__ void put_rows(const Fp8Args& a, float* y, int t, int 
       for (int j = 0; j < 16; ++j) stage[lane][j] = y[i + j];
       __syncwarp();
       const int col = n + i + (lane & 15);
-      for (int r = lane >> 4; r < 32 && t0 + r < a.M; r += 2)
-        if (col < a.N) put_one(a, stage[r][lane & 15], size_t(t0 + r) * a.ldo + col);
+      of_type(a.type, [&](auto type) {
+#pragma unroll
+        for (int r = 0; r < 32; r += 2) {
+          const int row = r + (lane >> 4);
+          if (t0 + row < a.M && col < a.N) put_one<decltype(type)::value>(a, stage[row][lane & 15], size_t(t0 + row) * a.ldo + col);
+        }
+      });
     }
   }
 }
@@ -325,8 +338,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
   }
 
   const int q = warp & 3, half = (warp - 4) >> 2, row = q * 32 + lane;
-  // one output (a byte; `c`: the token's place in bars->top)
-  auto put = [&](float y, float b, int n, int t) { put_one(a, a.bias != nullptr ? y + b : y, size_t(t) * a.ldo + n); };
+  // one output's byte; `c`: the token's place in bars->top
   auto put_byte = [&](float y, int c, int n, int t) {
     uint32_t top = 0;
 #pragma unroll
@@ -404,9 +416,11 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
           asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");    // before the next unit's
         } else if (live && n < a.N) {
           const float b = a.bias != nullptr ? bias_of(a, n) : 0.f;
+          of_type(a.type, [&](auto type) {
 #pragma unroll
-          for (int l = 0; l < H; ++l)
-            if (t0 + l < a.M) put(acc[l], b, n, t0 + l);
+            for (int l = 0; l < H; ++l)
+              if (t0 + l < a.M) put_one<decltype(type)::value>(a, a.bias != nullptr ? acc[l] + b : acc[l], size_t(t0 + l) * a.ldo + n);
+          });
         }
       } else {
         pair_cluster_sync();                                   // nothing is read from or loaded into a ring of the cluster any more
@@ -453,8 +467,13 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
         for (int i = half; live && i < mine; i += 2) put_byte(red[i * 128 + row], i, n, t0 + i);
       } else if (live && n < a.N) {
         const float b = a.bias != nullptr ? bias_of(a, n) : 0.f;
+        of_type(a.type, [&](auto type) {
 #pragma unroll 4
-        for (int i = half; i < mine; i += 2) put(sum_of(0, i), b, n, t0 + i);
+          for (int i = half; i < mine; i += 2) {
+            const float y = sum_of(0, i);
+            put_one<decltype(type)::value>(a, a.bias != nullptr ? y + b : y, size_t(t0 + i) * a.ldo + n);
+          }
+        });
       }
     }
   }
@@ -641,7 +660,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
         const float f = x * __shfl_sync(0xffffffffu, w32, k & 31), f_up = GLU ? x * __shfl_sync(0xffffffffu, u32, k & 31) : f;
         x = sx[size_t(min(k + 2, n_kb - 1)) * a.ld_sx];
         const int buf = c & 1;
-        live = live && __all_sync(0xffffffffu, mbar_wait(&bars->done[es], eph, abort_flag, a.status, 93, c));
+        live = live && __all_sync(0xffffffffu, mbar_wait_spin(&bars->done[es], eph, abort_flag, a.status, 93, c));
         tc_fence_after_sync();
         add_block<C, GLU ? C / 2 : C>(acc, taddr + buf * 256, f, f_up);
         tc_fence_before_sync();
