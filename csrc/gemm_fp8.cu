@@ -179,7 +179,9 @@ __device__ __forceinline__ void add_block(float* acc, uint32_t taddr, float s, f
 // The product the other way around: 128 weight rows on the TMEM lanes, NT tokens as columns, so that a thread adds NT / 2 numbers a block
 // whatever the rows are, and the weights, whose bytes are the time of such a pass, stream past once.  A step is two tiles of 128 x 128 weights:
 // two blocks of K of the same rows, or (GLU) gate and up rows of one block.  Where there are fewer tiles of rows than SMs, the CTAs of a
-// cluster have a part of K each and add their sums through distributed shared memory: CTA r finishes the tokens r, r + ks, ... in rank order.
+// cluster have a part of K each and add their sums through distributed shared memory: each finishes a run of the tokens, from the parts in
+// rank order.  Bound by the weights' bytes where there are many steps (5 tokens of 2 x 13824 x 5120 26 us, 5.4 TB/s), by the steps' handshakes with
+// 64 columns (5120 x 13824 19.6 us, 3.7 TB/s), by the start and the cluster's two barriers with few (one token of 5120 x 5120 8.4 us).
 template <int NT, bool GLU>
 struct Few {
   static constexpr int kX = NT * 128, kW = 128 * 128;
@@ -490,7 +492,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
 
 // ---- many tokens: pairs of CTAs, persistent ------------------------------------------------------------------------------------------
 // 256 tokens and 256 weight rows a pair (cta_group::2): a CTA has 128 of the tokens, loads those and half of the weight rows, and owns the
-// sums of its tokens.  Units that do not fill a round of all pairs take a launch of their own with KS pairs a unit, clusters of 2 KS: each pair
+// sums of its tokens.  Bound by the way from a product to the next but one, 785 to 810 cycles a block where the product takes 512, and by the card's
+// power (8192 x 5120 x 5120 190 us cold, 2260 TFLOP/s; 217 warm).  Units that do not fill a round of all pairs take a launch of their own with KS pairs a unit, clusters of 2 KS: each pair
 // has a part of K, and the sums of 128 / KS rows go to each of the CTAs that have the same tokens.
 constexpr int kPairThreads = 384;                // warp 0 loads, warp 1 issues the products, warps 4 .. 11 add them up
 // Registers: 168 a thread at launch (64512), then 56 for the first four warps and 216 for the other eight (62464): 128 sums and two reads of 16
@@ -788,8 +791,8 @@ int launch_pair(const Gpu& gpu, const CUtensorMap& tx, const CUtensorMap& tw, co
 // Times in microseconds, from layers of 1 to 4096 tokens (those of gate and up weights in brackets).  A pair of CTAs takes 0.44 (0.6) a block of K
 // whatever part of its 256 tokens there is, and 5 besides; the kernel for few tokens 0.6 a step with 16 token columns, 0.65 with 32, 0.78 (0.87)
 // with 64 and 1.25 with 128 (gate and up weights: 1.9, which pairs beat), but not less than its weights take from memory, and 2 besides.  Sums over
-// a cluster cost 3 or 4.  Both sides of the line, measured: 128 tokens of 5120 x 13824 30 us with 128 columns and 47 in pairs, 128 of 10240 x 8192 38
-// and 32; 64 of 2 x 13824 x 5120 38 and 48, 128 69 and 49.
+// a cluster cost 3 or 4.  Both sides of the line, measured: 128 tokens of 5120 x 13824 29 us with 128 columns and 31 in pairs, 128 of 10240 x 8192 38
+// and 32; 64 of 5120 x 13824 20 and 31, of 2 x 13824 x 5120 36 and 46, 128 70 and 49.
 struct Fp8Plan {
   int nt;                                                      // token columns of the kernel for few tokens; 0: pairs
   int ks;                                                      // pairs: parts of K of the units behind the last whole round
