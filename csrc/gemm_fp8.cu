@@ -493,7 +493,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
 // ---- many tokens: pairs of CTAs, persistent ------------------------------------------------------------------------------------------
 // 256 tokens and 256 weight rows a pair (cta_group::2): a CTA has 128 of the tokens, loads those and half of the weight rows, and owns the
 // sums of its tokens.  Bound by the way from a product to the next but one, 785 to 810 cycles a block where the product takes 512, and by the card's
-// power (8192 x 5120 x 5120 190 us cold, 2260 TFLOP/s; 217 warm).  Units that do not fill a round of all pairs take a launch of their own with KS pairs a unit, clusters of 2 KS: each pair
+// power (8192 x 5120 x 5120 190 us cold, 2260 TFLOP/s; 217 warm).  Units that do not fill a round of all pairs take a launch of their own with
+// KS pairs a unit, clusters of 2 KS: each pair
 // has a part of K, and the sums of 128 / KS rows go to each of the CTAs that have the same tokens.
 constexpr int kPairThreads = 384;                // warp 0 loads, warp 1 issues the products, warps 4 .. 11 add them up
 // Registers: 168 a thread at launch (64512), then 56 for the first four warps and 216 for the other eight (62464): 128 sums and two reads of 16
