@@ -465,8 +465,9 @@ int zse_attn_decode_q8(const ZseAttnQ8* a);
 
 // ---- fp8_rows.cu: rows in 8-bit floating point --------------------------------------------------------------------------
 // data e4m3 [M][columns], ld_data bytes apart; scale fp32 [columns / 128, rounded up][ld_scale], a row's number the last index: an
-// element is data * scale.  Columns: a multiple of 16; data 16-byte aligned.  type 0 fp16, 1 bfloat16, 2 fp32.  Rows that are read may not
-// share memory with those that are written.  The three calls below return the number of kernels launched.
+// element is data * scale.  Columns: a multiple of 16; data 16-byte aligned.  type 0 fp16, 1 bfloat16, 2 fp32.  What a call writes, scales
+// among it, may share no byte with what it reads or with what else it writes (ZSE_ERR_SHAPE); columns side by side of the same rows are
+// apart, and `normed` may be `add`.  The three calls below return the number of kernels launched.
 // residual fp32 [M][H] += the sum of n_planes planes fp32 [M][H] and of add [M][H] (type, or null); data, scale = RMSNorm(residual) *
 // weight (type), which also goes to `normed` [M][H] (type) unless that is null.  type 0 or 1, H up to 32768.
 typedef struct ZseNormFp8 {

@@ -50,13 +50,31 @@ __device__ __forceinline__ float hold_f16(float x) {
 template <>
 __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) { return pack_half2(hold_f16(a), hold_f16(b)); }
 
-// Whether `rows` rows of `bytes` bytes, ld bytes apart, at p share none with those at q: apart as a whole, or columns of the same rows.
-inline bool rows_apart(const void* p, long long bytes, long long ld, const void* q, long long q_bytes, long long q_ld, int rows) {
-  const long long d = reinterpret_cast<const uint8_t*>(q) - reinterpret_cast<const uint8_t*>(p);
-  if (d >= (rows - 1) * ld + bytes || -d >= (rows - 1) * q_ld + q_bytes) return true;
-  if (rows == 1 || ld != q_ld || ld <= 0) return false;
+// What a call reads or writes: rows of `bytes` bytes, ld bytes apart (p null: nothing).
+struct Fp8Span {
+  const void* p;
+  long long bytes, ld, rows;
+};
+// Whether two share no byte: apart as a whole, or columns side by side of the same rows (a single row may be one of any distance).
+inline bool spans_apart(const Fp8Span& a, const Fp8Span& b) {
+  if (a.p == nullptr || b.p == nullptr) return true;
+  const long long d = reinterpret_cast<const uint8_t*>(b.p) - reinterpret_cast<const uint8_t*>(a.p);
+  if (d >= (a.rows - 1) * a.ld + a.bytes || -d >= (b.rows - 1) * b.ld + b.bytes) return true;
+  const long long ld = a.rows == 1 ? b.ld : a.ld;
+  if ((a.rows == 1 && b.rows == 1) || (a.rows > 1 && b.rows > 1 && a.ld != b.ld) || ld <= 0) return false;
   const long long column = (d % ld + ld) % ld;
-  return column >= bytes && column + q_bytes <= ld;
+  return column >= a.bytes && column + b.bytes <= ld;
+}
+// Whether what is written shares no byte with anything else of the call: CTAs work on rows in any order.
+template <int W, int R>
+bool written_apart(const Fp8Span (&written)[W], const Fp8Span (&read)[R]) {
+  for (int i = 0; i < W; ++i) {
+    for (int j = 0; j < i; ++j)
+      if (!spans_apart(written[i], written[j])) return false;
+    for (int j = 0; j < R; ++j)
+      if (!spans_apart(written[i], read[j])) return false;
+  }
+  return true;
 }
 
 }  // namespace zse

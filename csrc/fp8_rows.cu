@@ -230,6 +230,11 @@ extern "C" int zse_add_rmsnorm_fp8(const ZseNormFp8* n) {
     return ZSE_ERR_ALIGN;
   const NormFp8 a{static_cast<float*>(n->residual), static_cast<const float*>(n->planes), n->add, n->weight, n->normed,
                   static_cast<uint8_t*>(n->data), static_cast<float*>(n->scale), ld_data, n->ld_scale, n->eps, n->n_planes, n->M, n->H};
+  const long long M = n->M, H = n->H, blocks = (H + kFp8Block - 1) / kFp8Block;
+  const void* normed = n->normed == n->add ? nullptr : n->normed;           // (in the place of add: each thread reads its own columns first)
+  const Fp8Span written[] = {{n->residual, M * H * 4, 0, 1}, {n->data, H, ld_data, M}, {n->scale, M * 4, n->ld_scale * 4, blocks}, {normed, M * H * 2, 0, 1}};
+  const Fp8Span read[] = {{n->n_planes > 0 ? n->planes : nullptr, M * H * 4 * n->n_planes, 0, 1}, {n->add, M * H * 2, 0, 1}, {n->weight, H * 2, 0, 1}};
+  if (!written_apart(written, read)) return ZSE_ERR_SHAPE;
   const cudaStream_t st = static_cast<cudaStream_t>(n->stream);
   const bool several = n->n_planes + (n->add != nullptr) > 1;
   if (n->type == kFp8F16) return several ? norm_fp8<__half, true>(a, st) : norm_fp8<__half, false>(a, st);
@@ -245,7 +250,9 @@ extern "C" int zse_quant_fp8(const ZseQuantFp8* q) {
   if (q->M == 1) one.ldx = one.ld_data = 0, q = &one;          // (a single row may have any)
   const int item = q->type == kFp8F32 ? 4 : 2;
   if (!aligned(q->x, 16) || q->ldx * item % 16 || !aligned(q->data, 16) || q->ld_data % 16 || !aligned(q->scale, 4)) return ZSE_ERR_ALIGN;
-  if (!rows_apart(q->x, (q->act == kFp8None ? 1ll : 2ll) * q->C * item, q->ldx * item, q->data, q->C, q->ld_data, q->M)) return ZSE_ERR_SHAPE;
+  const Fp8Span written[] = {{q->data, q->C, q->ld_data, q->M}, {q->scale, q->M * 4ll, q->ld_scale * 4, (q->C + kFp8Block - 1) / kFp8Block}};
+  const Fp8Span read[] = {{q->x, (q->act == kFp8None ? 1ll : 2ll) * q->C * item, q->ldx * item, q->M}};
+  if (!written_apart(written, read)) return ZSE_ERR_SHAPE;
   const cudaStream_t st = static_cast<cudaStream_t>(q->stream);
   switch (q->type) {
     case kFp8F16: return quant_fp8<__half>(*q, st);

@@ -960,7 +960,11 @@ extern "C" int zse_gemm_fp8(const ZseGemmFp8* g) {
   if (!aligned(g->x, 16) || !aligned(g->w, 16) || g->ldx % 16 || g->ldw % 16 || !aligned(g->sx, 4) || !aligned(g->sw, 4) ||
       (glu ? !aligned(g->out, 16) || g->ldo % 16 : !aligned(g->out, item) || !aligned(g->bias, g->bias_type == kFp8F32 ? 4 : 2)))
     return ZSE_ERR_ALIGN;
-  if (!rows_apart(g->x, g->K, g->ldx, g->out, (long long)g->N * item, g->ldo * item, g->M)) return ZSE_ERR_SHAPE;
+  const long long n_kb = (g->K + kFp8Block - 1) / kFp8Block, nbs = (g->N + kFp8Block - 1) / kFp8Block, parts = glu ? 2 : 1;
+  const Fp8Span written[] = {{g->out, (long long)g->N * item, g->ldo * item, g->M}, {glu ? g->out_scale : nullptr, g->M * 4ll, g->ld_os * 4, nbs}};
+  const Fp8Span read[] = {{g->x, g->K, g->ldx, g->M}, {g->sx, g->M * 4ll, g->ld_sx * 4, n_kb}, {g->w, g->K, g->ldw, parts * g->N},
+                          {g->sw, parts * nbs * n_kb * 4, 0, 1}, {g->bias, g->N * (g->bias_type == kFp8F32 ? 4ll : 2ll), 0, 1}};
+  if (!written_apart(written, read)) return ZSE_ERR_SHAPE;
   const Fp8Args a{static_cast<const float*>(g->sx), static_cast<const float*>(g->sw), g->bias, g->out, static_cast<float*>(g->out_scale),
                   g->ldo, g->ld_sx, g->ld_os, g->M, g->N, g->K, g->type, g->bias_type, g->act, static_cast<Status*>(g->status)};
   const cudaStream_t st = static_cast<cudaStream_t>(g->stream);

@@ -8,8 +8,8 @@ holds an infinity or a NaN reads back as NaN).
 checkpoints of such weights have.  With ``glu`` it is a gate and an up weight of N / 2 rows each, one after the other, and the up
 weight begins blocks of its own.
 
-The operators write memory of its own: rows that share bytes with those they are made of are refused on the GPU (columns of the
-same buffer side by side are fine, and so is ``add_rmsnorm_fp8`` with ``normed`` in the place of ``add``).
+The operators write memory of its own: data and scales (and ``add_rmsnorm_fp8``'s residual and ``normed``) that share bytes with anything
+else of the call are refused on the GPU.  Columns of the same buffer side by side are fine, and so is ``normed`` in the place of ``add``.
 """
 from __future__ import annotations
 
