@@ -14,8 +14,8 @@ namespace {
 
 // ---- residual += planes + 16-bit rows; out = RMSNorm(residual) * weight in 8 bits --------------------------------------------------
 // A warp has blocks of 128 columns, four columns a lane, which stay in registers between the sum and the rounding: every number is read once
-// and written once.  More than one addend is summed in 64 bits and the squares always are, so that the same row gives the same bytes
-// however it is split.
+// and written once.  More than one addend is summed in 64 bits and the squares always are, a block's by itself and then the blocks' in an
+// order of their own, so that the same row gives the same bytes however it is split over warps.
 struct NormFp8 {
   float* residual;
   const float* planes;
@@ -44,11 +44,34 @@ __device__ __forceinline__ float4 load4<bf16>(const bf16* p) {
   return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
 }
 
+// s[j], j < J: a lane's part of the sum of block j of the warp's.  Returns the whole sum of block lane >> (5 - log2 J), J rounded up to a power of
+// two: lanes whose numbers differ in one bit are added, from bit 4 down, the same way for every J.  Where a lane still has several blocks,
+// it keeps half of them and sends the other half: 9 exchanges for eight blocks, not 40.
+template <int J>
+__device__ __forceinline__ double block_sums(const double (&s)[J], int lane) {
+  constexpr int P = J == 1 ? 1 : J == 2 ? 2 : J <= 4 ? 4 : 8;
+  double t[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) t[j] = j < J ? s[j < J ? j : 0] : 0.;
+  int o = 16;
+#pragma unroll
+  for (int n = P / 2; n > 0; n /= 2, o /= 2) {
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      const bool upper = lane & o;
+      t[j] = (upper ? t[j + n] : t[j]) + __shfl_xor_sync(0xffffffffu, upper ? t[j] : t[j + n], o);
+    }
+  }
+#pragma unroll
+  for (; o > 0; o /= 2) t[0] += __shfl_xor_sync(0xffffffffu, t[0], o);
+  return t[0];
+}
+
 // SEVERAL: more than one addend.  (One, and 256 threads: as many rows on an SM as registers allow.)
 template <typename T, int J, int THREADS, bool SEVERAL>
 __global__ void __launch_bounds__(THREADS, THREADS > 256 || SEVERAL ? 1 : J <= 5 ? 6 : 4)
 add_rmsnorm_fp8_kernel(const NormFp8 a) {
-  __shared__ double red[32];
+  __shared__ double red[256];                                  // a block's sum of squares
   pdl_launch_dependents();
   pdl_wait();
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -85,18 +108,21 @@ add_rmsnorm_fp8_kernel(const NormFp8 a) {
       }
     }
   }
-  double ss = 0;
+  double ss[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const double b[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-    ss = fma(b[0], b[0], fma(b[1], b[1], fma(b[2], b[2], fma(b[3], b[3], ss))));
+    ss[j] = fma(b[0], b[0], fma(b[1], b[1], fma(b[2], b[2], b[3] * b[3])));
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (lane == 0) red[warp] = ss;
+  constexpr int kLanes = J == 1 ? 32 : J == 2 ? 16 : J <= 4 ? 8 : 4;         // that have the same block's sum
+  const double sum = block_sums<J>(ss, lane);
+  const int mine = warp + lane / kLanes * warps;
+  if (lane % kLanes == 0 && lane / kLanes < J && mine < blocks) red[mine] = sum;
   __syncthreads();
   double total = 0;
-  for (int w = 0; w < warps; ++w) total += red[w];
+  for (int b = lane; b < blocks; b += 32) total += red[b];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   const float inv = float(rsqrt(total / H + a.eps));
 #pragma unroll
   for (int j = 0; j < J; ++j) {
