@@ -263,7 +263,7 @@ class TorchOps:
                 raise ValueError(f"{name}: {' or '.join(map(str, dtypes))} with {len(shape)} dimensions expected beside the other "
                                  f"tensors, not {t.dtype} {tuple(t.shape)} on {t.device}")
             fits = t.shape[0] >= shape[0] and (len(shape) == 1 or (t.shape[1] >= shape[1] if apart else t.shape[1] == shape[1]))
-            packed = t.stride(-1) == 1 and (t.dim() == 1 or t.shape[0] == 1 or t.stride(0) >= t.shape[1]) if apart else t.is_contiguous()
+            packed = (t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() == 1 or t.shape[0] == 1 or t.stride(0) >= t.shape[1]) if apart else t.is_contiguous()
             if not fits or not packed:
                 raise ValueError(f"{name}: {'' if apart else 'packed '}rows {shape} expected, not {tuple(t.shape)} with strides {t.stride()}")
 

@@ -70,8 +70,8 @@ class Fp8Weight:
         device = data.get_device()
         if not scale.is_contiguous() or device != scale.get_device():
             raise ValueError("the scales have to be contiguous, and on the device of the data")
-        if bias is not None and (glu or bias.dtype not in BIAS_TYPES or bias.stride() != (1,) or len(bias) != shape[0]
-                                 or bias.get_device() != device):
+        if bias is not None and (glu or bias.dtype not in BIAS_TYPES or bias.shape != shape[:1]
+                                 or (bias.stride() != (1,) and shape[0] != 1) or bias.get_device() != device):
             raise ValueError(f"a bias of {shape[0]} numbers in fp16, bfloat16 or fp32 is expected beside the data, none for a gate and up weight")
         self.data, self.scale, self.bias, self.glu = data, scale, bias, glu
 
