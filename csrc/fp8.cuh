@@ -33,9 +33,9 @@ __device__ __forceinline__ uint32_t fp8_pack4(const float* y, float steps) {
 // an argument whose rounding weighs as much as |z| is large.  With the products the result is off by up to (10 + 1.25 |z|) 2^-24 of itself (gelu's z
 // comes out of five roundings: 10 + 6.25 |z|): 2^-19 at z = -20, 2^-17 at z = -80, where half a step of e4m3 is 2^-4; below z = -87 the
 // sigmoid is 0.  With expf and a division rows of 13824 took a third longer.
-template <int ACT>
-__device__ __forceinline__ float fp8_gated(float g, float u) {
-  const float z = ACT == kFp8Silu ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
+// (Where `act` is not a constant both z are computed and one is taken, without a branch.)
+__device__ __forceinline__ float fp8_gated(int act, float g, float u) {
+  const float z = act == kFp8Silu ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
   return g * sigmoid_fast(z) * u;
 }
 

@@ -188,7 +188,7 @@ quant_fp8_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ d
       if constexpr (ACT != kFp8None) {
         u[r].values(v);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) y[k] = fp8_gated<ACT>(y[k], v[k]);
+        for (int k = 0; k < 8; ++k) y[k] = fp8_gated(ACT, y[k], v[k]);
       }
       uint32_t top = 0;
 #pragma unroll

@@ -45,12 +45,6 @@ __device__ __forceinline__ float bias_of(const Fp8Args& a, int n) {
                                    : __half2float(static_cast<const __half*>(a.bias)[n]);
 }
 
-// (fp8_gated with the activation as an argument, without a branch)
-__device__ __forceinline__ float gated(int act, float g, float u) {
-  const float z = act == kFp8Silu ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
-  return g * sigmoid_fast(z) * u;
-}
-
 __device__ __forceinline__ void store32(void* p, const uint32_t* v) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
                "r"(v[6]), "r"(v[7])
@@ -131,7 +125,7 @@ __device__ __forceinline__ void put_gated(const Fp8Args& a, float* acc, int t, i
   auto gate = [&](auto act) {
 #pragma unroll
     for (int i = 0; i < O; ++i) {
-      const float y = fp8_gated<decltype(act)::value>(acc[i], acc[O + i]);
+      const float y = fp8_gated(decltype(act)::value, acc[i], acc[O + i]);
       acc[i] = n + (i & ~15) < a.N ? y : 0.f;
       top = max(top, abs_bits(acc[i]));
     }
@@ -406,7 +400,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
         if constexpr (GLU) {
 #pragma unroll
           for (int l = 0; l < H; ++l) {
-            const float y = gated(a.act, acc[l], acc[H + l]);
+            const float y = fp8_gated(a.act, acc[l], acc[H + l]);
             acc[l] = n < a.N ? y : 0.f;
             const uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(acc[l]));
             if (lane == 0) bars->top[q][half * H + l] = __uint_as_float(top);
@@ -460,7 +454,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
       };
       if constexpr (GLU) {
         for (int i = half; i < mine; i += 2) {
-          const float y = n < a.N ? gated(a.act, sum_of(0, i), sum_of(1, i)) : 0.f;
+          const float y = n < a.N ? fp8_gated(a.act, sum_of(0, i), sum_of(1, i)) : 0.f;
           red[i * 128 + row] = y;                              // (where this thread read its own part of the first sum)
           const uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(y));
           if (lane == 0) bars->top[q][i] = __uint_as_float(top);
@@ -526,11 +520,6 @@ __device__ __forceinline__ void umma_fp8_pair(uint32_t d_tmem, uint64_t a_desc, 
       "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
-}
-
-__device__ __forceinline__ void commit_to(uint64_t* bar, uint16_t ctas) {    // arrives at this offset in the CTAs of the cluster
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"(ctas)
-               : "memory");
 }
 
 // WIDE: see put_rows (true for GLU); TYPE: of the output, where WIDE (its own kernel for each type: the sums come out 2 to 4 % faster).
@@ -623,7 +612,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
           if (elect_one()) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) umma_fp8_pair(tmem + buf * 256, da + j * 2, db + j * 2, idesc, j != 0);
-            commit_to(&bars->done[s], uint16_t(3u << leader));
+            tc_commit_pair(&bars->done[s], uint16_t(3u << leader));
           }
           __syncwarp();
           if (++s == kPairStages) { s = 0; ph ^= 1; }

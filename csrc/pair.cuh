@@ -52,11 +52,12 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap,
       "l"(tmap), "r"(x), "r"(y), "r"(cluster_bar)
       : "memory");
 }
-__device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {          // arrives at this offset in both CTAs
+// Arrives at this offset in the CTAs of the cluster that `ctas` names, both of a cluster of two.
+__device__ __forceinline__ void tc_commit_pair(uint64_t* bar, uint16_t ctas = 3) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
           smem_u32(bar)),
-      "h"(uint16_t(3))
+      "h"(ctas)
       : "memory");
 }
 __device__ __forceinline__ void pair_cluster_sync() {
