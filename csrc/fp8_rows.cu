@@ -15,7 +15,8 @@ namespace {
 // ---- residual += planes + 16-bit rows; out = RMSNorm(residual) * weight in 8 bits --------------------------------------------------
 // A warp has blocks of 128 columns, four columns a lane, which stay in registers between the sum and the rounding: every number is read once
 // and written once.  More than one addend is summed in 64 bits and the squares always are, a block's by itself and then the blocks' in an
-// order of their own, so that the same row gives the same bytes however it is split over warps.
+// order of their own, so that the same row gives the same bytes however it is split over warps (8192 x 5120, one 16-bit addend: 98 us, and 95 with
+// sums by warp, whose order goes by the launch).  Bound by memory where there are many rows: with the norm in 16 bits as well 105 us, 5.2 TB/s.
 struct NormFp8 {
   float* residual;
   const float* planes;
@@ -257,9 +258,9 @@ extern "C" int zse_add_rmsnorm_fp8(const ZseNormFp8* n) {
   const NormFp8 a{static_cast<float*>(n->residual), static_cast<const float*>(n->planes), n->add, n->weight, n->normed,
                   static_cast<uint8_t*>(n->data), static_cast<float*>(n->scale), ld_data, n->ld_scale, n->eps, n->n_planes, n->M, n->H};
   const long long M = n->M, H = n->H, blocks = (H + kFp8Block - 1) / kFp8Block;
-  const void* normed = n->normed == n->add ? nullptr : n->normed;           // (in the place of add: each thread reads its own columns first)
-  const Fp8Span written[] = {{n->residual, M * H * 4, 0, 1}, {n->data, H, ld_data, M}, {n->scale, M * 4, n->ld_scale * 4, blocks}, {normed, M * H * 2, 0, 1}};
-  const Fp8Span read[] = {{n->n_planes > 0 ? n->planes : nullptr, M * H * 4 * n->n_planes, 0, 1}, {n->add, M * H * 2, 0, 1}, {n->weight, H * 2, 0, 1}};
+  const void* add = n->add == n->normed ? nullptr : n->add;                 // (normed in its place: each thread reads its own columns first)
+  const Fp8Span written[] = {{n->residual, M * H * 4, 0, 1}, {n->data, H, ld_data, M}, {n->scale, M * 4, n->ld_scale * 4, blocks}, {n->normed, M * H * 2, 0, 1}};
+  const Fp8Span read[] = {{n->n_planes > 0 ? n->planes : nullptr, M * H * 4 * n->n_planes, 0, 1}, {add, M * H * 2, 0, 1}, {n->weight, H * 2, 0, 1}};
   if (!written_apart(written, read)) return ZSE_ERR_SHAPE;
   const cudaStream_t st = static_cast<cudaStream_t>(n->stream);
   const bool several = n->n_planes + (n->add != nullptr) > 1;

@@ -35,6 +35,7 @@ LAST = (M - 1) * H                                                          # by
     dict(scale=AT[0] - 40, ld_scale=10), dict(scale=AT[4]),
     dict(normed=AT[2] + 2 * H), dict(normed=AT[2] - 16), dict(normed=AT[0]), dict(normed=AT[1] + 4 * M * H), dict(normed=AT[3]),
     dict(residual=AT[1]), dict(residual=AT[1] + 4 * M * H), dict(residual=AT[2]), dict(residual=AT[3]),
+    dict(add=AT[1] + 64, normed=AT[1] + 64), dict(add=AT[3], normed=AT[3]), dict(add=AT[0], normed=AT[0]), dict(add=AT[6], normed=AT[6]),
     dict(normed=AT[2], data=AT[2] + 16), dict(M=1, data=AT[2]), dict(M=1, normed=AT[2] + 16),
 ])
 def test_norm(call):
