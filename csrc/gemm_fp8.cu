@@ -115,8 +115,8 @@ __device__ __forceinline__ void put_rows(const Fp8Args& a, float* y, int t, int 
 }
 
 // act(gate) * up of 64 neighbouring outputs of a row (acc: gates, then ups), the other 64 of their block in the thread of the other half.
-// No branch an output: with one, each had to be done before the next began, 9000 cycles a unit instead of 1500 (4096 x 2 x 13824 x 5120 674 us
-// instead of 571).
+// No branch an output: with one, each had to be done before the next began, 9000 cycles a unit instead of 1500 (4096 x 2 x 13824 x 5120 651 us
+// instead of 594).
 // `live` is false where the sums are not there; every warp of the barrier calls it.
 __device__ __forceinline__ void put_gated(const Fp8Args& a, float* acc, int t, int n, int half, float (*tops)[128], int row, int barrier,
                                           int threads, bool live) {
@@ -175,7 +175,7 @@ __device__ __forceinline__ void add_block(float* acc, uint32_t taddr, float s, f
 // two blocks of K of the same rows, or (GLU) gate and up rows of one block.  Where there are fewer tiles of rows than SMs, the CTAs of a
 // cluster have a part of K each and add their sums through distributed shared memory: each finishes a run of the tokens, from the parts in
 // rank order.  Bound by the weights' bytes where there are many steps (5 tokens of 2 x 13824 x 5120 26 us, 5.4 TB/s), by the steps' handshakes with
-// 64 columns (5120 x 13824 19.6 us, 3.7 TB/s), by the start and the cluster's two barriers with few (one token of 5120 x 5120 8.4 us).
+// 64 columns (5120 x 13824 19.6 us, 3.7 TB/s), by the start and the cluster's three barriers with few (one token of 5120 x 5120 8.4 us).
 template <int NT, bool GLU>
 struct Few {
   static constexpr int kX = NT * 128, kW = 128 * 128;

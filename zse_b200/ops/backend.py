@@ -339,7 +339,8 @@ class TorchOps:
 
     def linear_fp8(self, w, x, M, out):
         """out [M, N] (fp16, bfloat16 or fp32) = x w^T + bias of the first M rows of ``x`` (``Fp8Rows``); ``w``: ``Fp8Weight``.  Sums in
-        fp32, rounded once; fp16 is held within +-65504.  K: a multiple of 16."""
+        fp32, rounded once; fp16 is held within +-65504.  K: a multiple of 16.  (A row's scale times a weight's has to be a normal number of
+        fp32: below 1e-38 it loses bits.)"""
         self._check_linear_fp8(w, x, M, out)
         if M == 0:
             return
